@@ -382,6 +382,45 @@ int pf_cross_entropy_gap_fwd(const void* logits, int l_dtype, const int64_t* tar
 int pf_cross_entropy_gap_bwd(const void* logits, int l_dtype, const int64_t* targets, const float* row_lse,
                              const float* dloss, const float* n_valid, void* dlogits, int dl_dtype, int64_t rows,
                              int64_t classes, int64_t ignore_index, int64_t group, int64_t gap, void* stream);
+/* ---- losses over the log-probabilities of given tokens (fine-tuning by preferences and policy gradients) -----------------
+ * Beside the cross entropy above; the reference's loss modules (pfeife/loss.py:4-70) stop there.  logits [B, T, V] (fp32, fp16
+ * or bf16; sb / st elements between sequences / rows, unit stride over the classes, no alignment asked for), labels int64
+ * [B, T] contiguous.  shift 0: row t is scored against label t; 1: against label t + 1, so that R = T - shift rows of a sequence are
+ * scored and the last one takes no part.  A row whose label is ignore_index is not read: its logprob is 0, its gradient zeros.
+ * Other labels outside [0, V) read nothing and give NaN.  p = softmax(logits / temperature).
+ *   pf_token_logprob_fwd   logprobs[b, t] = ln p[b, t, label], fp32 [B, R]; stats (optional) fp32 [B, R, 2]: what the backward needs
+ *   pf_token_logprob_bwd   dlogits[b, t, :] = g (onehot - p) / temperature in the logits' dtype, all B * T rows written (zeros where a
+ *                          row takes no part); g = coef[b * g_sb + t * g_st] (* scale[0]).  unless_one != 0: does nothing
+ *                          where scale[0] is 1, i.e. where dlogits already holds the gradient (pf_policy_loss writes it)
+ *   pf_preference_loss     sequences 2i (preferred) and 2i + 1: rewards[b] = beta (sum of its logprobs - ref[b]) (length_average:
+ *                          their mean), D = rewards[2i] - rewards[2i + 1], loss[0] = mean of -(1 - label_smoothing) ln sigma(D)
+ *                          - label_smoothing ln sigma(-D); coef[b] = d loss / d logprob of each of b's tokens and stats
+ *                          (optional) are what pf_token_logprob_bwd takes (g_sb = 1, g_st = 0).  workspace:
+ *                          pf_preference_workspace(B, T, shift) doubles
+ *   pf_policy_loss         r = exp(logprob - old), q = ref - logprob: loss[0] = sum of w (-min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A)
+ *                          + kl_coef k), kl[0] = sum of w k with k = exp(q) - q - 1 (ref_logprobs null: 0); old / ref fp32 [B, R],
+ *                          A = advantages[b * a_sb + t * a_st].  w = 1 / (tokens that count), by_sequence != 0: 1 / (such tokens of the
+ *                          sequence * sequences that have any); with no such token loss and kl are 0.  stats and coef (optional,
+ *                          both or neither) are what pf_token_logprob_bwd takes (g_sb = R, g_st = 1); dlogits (optional): the
+ *                          gradient, written in the same pass.  workspace: pf_policy_workspace(B, T, shift) doubles */
+int pf_token_logprob_fwd(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, int64_t sb, int64_t st,
+                         const int64_t* labels, int shift, int64_t ignore_index, double temperature, float* logprobs,
+                         float* stats, void* stream);
+int pf_token_logprob_bwd(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, int64_t sb, int64_t st,
+                         const int64_t* labels, int shift, int64_t ignore_index, double temperature, const float* stats,
+                         const float* coef, int64_t g_sb, int64_t g_st, const float* scale, int unless_one, void* dlogits,
+                         int64_t d_sb, int64_t d_st, void* stream);
+int64_t pf_preference_workspace(int64_t B, int64_t T, int shift);
+int pf_preference_loss(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, int64_t sb, int64_t st,
+                       const int64_t* labels, int shift, int64_t ignore_index, const float* ref, double beta,
+                       double label_smoothing, int length_average, float* loss, float* rewards, float* stats, float* coef,
+                       double* workspace, void* stream);
+int64_t pf_policy_workspace(int64_t B, int64_t T, int shift);
+int pf_policy_loss(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, int64_t sb, int64_t st,
+                   const int64_t* labels, int shift, int64_t ignore_index, double temperature, const float* old_logprobs,
+                   const float* advantages, int64_t a_sb, int64_t a_st, const float* ref_logprobs, double clip_low,
+                   double clip_high, double kl_coef, int by_sequence, float* loss, float* kl, float* logprobs, float* stats,
+                   float* coef, void* dlogits, int64_t d_sb, int64_t d_st, double* workspace, void* stream);
 /* Mean squared error (F.mse_loss, bench_models/models/train_sdxl.py:1422-1424):
  * loss[0] = mean((a-b)^2) computed in fp32; partial: fp32 [pf_reduce_workspace(n)]. */
 int64_t pf_reduce_workspace(int64_t n);
@@ -498,6 +537,18 @@ int pf_adam_step(const pf_adam_item* items_dev, int n_items, int64_t max_n, doub
 int pf_adam_step_chunks(const pf_adam_item* items_dev, const int64_t* chunk_ends_dev, int n_items, int64_t n_chunks,
                         double lr, double beta1, double beta2, double eps, double weight_decay, int64_t step, int adamw,
                         float* scaler_state, void* stream);
+
+/* AdamW whose moments are held in 8 bits: e4m3 codes (PF_ADAM8_BLOCK consecutive elements share an fp32 scale) of the first
+ * moment and of the second's square root, rounded up or down at random so that their mean is kept (bits of element, tensor and
+ * step: reproducible).  items_dev: n_items rows of eight 64-bit words in DEVICE memory, {param, grad, first moment's codes, its
+ * scales, root's codes, its scales, n, tensor}; pointers to fp32 params and gradients, n codes and ceil(n / PF_ADAM8_BLOCK) scales each;
+ * `tensor` is a number of the caller's that sets the rounding of one tensor apart from another's.  With both scale pointers null an
+ * item's moments are fp32 (exp_avg, exp_avg_sq).  No alignment is asked for beyond the types'.  chunk_ends_dev, n_chunks,
+ * step and scaler_state as for pf_adam_step_chunks.  Adds to what get_optimizer_cls offers (pfeife/option.py:9-29). */
+#define PF_ADAM8_BLOCK 256
+int pf_adam8_step(const int64_t* items_dev, const int64_t* chunk_ends_dev, int n_items, int64_t n_chunks, double lr,
+                  double beta1, double beta2, double eps, double weight_decay, int64_t step, float* scaler_state,
+                  void* stream);
 
 /* ---- dynamic loss scaling on the device ---------------------------------------------
  * torch.amp.GradScaler's rule without a host synchronisation.  `state` is float[8] in DEVICE

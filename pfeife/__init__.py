@@ -9,7 +9,7 @@ import sys
 import pfeife_amd
 from pfeife_amd import PipeOption  # noqa: F401
 
-for _name in ("option", "batch", "loss", "utils", "mp", "mp.net_states", "mp.partial", "mp.partial.module",
+for _name in ("option", "batch", "loss", "optim", "utils", "mp", "mp.net_states", "mp.partial", "mp.partial.module",
               "mp.worker", "schedule", "schedule.scheduler", "graph", "graph.partition_graph"):
     sys.modules["pfeife." + _name] = importlib.import_module("pfeife_amd." + _name)
 

@@ -30,6 +30,9 @@ void pf_set_error(const char* fmt, ...);
 // kernel may have; remembered per kernel and device.  Any thread.
 int pf_allow_lds(const void* kernel, size_t bytes, const char* who);
 
+// Under a loss scaler: step_size and the root of the second bias correction, of the device's count of completed steps, into state[4..5].
+void pf_adam_coefficients(float* state, double lr, double beta1, double beta2, void* stream);
+
 #define PF_REQUIRE(cond, ...)            \
   do {                                   \
     if (!(cond)) {                       \
@@ -235,6 +238,22 @@ __device__ __forceinline__ float pf_wave_max(float v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, PF_WAVE));
   return v;
+}
+
+// Which item holds a chunk: `ends`, the chunks up to and including each item's last, is searched by each wavefront, 64 ways at
+// a time (uniform result; the last end is past the chunk).
+__device__ __forceinline__ int pf_find_item(const int64_t* ends, int n_items, int64_t chunk) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, hi = n_items - 1;      // the item is one of these: the first whose end is past the chunk
+  while (lo < hi) {
+    const int step = (hi - lo + 64) / 64;
+    int at = lo + (lane + 1) * step - 1;
+    if (at > hi) at = hi;
+    const int k = __ffsll((unsigned long long)__ballot(ends[at] > chunk)) - 1;   // (the last item's end is)
+    hi = lo + (k + 1) * step - 1 < hi ? lo + (k + 1) * step - 1 : hi;
+    lo = lo + k * step;
+  }
+  return __builtin_amdgcn_readfirstlane(lo);
 }
 
 // Block-wide reductions for blocks of NW wavefronts; `sm` holds >= NW floats.

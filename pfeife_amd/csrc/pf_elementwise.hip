@@ -522,23 +522,12 @@ struct AdamCoef {
 // magnitude, so they are cut into chunks of 1024, and a workgroup updates one: all that is in flight then lies in a narrow window that moves over the
 // seven streams (see the top of this file).  2048 workgroups that stay, with consecutive chunks each, reach 5.2 TB/s over 268 M parameters, chunks dealt
 // out in turn 4.9, two chunks to a workgroup 5.7, one 6.2.  Everything is next used a step later and bypasses the caches.
-// Which item: `ends`, the chunks up to and including each item's last, is searched by each wavefront, 64 ways at a time.
 constexpr int ADAM_CHUNK = PF_ADAM_CHUNK;
 __global__ __launch_bounds__(256) void adam_chunk_kernel(const pf_adam_item* items, const int64_t* ends, int64_t first, int n_items, AdamCoef c,
                                                          const float* scaler_state) {
   if (!c.scaled(scaler_state)) return;
   const int64_t chunk = first + blockIdx.x;
-  const int lane = threadIdx.x & 63;
-  int lo = 0, hi = n_items - 1;      // the item is one of these: the first whose end is past the chunk
-  while (lo < hi) {
-    const int step = (hi - lo + 64) / 64;
-    int at = lo + (lane + 1) * step - 1;
-    if (at > hi) at = hi;
-    const int k = __ffsll((unsigned long long)__ballot(ends[at] > chunk)) - 1;   // (the last item's end is)
-    hi = lo + (k + 1) * step - 1 < hi ? lo + (k + 1) * step - 1 : hi;
-    lo = lo + k * step;
-  }
-  lo = __builtin_amdgcn_readfirstlane(lo);
+  const int lo = pf_find_item(ends, n_items, chunk);
   c.update4(items[lo], (chunk - (lo > 0 ? ends[lo - 1] : 0)) * ADAM_CHUNK + threadIdx.x * 4);
 }
 
@@ -1111,14 +1100,17 @@ int adam_launch(const pf_adam_item* items_dev, int n_items, int64_t max_n, doubl
 }
 }  // namespace
 
+void pf_adam_coefficients(float* state, double lr, double beta1, double beta2, void* stream) {
+  hipLaunchKernelGGL(adam_coefficients_kernel, dim3(1), dim3(1), 0, (hipStream_t)stream, state, lr, beta1, beta2);
+}
+
 extern "C" int pf_adam_step_chunks(const pf_adam_item* items_dev, const int64_t* chunk_ends_dev, int n_items, int64_t n_chunks, double lr,
                                    double beta1, double beta2, double eps, double weight_decay, int64_t step, int adamw,
                                    float* scaler_state, void* stream) {
   PF_REQUIRE(n_items >= 0 && n_chunks >= 0 && (scaler_state != nullptr || step >= 1), "pf_adam_step_chunks: bad arguments");
   if (n_items == 0 || n_chunks == 0) return PF_OK;
   PF_REQUIRE(items_dev != nullptr && chunk_ends_dev != nullptr, "pf_adam_step_chunks: bad item list");
-  if (scaler_state != nullptr)
-    hipLaunchKernelGGL(adam_coefficients_kernel, dim3(1), dim3(1), 0, (hipStream_t)stream, scaler_state, lr, beta1, beta2);
+  if (scaler_state != nullptr) pf_adam_coefficients(scaler_state, lr, beta1, beta2, stream);
   const AdamCoef c = adam_coef(lr, beta1, beta2, eps, weight_decay, scaler_state != nullptr ? 1 : step, adamw);
   for (int64_t first = 0; first < n_chunks; first += EW_MAX_BLOCKS) {      // (a launch has less than 2^32 threads)
     const int64_t blocks = n_chunks - first < EW_MAX_BLOCKS ? n_chunks - first : EW_MAX_BLOCKS;

@@ -21,6 +21,7 @@ ABI_VERSION = 6
 PF_F32, PF_F16, PF_BF16, PF_I64, PF_I32, PF_U8 = 0, 1, 2, 3, 4, 5
 ACT_NONE, ACT_GELU, ACT_GELU_TANH, ACT_SILU, ACT_RELU = 0, 1, 2, 3, 4
 ADAM_CHUNK = 1024   # PF_ADAM_CHUNK
+ADAM8_BLOCK = 256   # PF_ADAM8_BLOCK
 
 _DTYPE_CODE = {
     torch.float32: PF_F32,
@@ -91,7 +92,7 @@ class AttnDesc(Structure):
 
 
 # name -> argtypes (every function returns int unless listed in _RET_I64)
-_P, _I, _L, _F = c_void_p, c_int, c_int64, c_float
+_P, _I, _L, _F, _D = c_void_p, c_int, c_int64, c_float, ctypes.c_double
 _SIGNATURES = {
     "pf_init": [_I],
     "pf_graph_capture_begin": [_P],
@@ -131,6 +132,10 @@ _SIGNATURES = {
     "pf_cross_entropy_bwd": [_P, _I, _P, _P, _P, _P, _P, _I, _L, _L, _L, _P],
     "pf_cross_entropy_gap_fwd": [_P, _I, _P, _P, _P, _P, _L, _L, _L, _L, _L, _P],
     "pf_cross_entropy_gap_bwd": [_P, _I, _P, _P, _P, _P, _P, _I, _L, _L, _L, _L, _L, _P],
+    "pf_token_logprob_fwd": [_P, _I, _L, _L, _L, _L, _L, _P, _I, _L, _D, _P, _P, _P],
+    "pf_token_logprob_bwd": [_P, _I, _L, _L, _L, _L, _L, _P, _I, _L, _D, _P, _P, _L, _L, _P, _I, _P, _L, _L, _P],
+    "pf_preference_loss": [_P, _I, _L, _L, _L, _L, _L, _P, _I, _L, _P, _D, _D, _I, _P, _P, _P, _P, _P, _P],
+    "pf_policy_loss": [_P, _I, _L, _L, _L, _L, _L, _P, _I, _L, _D, _P, _P, _L, _L, _P, _D, _D, _D, _I, _P, _P, _P, _P, _P, _P, _L, _L, _P, _P],
     "pf_mse_fwd": [_P, _I, _P, _I, _P, _P, _L, _P],
     "pf_mse_bwd": [_P, _I, _P, _I, _P, _P, _I, _L, _P],
     "pf_sum_fwd": [_P, _I, _P, _P, _L, _P],
@@ -153,6 +158,7 @@ _SIGNATURES = {
                             ctypes.c_double, _I, _P, _P],
     "pf_adam_step_chunks": [_P, _P, _I, _L, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double,
                             ctypes.c_double, _L, _I, _P, _P],
+    "pf_adam8_step": [_P, _P, _I, _L, _D, _D, _D, _D, _D, _L, _P, _P],
     "pf_scale_by_state": [_P, _I, _P, _P, _I, _L, _P],
     "pf_scaler_unscale": [_P, _L, _P, _P],
     "pf_scaler_update": [_P, ctypes.c_double, ctypes.c_double, _I, _P],
@@ -168,7 +174,8 @@ _SIGNATURES = {
     "pf_mfma16_rate": [_I, _P, _L, _I, _P, _P],
 }
 _RET_I64 = {"pf_gemm_colsum_rows": [POINTER(GemmDesc)], "pf_colreduce_workspace": [_L, _L], "pf_reduce_workspace": [_L],
-            "pf_groupnorm_workspace": [_L, _L, _I],
+            "pf_groupnorm_workspace": [_L, _L, _I], "pf_policy_workspace": [_L, _L, _I],
+            "pf_preference_workspace": [_L, _L, _I],
             "pf_colsum_static_capacity": []}
 EXPORTED_SYMBOLS = sorted(list(_SIGNATURES) + list(_RET_I64) + ["pf_version", "pf_last_error"])
 
@@ -640,6 +647,36 @@ class HipKernels:
         return self._prep("pf_cross_entropy_gap_bwd" if gap else "pf_cross_entropy_bwd", args + ((group, gap) if gap else ()),
                           (logits, targets, row_lse, dloss, loss, dlogits), rows * classes * (_es(logits) + _es(dlogits)))
 
+    # -- losses over token log-probabilities: `rows` is (logits, B, T, V, sb, st, labels, shift, ignore_index, temperature) -------
+    def token_logprob_fwd(self, rows, logprobs, stats=None):
+        args = self._token_rows(rows) + (_ptr(logprobs), _ptr(stats))
+        return self._prep("pf_token_logprob_fwd", args, (rows, logprobs, stats))
+
+    def token_logprob_bwd(self, rows, stats, coef, g_strides, dlogits, d_strides, scale=None, unless_one=0):
+        args = self._token_rows(rows) + (_ptr(stats), _ptr(coef), *g_strides, _ptr(scale), int(unless_one), _ptr(dlogits), *d_strides)
+        return self._prep("pf_token_logprob_bwd", args, (rows, stats, coef, dlogits, scale))
+
+    def preference_workspace(self, B, T, shift):
+        return int(self.lib.pf_preference_workspace(B, T, int(shift)))
+
+    def preference_loss(self, rows, ref, beta, smoothing, average, loss, rewards, stats, coef, ws):
+        args = self._token_rows(rows)[:-1] + (_ptr(ref), beta, smoothing, int(average), _ptr(loss), _ptr(rewards), _ptr(stats), _ptr(coef), _ptr(ws))
+        return self._prep("pf_preference_loss", args, (rows, ref, loss, rewards, stats, coef, ws))
+
+    def policy_workspace(self, B, T, shift):
+        return int(self.lib.pf_policy_workspace(B, T, int(shift)))
+
+    def policy_loss(self, rows, old, adv, a_strides, ref, clip_low, clip_high, kl_coef, by_sequence, loss, kl, logprobs, stats, coef,
+                    dlogits, d_strides, ws):
+        args = self._token_rows(rows) + (_ptr(old), _ptr(adv), *a_strides, _ptr(ref), clip_low, clip_high, kl_coef, int(by_sequence),
+                                         _ptr(loss), _ptr(kl), _ptr(logprobs), _ptr(stats), _ptr(coef), _ptr(dlogits), *d_strides, _ptr(ws))
+        return self._prep("pf_policy_loss", args, (rows, old, adv, ref, loss, kl, logprobs, stats, coef, dlogits, ws))
+
+    @staticmethod
+    def _token_rows(rows):
+        logits, B, T, V, sb, st, labels, shift, ignore_index, temperature = rows
+        return (_ptr(logits), _dt(logits), B, T, V, sb, st, _ptr(labels), int(shift), ignore_index, temperature)
+
     def mse_fwd(self, a, b, partial, loss, n):
         args = (_ptr(a), _dt(a), _ptr(b), _dt(b), _ptr(partial), _ptr(loss), n)
         return self._prep("pf_mse_fwd", args, (a, b, partial, loss))
@@ -748,6 +785,23 @@ class HipKernels:
 
     def adam_step_scaled(self, table, n_items, n_chunks, lr, beta1, beta2, eps, weight_decay, adamw, state, stream):
         self._adam(table, n_items, n_chunks, lr, beta1, beta2, eps, weight_decay, 1, adamw, state.data_ptr(), stream)
+
+    def adam8_table(self, items):
+        """Device table of pf_adam8_step's items [(param, grad, m, m_scale, root, root_scale, tensor)] (scales None: moments
+        in 32 bits), then the running count of their chunks.  -> (table, items, chunks)"""
+        rows, ends, chunks = [], [], 0
+        for p, g, m, ms, r, rs, tensor in items:
+            n = p.numel()
+            rows += [_ptr(p), _ptr(g), _ptr(m), _ptr(ms) or 0, _ptr(r), _ptr(rs) or 0, n, tensor]
+            chunks += -(-n // ADAM_CHUNK)
+            ends.append(chunks)
+        return torch.tensor(rows + ends, dtype=torch.int64).to(items[0][0].device), len(ends), chunks
+
+    def adam8_step(self, table, n_items, n_chunks, lr, beta1, beta2, eps, weight_decay, step, state, stream):
+        at = table.data_ptr()
+        rc = self.lib.pf_adam8_step(at, at + 64 * n_items, n_items, n_chunks, lr, beta1, beta2, eps, weight_decay, step, _ptr(state), stream)
+        if rc != 0:
+            raise RuntimeError("pf_adam8_step failed: %s" % self.lib.pf_last_error().decode())
 
     # -- dynamic loss scaling (state: float32[8] on the device) ----------------------------
     def scale_by_state(self, src, state, dst, n):

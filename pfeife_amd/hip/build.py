@@ -28,6 +28,8 @@ SOURCES = [
     "pf_norm.hip",
     "pf_elementwise.hip",
     "pf_softmax_loss.hip",
+    "pf_token_loss.hip",
+    "pf_adam8.hip",
     "pf_batch.hip",
     "pf_mfma_rate.hip",
 ]

@@ -5,7 +5,13 @@ pfeife/loss.py:4-70).
 nn.CrossEntropyLoss computed by the pf_cross_entropy_fwd/bwd kernels when the
 logits live on the GPU; `SumLoss` uses pf_sum_fwd.  The wrappers are ordinary
 autograd nodes, so user code keeps calling `loss.backward()`.
+
+For fine-tuning a language model: `token_logprobs` (log-probabilities of given tokens),
+`preference_loss` (paired log ratios against a reference model) and `policy_loss` (clipped
+ratio with a KL term), each straight from the logits, and `PreferenceLoss` / `PolicyLoss`.
 """
+import math
+
 import torch
 import torch.nn as nn
 
@@ -88,6 +94,231 @@ def cross_entropy(logits, target, ignore_index=-100):
     return _CrossEntropyFn.apply(logits, target, ignore_index)
 
 
+_tables = {}
+
+
+def _table(t, who):
+    """The kernel table of the tensor's own device."""
+    if t.device.type != "cuda":
+        raise RuntimeError("%s: the HIP loss kernels need GPU tensors (got %s)" % (who, t.device))
+    k = _tables.get(t.device.index)
+    if k is None:
+        from .hip import HipKernels
+
+        with torch.cuda.device(t.device):
+            k = _tables[t.device.index] = HipKernels(t.device.index)
+    return k
+
+
+def _issue(t, launch):
+    """On the current stream of the tensor's device, whichever device is the current one."""
+    stream = torch.cuda.current_stream(t.device).cuda_stream
+    if torch.cuda.current_device() == t.device.index:
+        launch(stream)
+    else:
+        with torch.cuda.device(t.device):
+            launch(stream)
+
+
+def _check_rows(who, logits, labels, ignore_index, temperature, shift):
+    """What the three losses ask of their logits and labels.  -> (logits [B, T, V] with unit stride over the classes, labels [B, T])"""
+    if not torch.is_tensor(logits) or not torch.is_tensor(labels):
+        raise RuntimeError("%s: logits and labels are tensors" % who)
+    _table(logits, who)
+    if logits.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise RuntimeError("%s: logits are fp32, fp16 or bf16 (got %s)" % (who, logits.dtype))
+    if logits.dim() < 2 or logits.shape[-1] == 0:
+        raise RuntimeError("%s: logits are [..., tokens, classes] (got %s)" % (who, tuple(logits.shape)))
+    if labels.dtype != torch.int64 or labels.device != logits.device or labels.shape != logits.shape[:-1]:
+        raise RuntimeError("%s: labels are int64 %s on %s (got %s %s on %s)"
+                           % (who, tuple(logits.shape[:-1]), logits.device, labels.dtype, tuple(labels.shape), labels.device))
+    if not isinstance(ignore_index, int) or not isinstance(shift, (bool, int)) or shift not in (0, 1):
+        raise RuntimeError("%s: ignore_index is a whole number and shift a truth value" % who)
+    if not 1e-6 <= temperature <= 1e6:
+        raise RuntimeError("%s: temperature must lie in [1e-6, 1e6] (got %s)" % (who, temperature))
+    if logits.dim() != 3:
+        logits = logits.reshape((math.prod(logits.shape[:-2]),) + logits.shape[-2:])
+        labels = labels.reshape(logits.shape[:-1])
+    if logits.stride(-1) != 1 and logits.shape[-1] > 1:
+        logits = logits.contiguous()
+    return logits, labels.contiguous()
+
+
+def _constant(who, name, t, shapes, like):
+    """An operand that no gradient flows to, fp32 on the logits' device, of one of these shapes."""
+    if not torch.is_tensor(t) or not t.is_floating_point() or t.device != like.device or tuple(t.shape) not in shapes:
+        raise RuntimeError("%s: %s is a floating tensor of shape %s on %s (got %s)"
+                           % (who, name, " or ".join(map(str, shapes)), like.device,
+                              "%s %s on %s" % (t.dtype, tuple(t.shape), t.device) if torch.is_tensor(t) else type(t).__name__))
+    if t.requires_grad:
+        raise RuntimeError("%s: no gradient flows to %s: detach it" % (who, name))
+    return t.to(torch.float32)
+
+
+def _rows(logits, labels, cfg):
+    """The kernels' description of the rows; cfg = (shift, ignore_index, temperature)."""
+    B, T, V = logits.shape
+    return (logits, B, T, V, logits.stride(0), logits.stride(1), labels, *cfg)
+
+
+def _new(like, *shape, dtype=torch.float32):
+    return torch.empty(shape, dtype=dtype, device=like.device)
+
+
+def _logits_gradient(logits, labels, cfg, stats, coef, g_strides, scale=None, into=None, unless_one=0):
+    d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if into is None else into
+    _issue(logits, _table(logits, "").token_logprob_bwd(_rows(logits, labels, cfg), stats, coef, g_strides, d, d.stride()[:2], scale, unless_one))
+    return d
+
+
+def _as_scale(g):
+    return g if g.dtype == torch.float32 else g.to(torch.float32)
+
+
+class _TokenLogprobFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, cfg, want):
+        B, T, _ = logits.shape
+        out = _new(logits, B, max(0, T - cfg[0]))
+        stats = _new(logits, *out.shape, 2) if want else None
+        _issue(logits, _table(logits, "").token_logprob_fwd(_rows(logits, labels, cfg), out, stats))
+        if want:
+            ctx.save_for_backward(logits, labels, stats)
+            ctx.cfg = cfg
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        logits, labels, stats = ctx.saved_tensors
+        grad = _as_scale(grad)      # (any strides: a sum's gradient is one number)
+        return _logits_gradient(logits, labels, ctx.cfg, stats, grad, grad.stride()), None, None, None
+
+
+class _PreferenceFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, ref, cfg, beta, smoothing, average, want):
+        B, T, _ = logits.shape
+        k = _table(logits, "")
+        stats = _new(logits, B, max(0, T - cfg[0]), 2) if want else None
+        loss, rewards, coef = _new(logits), _new(logits, B), _new(logits, B)
+        _issue(logits, k.preference_loss(_rows(logits, labels, cfg), ref, beta, smoothing, average, loss, rewards, stats, coef,
+                                         _new(logits, k.preference_workspace(B, T, cfg[0]), dtype=torch.float64)))
+        if want:
+            ctx.save_for_backward(logits, labels, stats, coef)
+            ctx.cfg = cfg
+        ctx.mark_non_differentiable(rewards)
+        ctx.set_materialize_grads(False)
+        return loss, rewards
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, _):
+        logits, labels, stats, coef = ctx.saved_tensors
+        d = None if grad is None else _logits_gradient(logits, labels, ctx.cfg, stats, coef, (1, 0), _as_scale(grad))
+        return (d,) + (None,) * 7
+
+
+class _PolicyFn(torch.autograd.Function):
+    """The gradient of a loss that is itself the end (`loss.backward()`) is written by the forward pass, which has the row at
+    hand: a token's part of it depends on its own row alone.  The backward pass looks at what it is asked to multiply it
+    by, on the device: by one it has nothing to do, by anything else it computes the gradient from the logits."""
+
+    @staticmethod
+    def forward(ctx, logits, labels, old, adv, a_strides, ref, cfg, clip, kl_coef, by_sequence, want):
+        B, T, _ = logits.shape
+        k = _table(logits, "")
+        R = max(0, T - cfg[0])
+        loss, kl, logprobs = _new(logits), _new(logits), _new(logits, B, R)
+        stats, coef, d = (_new(logits, B, R, 2), _new(logits, B, R), torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)) \
+            if want else (None, None, None)
+        _issue(logits, k.policy_loss(_rows(logits, labels, cfg), old, adv, a_strides, ref, *clip, kl_coef, by_sequence, loss, kl, logprobs, stats,
+                                     coef, d, d.stride()[:2] if want else (0, 0), _new(logits, k.policy_workspace(B, T, cfg[0]), dtype=torch.float64)))
+        if want:
+            ctx.save_for_backward(logits, labels, stats, coef)
+            ctx.cfg, ctx.d, ctx.captured = cfg, d, torch.cuda.is_current_stream_capturing()
+        ctx.mark_non_differentiable(logprobs, kl)
+        ctx.set_materialize_grads(False)
+        return loss, logprobs, kl
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, *_):
+        logits, labels, stats, coef = ctx.saved_tensors
+        d = None
+        if grad is not None:
+            # handed out once (what has it may change it), and not from an eager forward pass to a graph, whose
+            # replays would find it changed
+            d, ctx.d = ctx.d, None
+            ready = d is not None and ctx.captured == torch.cuda.is_current_stream_capturing()
+            d = _logits_gradient(logits, labels, ctx.cfg, stats, coef, coef.stride(), _as_scale(grad), d if ready else None, int(ready))
+        return (d,) + (None,) * 10
+
+
+def token_logprobs(logits, labels, *, ignore_index=-100, temperature=1.0, shift=False):
+    """Log-probabilities of the labels: log softmax(logits / temperature)[label], fp32, with the gradient to the logits.
+
+    logits [..., T, V] (fp32, fp16 or bf16), labels int64 [..., T].  shift: row t is scored against label t + 1 (labels as
+    the model's own input), the result has T - 1 tokens.  Tokens whose label is `ignore_index` give 0 and take no part, whatever
+    their logits hold; labels outside the vocabulary give NaN."""
+    x, y = _check_rows("token_logprobs", logits, labels, ignore_index, temperature, shift)
+    cfg = (int(shift), ignore_index, float(temperature))
+    out = _TokenLogprobFn.apply(x, y, cfg, torch.is_grad_enabled() and x.requires_grad)
+    return out.reshape(logits.shape[:-2] + out.shape[1:])
+
+
+def preference_loss(logits, labels, ref_logprobs, *, beta=0.1, label_smoothing=0.0, length_average=False, ignore_index=-100, shift=False):
+    """Preference loss over pairs of answers; -> (loss, rewards).
+
+    logits [2P, T, V], labels int64 [2P, T]: sequences 2i (preferred) and 2i + 1 (rejected) are a pair, so that a batch split into
+    micro-batches of whole pairs keeps them together.  ref_logprobs [2P]: the sum (length_average: the mean) of the answer's
+    token log-probabilities under the reference model.  With s the same of this model, rewards = beta (s - ref) and D the preferred
+    minus the rejected reward, loss = mean of -(1 - label_smoothing) log sigmoid(D) - label_smoothing log sigmoid(-D).  The
+    gradient flows to the logits; `rewards` [2P] are for the log.  `shift` and `ignore_index` as for `token_logprobs`."""
+    who = "preference_loss"
+    x, y = _check_rows(who, logits, labels, ignore_index, 1.0, shift)
+    B = logits.shape[0]
+    if logits.dim() != 3 or B == 0 or B % 2:
+        raise RuntimeError("%s: logits are [2 * pairs, tokens, classes] (got %s)" % (who, tuple(logits.shape)))
+    if not math.isfinite(beta) or not 0.0 <= label_smoothing <= 1.0:
+        raise RuntimeError("%s: beta must be finite and label_smoothing lie in [0, 1]" % who)
+    ref = _constant(who, "ref_logprobs", ref_logprobs, [(B,)], logits).contiguous()
+    return _PreferenceFn.apply(x, y, ref, (int(shift), ignore_index, 1.0), float(beta), float(label_smoothing), bool(length_average),
+                               torch.is_grad_enabled() and x.requires_grad)
+
+
+def policy_loss(logits, labels, old_logprobs, advantages, ref_logprobs=None, *, clip=0.2, clip_high=None, kl_coef=0.0, temperature=1.0,
+                reduction="tokens", ignore_index=-100, shift=False):
+    """Clipped policy loss of sampled tokens with a KL term; -> (loss, logprobs, kl).
+
+    logits [B, T, V], labels int64 [B, T] (the tokens that were sampled), old_logprobs [B, T'] under the policy that sampled them,
+    advantages [B], [B, 1] or [B, T'], ref_logprobs [B, T'] under a reference model (T' = T - 1 with `shift`, else T).  With r =
+    exp(logprob - old) a token's loss is -min(r A, clamp(r, 1 - clip, 1 + clip_high) A) + kl_coef (exp(ref - logprob) - (ref -
+    logprob) - 1); clip_high defaults to clip.  reduction "tokens": the mean over all tokens that count; "sequences": the mean over
+    the sequences that have such tokens of their means; with none at all the loss is 0.  The gradient flows to the logits alone;
+    `logprobs` [B, T'] and `kl` (the KL term's mean) are for the log.  `ignore_index`, `shift` and `temperature` as for
+    `token_logprobs`; what the other operands hold at ignored tokens does not matter."""
+    who = "policy_loss"
+    x, y = _check_rows(who, logits, labels, ignore_index, temperature, shift)
+    if logits.dim() != 3:
+        raise RuntimeError("%s: logits are [sequences, tokens, classes] (got %s)" % (who, tuple(logits.shape)))
+    clip_high = clip if clip_high is None else clip_high
+    if not (0.0 <= clip < math.inf and 0.0 <= clip_high < math.inf) or not math.isfinite(kl_coef):
+        raise RuntimeError("%s: clip and clip_high must not be negative, and all coefficients finite" % who)
+    if reduction not in ("tokens", "sequences"):
+        raise RuntimeError("%s: reduction is 'tokens' or 'sequences' (got %r)" % (who, reduction))
+    if ref_logprobs is None and kl_coef != 0.0:
+        raise RuntimeError("%s: a KL term needs ref_logprobs" % who)
+    B, T = y.shape
+    R = max(0, T - int(shift))
+    old = _constant(who, "old_logprobs", old_logprobs, [(B, R)], logits).contiguous()
+    adv = _constant(who, "advantages", advantages, [(B,), (B, 1), (B, R)], logits)
+    ref = None if ref_logprobs is None else _constant(who, "ref_logprobs", ref_logprobs, [(B, R)], logits).contiguous()
+    a_strides = (adv.stride(0), adv.stride(1) if adv.dim() == 2 and adv.shape[1] > 1 else 0)
+    return _PolicyFn.apply(x, y, old, adv, a_strides, ref, (int(shift), ignore_index, float(temperature)), (float(clip), float(clip_high)),
+                           float(kl_coef), reduction == "sequences", torch.is_grad_enabled() and x.requires_grad)
+
+
 class LossWrapper(nn.Module):
     def forward(self, input, target, model=None):
         return _SumFn.apply(input)
@@ -151,3 +382,26 @@ class HFCrossEntropyLoss(LossWrapper):
 
     def forward(self, input, target, model=None):
         return cross_entropy(input.logits.view(-1, self.num_labels), target)
+
+
+class PreferenceLoss(LossWrapper):
+    """`preference_loss` of the logits (or of an output that has `.logits`); target: (labels, ref_logprobs)."""
+
+    def __init__(self, **kwargs):
+        super().__init__()
+        self.kwargs = kwargs
+
+    def forward(self, input, target, model=None):
+        labels, ref_logprobs = target
+        return preference_loss(getattr(input, "logits", input), labels, ref_logprobs, **self.kwargs)[0]
+
+
+class PolicyLoss(LossWrapper):
+    """`policy_loss` of the logits (or of an output that has `.logits`); target: (labels, old_logprobs, advantages[, ref_logprobs])."""
+
+    def __init__(self, **kwargs):
+        super().__init__()
+        self.kwargs = kwargs
+
+    def forward(self, input, target, model=None):
+        return policy_loss(getattr(input, "logits", input), *target, **self.kwargs)[0]

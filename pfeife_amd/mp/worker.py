@@ -21,6 +21,7 @@ import torch
 from ..executor.lowering import BufferPool, Lowerer, ParamStore, Unsupported
 from ..executor.merge import MicroBatchLayout
 from ..executor.values import Val
+from ..optim import AdamW8bit
 from ..option import get_optimizer_cls
 from ..schedule.scheduler import PipeSchedParams, SingleCommScheduler, StepWork, serialize_ranks
 from ..utils import fmem, get_logger
@@ -802,6 +803,8 @@ class StageWorker:
         adam = None
         if opt is not None and self._fused_adam_applicable(opt):
             adam = self._fused_adam_prepare(opt, self.dyn_scale)
+        elif type(opt) is AdamW8bit and hasattr(self.kernels, "adam8_step"):
+            adam = self._adam8_prepare(opt, self.dyn_scale)
         if settle is not None:
             settle()
         if self.dyn_scale:
@@ -890,6 +893,19 @@ class StageWorker:
                     else:
                         for st in state:
                             st["step"] += 1
+
+        return step
+
+    def _adam8_prepare(self, opt, scaled):
+        """The same for AdamW8bit, whose own step() cannot know of an overflow without a read from the device."""
+        work, fresh = opt._prepare(self.kernels)
+
+        def step():
+            if scaled and fresh:
+                self._seed_device_step_count(opt, [(g, None, states, None) for g, states, _, _ in work])
+            for g, states, _, table in work:
+                opt._launch(self.kernels, g, states, table, self.stream(), self.scaler_state if scaled else None)
+                self._host_steps_stale = scaled
 
         return step
 

@@ -16,6 +16,7 @@ import logging
 import torch
 import torch.optim as optim
 
+from .optim import AdamW8bit
 from .utils import set_logger_level
 
 default_optimizer = dict(type="adam", lr=1e-5)
@@ -23,6 +24,7 @@ default_optimizer = dict(type="adam", lr=1e-5)
 _OPTIMIZERS = {
     "adam": optim.Adam,
     "adamw": optim.AdamW,
+    "adamw8bit": AdamW8bit,
     "adagrad": optim.Adagrad,
     "adamax": optim.Adamax,
     "asgd": optim.ASGD,
