@@ -21,7 +21,8 @@ struct TokenRows {
   int64_t B, T, V;
   int64_t ignore_index;
   int shift;
-  float c, c_lo;          // log2(e) / temperature, and what its rounding lost
+  float c;                // log2(e) / temperature
+  double c_off;           // what its rounding added to it, relative
   double inv_temp;
 };
 struct GradRows {
@@ -35,75 +36,367 @@ __device__ __forceinline__ LabelKind label_kind(const TokenRows& r, int64_t y) {
   return y >= 0 && y < r.V ? LABEL_OK : LABEL_BAD;
 }
 
-struct RowStats { float m, z; };
+// ---- a row's sum of exponentials --------------------------------------------------------------------------------------------
+// A row is read once, 16 bytes to a lane and access at whatever alignment it has, NV accesses of a lane in flight; the row stays in the
+// registers that it was loaded to, so that a gradient of the same pass is formed from there.  Each lane sums 2^(x c - ref) against a
+// reference of its own, the whole number from its largest x c on: no exchange between lanes before the end, and one FMA and one exponential
+// to an element.  Sums of eight go into a double.  What such arithmetic cannot do (a row of nothing but the lowest values, where
+// x c overflows, infinities, NaN) shows as a sum that is not a positive number, and is done again as (x - m) c.
+typedef uint32_t raw4 __attribute__((ext_vector_type(4)));
+typedef uint32_t raw4_any __attribute__((ext_vector_type(4), aligned(2)));      // (the memory unit takes any alignment)
 
-// Maximum and sum of exponentials of one row by the whole workgroup (256 threads).
-template <int DT>
-__device__ RowStats row_stats(const TokenRows& r, const void* x, int64_t at, float* sm) {
-  float m = -INFINITY;
-  for (int64_t j = threadIdx.x; j < r.V; j += 256) m = fmaxf(m, Codec<DT>::load(x, at + j));
-  m = pf_block_max<4>(m, sm);
-  float z = 0.f;
-  for (int64_t j = threadIdx.x; j < r.V; j += 256) {
-    const float t = Codec<DT>::load(x, at + j) - m;
-    z += exp2f(fmaf(t, r.c, t == -INFINITY ? 0.f : t * r.c_lo));      // (a sum of many tokens' logprobs would show c's rounding)
-  }
-  return {m, pf_block_sum<4>(z, sm)};
-}
+template <int DT> constexpr int VE = DT == PF_F32 ? 4 : 8;       // elements of 16 bytes
 
 template <int DT>
-__device__ __forceinline__ double row_logprob(const TokenRows& r, int64_t at, int64_t y, const RowStats& s) {
-  return ((double)Codec<DT>::load(r.logits, at + y) - (double)s.m) * r.inv_temp - log((double)s.z);
-}
-
-// dx = g (onehot - p) / temperature over one row
-template <int DT>
-__device__ __forceinline__ void row_gradient(const TokenRows& r, int64_t at, int64_t y, float m, float inv_z, float g, void* dx, int64_t to) {
-  g *= (float)r.inv_temp;
-  for (int64_t j = threadIdx.x; j < r.V; j += 256) {
-    const float p = exp2f((Codec<DT>::load(r.logits, at + j) - m) * r.c) * inv_z;
-    Codec<DT>::store(dx, to + j, g * ((j == y ? 1.f : 0.f) - p));
-  }
-}
-template <int DT>
-__device__ __forceinline__ void row_zeros(const TokenRows& r, void* dx, int64_t to) {
-  for (int64_t j = threadIdx.x; j < r.V; j += 256) Codec<DT>::store(dx, to + j, 0.f);
-}
-
-// stats[row] = {maximum, 1 / sum}; for rows that take no part {0, 0}
-template <int DT, typename Out>
-__global__ __launch_bounds__(256) void token_logprob_kernel(const TokenRows r, Out* logprobs, float2* stats) {
-  __shared__ float sm[4];
-  const int64_t R = r.T - r.shift, rows = r.B * R;
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const int64_t b = row / R, t = row % R, at = b * r.sb + t * r.st;
-    const int64_t y = r.labels[b * r.T + t + r.shift];
-    const LabelKind kind = label_kind(r, y);
-    RowStats s = {0.f, 0.f};
-    if (kind == LABEL_OK) s = row_stats<DT>(r, r.logits, at, sm);
-    if (threadIdx.x == 0) {
-      logprobs[row] = kind == LABEL_OK ? (Out)row_logprob<DT>(r, at, y, s) : kind == LABEL_BAD ? (Out)NAN : (Out)0;
-      if (stats) stats[row] = kind == LABEL_OK ? make_float2(s.m, 1.f / s.z) : make_float2(0.f, kind == LABEL_BAD ? NAN : 0.f);
+__device__ __forceinline__ void unpack(const raw4& w, float (&x)[VE<DT>]) {
+  if constexpr (DT == PF_F32) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = __uint_as_float(w[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (DT == PF_BF16) {
+        x[2 * k] = __uint_as_float(w[k] << 16);
+        x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+      } else {
+        x[2 * k] = pf_f16_bits_to_f32((uint16_t)(w[k] & 0xffffu));
+        x[2 * k + 1] = pf_f16_bits_to_f32((uint16_t)(w[k] >> 16));
+      }
     }
+  }
+}
+template <int DT>
+__device__ __forceinline__ raw4 pack(const float (&x)[VE<DT>]) {
+  raw4 w;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (DT == PF_F32) w[k] = __float_as_uint(x[k]);
+    else if constexpr (DT == PF_BF16) w[k] = pf_pack2_bf16(x[2 * k], x[2 * k + 1]);
+    else w[k] = pf_pack2_f16(x[2 * k], x[2 * k + 1]);
+  }
+  return w;
+}
+constexpr float NOTHING = -1e30f;      // the reference of a lane that has seen nothing
+
+// the largest of three, NaN aside (one instruction: fmaxf would first quieten each operand)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+  return d;
+}
+// the largest of a vector's elements and `top`
+template <int DT>
+__device__ __forceinline__ float max_of(const raw4& w, float top) {
+  if constexpr (DT == PF_F32) {
+    return max3(max3(top, __uint_as_float(w[0]), __uint_as_float(w[1])), __uint_as_float(w[2]), __uint_as_float(w[3]));
+  } else if constexpr (DT == PF_BF16) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) top = max3(top, __uint_as_float(w[k] & 0xffff0000u), __uint_as_float(w[k] << 16));
+    return top;
+  } else {
+    uint32_t m, n;
+    asm("v_pk_max_f16 %0, %1, %2" : "=v"(m) : "v"(w[0]), "v"(w[1]));
+    asm("v_pk_max_f16 %0, %1, %2" : "=v"(n) : "v"(w[2]), "v"(w[3]));
+    asm("v_pk_max_f16 %0, %1, %2" : "=v"(m) : "v"(m), "v"(n));
+    return max3(top, pf_f16_bits_to_f32((uint16_t)(m & 0xffffu)), pf_f16_bits_to_f32((uint16_t)(m >> 16)));
+  }
+}
+
+// Sum of 2^(x c - ref), ref a whole number, so that sums of different references meet without a rounding.  With FIRST also that of
+// x 2^(x c - ref): what c's rounding does to the sum is some 1e-8 times the mean of x, of one sign in every row, and a sum over the tokens
+// of a sequence shows it.
+template <bool FIRST> struct Sums {
+  float ref = NOTHING;
+  double s = 0.0, s1 = 0.0;
+  __device__ __forceinline__ void raise(float top) {      // the reference to the whole number from top on, if that is more
+    top = ceilf(top);
+    const float to = max3(ref, top, top);
+    const int by = (int)(ref - to);
+    s = ldexp(s, by);
+    if (FIRST) s1 = ldexp(s1, by);
+    ref = to;
+  }
+  template <int N> __device__ __forceinline__ void add(const float (&x)[N], float c, bool valid) {
+    float e[N], f = 0.f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      e[k] = __builtin_amdgcn_exp2f(fmaf(x[k], c, -ref));
+      if (FIRST) f = fmaf(e[k], max3(x[k], NOTHING, NOTHING), f);      // (0 of -inf)
+    }
+#pragma unroll
+    for (int d = N / 2; d > 0; d >>= 1)
+#pragma unroll
+      for (int k = 0; k < d; ++k) e[k] += e[k + d];
+    s += (double)(valid ? e[0] : 0.f);
+    if (FIRST) s1 += (double)(valid ? f : 0.f);
+  }
+  __device__ __forceinline__ void join(float other, double os, double os1) {
+    const float to = max3(ref, other, other);
+    const int a = (int)(ref - to), b = (int)(other - to);
+    s = ldexp(s, a) + ldexp(os, b);
+    if (FIRST) s1 = ldexp(s1, a) + ldexp(os1, b);
+    ref = to;
+  }
+  __device__ __forceinline__ void join_lanes(int width) {
+    for (int o = width / 2; o > 0; o >>= 1) {
+      const float other = __shfl_xor(ref, o, 64);
+      const double os = __shfl_xor(s, o, 64), os1 = FIRST ? __shfl_xor(s1, o, 64) : 0.0;
+      join(other, os, os1);
+    }
+  }
+};
+
+// The whole row's: by one wavefront, or by the workgroup (`sm`: a slot to each wavefront).
+template <bool FIRST> struct SumSlots { float ref[16]; double s[16], s1[16]; };
+template <bool ONE, bool FIRST>
+__device__ __forceinline__ void join_row(Sums<FIRST>& a, SumSlots<FIRST>* sm) {
+  a.join_lanes(64);
+  if constexpr (!ONE) {
+    const int waves = blockDim.x >> 6, lane = threadIdx.x & 63;
+    if (waves == 1) return;
+    __syncthreads();
+    if (lane == 0) {
+      sm->ref[threadIdx.x >> 6] = a.ref;
+      sm->s[threadIdx.x >> 6] = a.s;
+      if (FIRST) sm->s1[threadIdx.x >> 6] = a.s1;
+    }
+    __syncthreads();
+    const int at = lane & 15;            // (lanes 16 apart hold the same)
+    const bool in = at < waves;
+    a.ref = in ? sm->ref[at] : NOTHING;
+    a.s = in ? sm->s[at] : 0.0;
+    if (FIRST) a.s1 = in ? sm->s1[at] : 0.0;
+    a.join_lanes(16);
+  }
+}
+
+// What follows from a row's sums.  slow: p = 2^((x - ref) c) inv, else 2^(x c - ref) inv
+struct RowStats { float ref, inv; bool slow; double logprob; };
+__device__ __forceinline__ float2 pack_stats(const RowStats& s) { return make_float2(s.ref, s.slow ? -s.inv : s.inv); }
+
+// The row by (x - m) c, an element at a time; -> its sum
+template <int DT, bool ONE>
+__device__ double slow_sums(const char* x, int V, float c, float* m_out, double* shared) {
+  const int tid = ONE ? (threadIdx.x & 63) : threadIdx.x, n = ONE ? 64 : blockDim.x, waves = ONE ? 1 : blockDim.x >> 6;
+  float m = -INFINITY;
+  for (int j = tid; j < V; j += n) m = fmaxf(m, Codec<DT>::load(x, j));
+  m = pf_wave_max(m);
+  if (waves > 1) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = (double)m;
+    __syncthreads();
+    for (int w = 0; w < waves; ++w) m = fmaxf(m, (float)shared[w]);
+  }
+  double z = 0.0;
+  for (int j = tid; j < V; j += n) z += (double)exp2f((Codec<DT>::load(x, j) - m) * c);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) z += __shfl_xor(z, o, 64);
+  if (waves > 1) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = z;
+    __syncthreads();
+    z = 0.0;
+    for (int w = 0; w < waves; ++w) z += shared[w];
+  }
+  *m_out = m;
+  return z;
+}
+
+template <int DT> constexpr int pf_es = DT == PF_F32 ? 4 : 2;
+
+// LOOP: the row takes several tiles of NV vectors to a lane; else one (rows of no vector at all have none).
+template <int DT, int NV, bool ONE, bool LOOP> struct RowReader {
+  const char* x;       // the row
+  int V, full, tail;   // elements, whole vectors, elements behind them
+  int tid, n;          // this lane among those of the row
+  raw4 v[NV];
+  float last;          // the element behind the vectors that this lane has (tid < tail)
+
+  __device__ __forceinline__ RowReader(const void* row, int64_t at, int64_t classes)
+      : x((const char*)row + at * pf_es<DT>), V((int)classes), full((int)classes / VE<DT>), tail((int)classes % VE<DT>), tid(ONE ? (threadIdx.x & 63) : threadIdx.x),
+        n(ONE ? 64 : blockDim.x) {}
+
+  __device__ __forceinline__ int tiles() const { return full == 0 ? 0 : LOOP ? (full + n * NV - 1) / (n * NV) : 1; }
+  __device__ __forceinline__ void load_tail() {
+    last = -INFINITY;
+    if (tid < tail) last = Codec<DT>::load(x, full * VE<DT> + tid);
+  }
+  // lanes that have an i-th vector of a tile: those below this (uniform)
+  __device__ __forceinline__ int left(int tile, int i) const { return full - (tile * NV + i) * n; }
+  __device__ __forceinline__ void load(int tile) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      int k = (tile * NV + i) * n + tid;
+      if (k > full - 1) k = full - 1;
+      v[i] = *(const raw4_any*)(x + (uint32_t)k * 16u);
+    }
+  }
+  template <bool FIRST> __device__ __forceinline__ void sum(int tile, float c, Sums<FIRST>& a) {
+    float top = NOTHING;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) top = max_of<DT>(v[i], top);
+    a.raise(top * c);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      asm("" : "+v"(v[i]));      // (what the maximum unpacked is not worth keeping)
+      float e[VE<DT>];
+      unpack<DT>(v[i], e);
+      a.add(e, c, tid < left(tile, i));      // (lanes past the end hold the last vector again)
+    }
+  }
+  template <bool FIRST> __device__ __forceinline__ void sum_tail(float c, Sums<FIRST>& a) {
+    if (tail == 0) return;
+    float e[1] = {last};
+    a.raise(last * c);
+    a.add(e, c, tid < tail);
+  }
+};
+
+template <int DT> __device__ __forceinline__ float element(const char* x, int j) { return Codec<DT>::load(x, j); }
+
+// Statistics of a row whose label counts; the logprob where `lane_wants` (all lanes for the policy, one otherwise).
+template <bool FIRST, int DT, int NV, bool ONE, bool LOOP>
+__device__ __forceinline__ RowStats row_stats(const TokenRows& r, RowReader<DT, NV, ONE, LOOP>& row, float xy, SumSlots<FIRST>* sm, bool lane_wants) {
+  Sums<FIRST> a;
+  row.load_tail();
+  const int tiles = row.tiles();
+  for (int tile = 0; tile < tiles; ++tile) {
+    row.load(tile);
+    row.sum(tile, r.c, a);
+  }
+  row.sum_tail(r.c, a);
+  join_row<ONE, FIRST>(a, sm);
+  RowStats o = {a.ref, 0.f, !(a.s > 0.0 && a.s < INFINITY), 0.0};
+  if (o.slow) {
+    a.s = slow_sums<DT, ONE>(row.x, row.V, r.c, &o.ref, sm ? sm->s : nullptr);
+    o.logprob = ((double)xy - (double)o.ref) * r.inv_temp - log(a.s);
+  } else if (lane_wants) {
+    if (FIRST)   // ln sum exp(x / temperature) = ln sum 2^(x c) - c's relative error times the mean of x / temperature
+      o.logprob = (double)xy * r.inv_temp - ((double)a.ref * 0.693147180559945309 + log(a.s) - r.c_off * r.inv_temp * (a.s1 / a.s));
+    else
+      o.logprob = ((double)xy * (double)r.c - (double)a.ref) * 0.693147180559945309 - log(a.s);
+  }
+  o.inv = (float)(1.0 / a.s);
+  return o;
+}
+
+template <int DT> __device__ __forceinline__ void store_vector(char* dx, int k, const raw4& w) { *(raw4_any*)(dx + (uint32_t)k * 16u) = w; }
+
+// What a lane needs for dx = g (onehot - p) / temperature = scaled 2^(..), scaled = -g inv / temperature; and the whole of it at the label
+struct RowGrad { float scaled, at_label; };
+template <bool SLOW> __device__ __forceinline__ float power(float x, const RowStats& s, float c) {
+  return __builtin_amdgcn_exp2f(SLOW ? (x - s.ref) * c : fmaf(x, c, -s.ref));
+}
+__device__ __forceinline__ RowGrad row_grad(const TokenRows& r, const RowStats& s, float g, float xy) {
+  g *= (float)r.inv_temp;
+  const float scaled = -g * s.inv;
+  return {scaled, fmaf(scaled, s.slow ? power<true>(xy, s, r.c) : power<false>(xy, s, r.c), g)};
+}
+// of the vector at dx; label: whose element in it, else negative or VE and more
+template <int DT, bool SLOW>
+__device__ __forceinline__ void gradient_vector(raw4 w, int label, const RowStats& s, const RowGrad& g, float c, char* dx) {
+  asm volatile("" : "+v"(w));      // (unpacked here and not before: a tile's elements would not fit the registers)
+  float x[VE<DT>];
+  unpack<DT>(w, x);
+#pragma unroll
+  for (int e = 0; e < VE<DT>; ++e) x[e] = g.scaled * power<SLOW>(x[e], s, c);
+  *(raw4_any*)dx = pack<DT>(x);
+  if ((unsigned)label < (unsigned)VE<DT>) Codec<DT>::store(dx, label, g.at_label);      // (the same lane, behind its vector)
+}
+template <int DT>
+__device__ __forceinline__ void gradient_element(float x, int j, int y, const RowStats& s, const RowGrad& g, float c, char* dx) {
+  Codec<DT>::store(dx, j, j == y ? g.at_label : g.scaled * (s.slow ? power<true>(x, s, c) : power<false>(x, s, c)));
+}
+
+template <int DT>
+__device__ __forceinline__ void fill_row(char* dx, int V, float value, int tid, int n) {
+  float x[VE<DT>];
+#pragma unroll
+  for (int e = 0; e < VE<DT>; ++e) x[e] = value;
+  const raw4 w = pack<DT>(x);
+  const int full = V / VE<DT>;
+  for (int k = tid; k < full; k += n) store_vector<DT>(dx, k, w);
+  if (tid < V % VE<DT>) Codec<DT>::store(dx, (int64_t)full * VE<DT> + tid, value);
+}
+
+// The row of a workgroup or, with ONE, of a wavefront (four to a workgroup): sequence b, place t (uniform)
+template <bool ONE> __device__ __forceinline__ int row_of_group() {
+  return ONE ? (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : (int)blockIdx.x;
+}
+
+// stats[row] = {reference, 1 / sum}; for rows that take no part {0, 0}
+template <int DT, int NV, bool ONE, bool LOOP, typename Out>
+__global__ __launch_bounds__(ONE ? 256 : 1024) void token_logprob_kernel(const TokenRows r, int b0, Out* logprobs, float2* stats) {
+  constexpr bool FIRST = sizeof(Out) == 8;
+  __shared__ SumSlots<FIRST> slots[1];
+  const int R = (int)r.T - r.shift, t = row_of_group<ONE>();
+  const int64_t b = b0 + (int)blockIdx.y;
+  if (t >= R) return;
+  const int64_t y = r.labels[b * r.T + t + r.shift], at = b * R + t;
+  const LabelKind kind = label_kind(r, y);
+  RowStats s = {0.f, kind == LABEL_BAD ? NAN : 0.f, false, kind == LABEL_BAD ? (double)NAN : 0.0};
+  const int tid = ONE ? threadIdx.x & 63 : threadIdx.x;
+  if (kind == LABEL_OK) {
+    RowReader<DT, NV, ONE, LOOP> row(r.logits, b * r.sb + t * r.st, r.V);
+    s = row_stats<FIRST>(r, row, element<DT>(row.x, (int)y), slots, tid == 0);
+  }
+  if (tid == 0) {
+    logprobs[at] = (Out)s.logprob;
+    if (stats) stats[at] = pack_stats(s);
   }
 }
 
 // dlogits from the rows' statistics and g = coef[b * g_sb + t * g_st] (* scale[0]).  unless_one: nothing is done where scale[0] is one.
+// A wavefront to 64 * GNV vectors of a row, without a word to others.  Rows are taken from the last one back: what the forward pass read
+// last is what the caches may still hold.
+constexpr int GNV = 4;
 template <int DT>
 __global__ __launch_bounds__(256) void token_gradient_kernel(const TokenRows r, const GradRows d, const float2* stats, const float* coef,
-                                                             int64_t g_sb, int64_t g_st, const float* scale, int unless_one) {
+                                                             int64_t g_sb, int64_t g_st, const float* scale, int unless_one, unsigned pieces) {
   const float by = scale ? scale[0] : 1.f;
   if (unless_one && by == 1.f) return;
-  const int64_t R = r.T - r.shift, rows = r.B * r.T;
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const int64_t b = row / r.T, t = row % r.T, at = b * r.sb + t * r.st, to = b * d.sb + t * d.st;
-    const int64_t y = t < R ? r.labels[row + r.shift] : 0;
-    const LabelKind kind = t < R ? label_kind(r, y) : LABEL_SKIP;
-    if (kind == LABEL_SKIP) {
-      row_zeros<DT>(r, d.dx, to);
-    } else {
-      const float2 s = stats[b * R + t];
-      row_gradient<DT>(r, at, y, s.x, s.y, coef[b * g_sb + t * g_st] * by, d.dx, to);
+  const int64_t R = r.T - r.shift, units = r.T * pieces;
+  const int lane = threadIdx.x & 63, V = (int)r.V, full = V / VE<DT>, tail = V % VE<DT>;
+  for (int64_t b = r.B - 1 - (int64_t)blockIdx.y; b >= 0; b -= gridDim.y) {
+    for (int64_t u = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); u < units; u += (int64_t)gridDim.x * 4) {
+      const int64_t t = r.T - 1 - u / pieces;
+      const int piece = (int)(u % pieces), k0 = piece * 64 * GNV + lane;
+      char* dx = (char*)d.dx + (b * d.sb + t * d.st) * pf_es<DT>;
+      const int64_t y = t < R ? r.labels[b * r.T + t + r.shift] : 0;
+      const LabelKind kind = t < R ? label_kind(r, y) : LABEL_SKIP;
+      if (kind == LABEL_SKIP) {
+#pragma unroll
+        for (int i = 0; i < GNV; ++i)
+          if (k0 + i * 64 < full) store_vector<DT>(dx, k0 + i * 64, raw4{0, 0, 0, 0});
+        if (piece == (int)pieces - 1 && lane < tail) Codec<DT>::store(dx, (int64_t)full * VE<DT> + lane, 0.f);
+        continue;
+      }
+      const int yi = kind == LABEL_OK ? (int)y : -1;      // (no vector's and no element's)
+      const char* x = (const char*)r.logits + (b * r.sb + t * r.st) * pf_es<DT>;
+      raw4 v[GNV];
+      if (full > 0) {
+#pragma unroll
+        for (int i = 0; i < GNV; ++i) {
+          const int k = k0 + i * 64;
+          v[i] = *(const raw4_any*)(x + (uint32_t)(k < full ? k : full - 1) * 16u);
+        }
+      }
+      const float2 packed = stats[b * R + t];
+      const RowStats s = {packed.x, fabsf(packed.y), packed.y < 0.f, 0.0};
+      const RowGrad g = row_grad(r, s, coef[b * g_sb + t * g_st] * by, kind == LABEL_OK ? element<DT>(x, yi) : NAN);
+      if (s.slow) {
+#pragma unroll
+        for (int i = 0; i < GNV; ++i)
+          if (k0 + i * 64 < full) gradient_vector<DT, true>(v[i], yi - (k0 + i * 64) * VE<DT>, s, g, r.c, dx + (uint32_t)(k0 + i * 64) * 16u);
+      } else {
+#pragma unroll
+        for (int i = 0; i < GNV; ++i)
+          if (k0 + i * 64 < full) gradient_vector<DT, false>(v[i], yi - (k0 + i * 64) * VE<DT>, s, g, r.c, dx + (uint32_t)(k0 + i * 64) * 16u);
+      }
+      if (piece == (int)pieces - 1 && lane < tail) {
+        const int j = full * VE<DT> + lane;
+        gradient_element<DT>(element<DT>(x, j), j, yi, s, g, r.c, dx);
+      }
     }
   }
 }
@@ -113,46 +406,42 @@ __device__ __forceinline__ double wave_sum(double v) {
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
 }
-template <int NW>
-__device__ __forceinline__ double block_sum(double v, double* sm) {
-  v = wave_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = v;
-  __syncthreads();
-  double s = 0.0;
-#pragma unroll
-  for (int i = 0; i < NW; ++i) s += sm[i];
-  return s;
-}
 
 // ---- preference ------------------------------------------------------------------------------------------------------------
-// A workgroup to a pair (sequences 2i, 2i + 1):  reward = beta (sum or mean of logprobs - ref),  D = reward_2i - reward_2i+1,
+// A workgroup to a pair, half of it to a sequence (2i, 2i + 1):  reward = beta (sum or mean of logprobs - ref),  D = reward_2i - reward_2i+1,
 //   loss_i = -(1 - e) ln sigma(D) - e ln sigma(-D),   d loss_i / dD = sigma(D) - (1 - e).
 __device__ __forceinline__ double softplus(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }   // -ln sigma(-x)
 
-__global__ __launch_bounds__(256) void preference_pair_kernel(const double* logprobs, const int64_t* labels, int64_t T, int shift, int64_t ignore_index,
+__global__ __launch_bounds__(512) void preference_pair_kernel(const double* logprobs, const int64_t* labels, int64_t T, int shift, int64_t ignore_index,
                                                               const float* ref, double beta, double smoothing, int average, int64_t pairs,
                                                               float* rewards, float* coef, double* pair_loss) {
-  __shared__ double sm[4];
+  __shared__ double sums[8], counts[8];
   const int64_t R = T - shift;
+  const int half = threadIdx.x >> 8;
   for (int64_t i = blockIdx.x; i < pairs; i += gridDim.x) {
-    double reward[2], per_token[2];
-    for (int k = 0; k < 2; ++k) {
-      const int64_t b = 2 * i + k;
-      double s = 0.0, n = 0.0;
-      for (int64_t t = threadIdx.x; t < R; t += 256) {
-        s += logprobs[b * R + t];
-        if (average) n += labels[b * T + t + shift] != ignore_index ? 1.0 : 0.0;
-      }
-      s = block_sum<4>(s, sm);
-      per_token[k] = 1.0;
-      if (average) {
-        n = block_sum<4>(n, sm);
-        per_token[k] = n > 0.0 ? 1.0 / n : 0.0;
-      }
-      reward[k] = beta * (s * per_token[k] - (double)ref[b]);
+    const int64_t b = 2 * i + half;
+    double s = 0.0, n = 0.0;
+#pragma unroll 8
+    for (int64_t t = threadIdx.x & 255; t < R; t += 256) s += logprobs[b * R + t];
+    if (average)
+#pragma unroll 8
+      for (int64_t t = threadIdx.x & 255; t < R; t += 256) n += labels[b * T + t + shift] != ignore_index ? 1.0 : 0.0;
+    s = wave_sum(s);
+    n = wave_sum(n);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+      sums[threadIdx.x >> 6] = s;
+      counts[threadIdx.x >> 6] = n;
     }
+    __syncthreads();
     if (threadIdx.x == 0) {
+      double reward[2], per_token[2];
+      for (int k = 0; k < 2; ++k) {
+        const double total = sums[4 * k] + sums[4 * k + 1] + sums[4 * k + 2] + sums[4 * k + 3];
+        const double count = counts[4 * k] + counts[4 * k + 1] + counts[4 * k + 2] + counts[4 * k + 3];
+        per_token[k] = !average ? 1.0 : count > 0.0 ? 1.0 / count : 0.0;
+        reward[k] = beta * (total * per_token[k] - (double)ref[2 * i + k]);
+      }
       const double D = reward[0] - reward[1];
       const double up = 1.0 / (1.0 + exp(-D)) - (1.0 - smoothing);
       pair_loss[i] = (1.0 - smoothing) * softplus(-D) + smoothing * softplus(D);
@@ -164,32 +453,48 @@ __global__ __launch_bounds__(256) void preference_pair_kernel(const double* logp
   }
 }
 
-// out[k] = sum over n of in[k * n + i] (* scale), in double
-__global__ __launch_bounds__(256) void sums_kernel(const double* in, int64_t n, double scale, float* out0, float* out1) {
-  __shared__ double sm[4];
-  for (int k = 0; k < (out1 ? 2 : 1); ++k) {
+// out_k = scale * sum over n of in[k * n + i], in double
+__global__ __launch_bounds__(1024) void sums_kernel(const double* in, int64_t n, double scale, float* out0, float* out1) {
+  __shared__ double sm[2][16];
+  double a = 0.0, c = 0.0;
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < n; i += 1024) {
+    a += in[i];
+    if (out1) c += in[n + i];
+  }
+  a = wave_sum(a);
+  c = wave_sum(c);
+  if ((threadIdx.x & 63) == 0) {
+    sm[0][threadIdx.x >> 6] = a;
+    sm[1][threadIdx.x >> 6] = c;
+  }
+  __syncthreads();
+  if (threadIdx.x < 2 && (threadIdx.x == 0 || out1)) {
     double s = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += 256) s += in[k * n + i];
-    s = block_sum<4>(s, sm);
-    if (threadIdx.x == 0) (k ? out1 : out0)[0] = (float)(s * scale);
+    for (int i = 0; i < 16; ++i) s += sm[threadIdx.x][i];
+    (threadIdx.x ? out1 : out0)[0] = (float)(s * scale);
   }
 }
 
 // ---- policy ----------------------------------------------------------------------------------------------------------------
 // weight of every token of sequence b: 1 / (tokens that count), or by_sequence 1 / (its own such tokens * sequences that have any)
-__global__ __launch_bounds__(256) void token_weights_kernel(const TokenRows r, int by_sequence, double* weights) {
-  __shared__ double sm[4];
+__global__ __launch_bounds__(1024) void token_weights_kernel(const TokenRows r, int by_sequence, double* weights) {
+  __shared__ double sm[16];
   const int64_t R = r.T - r.shift;
   double total = 0.0;
-  for (int64_t b = 0; b < r.B; ++b) {
+  for (int64_t b = threadIdx.x >> 6; b < r.B; b += 16) {      // a wavefront to a sequence
     double n = 0.0;
-    for (int64_t t = threadIdx.x; t < R; t += 256) n += r.labels[b * r.T + t + r.shift] != r.ignore_index ? 1.0 : 0.0;
-    n = block_sum<4>(n, sm);
-    if (threadIdx.x == 0) weights[b] = n;
+#pragma unroll 8
+    for (int64_t t = threadIdx.x & 63; t < R; t += 64) n += r.labels[b * r.T + t + r.shift] != r.ignore_index ? 1.0 : 0.0;
+    n = wave_sum(n);
+    if ((threadIdx.x & 63) == 0) weights[b] = n;
     total += by_sequence ? (n > 0.0 ? 1.0 : 0.0) : n;
   }
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = total;
   __syncthreads();
-  for (int64_t b = threadIdx.x; b < r.B; b += 256) {
+  total = 0.0;
+  for (int i = 0; i < 16; ++i) total += sm[i];
+  for (int64_t b = threadIdx.x; b < r.B; b += 1024) {
     const double n = weights[b];
     weights[b] = n > 0.0 ? 1.0 / (by_sequence ? n * total : total) : 0.0;
   }
@@ -200,71 +505,132 @@ struct PolicyArgs {
   const float* ref;      // [B, R] or null
   const float* adv;
   int64_t a_sb, a_st;
-  double low, high, kl_coef;
+  double low, high;      // ln(1 - clip_low), ln(1 + clip_high)
+  float low_ratio, high_ratio, kl_coef;
 };
 
-// One token:  -min(r A, clip(r) A) + kl_coef (e^q - q - 1)  with r = e^(logprob - old), q = ref - logprob; g is its derivative by
-// the logprob (at the clip's borders that of r A).
-struct TokenTerms { double loss, kl, g; };
-__device__ __forceinline__ TokenTerms policy_token(const PolicyArgs& a, int64_t row, int64_t b, int64_t t, double logprob) {
-  const double ratio = exp(logprob - (double)a.old[row]);
-  const double A = (double)a.adv[b * a.a_sb + t * a.a_st];
-  const double clipped = ratio < a.low ? a.low : ratio > a.high ? a.high : ratio;
-  const bool outside = A >= 0.0 ? ratio > a.high : ratio < a.low;
+// One token:  -min(r A, clip(r) A) + kl_coef (e^q - q - 1)  with r = e^d, d = logprob - old, q = ref - logprob; g is its derivative by the
+// logprob (at the clip's borders that of r A).  The differences and the comparison are in double; e^q - 1 - q is summed up as
+// the series it is where the subtraction would lose its digits.
+struct TokenTerms { float loss, kl, g; };
+__device__ __forceinline__ TokenTerms policy_token(const PolicyArgs& a, float old, float A, float ref, double logprob) {
+  const double d = logprob - (double)old;
+  const float ratio = expf((float)d);
+  const bool outside = A >= 0.f ? d > a.high : d < a.low;
   TokenTerms o;
-  o.loss = -(outside ? clipped : ratio) * A;
-  o.g = outside ? 0.0 : -ratio * A;
-  o.kl = 0.0;
+  o.loss = -(outside ? (A >= 0.f ? a.high_ratio : a.low_ratio) : ratio) * A;
+  o.g = outside ? 0.f : -ratio * A;
+  o.kl = 0.f;
   if (a.ref) {
-    const double q = (double)a.ref[row] - logprob, e = expm1(q);
-    o.kl = e - q;
-    o.loss += a.kl_coef * o.kl;
-    o.g -= a.kl_coef * e;
+    const double dq = (double)ref - logprob;
+    const float q = (float)dq;
+    float e, k;
+    if (fabsf(q) < 0.5f) {      // q^2 / 2! + q^3 / 3! + ...: eight terms leave 2^-26 of it
+      float h = fmaf(q, 1.f / 9.f, 1.f);
+      h = fmaf(h * q, 1.f / 8.f, 1.f);
+      h = fmaf(h * q, 1.f / 7.f, 1.f);
+      h = fmaf(h * q, 1.f / 6.f, 1.f);
+      h = fmaf(h * q, 1.f / 5.f, 1.f);
+      h = fmaf(h * q, 1.f / 4.f, 1.f);
+      h = fmaf(h * q, 1.f / 3.f, 1.f);
+      k = 0.5f * q * q * h;
+      e = q + k;
+    } else {
+      e = expf(q) - 1.f;
+      k = e - q;
+    }
+    o.kl = k;
+    o.loss = fmaf(a.kl_coef, k, o.loss);
+    o.g = fmaf(-a.kl_coef, e, o.g);
   }
   return o;
 }
 
 // A row's log-probability, its part of the loss and, where wanted, its gradient.  terms: [2][B * R], weighted
-template <int DT>
-__global__ __launch_bounds__(256) void policy_kernel(const TokenRows r, const GradRows d, const PolicyArgs a, const double* weights, float* logprobs,
-                                                     float2* stats, float* coef, double* terms) {
-  __shared__ float sm[4];
-  __shared__ float shared_g;
-  const int64_t R = r.T - r.shift, all = r.B * R, rows = r.B * r.T;
-  for (int64_t place = blockIdx.x; place < rows; place += gridDim.x) {
-    const int64_t b = place / r.T, t = place % r.T, at = b * r.sb + t * r.st, to = b * d.sb + t * d.st, row = b * R + t;
-    const int64_t y = t < R ? r.labels[place + r.shift] : 0;
-    const LabelKind kind = t < R ? label_kind(r, y) : LABEL_SKIP;
-    RowStats s = {0.f, 0.f};
-    if (kind == LABEL_OK) s = row_stats<DT>(r, r.logits, at, sm);
-    if (threadIdx.x == 0 && t < R) {
-      TokenTerms o = {0.0, 0.0, 0.0};
-      double lp = 0.0;
-      if (kind != LABEL_SKIP) {
-        lp = kind == LABEL_OK ? row_logprob<DT>(r, at, y, s) : (double)NAN;
-        o = policy_token(a, row, b, t, lp);
-      }
-      const double w = weights[b];
-      logprobs[row] = (float)lp;
-      terms[row] = kind == LABEL_SKIP ? 0.0 : w * o.loss;
-      terms[all + row] = kind == LABEL_SKIP ? 0.0 : w * o.kl;
-      const float g = kind == LABEL_SKIP ? 0.f : (float)(w * o.g);
-      shared_g = g;
+template <int DT, int NV, bool ONE, bool LOOP>
+__global__ __launch_bounds__(ONE ? 256 : 1024) void policy_kernel(const TokenRows r, int b0, const GradRows d, const PolicyArgs a, const double* weights,
+                                                                  float* logprobs, float2* stats, float* coef, double* terms) {
+  __shared__ SumSlots<false> slots[1];
+  const int T = (int)r.T, R = T - r.shift, t = row_of_group<ONE>();
+  const int64_t b = b0 + (int)blockIdx.y, at = b * R + t;
+  if (t >= T) return;
+  const int tid = ONE ? threadIdx.x & 63 : threadIdx.x, n = ONE ? 64 : blockDim.x;
+  const int64_t y = t < R ? r.labels[b * T + t + r.shift] : 0;
+  const LabelKind kind = t < R ? label_kind(r, y) : LABEL_SKIP;
+  char* dx = (char*)d.dx + (b * d.sb + t * d.st) * pf_es<DT>;
+  if (kind != LABEL_OK) {
+    const float none = kind == LABEL_BAD ? NAN : 0.f;
+    if (tid == 0 && t < R) {
+      logprobs[at] = none;
+      terms[at] = terms[r.B * R + at] = none;
       if (coef) {
-        coef[row] = g;
-        stats[row] = kind == LABEL_OK ? make_float2(s.m, 1.f / s.z) : make_float2(0.f, kind == LABEL_BAD ? NAN : 0.f);
+        coef[at] = none;
+        stats[at] = make_float2(0.f, none);
       }
     }
-    if (!d.dx) continue;
-    __syncthreads();
-    if (kind == LABEL_SKIP) row_zeros<DT>(r, d.dx, to);
-    else row_gradient<DT>(r, at, y, s.m, kind == LABEL_OK ? 1.f / s.z : NAN, shared_g, d.dx, to);
-    __syncthreads();
+    if (d.dx) fill_row<DT>(dx, (int)r.V, none, tid, n);
+    return;
+  }
+  const float old = a.old[at], A = a.adv[b * a.a_sb + t * a.a_st], ref = a.ref ? a.ref[at] : 0.f;
+  const double w = weights[b];
+  RowReader<DT, NV, ONE, LOOP> row(r.logits, b * r.sb + t * r.st, r.V);
+  const float xy = element<DT>(row.x, (int)y);
+  const RowStats s = row_stats<false>(r, row, xy, slots, true);
+  const TokenTerms o = policy_token(a, old, A, ref, s.logprob);
+  const float g = (float)(w * (double)o.g);
+  if (tid == 0) {
+    logprobs[at] = (float)s.logprob;
+    terms[at] = w * (double)o.loss;
+    terms[r.B * R + at] = w * (double)o.kl;
+    if (coef) {
+      coef[at] = g;
+      stats[at] = pack_stats(s);
+    }
+  }
+  if (!d.dx) return;
+  const RowGrad rg = row_grad(r, s, g, xy);
+  const int tiles = row.tiles(), mine = (int)y - tid * VE<DT>;
+  for (int tile = tiles - 1; tile >= 0; --tile) {
+    if (LOOP && tile != tiles - 1) row.load(tile);      // (the last one is still there)
+    char* to = dx + (size_t)((unsigned)(tile * NV * n) * 16u);
+    if (s.slow) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (tid < row.left(tile, i))
+          gradient_vector<DT, true>(row.v[i], mine - (tile * NV + i) * n * VE<DT>, s, rg, r.c, to + (unsigned)(i * n) * 16u + (unsigned)tid * 16u);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (tid < row.left(tile, i))
+          gradient_vector<DT, false>(row.v[i], mine - (tile * NV + i) * n * VE<DT>, s, rg, r.c, to + (unsigned)(i * n) * 16u + (unsigned)tid * 16u);
+    }
+  }
+  if (tid < row.tail) {
+    const int j = row.full * VE<DT> + tid;
+    gradient_element<DT>(row.last, j, (int)y, s, rg, r.c, dx);
   }
 }
 
-constexpr int64_t MAX_BLOCKS = 1 << 20;
-inline dim3 rows_grid(int64_t rows) { return dim3((unsigned)(rows < MAX_BLOCKS ? rows : MAX_BLOCKS)); }
+// ---- launches --------------------------------------------------------------------------------------------------------------
+// How a row is dealt out.  NV accesses of a lane in flight, WAVES wavefronts to a row; ONE: a wavefront alone, four rows to a workgroup; LOOP: in
+// several tiles.
+struct RowPlan { int nv, waves; bool one, loop; };
+RowPlan row_plan(int dtype, int64_t V) {
+  const int64_t full = V / (dtype == PF_F32 ? 4 : 8);
+  if (full <= 64 * 4) return {4, 1, true, false};
+  const int nv = full <= 64 * 4 * 4 ? 4 : full <= 64 * 16 * 16 ? 16 : 8;
+  const int64_t waves = (full + 64 * nv - 1) / (64 * nv);
+  return {nv, (int)(waves < 16 ? waves : 16), false, waves > 16};
+}
+// rows along x, sequences along y; a launch has less than 2^32 threads, and kernels loop over what is beyond
+dim3 rows_grid(int64_t units, int64_t B, int per_group, int threads, int64_t most = 1ll << 40) {
+  const int64_t y = B < 65535 ? B : 65535;
+  int64_t x = (units + per_group - 1) / per_group, limit = ((1ll << 32) - 1) / threads / y;
+  if (limit > most / y) limit = most / y;
+  if (limit < 1) limit = 1;
+  if (x > limit) x = limit;
+  return dim3((unsigned)(x < 1 ? 1 : x), (unsigned)y);
+}
 
 int check_rows(const char* who, const void* logits, int dtype, int64_t B, int64_t T, int64_t V, int64_t sb, int64_t st, const int64_t* labels, int shift,
                double temperature) {
@@ -273,14 +639,15 @@ int check_rows(const char* who, const void* logits, int dtype, int64_t B, int64_
   PF_REQUIRE(shift == 0 || shift == 1, "%s: shift is 0 or 1", who);
   PF_REQUIRE(temperature > 0.0 && temperature >= 1e-6 && temperature <= 1e6, "%s: temperature must lie in [1e-6, 1e6]", who);
   PF_REQUIRE(B * T == 0 || (logits && labels), "%s: null pointer", who);
-  PF_REQUIRE(T < (1ll << 31) && B < (1ll << 31) && B * T < (1ll << 40), "%s: too many rows", who);
+  PF_REQUIRE(T <= (1ll << 21) && B < (1ll << 31), "%s: too many rows", who);
+  PF_REQUIRE(V <= (1ll << 28), "%s: too many classes", who);
   return PF_OK;
 }
 
 TokenRows token_rows(const void* logits, int64_t B, int64_t T, int64_t V, int64_t sb, int64_t st, const int64_t* labels, int shift,
                      int64_t ignore_index, double temperature) {
   const double c = 1.4426950408889634 / temperature;
-  return {logits, sb, st, labels, B, T, V, ignore_index, shift, (float)c, (float)(c - (double)(float)c), 1.0 / temperature};
+  return {logits, sb, st, labels, B, T, V, ignore_index, shift, (float)c, (double)(float)c / c - 1.0, 1.0 / temperature};
 }
 
 }  // namespace
@@ -291,6 +658,22 @@ TokenRows token_rows(const void* logits, int64_t B, int64_t T, int64_t V, int64_
     else if (dt == PF_F16) { CALL(PF_F16); } \
     else { CALL(PF_BF16); }                  \
   } while (0)
+// CALL(dtype, NV, ONE) with grid, block and b0 for rows of V classes: a launch has less than 2^32 threads, so many sequences go in several
+#define PF_BY_ROW(dt, V, rows, B, CALL)                                                             \
+  do {                                                                                              \
+    const RowPlan plan = row_plan(dt, V);                                                           \
+    const dim3 block(plan.one ? 256 : 64 * plan.waves);                                             \
+    const unsigned groups = (unsigned)(plan.one ? ((rows) + 3) / 4 : (rows));                       \
+    int64_t most = ((1ll << 32) - 1) / ((int64_t)groups * block.x);                                 \
+    if (most > 65535) most = 65535;                                                                 \
+    for (int64_t b0 = 0; b0 < (B); b0 += most) {                                                    \
+      const dim3 grid(groups, (unsigned)((B) - b0 < most ? (B) - b0 : most));                       \
+      if (plan.one) { PF_BY_DTYPE(dt, CALL##_ONE); }                                                \
+      else if (plan.loop) { PF_BY_DTYPE(dt, CALL##_LOOP); }                                         \
+      else if (plan.nv == 4) { PF_BY_DTYPE(dt, CALL##_FEW); }                                       \
+      else { PF_BY_DTYPE(dt, CALL##_MANY); }                                                        \
+    }                                                                                               \
+  } while (0)
 
 extern "C" int pf_token_logprob_fwd(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, int64_t sb, int64_t st, const int64_t* labels,
                                     int shift, int64_t ignore_index, double temperature, float* logprobs, float* stats, void* stream) {
@@ -298,8 +681,12 @@ extern "C" int pf_token_logprob_fwd(const void* logits, int dtype, int64_t B, in
   if (B == 0 || T <= shift) return PF_OK;
   PF_REQUIRE(logprobs, "pf_token_logprob_fwd: null pointer");
   const TokenRows r = token_rows(logits, B, T, V, sb, st, labels, shift, ignore_index, temperature);
-#define CALL(DT) hipLaunchKernelGGL((token_logprob_kernel<DT, float>), rows_grid(B * (T - shift)), dim3(256), 0, (hipStream_t)stream, r, logprobs, (float2*)stats)
-  PF_BY_DTYPE(dtype, CALL);
+#define CALL(DT, NV, ONE, LOOP) hipLaunchKernelGGL((token_logprob_kernel<DT, NV, ONE, LOOP, float>), grid, block, 0, (hipStream_t)stream, r, (int)b0, logprobs, (float2*)stats)
+#define CALL_ONE(DT) CALL(DT, 4, true, false)
+#define CALL_FEW(DT) CALL(DT, 4, false, false)
+#define CALL_MANY(DT) CALL(DT, 16, false, false)
+#define CALL_LOOP(DT) CALL(DT, 8, false, true)
+  PF_BY_ROW(dtype, V, T - shift, B, CALL);
 #undef CALL
   PF_CHECK_LAUNCH("pf_token_logprob_fwd");
   return PF_OK;
@@ -315,9 +702,12 @@ extern "C" int pf_token_logprob_bwd(const void* logits, int dtype, int64_t B, in
   PF_REQUIRE(dlogits && (T <= shift || (stats && coef)), "pf_token_logprob_bwd: null pointer");
   const TokenRows r = token_rows(logits, B, T, V, sb, st, labels, shift, ignore_index, temperature);
   const GradRows d = {dlogits, d_sb, d_st};
-#define CALL(DT)                                                                                                                        \
-  hipLaunchKernelGGL(token_gradient_kernel<DT>, rows_grid(B * T), dim3(256), 0, (hipStream_t)stream, r, d, (const float2*)stats, coef, g_sb, g_st, \
-                     scale, unless_one)
+  const int64_t full = V / (dtype == PF_F32 ? 4 : 8), pieces = full > 64 * GNV ? (full + 64 * GNV - 1) / (64 * GNV) : 1;
+  // (with unless_one most calls have nothing to do: few workgroups, that loop where there is something)
+  const dim3 grid = rows_grid(T * pieces, B, 4, 256, unless_one ? 2048 : 1ll << 40);
+#define CALL(DT)                                                                                                                                 \
+  hipLaunchKernelGGL(token_gradient_kernel<DT>, grid, dim3(256), 0, (hipStream_t)stream, r, d, (const float2*)stats, coef, g_sb, g_st, scale, unless_one, \
+                     (unsigned)pieces)
   PF_BY_DTYPE(dtype, CALL);
 #undef CALL
   PF_CHECK_LAUNCH("pf_token_logprob_bwd");
@@ -337,13 +727,13 @@ extern "C" int pf_preference_loss(const void* logits, int dtype, int64_t B, int6
   double* logprobs = workspace + pairs;
   if (R > 0) {
     const TokenRows r = token_rows(logits, B, T, V, sb, st, labels, shift, ignore_index, 1.0);
-#define CALL(DT) hipLaunchKernelGGL((token_logprob_kernel<DT, double>), rows_grid(B * R), dim3(256), 0, (hipStream_t)stream, r, logprobs, (float2*)stats)
-    PF_BY_DTYPE(dtype, CALL);
+#define CALL(DT, NV, ONE, LOOP) hipLaunchKernelGGL((token_logprob_kernel<DT, NV, ONE, LOOP, double>), grid, block, 0, (hipStream_t)stream, r, (int)b0, logprobs, (float2*)stats)
+    PF_BY_ROW(dtype, V, R, B, CALL);
 #undef CALL
   }
-  hipLaunchKernelGGL(preference_pair_kernel, rows_grid(pairs), dim3(256), 0, (hipStream_t)stream, logprobs, labels, R + shift, shift, ignore_index, ref,
+  hipLaunchKernelGGL(preference_pair_kernel, dim3((unsigned)(pairs < 65536 ? pairs : 65536)), dim3(512), 0, (hipStream_t)stream, logprobs, labels, R + shift, shift, ignore_index, ref,
                      beta, label_smoothing, length_average, pairs, rewards, coef, workspace);
-  hipLaunchKernelGGL(sums_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, workspace, pairs, 1.0 / (double)pairs, loss, (float*)nullptr);
+  hipLaunchKernelGGL(sums_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, workspace, pairs, 1.0 / (double)pairs, loss, (float*)nullptr);
   PF_CHECK_LAUNCH("pf_preference_loss");
   return PF_OK;
 }
@@ -364,17 +754,18 @@ extern "C" int pf_policy_loss(const void* logits, int dtype, int64_t B, int64_t 
   hipStream_t s = (hipStream_t)stream;
   const TokenRows r = token_rows(logits, B, T, V, sb, st, labels, shift, ignore_index, temperature);
   const GradRows d = {dlogits, d_sb, d_st};
-  const PolicyArgs a = {old_logprobs, ref_logprobs, advantages, a_sb, a_st, 1.0 - clip_low, 1.0 + clip_high, kl_coef};
+  const PolicyArgs a = {old_logprobs, ref_logprobs, advantages, a_sb, a_st, clip_low < 1.0 ? log1p(-clip_low) : -INFINITY, log1p(clip_high),
+                        (float)(1.0 - clip_low), (float)(1.0 + clip_high), (float)kl_coef};
   const int64_t R = T > shift ? T - shift : 0;
   double* terms = workspace ? workspace + B : nullptr;
   if (B * T > 0 && (R > 0 || dlogits)) {
-    if (R > 0) hipLaunchKernelGGL(token_weights_kernel, dim3(1), dim3(256), 0, s, r, by_sequence, workspace);
-#define CALL(DT) \
-  hipLaunchKernelGGL(policy_kernel<DT>, rows_grid(B * T), dim3(256), 0, s, r, d, a, workspace, logprobs, (float2*)stats, coef, terms)
-    PF_BY_DTYPE(dtype, CALL);
+    if (R > 0) hipLaunchKernelGGL(token_weights_kernel, dim3(1), dim3(1024), 0, s, r, by_sequence, workspace);
+#define CALL(DT, NV, ONE, LOOP) \
+  hipLaunchKernelGGL((policy_kernel<DT, NV, ONE, LOOP>), grid, block, 0, s, r, (int)b0, d, a, workspace, logprobs, (float2*)stats, coef, terms)
+    PF_BY_ROW(dtype, V, dlogits ? T : R, B, CALL);
 #undef CALL
   }
-  hipLaunchKernelGGL(sums_kernel, dim3(1), dim3(256), 0, s, terms, B * R, 1.0, loss, kl);
+  hipLaunchKernelGGL(sums_kernel, dim3(1), dim3(1024), 0, s, terms, B * R, 1.0, loss, kl);
   PF_CHECK_LAUNCH("pf_policy_loss");
   return PF_OK;
 }
