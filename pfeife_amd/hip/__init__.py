@@ -217,7 +217,8 @@ def last_error():
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr()
+    """of a tensor, or of nothing; a place inside a tensor that the caller keeps is given as an address"""
+    return t if t is None or isinstance(t, int) else t.data_ptr()
 
 
 def _es(t):
@@ -795,7 +796,8 @@ class HipKernels:
             rows += [_ptr(p), _ptr(g), _ptr(m), _ptr(ms) or 0, _ptr(r), _ptr(rs) or 0, n, tensor]
             chunks += -(-n // ADAM_CHUNK)
             ends.append(chunks)
-        return torch.tensor(rows + ends, dtype=torch.int64).to(items[0][0].device), len(ends), chunks
+        # (pinned, so that a table of new gradients does not make the host wait for the device)
+        return torch.tensor(rows + ends, dtype=torch.int64, pin_memory=True).to(items[0][0].device, non_blocking=True), len(ends), chunks
 
     def adam8_step(self, table, n_items, n_chunks, lr, beta1, beta2, eps, weight_decay, step, state, stream):
         at = table.data_ptr()

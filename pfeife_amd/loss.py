@@ -95,14 +95,16 @@ def cross_entropy(logits, target, ignore_index=-100):
 
 
 _tables = {}
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _table(t, who):
     """The kernel table of the tensor's own device."""
-    if t.device.type != "cuda":
-        raise RuntimeError("%s: the HIP loss kernels need GPU tensors (got %s)" % (who, t.device))
-    k = _tables.get(t.device.index)
+    k = _tables.get(t.get_device())
     if k is None:
+        if t.device.type != "cuda":
+            raise RuntimeError("%s: the HIP loss kernels need GPU tensors (got %s)" % (who, t.device))
         from .hip import HipKernels
 
         with torch.cuda.device(t.device):
@@ -112,12 +114,15 @@ def _table(t, who):
 
 def _issue(t, launch):
     """On the current stream of the tensor's device, whichever device is the current one."""
-    stream = torch.cuda.current_stream(t.device).cuda_stream
-    if torch.cuda.current_device() == t.device.index:
-        launch(stream)
+    index = t.get_device()
+    if torch.cuda.current_device() == index:
+        launch(_raw_stream(index))
     else:
-        with torch.cuda.device(t.device):
-            launch(stream)
+        with torch.cuda.device(index):
+            launch(_raw_stream(index))
+
+
+_LOGITS = (torch.float32, torch.float16, torch.bfloat16)
 
 
 def _check_rows(who, logits, labels, ignore_index, temperature, shift):
@@ -125,40 +130,40 @@ def _check_rows(who, logits, labels, ignore_index, temperature, shift):
     if not torch.is_tensor(logits) or not torch.is_tensor(labels):
         raise RuntimeError("%s: logits and labels are tensors" % who)
     _table(logits, who)
-    if logits.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+    shape = logits.shape
+    if logits.dtype not in _LOGITS:
         raise RuntimeError("%s: logits are fp32, fp16 or bf16 (got %s)" % (who, logits.dtype))
-    if logits.dim() < 2 or logits.shape[-1] == 0:
-        raise RuntimeError("%s: logits are [..., tokens, classes] (got %s)" % (who, tuple(logits.shape)))
-    if labels.dtype != torch.int64 or labels.device != logits.device or labels.shape != logits.shape[:-1]:
+    if len(shape) < 2 or shape[-1] == 0:
+        raise RuntimeError("%s: logits are [..., tokens, classes] (got %s)" % (who, tuple(shape)))
+    if labels.dtype != torch.int64 or labels.get_device() != logits.get_device() or labels.shape != shape[:-1]:
         raise RuntimeError("%s: labels are int64 %s on %s (got %s %s on %s)"
-                           % (who, tuple(logits.shape[:-1]), logits.device, labels.dtype, tuple(labels.shape), labels.device))
+                           % (who, tuple(shape[:-1]), logits.device, labels.dtype, tuple(labels.shape), labels.device))
     if not isinstance(ignore_index, int) or not isinstance(shift, (bool, int)) or shift not in (0, 1):
         raise RuntimeError("%s: ignore_index is a whole number and shift a truth value" % who)
     if not 1e-6 <= temperature <= 1e6:
         raise RuntimeError("%s: temperature must lie in [1e-6, 1e6] (got %s)" % (who, temperature))
-    if logits.dim() != 3:
-        logits = logits.reshape((math.prod(logits.shape[:-2]),) + logits.shape[-2:])
+    if len(shape) != 3:
+        logits = logits.reshape((math.prod(shape[:-2]),) + shape[-2:])
         labels = labels.reshape(logits.shape[:-1])
-    if logits.stride(-1) != 1 and logits.shape[-1] > 1:
+    if logits.stride(-1) != 1 and shape[-1] > 1:
         logits = logits.contiguous()
     return logits, labels.contiguous()
 
 
 def _constant(who, name, t, shapes, like):
     """An operand that no gradient flows to, fp32 on the logits' device, of one of these shapes."""
-    if not torch.is_tensor(t) or not t.is_floating_point() or t.device != like.device or tuple(t.shape) not in shapes:
+    if not torch.is_tensor(t) or not t.is_floating_point() or t.get_device() != like.get_device() or t.shape not in shapes:
         raise RuntimeError("%s: %s is a floating tensor of shape %s on %s (got %s)"
                            % (who, name, " or ".join(map(str, shapes)), like.device,
                               "%s %s on %s" % (t.dtype, tuple(t.shape), t.device) if torch.is_tensor(t) else type(t).__name__))
     if t.requires_grad:
         raise RuntimeError("%s: no gradient flows to %s: detach it" % (who, name))
-    return t.to(torch.float32)
+    return t if t.dtype == torch.float32 else t.to(torch.float32)
 
 
 def _rows(logits, labels, cfg):
     """The kernels' description of the rows; cfg = (shift, ignore_index, temperature)."""
-    B, T, V = logits.shape
-    return (logits, B, T, V, logits.stride(0), logits.stride(1), labels, *cfg)
+    return (logits, *logits.shape, *logits.stride()[:2], labels, *cfg)
 
 
 def _new(like, *shape, dtype=torch.float32):
@@ -200,13 +205,16 @@ class _PreferenceFn(torch.autograd.Function):
     def forward(ctx, logits, labels, ref, cfg, beta, smoothing, average, want):
         B, T, _ = logits.shape
         k = _table(logits, "")
-        stats = _new(logits, B, max(0, T - cfg[0]), 2) if want else None
-        loss, rewards, coef = _new(logits), _new(logits, B), _new(logits, B)
-        _issue(logits, k.preference_loss(_rows(logits, labels, cfg), ref, beta, smoothing, average, loss, rewards, stats, coef,
-                                         _new(logits, k.preference_workspace(B, T, cfg[0]), dtype=torch.float64)))
+        n, rows = k.preference_workspace(B, T, cfg[0]), B * max(0, T - cfg[0])
+        # the kernels' scratch, and behind it what the backward pass takes: {reference, 1 / sum} of every row, a factor of every sequence
+        work = _new(logits, n + rows + (B + 1) // 2, dtype=torch.float64)
+        at = work.data_ptr()
+        stats, coef = at + 8 * n, at + 8 * (n + rows)
+        loss, rewards = _new(logits), _new(logits, B)
+        _issue(logits, k.preference_loss(_rows(logits, labels, cfg), ref, beta, smoothing, average, loss, rewards, stats if want else None, coef, work))
         if want:
-            ctx.save_for_backward(logits, labels, stats, coef)
-            ctx.cfg = cfg
+            ctx.save_for_backward(logits, labels, work)
+            ctx.cfg, ctx.at = cfg, (stats, coef)
         ctx.mark_non_differentiable(rewards)
         ctx.set_materialize_grads(False)
         return loss, rewards
@@ -214,8 +222,8 @@ class _PreferenceFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad, _):
-        logits, labels, stats, coef = ctx.saved_tensors
-        d = None if grad is None else _logits_gradient(logits, labels, ctx.cfg, stats, coef, (1, 0), _as_scale(grad))
+        logits, labels, _ = ctx.saved_tensors
+        d = None if grad is None else _logits_gradient(logits, labels, ctx.cfg, *ctx.at, (1, 0), _as_scale(grad))
         return (d,) + (None,) * 7
 
 
@@ -229,14 +237,23 @@ class _PolicyFn(torch.autograd.Function):
         B, T, _ = logits.shape
         k = _table(logits, "")
         R = max(0, T - cfg[0])
+        n = k.policy_workspace(B, T, cfg[0])
         loss, kl, logprobs = _new(logits), _new(logits), _new(logits, B, R)
-        stats, coef, d = (_new(logits, B, R, 2), _new(logits, B, R), torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)) \
-            if want else (None, None, None)
+        stats = coef = d = None
+        strides = (0, 0)
+        if want:      # behind the kernels' scratch what the backward pass takes: {reference, 1 / sum} and a factor of every row
+            work = _new(logits, n + B * R + (B * R + 1) // 2, dtype=torch.float64)
+            stats = work.data_ptr() + 8 * n
+            coef = stats + 8 * B * R
+            d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+            strides = d.stride()[:2]
+        else:
+            work = _new(logits, n, dtype=torch.float64)
         _issue(logits, k.policy_loss(_rows(logits, labels, cfg), old, adv, a_strides, ref, *clip, kl_coef, by_sequence, loss, kl, logprobs, stats,
-                                     coef, d, d.stride()[:2] if want else (0, 0), _new(logits, k.policy_workspace(B, T, cfg[0]), dtype=torch.float64)))
+                                     coef, d, strides, work))
         if want:
-            ctx.save_for_backward(logits, labels, stats, coef)
-            ctx.cfg, ctx.d, ctx.captured = cfg, d, torch.cuda.is_current_stream_capturing()
+            ctx.save_for_backward(logits, labels, work)
+            ctx.cfg, ctx.at, ctx.d, ctx.captured = cfg, (stats, coef, (R, 1)), d, torch.cuda.is_current_stream_capturing()
         ctx.mark_non_differentiable(logprobs, kl)
         ctx.set_materialize_grads(False)
         return loss, logprobs, kl
@@ -244,14 +261,14 @@ class _PolicyFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad, *_):
-        logits, labels, stats, coef = ctx.saved_tensors
+        logits, labels, _ = ctx.saved_tensors
         d = None
         if grad is not None:
             # handed out once (what has it may change it), and not from an eager forward pass to a graph, whose
             # replays would find it changed
             d, ctx.d = ctx.d, None
             ready = d is not None and ctx.captured == torch.cuda.is_current_stream_capturing()
-            d = _logits_gradient(logits, labels, ctx.cfg, stats, coef, coef.stride(), _as_scale(grad), d if ready else None, int(ready))
+            d = _logits_gradient(logits, labels, ctx.cfg, *ctx.at, _as_scale(grad), d if ready else None, int(ready))
         return (d,) + (None,) * 10
 
 

@@ -898,14 +898,17 @@ class StageWorker:
 
     def _adam8_prepare(self, opt, scaled):
         """The same for AdamW8bit, whose own step() cannot know of an overflow without a read from the device."""
-        work, fresh = opt._prepare(self.kernels)
+        lane = self.stream_obj if self.stream_obj is not None else torch.cuda.default_stream(self.device)
+        with torch.cuda.stream(lane):
+            work, fresh = opt._prepare(self.kernels)
 
         def step():
             if scaled and fresh:
-                self._seed_device_step_count(opt, [(g, None, states, None) for g, states, _, _ in work])
-            for g, states, _, table in work:
-                opt._launch(self.kernels, g, states, table, self.stream(), self.scaler_state if scaled else None)
-                self._host_steps_stale = scaled
+                self._seed_device_step_count(opt, [(w[0], None, w[1], None) for w in work])
+            with torch.cuda.stream(lane):
+                for g, states, _, table, copies in work:
+                    opt._launch(self.kernels, g, states, table, copies, lane.cuda_stream, self.scaler_state if scaled else None)
+                    self._host_steps_stale = scaled
 
         return step
 

@@ -7,6 +7,7 @@ A parameter of `min_8bit_size` elements or more keeps its moments as e4m3 codes 
 import torch
 
 from .hip import ADAM8_BLOCK
+from .loss import _raw_stream, _table
 
 
 class AdamW8bit(torch.optim.Optimizer):
@@ -53,51 +54,63 @@ class AdamW8bit(torch.optim.Optimizer):
         return st
 
     @staticmethod
-    def _check(p, st):
-        """The operands as the kernel addresses them: (gradient, first moment, its scales, second moment, its scales)"""
-        g = p.grad
+    def _operands(p, st):
+        """(first moment, its scales, second moment, its scales)"""
+        if "exp_avg_scale" in st:
+            return st["exp_avg"], st["exp_avg_scale"], st["exp_avg_sq_root"], st["exp_avg_sq_root_scale"]
+        return st["exp_avg"], None, st["exp_avg_sq"], None
+
+    @staticmethod
+    def _check(p, g, ops):
+        """The gradient as the kernel addresses it; errors where it, the parameter or the state is not what the kernel takes."""
         if p.device.type != "cuda":
             raise RuntimeError("AdamW8bit: the HIP step needs GPU parameters (got %s)" % p.device)
         if g.is_sparse or g.dtype != torch.float32 or g.device != p.device:
             raise RuntimeError("AdamW8bit: gradients are dense fp32 on the parameter's device (got %s %s on %s)" % (g.layout, g.dtype, g.device))
-        if not torch.empty_like(p, device="meta").stride() == p.stride():
+        if not p.is_contiguous() and torch.empty_like(p, device="meta").stride() != p.stride():
             raise RuntimeError("AdamW8bit: a parameter's elements have to lie in memory without gaps (strides %s)" % (p.stride(),))
-        if g.stride() != p.stride():
-            g = torch.empty_like(p).copy_(g)
-        if "exp_avg_scale" in st:
-            ops = [(st["exp_avg"], torch.float8_e4m3fn, p.numel()), (st["exp_avg_scale"], torch.float32, -(-p.numel() // ADAM8_BLOCK)),
-                   (st["exp_avg_sq_root"], torch.float8_e4m3fn, p.numel()), (st["exp_avg_sq_root_scale"], torch.float32, -(-p.numel() // ADAM8_BLOCK))]
+        n = p.numel()
+        if ops[1] is not None:
+            fits = all(t.dtype == dtype and t.numel() == size and t.is_contiguous() and t.device == p.device for t, dtype, size in
+                       zip(ops, (torch.float8_e4m3fn, torch.float32) * 2, (n, -(-n // ADAM8_BLOCK)) * 2))
         else:
-            ops = [(st["exp_avg"], torch.float32, p.numel()), None, (st["exp_avg_sq"], torch.float32, p.numel()), None]
-        for op in ops:
-            if op is not None and (op[0].dtype != op[1] or op[0].numel() != op[2] or op[0].device != p.device
-                                   or op[0].dim() == 1 and not op[0].is_contiguous() or op[0].dim() > 1 and op[0].stride() != p.stride()):
-                raise RuntimeError("AdamW8bit: the optimizer's state does not fit its parameter of shape %s" % (tuple(p.shape),))
-        return (g,) + tuple(None if op is None else op[0] for op in ops)
+            fits = all(t.dtype == torch.float32 and t.numel() == n and t.device == p.device and (t.stride() == p.stride() or t.dim() == 1 and t.is_contiguous())
+                       for t in ops[::2])
+        if not fits:
+            raise RuntimeError("AdamW8bit: the optimizer's state does not fit its parameter of shape %s" % (tuple(p.shape),))
+        return g if g.stride() == p.stride() or g.is_contiguous() and p.is_contiguous() else torch.empty_like(p)     # (of another layout: copied for each step)
 
     def _prepare(self, kernels):
-        """[(group, states, table, items, chunks)] of what has a gradient, parameters at one step count together, and whether a table is new."""
+        """[(group, states, device, table, copies)] of what has a gradient, parameters at one step count together, and whether a table
+        is new.  A table holds addresses: it is made again when one of them is another, or the stream is.  Reads no gradient."""
         cache = self.__dict__.setdefault("_tables", {})
         work, fresh, place = [], False, 0
         for gi, group in enumerate(self.param_groups):
             by_step = {}
             for p in group["params"]:
                 place += 1
-                if p.grad is None or p.numel() == 0:
+                g = p.grad
+                if g is None or p.numel() == 0:
                     continue
                 st = self._init_state(p, group)
-                by_step.setdefault((float(st["step"]), p.device), []).append((p, st, place - 1))
-            for n, (_, found) in enumerate(sorted(by_step.items(), key=lambda kv: (kv[0][0], str(kv[0][1])))):
-                items = []
-                for p, st, index in found:
-                    g, m, ms, r, rs = self._check(p, st)
-                    items.append((p.data, g, m, ms, r, rs, index))
-                key = [(i[6], i[0].numel()) + tuple(None if t is None else t.data_ptr() for t in i[:6]) for i in items]
+                key = (float(st["step"]), p.get_device())
+                found = by_step.get(key)
+                if found is None:
+                    found = by_step[key] = ([], [], [])
+                ops = self._operands(p, st)
+                found[0].append(st)
+                found[1].append((p, g, ops, place - 1))
+                found[2].append((place, *[t if t is None else (t.data_ptr(), t.dtype, t.numel()) for t in (p, g, *ops)], g.stride(), p.stride()))
+            for n, key in enumerate(sorted(by_step)):
+                states, params, now = by_step[key]
+                now.append(_raw_stream(key[1]) if key[1] >= 0 else None)
                 ent = cache.get((gi, n))
-                if ent is None or ent[0] != key:
+                if ent is None or ent[0] != now:
                     fresh = True
-                    ent = cache[gi, n] = (key, kernels.adam8_table(items))
-                work.append((group, [st for _, st, _ in found], items, ent[1]))
+                    items = [(p.data, self._check(p, g, ops), *ops, index) for p, g, ops, index in params]
+                    copies = [(i[1], g) for (_, g, _, _), i in zip(params, items) if i[1] is not g]
+                    ent = cache[gi, n] = (now, kernels.adam8_table(items), copies)
+                work.append((group, states, params[0][0].device, *ent[1:]))
         return work, fresh
 
     @torch.no_grad()
@@ -109,24 +122,31 @@ class AdamW8bit(torch.optim.Optimizer):
         first = next((p for g in self.param_groups for p in g["params"] if p.grad is not None), None)
         if first is None:
             return loss
-        from .loss import _table
-
-        if first.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+        if first.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW8bit: a step cannot be captured into a graph: its count would stay the same")
         kernels = _table(first, "AdamW8bit")
-        for group, states, items, table in self._prepare(kernels)[0]:
-            device = items[0][0].device
-            with torch.cuda.device(device):
-                self._launch(_table(items[0][0], "AdamW8bit"), group, states, table, torch.cuda.current_stream(device).cuda_stream)
+        for group, states, device, table, copies in self._prepare(kernels)[0]:
+            if device.index == torch.cuda.current_device():
+                self._launch(kernels, group, states, table, copies, _raw_stream(device.index))
+            else:
+                with torch.cuda.device(device):
+                    self._launch(kernels, group, states, table, copies, _raw_stream(device.index))
         return loss
 
     @staticmethod
-    def _launch(kernels, group, states, table, stream, scaler_state=None):
-        """One launch; with a loss scaler's state the count of steps is the device's, and the states' entries are not touched."""
+    def _launch(kernels, group, states, table, copies, stream, scaler_state=None):
+        """One launch, on the current stream; with a loss scaler's state the count of steps is the device's, and the states' entries are not
+        touched."""
+        for mine, g in copies:
+            mine.copy_(g)
         b1, b2 = group["betas"]
         step = int(states[0]["step"]) + 1
         kernels.adam8_step(*table, float(group["lr"]), float(b1), float(b2), float(group["eps"]), float(group["weight_decay"]), step,
                            scaler_state, stream)
         if scaler_state is None:
-            for st in states:
-                st["step"] += 1
+            steps = [st["step"] for st in states]
+            if all(map(torch.is_tensor, steps)):
+                torch._foreach_add_(steps, 1)
+            else:
+                for st in states:
+                    st["step"] += 1
