@@ -121,14 +121,14 @@ template <bool FIRST> struct Sums {
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       e[k] = __builtin_amdgcn_exp2f(fmaf(x[k], c, -ref));
-      if (FIRST) f = fmaf(e[k], max3(x[k], NOTHING, NOTHING), f);      // (0 of -inf)
+      if (FIRST) f = fmaf(e[k], x[k], f);
     }
 #pragma unroll
     for (int d = N / 2; d > 0; d >>= 1)
 #pragma unroll
       for (int k = 0; k < d; ++k) e[k] += e[k + d];
     s += (double)(valid ? e[0] : 0.f);
-    if (FIRST) s1 += (double)(valid ? f : 0.f);
+    if (FIRST) s1 += (double)(valid && f == f ? f : 0.f);      // (0 times -inf: a masked class among the eight leaves them out of the mean)
   }
   __device__ __forceinline__ void join(float other, double os, double os1) {
     const float to = max3(ref, other, other);
@@ -204,31 +204,46 @@ __device__ double slow_sums(const char* x, int V, float c, float* m_out, double*
 
 template <int DT> constexpr int pf_es = DT == PF_F32 ? 4 : 2;
 
+// A row in vectors of 16 bytes from the first address of `where` (the row itself, or its gradient) that is a multiple of 16 on: `head` elements
+// stand before them and less than a vector's behind them, those of both ends a lane each.
+template <int DT> struct Split {
+  int head, full, loose;      // elements before the vectors, vectors, elements at both ends
+  __device__ __forceinline__ Split(const char* where, int V) {
+    head = (int)((16u - ((uint32_t)(uintptr_t)where & 15u)) & 15u) / pf_es<DT>;
+    if (head > V) head = V;
+    full = (V - head) / VE<DT>;
+    loose = V - full * VE<DT>;
+  }
+  __device__ __forceinline__ int element(int lane) const { return lane < head ? lane : full * VE<DT> + lane; }      // (lane < loose)
+  __device__ __forceinline__ size_t start() const { return (size_t)head * pf_es<DT>; }
+};
+
 // LOOP: the row takes several tiles of NV vectors to a lane; else one (rows of no vector at all have none).
 template <int DT, int NV, bool ONE, bool LOOP> struct RowReader {
   const char* x;       // the row
-  int V, full, tail;   // elements, whole vectors, elements behind them
+  Split<DT> cut;
+  int full;            // its vectors
   int tid, n;          // this lane among those of the row
   raw4 v[NV];
-  float last;          // the element behind the vectors that this lane has (tid < tail)
+  float last;          // the loose element that this lane has (tid < cut.loose)
 
-  __device__ __forceinline__ RowReader(const void* row, int64_t at, int64_t classes)
-      : x((const char*)row + at * pf_es<DT>), V((int)classes), full((int)classes / VE<DT>), tail((int)classes % VE<DT>), tid(ONE ? (threadIdx.x & 63) : threadIdx.x),
-        n(ONE ? 64 : blockDim.x) {}
+  __device__ __forceinline__ RowReader(const char* row, const char* where, int V)
+      : x(row), cut(where, V), full(cut.full), tid(ONE ? (threadIdx.x & 63) : threadIdx.x), n(ONE ? 64 : blockDim.x) {}
 
   __device__ __forceinline__ int tiles() const { return full == 0 ? 0 : LOOP ? (full + n * NV - 1) / (n * NV) : 1; }
-  __device__ __forceinline__ void load_tail() {
+  __device__ __forceinline__ void load_loose() {
     last = -INFINITY;
-    if (tid < tail) last = Codec<DT>::load(x, full * VE<DT> + tid);
+    if (tid < cut.loose) last = Codec<DT>::load(x, cut.element(tid));
   }
   // lanes that have an i-th vector of a tile: those below this (uniform)
   __device__ __forceinline__ int left(int tile, int i) const { return full - (tile * NV + i) * n; }
   __device__ __forceinline__ void load(int tile) {
+    const char* from = x + cut.start();
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       int k = (tile * NV + i) * n + tid;
       if (k > full - 1) k = full - 1;
-      v[i] = *(const raw4_any*)(x + (uint32_t)k * 16u);
+      v[i] = *(const raw4_any*)(from + (uint32_t)k * 16u);
     }
   }
   template <bool FIRST> __device__ __forceinline__ void sum(int tile, float c, Sums<FIRST>& a) {
@@ -244,11 +259,11 @@ template <int DT, int NV, bool ONE, bool LOOP> struct RowReader {
       a.add(e, c, tid < left(tile, i));      // (lanes past the end hold the last vector again)
     }
   }
-  template <bool FIRST> __device__ __forceinline__ void sum_tail(float c, Sums<FIRST>& a) {
-    if (tail == 0) return;
+  template <bool FIRST> __device__ __forceinline__ void sum_loose(float c, Sums<FIRST>& a) {
+    if (cut.loose == 0) return;
     float e[1] = {last};
     a.raise(last * c);
-    a.add(e, c, tid < tail);
+    a.add(e, c, tid < cut.loose);
   }
 };
 
@@ -258,17 +273,17 @@ template <int DT> __device__ __forceinline__ float element(const char* x, int j)
 template <bool FIRST, int DT, int NV, bool ONE, bool LOOP>
 __device__ __forceinline__ RowStats row_stats(const TokenRows& r, RowReader<DT, NV, ONE, LOOP>& row, float xy, SumSlots<FIRST>* sm, bool lane_wants) {
   Sums<FIRST> a;
-  row.load_tail();
+  row.load_loose();
   const int tiles = row.tiles();
   for (int tile = 0; tile < tiles; ++tile) {
     row.load(tile);
     row.sum(tile, r.c, a);
   }
-  row.sum_tail(r.c, a);
+  row.sum_loose(r.c, a);
   join_row<ONE, FIRST>(a, sm);
   RowStats o = {a.ref, 0.f, !(a.s > 0.0 && a.s < INFINITY), 0.0};
   if (o.slow) {
-    a.s = slow_sums<DT, ONE>(row.x, row.V, r.c, &o.ref, sm ? sm->s : nullptr);
+    a.s = slow_sums<DT, ONE>(row.x, (int)r.V, r.c, &o.ref, sm ? sm->s : nullptr);
     o.logprob = ((double)xy - (double)o.ref) * r.inv_temp - log(a.s);
   } else if (lane_wants) {
     if (FIRST)   // ln sum exp(x / temperature) = ln sum 2^(x c) - c's relative error times the mean of x / temperature
@@ -280,7 +295,11 @@ __device__ __forceinline__ RowStats row_stats(const TokenRows& r, RowReader<DT, 
   return o;
 }
 
-template <int DT> __device__ __forceinline__ void store_vector(char* dx, int k, const raw4& w) { *(raw4_any*)(dx + (uint32_t)k * 16u) = w; }
+// PAST: past the caches
+template <bool PAST> __device__ __forceinline__ void store_vector(char* dx, const raw4& w) {
+  if (PAST) __builtin_nontemporal_store(w, (raw4_any*)dx);
+  else *(raw4_any*)dx = w;
+}
 
 // What a lane needs for dx = g (onehot - p) / temperature = scaled 2^(..), scaled = -g inv / temperature; and the whole of it at the label
 struct RowGrad { float scaled, at_label; };
@@ -293,14 +312,14 @@ __device__ __forceinline__ RowGrad row_grad(const TokenRows& r, const RowStats& 
   return {scaled, fmaf(scaled, s.slow ? power<true>(xy, s, r.c) : power<false>(xy, s, r.c), g)};
 }
 // of the vector at dx; label: whose element in it, else negative or VE and more
-template <int DT, bool SLOW>
+template <int DT, bool SLOW, bool PAST>
 __device__ __forceinline__ void gradient_vector(raw4 w, int label, const RowStats& s, const RowGrad& g, float c, char* dx) {
   asm volatile("" : "+v"(w));      // (unpacked here and not before: a tile's elements would not fit the registers)
   float x[VE<DT>];
   unpack<DT>(w, x);
 #pragma unroll
   for (int e = 0; e < VE<DT>; ++e) x[e] = g.scaled * power<SLOW>(x[e], s, c);
-  *(raw4_any*)dx = pack<DT>(x);
+  store_vector<PAST>(dx, pack<DT>(x));
   if ((unsigned)label < (unsigned)VE<DT>) Codec<DT>::store(dx, label, g.at_label);      // (the same lane, behind its vector)
 }
 template <int DT>
@@ -308,15 +327,15 @@ __device__ __forceinline__ void gradient_element(float x, int j, int y, const Ro
   Codec<DT>::store(dx, j, j == y ? g.at_label : g.scaled * (s.slow ? power<true>(x, s, c) : power<false>(x, s, c)));
 }
 
-template <int DT>
+template <int DT, bool PAST>
 __device__ __forceinline__ void fill_row(char* dx, int V, float value, int tid, int n) {
   float x[VE<DT>];
 #pragma unroll
   for (int e = 0; e < VE<DT>; ++e) x[e] = value;
   const raw4 w = pack<DT>(x);
-  const int full = V / VE<DT>;
-  for (int k = tid; k < full; k += n) store_vector<DT>(dx, k, w);
-  if (tid < V % VE<DT>) Codec<DT>::store(dx, (int64_t)full * VE<DT> + tid, value);
+  const Split<DT> cut(dx, V);
+  for (int k = tid; k < cut.full; k += n) store_vector<PAST>(dx + cut.start() + (uint32_t)k * 16u, w);
+  if (tid < cut.loose) Codec<DT>::store(dx, cut.element(tid), value);
 }
 
 // The row of a workgroup or, with ONE, of a wavefront (four to a workgroup): sequence b, place t (uniform)
@@ -337,7 +356,8 @@ __global__ __launch_bounds__(ONE ? 256 : 1024) void token_logprob_kernel(const T
   RowStats s = {0.f, kind == LABEL_BAD ? NAN : 0.f, false, kind == LABEL_BAD ? (double)NAN : 0.0};
   const int tid = ONE ? threadIdx.x & 63 : threadIdx.x;
   if (kind == LABEL_OK) {
-    RowReader<DT, NV, ONE, LOOP> row(r.logits, b * r.sb + t * r.st, r.V);
+    const char* x = (const char*)r.logits + (b * r.sb + t * r.st) * pf_es<DT>;
+    RowReader<DT, NV, ONE, LOOP> row(x, x, (int)r.V);
     s = row_stats<FIRST>(r, row, element<DT>(row.x, (int)y), slots, tid == 0);
   }
   if (tid == 0) {
@@ -350,53 +370,55 @@ __global__ __launch_bounds__(ONE ? 256 : 1024) void token_logprob_kernel(const T
 // A wavefront to 64 * GNV vectors of a row, without a word to others.  Rows are taken from the last one back: what the forward pass read
 // last is what the caches may still hold.
 constexpr int GNV = 4;
-template <int DT>
+template <int DT, bool PAST>
 __global__ __launch_bounds__(256) void token_gradient_kernel(const TokenRows r, const GradRows d, const float2* stats, const float* coef,
                                                              int64_t g_sb, int64_t g_st, const float* scale, int unless_one, unsigned pieces) {
   const float by = scale ? scale[0] : 1.f;
   if (unless_one && by == 1.f) return;
   const int64_t R = r.T - r.shift, units = r.T * pieces;
-  const int lane = threadIdx.x & 63, V = (int)r.V, full = V / VE<DT>, tail = V % VE<DT>;
+  const int lane = threadIdx.x & 63;
   for (int64_t b = r.B - 1 - (int64_t)blockIdx.y; b >= 0; b -= gridDim.y) {
     for (int64_t u = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); u < units; u += (int64_t)gridDim.x * 4) {
       const int64_t t = r.T - 1 - u / pieces;
-      const int piece = (int)(u % pieces), k0 = piece * 64 * GNV + lane;
+      const int piece = (int)(u % pieces);
       char* dx = (char*)d.dx + (b * d.sb + t * d.st) * pf_es<DT>;
+      const Split<DT> cut(dx, (int)r.V);
+      const int first = piece * 64 * GNV + lane;      // this lane's vectors: this one and every 64th from it on
+      const bool loose = piece == 0 && lane < cut.loose;
       const int64_t y = t < R ? r.labels[b * r.T + t + r.shift] : 0;
       const LabelKind kind = t < R ? label_kind(r, y) : LABEL_SKIP;
+      char* to = dx + cut.start() + (uint32_t)first * 16u;
       if (kind == LABEL_SKIP) {
 #pragma unroll
         for (int i = 0; i < GNV; ++i)
-          if (k0 + i * 64 < full) store_vector<DT>(dx, k0 + i * 64, raw4{0, 0, 0, 0});
-        if (piece == (int)pieces - 1 && lane < tail) Codec<DT>::store(dx, (int64_t)full * VE<DT> + lane, 0.f);
+          if (first + i * 64 < cut.full) store_vector<PAST>(to + i * 1024, raw4{0, 0, 0, 0});
+        if (loose) Codec<DT>::store(dx, cut.element(lane), 0.f);
         continue;
       }
-      const int yi = kind == LABEL_OK ? (int)y : -1;      // (no vector's and no element's)
       const char* x = (const char*)r.logits + (b * r.sb + t * r.st) * pf_es<DT>;
+      const int yi = kind == LABEL_OK ? (int)y : -1;      // (no vector's and no element's)
       raw4 v[GNV];
-      if (full > 0) {
+      if (cut.full > 0) {
 #pragma unroll
         for (int i = 0; i < GNV; ++i) {
-          const int k = k0 + i * 64;
-          v[i] = *(const raw4_any*)(x + (uint32_t)(k < full ? k : full - 1) * 16u);
+          const int k = first + i * 64;
+          v[i] = *(const raw4_any*)(x + cut.start() + (uint32_t)(k < cut.full ? k : cut.full - 1) * 16u);
         }
       }
       const float2 packed = stats[b * R + t];
       const RowStats s = {packed.x, fabsf(packed.y), packed.y < 0.f, 0.0};
       const RowGrad g = row_grad(r, s, coef[b * g_sb + t * g_st] * by, kind == LABEL_OK ? element<DT>(x, yi) : NAN);
+      const int label = yi < cut.head ? -1 : yi - cut.head - first * VE<DT>;
       if (s.slow) {
 #pragma unroll
         for (int i = 0; i < GNV; ++i)
-          if (k0 + i * 64 < full) gradient_vector<DT, true>(v[i], yi - (k0 + i * 64) * VE<DT>, s, g, r.c, dx + (uint32_t)(k0 + i * 64) * 16u);
+          if (first + i * 64 < cut.full) gradient_vector<DT, true, PAST>(v[i], label - i * 64 * VE<DT>, s, g, r.c, to + i * 1024);
       } else {
 #pragma unroll
         for (int i = 0; i < GNV; ++i)
-          if (k0 + i * 64 < full) gradient_vector<DT, false>(v[i], yi - (k0 + i * 64) * VE<DT>, s, g, r.c, dx + (uint32_t)(k0 + i * 64) * 16u);
+          if (first + i * 64 < cut.full) gradient_vector<DT, false, PAST>(v[i], label - i * 64 * VE<DT>, s, g, r.c, to + i * 1024);
       }
-      if (piece == (int)pieces - 1 && lane < tail) {
-        const int j = full * VE<DT> + lane;
-        gradient_element<DT>(element<DT>(x, j), j, yi, s, g, r.c, dx);
-      }
+      if (loose) gradient_element<DT>(element<DT>(x, cut.element(lane)), cut.element(lane), yi, s, g, r.c, dx);
     }
   }
 }
@@ -407,66 +429,124 @@ __device__ __forceinline__ double wave_sum(double v) {
   return v;
 }
 
+// sum of f(i) for i = first, first + n, ... below `end`, eight of them requested at a time
+template <typename F> __device__ __forceinline__ double sum_in_eights(int64_t first, int64_t end, int64_t n, F f) {
+  double s = 0.0;
+  for (int64_t i = first; i < end; i += 8 * n) {
+    double x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = f(i + j * n < end ? i + j * n : end - 1);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += i + j * n < end ? x[j] : 0.0;
+  }
+  return s;
+}
+
 // ---- preference ------------------------------------------------------------------------------------------------------------
 // A workgroup to a pair, half of it to a sequence (2i, 2i + 1):  reward = beta (sum or mean of logprobs - ref),  D = reward_2i - reward_2i+1,
 //   loss_i = -(1 - e) ln sigma(D) - e ln sigma(-D),   d loss_i / dD = sigma(D) - (1 - e).
 __device__ __forceinline__ double softplus(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }   // -ln sigma(-x)
 
-__global__ __launch_bounds__(512) void preference_pair_kernel(const double* logprobs, const int64_t* labels, int64_t T, int shift, int64_t ignore_index,
-                                                              const float* ref, double beta, double smoothing, int average, int64_t pairs,
-                                                              float* rewards, float* coef, double* pair_loss) {
+struct PairArgs {
+  const double* logprobs;
+  const int64_t* labels;
+  int64_t T;
+  int shift;
+  int64_t ignore_index;
+  const float* ref;
+  double beta, smoothing;
+  int average;
+  int64_t pairs;
+  float* rewards;
+  float* coef;
+};
+// sum of the logprobs of sequence b's tokens and, for an average, how many count: this lane's part, lane of n
+__device__ __forceinline__ void sequence_part(const PairArgs& a, int64_t b, int lane, int n, double& s, double& count) {
+  const int64_t R = a.T - a.shift;
+  s = sum_in_eights(lane, R, n, [&](int64_t t) { return a.logprobs[b * R + t]; });
+  count = a.average ? sum_in_eights(lane, R, n, [&](int64_t t) { return a.labels[b * a.T + t + a.shift] != a.ignore_index ? 1.0 : 0.0; }) : 0.0;
+}
+// -> the pair's loss
+__device__ double pair_terms(const PairArgs& a, int64_t i, const double (&total)[2], const double (&count)[2]) {
+  double reward[2], per_token[2];
+  for (int k = 0; k < 2; ++k) {
+    per_token[k] = !a.average ? 1.0 : count[k] > 0.0 ? 1.0 / count[k] : 0.0;
+    reward[k] = a.beta * (total[k] * per_token[k] - (double)a.ref[2 * i + k]);
+  }
+  const double D = reward[0] - reward[1], up = 1.0 / (1.0 + exp(-D)) - (1.0 - a.smoothing);
+  for (int k = 0; k < 2; ++k) {
+    a.rewards[2 * i + k] = (float)reward[k];
+    a.coef[2 * i + k] = (float)((k ? -up : up) * a.beta * per_token[k] / (double)a.pairs);
+  }
+  return (1.0 - a.smoothing) * softplus(-D) + a.smoothing * softplus(D);
+}
+
+__global__ __launch_bounds__(512) void preference_pair_kernel(const PairArgs a, double* pair_loss) {
   __shared__ double sums[8], counts[8];
-  const int64_t R = T - shift;
-  const int half = threadIdx.x >> 8;
-  for (int64_t i = blockIdx.x; i < pairs; i += gridDim.x) {
-    const int64_t b = 2 * i + half;
-    double s = 0.0, n = 0.0;
-#pragma unroll 8
-    for (int64_t t = threadIdx.x & 255; t < R; t += 256) s += logprobs[b * R + t];
-    if (average)
-#pragma unroll 8
-      for (int64_t t = threadIdx.x & 255; t < R; t += 256) n += labels[b * T + t + shift] != ignore_index ? 1.0 : 0.0;
+  const int wave = threadIdx.x >> 6;
+  for (int64_t i = blockIdx.x; i < a.pairs; i += gridDim.x) {
+    double s, n;
+    sequence_part(a, 2 * i + (threadIdx.x >> 8), threadIdx.x & 255, 256, s, n);
     s = wave_sum(s);
     n = wave_sum(n);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) {
-      sums[threadIdx.x >> 6] = s;
-      counts[threadIdx.x >> 6] = n;
+      sums[wave] = s;
+      counts[wave] = n;
     }
     __syncthreads();
     if (threadIdx.x == 0) {
-      double reward[2], per_token[2];
+      double total[2], count[2];
       for (int k = 0; k < 2; ++k) {
-        const double total = sums[4 * k] + sums[4 * k + 1] + sums[4 * k + 2] + sums[4 * k + 3];
-        const double count = counts[4 * k] + counts[4 * k + 1] + counts[4 * k + 2] + counts[4 * k + 3];
-        per_token[k] = !average ? 1.0 : count > 0.0 ? 1.0 / count : 0.0;
-        reward[k] = beta * (total * per_token[k] - (double)ref[2 * i + k]);
+        total[k] = sums[4 * k] + sums[4 * k + 1] + sums[4 * k + 2] + sums[4 * k + 3];
+        count[k] = counts[4 * k] + counts[4 * k + 1] + counts[4 * k + 2] + counts[4 * k + 3];
       }
-      const double D = reward[0] - reward[1];
-      const double up = 1.0 / (1.0 + exp(-D)) - (1.0 - smoothing);
-      pair_loss[i] = (1.0 - smoothing) * softplus(-D) + smoothing * softplus(D);
-      for (int k = 0; k < 2; ++k) {
-        rewards[2 * i + k] = (float)reward[k];
-        coef[2 * i + k] = (float)((k ? -up : up) * beta * per_token[k] / (double)pairs);
-      }
+      pair_loss[i] = pair_terms(a, i, total, count);
     }
   }
+}
+
+// All pairs by one workgroup, and their mean: the wavefronts share the sequences, a lane each takes a pair.
+constexpr int FEW_SEQUENCES = 64;
+__global__ __launch_bounds__(1024) void preference_few_kernel(const PairArgs a, float* loss) {
+  __shared__ double sums[FEW_SEQUENCES][16], counts[FEW_SEQUENCES][16];
+  const int B = 2 * (int)a.pairs, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int share = B <= 2 ? 8 : B <= 4 ? 4 : B <= 8 ? 2 : 1;      // wavefronts to a sequence
+  for (int b = wave / share; b < B; b += 16 / share) {
+    double s, n;
+    sequence_part(a, b, (wave % share) * 64 + lane, share * 64, s, n);
+    s = wave_sum(s);
+    n = wave_sum(n);
+    if (lane == 0) {
+      sums[b][wave % share] = s;
+      counts[b][wave % share] = n;
+    }
+  }
+  __syncthreads();
+  if (wave != 0) return;
+  double mine = 0.0;
+  if (lane < (int)a.pairs) {
+    double total[2] = {0.0, 0.0}, count[2] = {0.0, 0.0};
+    for (int k = 0; k < 2; ++k)
+      for (int j = 0; j < share; ++j) {
+        total[k] += sums[2 * lane + k][j];
+        count[k] += counts[2 * lane + k][j];
+      }
+    mine = pair_terms(a, lane, total, count);
+  }
+  mine = wave_sum(mine);
+  if (lane == 0) loss[0] = (float)(mine / (double)a.pairs);
 }
 
 // out_k = scale * sum over n of in[k * n + i], in double
 __global__ __launch_bounds__(1024) void sums_kernel(const double* in, int64_t n, double scale, float* out0, float* out1) {
   __shared__ double sm[2][16];
-  double a = 0.0, c = 0.0;
-#pragma unroll 4
-  for (int64_t i = threadIdx.x; i < n; i += 1024) {
-    a += in[i];
-    if (out1) c += in[n + i];
-  }
-  a = wave_sum(a);
-  c = wave_sum(c);
-  if ((threadIdx.x & 63) == 0) {
-    sm[0][threadIdx.x >> 6] = a;
-    sm[1][threadIdx.x >> 6] = c;
+  double total[2] = {0.0, 0.0};
+  total[0] = sum_in_eights(threadIdx.x, n, 1024, [&](int64_t i) { return in[i]; });
+  if (out1) total[1] = sum_in_eights(threadIdx.x, n, 1024, [&](int64_t i) { return in[n + i]; });
+  for (int k = 0; k < 2; ++k) {
+    total[k] = wave_sum(total[k]);
+    if ((threadIdx.x & 63) == 0) sm[k][threadIdx.x >> 6] = total[k];
   }
   __syncthreads();
   if (threadIdx.x < 2 && (threadIdx.x == 0 || out1)) {
@@ -480,23 +560,27 @@ __global__ __launch_bounds__(1024) void sums_kernel(const double* in, int64_t n,
 // weight of every token of sequence b: 1 / (tokens that count), or by_sequence 1 / (its own such tokens * sequences that have any)
 __global__ __launch_bounds__(1024) void token_weights_kernel(const TokenRows r, int by_sequence, double* weights) {
   __shared__ double sm[16];
-  const int64_t R = r.T - r.shift;
+  const int64_t R = r.T - r.shift, all = r.B * r.T;
   double total = 0.0;
-  for (int64_t b = threadIdx.x >> 6; b < r.B; b += 16) {      // a wavefront to a sequence
-    double n = 0.0;
-#pragma unroll 8
-    for (int64_t t = threadIdx.x & 63; t < R; t += 64) n += r.labels[b * r.T + t + r.shift] != r.ignore_index ? 1.0 : 0.0;
-    n = wave_sum(n);
-    if ((threadIdx.x & 63) == 0) weights[b] = n;
-    total += by_sequence ? (n > 0.0 ? 1.0 : 0.0) : n;
+  if (by_sequence) {      // a wavefront to a sequence
+    for (int64_t b = threadIdx.x >> 6; b < r.B; b += 16) {
+      const double n = wave_sum(sum_in_eights(threadIdx.x & 63, R, 64, [&](int64_t t) { return r.labels[b * r.T + t + r.shift] != r.ignore_index ? 1.0 : 0.0; }));
+      if ((threadIdx.x & 63) == 0) weights[b] = n;
+      total += n > 0.0 ? 1.0 : 0.0;
+    }
+  } else {
+    double n = sum_in_eights(threadIdx.x, all, 1024, [&](int64_t i) { return r.labels[i] != r.ignore_index ? 1.0 : 0.0; });
+    if (r.shift)      // no row is scored against a sequence's first label
+      for (int64_t b = threadIdx.x; b < r.B; b += 1024) n -= r.labels[b * r.T] != r.ignore_index ? 1.0 : 0.0;
+    total = wave_sum(n);
   }
   if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = total;
   __syncthreads();
   total = 0.0;
   for (int i = 0; i < 16; ++i) total += sm[i];
   for (int64_t b = threadIdx.x; b < r.B; b += 1024) {
-    const double n = weights[b];
-    weights[b] = n > 0.0 ? 1.0 / (by_sequence ? n * total : total) : 0.0;
+    const double n = by_sequence ? weights[b] * total : total;
+    weights[b] = n > 0.0 ? 1.0 / n : 0.0;
   }
 }
 
@@ -547,7 +631,7 @@ __device__ __forceinline__ TokenTerms policy_token(const PolicyArgs& a, float ol
 }
 
 // A row's log-probability, its part of the loss and, where wanted, its gradient.  terms: [2][B * R], weighted
-template <int DT, int NV, bool ONE, bool LOOP>
+template <int DT, int NV, bool ONE, bool LOOP, bool PAST>
 __global__ __launch_bounds__(ONE ? 256 : 1024) void policy_kernel(const TokenRows r, int b0, const GradRows d, const PolicyArgs a, const double* weights,
                                                                   float* logprobs, float2* stats, float* coef, double* terms) {
   __shared__ SumSlots<false> slots[1];
@@ -568,12 +652,13 @@ __global__ __launch_bounds__(ONE ? 256 : 1024) void policy_kernel(const TokenRow
         stats[at] = make_float2(0.f, none);
       }
     }
-    if (d.dx) fill_row<DT>(dx, (int)r.V, none, tid, n);
+    if (d.dx) fill_row<DT, PAST>(dx, (int)r.V, none, tid, n);
     return;
   }
   const float old = a.old[at], A = a.adv[b * a.a_sb + t * a.a_st], ref = a.ref ? a.ref[at] : 0.f;
   const double w = weights[b];
-  RowReader<DT, NV, ONE, LOOP> row(r.logits, b * r.sb + t * r.st, r.V);
+  const char* x = (const char*)r.logits + (b * r.sb + t * r.st) * pf_es<DT>;
+  RowReader<DT, NV, ONE, LOOP> row(x, d.dx ? dx : x, (int)r.V);
   const float xy = element<DT>(row.x, (int)y);
   const RowStats s = row_stats<false>(r, row, xy, slots, true);
   const TokenTerms o = policy_token(a, old, A, ref, s.logprob);
@@ -589,39 +674,46 @@ __global__ __launch_bounds__(ONE ? 256 : 1024) void policy_kernel(const TokenRow
   }
   if (!d.dx) return;
   const RowGrad rg = row_grad(r, s, g, xy);
-  const int tiles = row.tiles(), mine = (int)y - tid * VE<DT>;
+  const int tiles = row.tiles(), label = (int)y < row.cut.head ? -1 : (int)y - row.cut.head - tid * VE<DT>;
   for (int tile = tiles - 1; tile >= 0; --tile) {
     if (LOOP && tile != tiles - 1) row.load(tile);      // (the last one is still there)
-    char* to = dx + (size_t)((unsigned)(tile * NV * n) * 16u);
+    char* to = dx + row.cut.start() + (size_t)((unsigned)(tile * NV * n) * 16u);
     if (s.slow) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (tid < row.left(tile, i))
-          gradient_vector<DT, true>(row.v[i], mine - (tile * NV + i) * n * VE<DT>, s, rg, r.c, to + (unsigned)(i * n) * 16u + (unsigned)tid * 16u);
+          gradient_vector<DT, true, PAST>(row.v[i], label - (tile * NV + i) * n * VE<DT>, s, rg, r.c, to + (unsigned)(i * n) * 16u + (unsigned)tid * 16u);
     } else {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (tid < row.left(tile, i))
-          gradient_vector<DT, false>(row.v[i], mine - (tile * NV + i) * n * VE<DT>, s, rg, r.c, to + (unsigned)(i * n) * 16u + (unsigned)tid * 16u);
+          gradient_vector<DT, false, PAST>(row.v[i], label - (tile * NV + i) * n * VE<DT>, s, rg, r.c, to + (unsigned)(i * n) * 16u + (unsigned)tid * 16u);
     }
   }
-  if (tid < row.tail) {
-    const int j = row.full * VE<DT> + tid;
-    gradient_element<DT>(row.last, j, (int)y, s, rg, r.c, dx);
-  }
+  if (tid < row.cut.loose) gradient_element<DT>(row.last, row.cut.element(tid), (int)y, s, rg, r.c, dx);
 }
 
 // ---- launches --------------------------------------------------------------------------------------------------------------
 // How a row is dealt out.  NV accesses of a lane in flight, WAVES wavefronts to a row; ONE: a wavefront alone, four rows to a workgroup; LOOP: in
-// several tiles.
+// several tiles.  A row that is only read goes through eight wavefronts at most, so that several workgroups share a CU and one loads while
+// another sums: us for 400 MB, 2 wavefronts of 8 / 4 of 4 at 8192 classes 69 / 72 (in bf16), 8 of 8 / 4 of 16 at 32000 67 / 69, 13 wavefronts of 8 /
+// loops of 8 at 49999 88 / 59, 13 of 16 / loops at 100000 91 / 75.  One whose gradient follows is kept whole as far as registers go: 4 wavefronts of 4 /
+// 2 of 8 at 8192 191 / 197, 8 of 8 / 4 of 16 at 32000 187 / 190, 13 of 8 / 7 of 16 at 49999 208 / 176, 13 of 16 / loops of 8 at 100000 195 / 219.
 struct RowPlan { int nv, waves; bool one, loop; };
-RowPlan row_plan(int dtype, int64_t V) {
+RowPlan row_plan(int dtype, int64_t V, bool gradient) {
   const int64_t full = V / (dtype == PF_F32 ? 4 : 8);
+  const auto waves = [&](int nv) { return (int)((full + 64 * nv - 1) / (64 * nv)); };
   if (full <= 64 * 4) return {4, 1, true, false};
-  const int nv = full <= 64 * 4 * 4 ? 4 : full <= 64 * 16 * 16 ? 16 : 8;
-  const int64_t waves = (full + 64 * nv - 1) / (64 * nv);
-  return {nv, (int)(waves < 16 ? waves : 16), false, waves > 16};
+  if (gradient && full <= 64 * 4 * 4) return {4, waves(4), false, false};
+  if (full <= 64 * 8 * 8) return {8, waves(8), false, false};
+  if (gradient && full <= 64 * 16 * 16) return {16, waves(16), false, false};
+  return {8, gradient ? 16 : 8, false, true};
 }
+// A gradient of this many bytes goes past the caches, which it would only empty of logits that are still to be read: preference loss at [4, 2048] x
+// 32000 in bf16 272 -> 232 us, policy loss 198 -> 190.  In the policy loss's one pass that holds for rows of whole cache lines; a line that two workgroups
+// write goes out twice (49999 classes in fp16 172 -> 179, 10007 in fp32 230 -> 243).
+constexpr int64_t PAST_BYTES = 256ll << 20;
+
 // rows along x, sequences along y; a launch has less than 2^32 threads, and kernels loop over what is beyond
 dim3 rows_grid(int64_t units, int64_t B, int per_group, int threads, int64_t most = 1ll << 40) {
   const int64_t y = B < 65535 ? B : 65535;
@@ -658,22 +750,32 @@ TokenRows token_rows(const void* logits, int64_t B, int64_t T, int64_t V, int64_
     else if (dt == PF_F16) { CALL(PF_F16); } \
     else { CALL(PF_BF16); }                  \
   } while (0)
-// CALL(dtype, NV, ONE) with grid, block and b0 for rows of V classes: a launch has less than 2^32 threads, so many sequences go in several
-#define PF_BY_ROW(dt, V, rows, B, CALL)                                                             \
+// CALL(dtype, NV, ONE, LOOP), or OTHER where a plan for a gradient has another kernel, with grid, block and b0 for rows of V classes: a
+// launch has less than 2^32 threads, so many sequences go in several
+#define PF_ONE(DT) CALL(DT, 4, true, false)
+#define PF_SOME(DT) CALL(DT, 8, false, false)
+#define PF_LOOP(DT) CALL(DT, 8, false, true)
+#define PF_FEW(DT) CALL(DT, 4, false, false)
+#define PF_MANY(DT) CALL(DT, 16, false, false)
+#define PF_BY_ROW(dt, V, rows, B, gradient, OTHER)                                                  \
   do {                                                                                              \
-    const RowPlan plan = row_plan(dt, V);                                                           \
+    const RowPlan plan = row_plan(dt, V, gradient);                                                 \
     const dim3 block(plan.one ? 256 : 64 * plan.waves);                                             \
     const unsigned groups = (unsigned)(plan.one ? ((rows) + 3) / 4 : (rows));                       \
     int64_t most = ((1ll << 32) - 1) / ((int64_t)groups * block.x);                                 \
     if (most > 65535) most = 65535;                                                                 \
     for (int64_t b0 = 0; b0 < (B); b0 += most) {                                                    \
       const dim3 grid(groups, (unsigned)((B) - b0 < most ? (B) - b0 : most));                       \
-      if (plan.one) { PF_BY_DTYPE(dt, CALL##_ONE); }                                                \
-      else if (plan.loop) { PF_BY_DTYPE(dt, CALL##_LOOP); }                                         \
-      else if (plan.nv == 4) { PF_BY_DTYPE(dt, CALL##_FEW); }                                       \
-      else { PF_BY_DTYPE(dt, CALL##_MANY); }                                                        \
+      if (plan.one) { PF_BY_DTYPE(dt, PF_ONE); }                                                    \
+      else if (plan.loop) { PF_BY_DTYPE(dt, PF_LOOP); }                                             \
+      else if (plan.nv == 8) { PF_BY_DTYPE(dt, PF_SOME); }                                          \
+      OTHER(dt)                                                                                     \
     }                                                                                               \
   } while (0)
+#define PF_NO_OTHER(dt)
+#define PF_FEW_OR_MANY(dt)                                                                          \
+  else if (plan.nv == 4) { PF_BY_DTYPE(dt, PF_FEW); }                                               \
+  else { PF_BY_DTYPE(dt, PF_MANY); }
 
 extern "C" int pf_token_logprob_fwd(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, int64_t sb, int64_t st, const int64_t* labels,
                                     int shift, int64_t ignore_index, double temperature, float* logprobs, float* stats, void* stream) {
@@ -682,11 +784,7 @@ extern "C" int pf_token_logprob_fwd(const void* logits, int dtype, int64_t B, in
   PF_REQUIRE(logprobs, "pf_token_logprob_fwd: null pointer");
   const TokenRows r = token_rows(logits, B, T, V, sb, st, labels, shift, ignore_index, temperature);
 #define CALL(DT, NV, ONE, LOOP) hipLaunchKernelGGL((token_logprob_kernel<DT, NV, ONE, LOOP, float>), grid, block, 0, (hipStream_t)stream, r, (int)b0, logprobs, (float2*)stats)
-#define CALL_ONE(DT) CALL(DT, 4, true, false)
-#define CALL_FEW(DT) CALL(DT, 4, false, false)
-#define CALL_MANY(DT) CALL(DT, 16, false, false)
-#define CALL_LOOP(DT) CALL(DT, 8, false, true)
-  PF_BY_ROW(dtype, V, T - shift, B, CALL);
+  PF_BY_ROW(dtype, V, T - shift, B, false, PF_NO_OTHER);
 #undef CALL
   PF_CHECK_LAUNCH("pf_token_logprob_fwd");
   return PF_OK;
@@ -705,9 +803,12 @@ extern "C" int pf_token_logprob_bwd(const void* logits, int dtype, int64_t B, in
   const int64_t full = V / (dtype == PF_F32 ? 4 : 8), pieces = full > 64 * GNV ? (full + 64 * GNV - 1) / (64 * GNV) : 1;
   // (with unless_one most calls have nothing to do: few workgroups, that loop where there is something)
   const dim3 grid = rows_grid(T * pieces, B, 4, 256, unless_one ? 2048 : 1ll << 40);
-#define CALL(DT)                                                                                                                                 \
-  hipLaunchKernelGGL(token_gradient_kernel<DT>, grid, dim3(256), 0, (hipStream_t)stream, r, d, (const float2*)stats, coef, g_sb, g_st, scale, unless_one, \
-                     (unsigned)pieces)
+  const bool past = B * T * V * pf_dtype_size(dtype) >= PAST_BYTES;
+#define CALL(DT)                                                                                                                                       \
+  if (past) hipLaunchKernelGGL((token_gradient_kernel<DT, true>), grid, dim3(256), 0, (hipStream_t)stream, r, d, (const float2*)stats, coef, g_sb, g_st, scale, \
+                               unless_one, (unsigned)pieces);                                                                                            \
+  else hipLaunchKernelGGL((token_gradient_kernel<DT, false>), grid, dim3(256), 0, (hipStream_t)stream, r, d, (const float2*)stats, coef, g_sb, g_st, scale, \
+                          unless_one, (unsigned)pieces)
   PF_BY_DTYPE(dtype, CALL);
 #undef CALL
   PF_CHECK_LAUNCH("pf_token_logprob_bwd");
@@ -728,12 +829,17 @@ extern "C" int pf_preference_loss(const void* logits, int dtype, int64_t B, int6
   if (R > 0) {
     const TokenRows r = token_rows(logits, B, T, V, sb, st, labels, shift, ignore_index, 1.0);
 #define CALL(DT, NV, ONE, LOOP) hipLaunchKernelGGL((token_logprob_kernel<DT, NV, ONE, LOOP, double>), grid, block, 0, (hipStream_t)stream, r, (int)b0, logprobs, (float2*)stats)
-    PF_BY_ROW(dtype, V, R, B, CALL);
+    PF_BY_ROW(dtype, V, R, B, false, PF_NO_OTHER);
 #undef CALL
   }
-  hipLaunchKernelGGL(preference_pair_kernel, dim3((unsigned)(pairs < 65536 ? pairs : 65536)), dim3(512), 0, (hipStream_t)stream, logprobs, labels, R + shift, shift, ignore_index, ref,
-                     beta, label_smoothing, length_average, pairs, rewards, coef, workspace);
-  hipLaunchKernelGGL(sums_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, workspace, pairs, 1.0 / (double)pairs, loss, (float*)nullptr);
+  const PairArgs a = {logprobs, labels, R + shift, shift, ignore_index, ref, beta, label_smoothing, length_average, pairs, rewards, coef};
+  // one workgroup reads some 50 KB a microsecond: beyond that what a second launch costs is less ([4, 2047] 5.2 us against 6.1 + 4.6)
+  if (B <= FEW_SEQUENCES && B * R <= 32768) {
+    hipLaunchKernelGGL(preference_few_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, a, loss);
+  } else {
+    hipLaunchKernelGGL(preference_pair_kernel, dim3((unsigned)(pairs < 65536 ? pairs : 65536)), dim3(512), 0, (hipStream_t)stream, a, workspace);
+    hipLaunchKernelGGL(sums_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, workspace, pairs, 1.0 / (double)pairs, loss, (float*)nullptr);
+  }
   PF_CHECK_LAUNCH("pf_preference_loss");
   return PF_OK;
 }
@@ -760,9 +866,12 @@ extern "C" int pf_policy_loss(const void* logits, int dtype, int64_t B, int64_t 
   double* terms = workspace ? workspace + B : nullptr;
   if (B * T > 0 && (R > 0 || dlogits)) {
     if (R > 0) hipLaunchKernelGGL(token_weights_kernel, dim3(1), dim3(1024), 0, s, r, by_sequence, workspace);
-#define CALL(DT, NV, ONE, LOOP) \
-  hipLaunchKernelGGL((policy_kernel<DT, NV, ONE, LOOP>), grid, block, 0, s, r, (int)b0, d, a, workspace, logprobs, (float2*)stats, coef, terms)
-    PF_BY_ROW(dtype, V, dlogits ? T : R, B, CALL);
+    const int64_t es = pf_dtype_size(dtype);
+    const bool past = dlogits && B * T * V * es >= PAST_BYTES && pf_aligned(dlogits, 128) && V * es % 128 == 0 && d_sb * es % 128 == 0 && d_st * es % 128 == 0;
+#define CALL(DT, NV, ONE, LOOP)                                                                                                                     \
+  if (past) hipLaunchKernelGGL((policy_kernel<DT, NV, ONE, LOOP, true>), grid, block, 0, s, r, (int)b0, d, a, workspace, logprobs, (float2*)stats, coef, terms); \
+  else hipLaunchKernelGGL((policy_kernel<DT, NV, ONE, LOOP, false>), grid, block, 0, s, r, (int)b0, d, a, workspace, logprobs, (float2*)stats, coef, terms)
+    PF_BY_ROW(dtype, V, dlogits ? T : R, B, dlogits != nullptr, PF_FEW_OR_MANY);
 #undef CALL
   }
   hipLaunchKernelGGL(sums_kernel, dim3(1), dim3(1024), 0, s, terms, B * R, 1.0, loss, kl);

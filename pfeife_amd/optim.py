@@ -43,7 +43,7 @@ class AdamW8bit(torch.optim.Optimizer):
         st = self.state[p]
         if len(st) == 0:
             n = p.numel()
-            st["step"] = torch.tensor(0.0, dtype=torch.float32)
+            st["step"] = 0
             if n < max(1, group["min_8bit_size"]):
                 st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
                 st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
@@ -144,9 +144,5 @@ class AdamW8bit(torch.optim.Optimizer):
         kernels.adam8_step(*table, float(group["lr"]), float(b1), float(b2), float(group["eps"]), float(group["weight_decay"]), step,
                            scaler_state, stream)
         if scaler_state is None:
-            steps = [st["step"] for st in states]
-            if all(map(torch.is_tensor, steps)):
-                torch._foreach_add_(steps, 1)
-            else:
-                for st in states:
-                    st["step"] += 1
+            for st in states:      # (a number: adding one to a hundred tensors takes longer than the launch)
+                st["step"] = step

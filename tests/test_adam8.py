@@ -50,6 +50,7 @@ def test_loading_keeps_the_codes_types():
     st["exp_avg_scale"].fill_(0.5)
     other = AdamW8bit([q])
     other.load_state_dict(opt.state_dict())
-    for key, t in st.items():
+    assert other.state[q]["step"] == 0
+    for key, t in ((k, t) for k, t in st.items() if k != "step"):
         mine = other.state[q][key]
-        assert mine.dtype == t.dtype and torch.equal(mine.float(), t.float()) and (key == "step" or mine.data_ptr() != t.data_ptr()), key
+        assert mine.dtype == t.dtype and torch.equal(mine.float(), t.float()) and mine.data_ptr() != t.data_ptr(), key
