@@ -37,8 +37,7 @@ __device__ __forceinline__ LabelKind label_kind(const TokenRows& r, int64_t y) {
 }
 
 // ---- a row's sum of exponentials --------------------------------------------------------------------------------------------
-// A row is read once, 16 bytes to a lane and access at whatever alignment it has, NV accesses of a lane in flight; the row stays in the
-// registers that it was loaded to, so that a gradient of the same pass is formed from there.  Each lane sums 2^(x c - ref) against a
+// A row is read once, 16 bytes to a lane and access, NV accesses of a lane in flight; the row stays in the registers that it was loaded to, so that a gradient of the same pass is formed from there.  Each lane sums 2^(x c - ref) against a
 // reference of its own, the whole number from its largest x c on: no exchange between lanes before the end, and one FMA and one exponential
 // to an element.  Sums of eight go into a double.  What such arithmetic cannot do (a row of nothing but the lowest values, where
 // x c overflows, infinities, NaN) shows as a sum that is not a positive number, and is done again as (x - m) c.
@@ -319,8 +318,12 @@ __device__ __forceinline__ void gradient_vector(raw4 w, int label, const RowStat
   unpack<DT>(w, x);
 #pragma unroll
   for (int e = 0; e < VE<DT>; ++e) x[e] = g.scaled * power<SLOW>(x[e], s, c);
+  if ((unsigned)label < (unsigned)VE<DT>) {
+    asm volatile("" : "+v"(label));      // (compared here and not ahead for every vector of a tile)
+#pragma unroll
+    for (int e = 0; e < VE<DT>; ++e) x[e] = e == label ? g.at_label : x[e];
+  }
   store_vector<PAST>(dx, pack<DT>(x));
-  if ((unsigned)label < (unsigned)VE<DT>) Codec<DT>::store(dx, label, g.at_label);      // (the same lane, behind its vector)
 }
 template <int DT>
 __device__ __forceinline__ void gradient_element(float x, int j, int y, const RowStats& s, const RowGrad& g, float c, char* dx) {
@@ -338,17 +341,17 @@ __device__ __forceinline__ void fill_row(char* dx, int V, float value, int tid, 
   if (tid < cut.loose) Codec<DT>::store(dx, cut.element(tid), value);
 }
 
-// The row of a workgroup or, with ONE, of a wavefront (four to a workgroup): sequence b, place t (uniform)
-template <bool ONE> __device__ __forceinline__ int row_of_group() {
-  return ONE ? (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : (int)blockIdx.x;
+// The place of a workgroup's row in its sequence or, with ONE, of a wavefront's (four to a workgroup), uniform; the sequence is b0 + blockIdx.y
+template <bool ONE> __device__ __forceinline__ int row_of_group(int t0) {
+  return t0 + (ONE ? (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : (int)blockIdx.x);
 }
 
 // stats[row] = {reference, 1 / sum}; for rows that take no part {0, 0}
 template <int DT, int NV, bool ONE, bool LOOP, typename Out>
-__global__ __launch_bounds__(ONE ? 256 : 1024) void token_logprob_kernel(const TokenRows r, int b0, Out* logprobs, float2* stats) {
+__global__ __launch_bounds__(ONE ? 256 : 1024) void token_logprob_kernel(const TokenRows r, int b0, int t0, Out* logprobs, float2* stats) {
   constexpr bool FIRST = sizeof(Out) == 8;
   __shared__ SumSlots<FIRST> slots[1];
-  const int R = (int)r.T - r.shift, t = row_of_group<ONE>();
+  const int R = (int)r.T - r.shift, t = row_of_group<ONE>(t0);
   const int64_t b = b0 + (int)blockIdx.y;
   if (t >= R) return;
   const int64_t y = r.labels[b * r.T + t + r.shift], at = b * R + t;
@@ -507,7 +510,7 @@ __global__ __launch_bounds__(512) void preference_pair_kernel(const PairArgs a, 
 }
 
 // All pairs by one workgroup, and their mean: the wavefronts share the sequences, a lane each takes a pair.
-constexpr int FEW_SEQUENCES = 64;
+constexpr int FEW_SEQUENCES = 32;
 __global__ __launch_bounds__(1024) void preference_few_kernel(const PairArgs a, float* loss) {
   __shared__ double sums[FEW_SEQUENCES][16], counts[FEW_SEQUENCES][16];
   const int B = 2 * (int)a.pairs, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -632,10 +635,10 @@ __device__ __forceinline__ TokenTerms policy_token(const PolicyArgs& a, float ol
 
 // A row's log-probability, its part of the loss and, where wanted, its gradient.  terms: [2][B * R], weighted
 template <int DT, int NV, bool ONE, bool LOOP, bool PAST>
-__global__ __launch_bounds__(ONE ? 256 : 1024) void policy_kernel(const TokenRows r, int b0, const GradRows d, const PolicyArgs a, const double* weights,
+__global__ __launch_bounds__(ONE ? 256 : 1024) void policy_kernel(const TokenRows r, int b0, int t0, const GradRows d, const PolicyArgs a, const double* weights,
                                                                   float* logprobs, float2* stats, float* coef, double* terms) {
   __shared__ SumSlots<false> slots[1];
-  const int T = (int)r.T, R = T - r.shift, t = row_of_group<ONE>();
+  const int T = (int)r.T, R = T - r.shift, t = row_of_group<ONE>(t0);
   const int64_t b = b0 + (int)blockIdx.y, at = b * R + t;
   if (t >= T) return;
   const int tid = ONE ? threadIdx.x & 63 : threadIdx.x, n = ONE ? 64 : blockDim.x;
@@ -731,7 +734,7 @@ int check_rows(const char* who, const void* logits, int dtype, int64_t B, int64_
   PF_REQUIRE(shift == 0 || shift == 1, "%s: shift is 0 or 1", who);
   PF_REQUIRE(temperature > 0.0 && temperature >= 1e-6 && temperature <= 1e6, "%s: temperature must lie in [1e-6, 1e6]", who);
   PF_REQUIRE(B * T == 0 || (logits && labels), "%s: null pointer", who);
-  PF_REQUIRE(T <= (1ll << 21) && B < (1ll << 31), "%s: too many rows", who);
+  PF_REQUIRE(T <= (1ll << 30) && B < (1ll << 31), "%s: too many rows", who);
   PF_REQUIRE(V <= (1ll << 28), "%s: too many classes", who);
   return PF_OK;
 }
@@ -750,26 +753,30 @@ TokenRows token_rows(const void* logits, int64_t B, int64_t T, int64_t V, int64_
     else if (dt == PF_F16) { CALL(PF_F16); } \
     else { CALL(PF_BF16); }                  \
   } while (0)
-// CALL(dtype, NV, ONE, LOOP), or OTHER where a plan for a gradient has another kernel, with grid, block and b0 for rows of V classes: a
-// launch has less than 2^32 threads, so many sequences go in several
+// CALL(dtype, NV, ONE, LOOP), or OTHER where a plan for a gradient has another kernel, with grid, block, b0 and t0 for rows of V classes: a
+// launch has less than 2^32 threads, so many rows or sequences go in several
 #define PF_ONE(DT) CALL(DT, 4, true, false)
 #define PF_SOME(DT) CALL(DT, 8, false, false)
 #define PF_LOOP(DT) CALL(DT, 8, false, true)
 #define PF_FEW(DT) CALL(DT, 4, false, false)
 #define PF_MANY(DT) CALL(DT, 16, false, false)
+constexpr int64_t ROWS_MOST = 1 << 20;
 #define PF_BY_ROW(dt, V, rows, B, gradient, OTHER)                                                  \
   do {                                                                                              \
     const RowPlan plan = row_plan(dt, V, gradient);                                                 \
     const dim3 block(plan.one ? 256 : 64 * plan.waves);                                             \
-    const unsigned groups = (unsigned)(plan.one ? ((rows) + 3) / 4 : (rows));                       \
-    int64_t most = ((1ll << 32) - 1) / ((int64_t)groups * block.x);                                 \
-    if (most > 65535) most = 65535;                                                                 \
-    for (int64_t b0 = 0; b0 < (B); b0 += most) {                                                    \
-      const dim3 grid(groups, (unsigned)((B) - b0 < most ? (B) - b0 : most));                       \
-      if (plan.one) { PF_BY_DTYPE(dt, PF_ONE); }                                                    \
-      else if (plan.loop) { PF_BY_DTYPE(dt, PF_LOOP); }                                             \
-      else if (plan.nv == 8) { PF_BY_DTYPE(dt, PF_SOME); }                                          \
-      OTHER(dt)                                                                                     \
+    for (int64_t t0 = 0; t0 < (rows); t0 += ROWS_MOST) {                                            \
+      const int64_t here = (rows) - t0 < ROWS_MOST ? (rows) - t0 : ROWS_MOST;                       \
+      const unsigned groups = (unsigned)(plan.one ? (here + 3) / 4 : here);                         \
+      int64_t most = ((1ll << 32) - 1) / ((int64_t)groups * block.x);                               \
+      if (most > 65535) most = 65535;                                                               \
+      for (int64_t b0 = 0; b0 < (B); b0 += most) {                                                  \
+        const dim3 grid(groups, (unsigned)((B) - b0 < most ? (B) - b0 : most));                     \
+        if (plan.one) { PF_BY_DTYPE(dt, PF_ONE); }                                                  \
+        else if (plan.loop) { PF_BY_DTYPE(dt, PF_LOOP); }                                           \
+        else if (plan.nv == 8) { PF_BY_DTYPE(dt, PF_SOME); }                                        \
+        OTHER(dt)                                                                                   \
+      }                                                                                             \
     }                                                                                               \
   } while (0)
 #define PF_NO_OTHER(dt)
@@ -783,7 +790,7 @@ extern "C" int pf_token_logprob_fwd(const void* logits, int dtype, int64_t B, in
   if (B == 0 || T <= shift) return PF_OK;
   PF_REQUIRE(logprobs, "pf_token_logprob_fwd: null pointer");
   const TokenRows r = token_rows(logits, B, T, V, sb, st, labels, shift, ignore_index, temperature);
-#define CALL(DT, NV, ONE, LOOP) hipLaunchKernelGGL((token_logprob_kernel<DT, NV, ONE, LOOP, float>), grid, block, 0, (hipStream_t)stream, r, (int)b0, logprobs, (float2*)stats)
+#define CALL(DT, NV, ONE, LOOP) hipLaunchKernelGGL((token_logprob_kernel<DT, NV, ONE, LOOP, float>), grid, block, 0, (hipStream_t)stream, r, (int)b0, (int)t0, logprobs, (float2*)stats)
   PF_BY_ROW(dtype, V, T - shift, B, false, PF_NO_OTHER);
 #undef CALL
   PF_CHECK_LAUNCH("pf_token_logprob_fwd");
@@ -828,13 +835,14 @@ extern "C" int pf_preference_loss(const void* logits, int dtype, int64_t B, int6
   double* logprobs = workspace + pairs;
   if (R > 0) {
     const TokenRows r = token_rows(logits, B, T, V, sb, st, labels, shift, ignore_index, 1.0);
-#define CALL(DT, NV, ONE, LOOP) hipLaunchKernelGGL((token_logprob_kernel<DT, NV, ONE, LOOP, double>), grid, block, 0, (hipStream_t)stream, r, (int)b0, logprobs, (float2*)stats)
+#define CALL(DT, NV, ONE, LOOP) hipLaunchKernelGGL((token_logprob_kernel<DT, NV, ONE, LOOP, double>), grid, block, 0, (hipStream_t)stream, r, (int)b0, (int)t0, logprobs, (float2*)stats)
     PF_BY_ROW(dtype, V, R, B, false, PF_NO_OTHER);
 #undef CALL
   }
   const PairArgs a = {logprobs, labels, R + shift, shift, ignore_index, ref, beta, label_smoothing, length_average, pairs, rewards, coef};
-  // one workgroup reads some 50 KB a microsecond: beyond that what a second launch costs is less ([4, 2047] 5.2 us against 6.1 + 4.6)
-  if (B <= FEW_SEQUENCES && B * R <= 32768) {
+  // one workgroup saves a launch and reads less at a time: us of it / of the two, [2, 128] 4.3 / 6.1, [4, 2047] 5.5 / 6.9, [16, 1024] 7.1 / 7.9,
+  // [32, 1024] 10.8 / 10.2, [64, 2048] 32 / 19
+  if (B <= FEW_SEQUENCES && B * R <= 16384) {
     hipLaunchKernelGGL(preference_few_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, a, loss);
   } else {
     hipLaunchKernelGGL(preference_pair_kernel, dim3((unsigned)(pairs < 65536 ? pairs : 65536)), dim3(512), 0, (hipStream_t)stream, a, workspace);
@@ -869,8 +877,8 @@ extern "C" int pf_policy_loss(const void* logits, int dtype, int64_t B, int64_t 
     const int64_t es = pf_dtype_size(dtype);
     const bool past = dlogits && B * T * V * es >= PAST_BYTES && pf_aligned(dlogits, 128) && V * es % 128 == 0 && d_sb * es % 128 == 0 && d_st * es % 128 == 0;
 #define CALL(DT, NV, ONE, LOOP)                                                                                                                     \
-  if (past) hipLaunchKernelGGL((policy_kernel<DT, NV, ONE, LOOP, true>), grid, block, 0, s, r, (int)b0, d, a, workspace, logprobs, (float2*)stats, coef, terms); \
-  else hipLaunchKernelGGL((policy_kernel<DT, NV, ONE, LOOP, false>), grid, block, 0, s, r, (int)b0, d, a, workspace, logprobs, (float2*)stats, coef, terms)
+  if (past) hipLaunchKernelGGL((policy_kernel<DT, NV, ONE, LOOP, true>), grid, block, 0, s, r, (int)b0, (int)t0, d, a, workspace, logprobs, (float2*)stats, coef, terms); \
+  else hipLaunchKernelGGL((policy_kernel<DT, NV, ONE, LOOP, false>), grid, block, 0, s, r, (int)b0, (int)t0, d, a, workspace, logprobs, (float2*)stats, coef, terms)
     PF_BY_ROW(dtype, V, dlogits ? T : R, B, dlogits != nullptr, PF_FEW_OR_MANY);
 #undef CALL
   }

@@ -180,6 +180,24 @@ def _as_scale(g):
     return g if g.dtype == torch.float32 else g.to(torch.float32)
 
 
+class _NoContext:
+    """Stands for autograd's where no gradient is asked for: its bookkeeping takes longer than a small call."""
+
+    @staticmethod
+    def mark_non_differentiable(*_):
+        pass
+
+    @staticmethod
+    def set_materialize_grads(_):
+        pass
+
+
+def _apply(fn, logits, *args):
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return fn.apply(logits, *args, True)
+    return fn.forward(_NoContext, logits, *args, False)
+
+
 class _TokenLogprobFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, cfg, want):
@@ -280,8 +298,8 @@ def token_logprobs(logits, labels, *, ignore_index=-100, temperature=1.0, shift=
     their logits hold; labels outside the vocabulary give NaN."""
     x, y = _check_rows("token_logprobs", logits, labels, ignore_index, temperature, shift)
     cfg = (int(shift), ignore_index, float(temperature))
-    out = _TokenLogprobFn.apply(x, y, cfg, torch.is_grad_enabled() and x.requires_grad)
-    return out.reshape(logits.shape[:-2] + out.shape[1:])
+    out = _apply(_TokenLogprobFn, x, y, cfg)
+    return out if logits.dim() == 3 else out.reshape(logits.shape[:-2] + out.shape[1:])
 
 
 def preference_loss(logits, labels, ref_logprobs, *, beta=0.1, label_smoothing=0.0, length_average=False, ignore_index=-100, shift=False):
@@ -289,7 +307,7 @@ def preference_loss(logits, labels, ref_logprobs, *, beta=0.1, label_smoothing=0
 
     logits [2P, T, V], labels int64 [2P, T]: sequences 2i (preferred) and 2i + 1 (rejected) are a pair, so that a batch split into
     micro-batches of whole pairs keeps them together.  ref_logprobs [2P]: the sum (length_average: the mean) of the answer's
-    token log-probabilities under the reference model.  With s the same of this model, rewards = beta (s - ref) and D the preferred
+    token log-probabilities under the reference model (of no token: 0).  With s the same of this model, rewards = beta (s - ref) and D the preferred
     minus the rejected reward, loss = mean of -(1 - label_smoothing) log sigmoid(D) - label_smoothing log sigmoid(-D).  The
     gradient flows to the logits; `rewards` [2P] are for the log.  `shift` and `ignore_index` as for `token_logprobs`."""
     who = "preference_loss"
@@ -300,8 +318,7 @@ def preference_loss(logits, labels, ref_logprobs, *, beta=0.1, label_smoothing=0
     if not math.isfinite(beta) or not 0.0 <= label_smoothing <= 1.0:
         raise RuntimeError("%s: beta must be finite and label_smoothing lie in [0, 1]" % who)
     ref = _constant(who, "ref_logprobs", ref_logprobs, [(B,)], logits).contiguous()
-    return _PreferenceFn.apply(x, y, ref, (int(shift), ignore_index, 1.0), float(beta), float(label_smoothing), bool(length_average),
-                               torch.is_grad_enabled() and x.requires_grad)
+    return _apply(_PreferenceFn, x, y, ref, (int(shift), ignore_index, 1.0), float(beta), float(label_smoothing), bool(length_average))
 
 
 def policy_loss(logits, labels, old_logprobs, advantages, ref_logprobs=None, *, clip=0.2, clip_high=None, kl_coef=0.0, temperature=1.0,
@@ -314,7 +331,8 @@ def policy_loss(logits, labels, old_logprobs, advantages, ref_logprobs=None, *, 
     logprob) - 1); clip_high defaults to clip.  reduction "tokens": the mean over all tokens that count; "sequences": the mean over
     the sequences that have such tokens of their means; with none at all the loss is 0.  The gradient flows to the logits alone;
     `logprobs` [B, T'] and `kl` (the KL term's mean) are for the log.  `ignore_index`, `shift` and `temperature` as for
-    `token_logprobs`; what the other operands hold at ignored tokens does not matter."""
+    `token_logprobs`; what the other operands hold at ignored tokens does not matter.  A backward pass captured into a graph of its own is
+    replayed once for every replay of the forward pass's graph."""
     who = "policy_loss"
     x, y = _check_rows(who, logits, labels, ignore_index, temperature, shift)
     if logits.dim() != 3:
@@ -332,8 +350,8 @@ def policy_loss(logits, labels, old_logprobs, advantages, ref_logprobs=None, *, 
     adv = _constant(who, "advantages", advantages, [(B,), (B, 1), (B, R)], logits)
     ref = None if ref_logprobs is None else _constant(who, "ref_logprobs", ref_logprobs, [(B, R)], logits).contiguous()
     a_strides = (adv.stride(0), adv.stride(1) if adv.dim() == 2 and adv.shape[1] > 1 else 0)
-    return _PolicyFn.apply(x, y, old, adv, a_strides, ref, (int(shift), ignore_index, float(temperature)), (float(clip), float(clip_high)),
-                           float(kl_coef), reduction == "sequences", torch.is_grad_enabled() and x.requires_grad)
+    return _apply(_PolicyFn, x, y, old, adv, a_strides, ref, (int(shift), ignore_index, float(temperature)), (float(clip), float(clip_high)),
+                  float(kl_coef), reduction == "sequences")
 
 
 class LossWrapper(nn.Module):

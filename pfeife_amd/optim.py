@@ -29,6 +29,7 @@ class AdamW8bit(torch.optim.Optimizer):
         super().add_param_group(param_group)
         for p in self.param_groups[-1]["params"]:
             if p.dtype != torch.float32:
+                self.param_groups.pop()
                 raise RuntimeError("AdamW8bit: parameters are fp32 (got %s)" % p.dtype)
 
     def load_state_dict(self, state_dict):
@@ -44,7 +45,7 @@ class AdamW8bit(torch.optim.Optimizer):
         if len(st) == 0:
             n = p.numel()
             st["step"] = 0
-            if n < max(1, group["min_8bit_size"]):
+            if n < max(1, group.get("min_8bit_size", self.defaults["min_8bit_size"])):
                 st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
                 st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
             else:
