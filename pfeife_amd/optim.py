@@ -84,14 +84,18 @@ class AdamW8bit(torch.optim.Optimizer):
     def _prepare(self, kernels):
         """[(group, states, device, table, copies)] of what has a gradient, parameters at one step count together, and whether a table
         is new.  A table holds addresses: it is made again when one of them is another, or the stream is.  Reads no gradient."""
+        seen = self.__dict__.get("_seen")
+        if seen is not None and self._as_seen(*seen[0]):
+            return seen[1], False
         cache = self.__dict__.setdefault("_tables", {})
-        work, fresh, place = [], False, 0
+        work, fresh, place, records, plain = [], False, 0, [], True
         for gi, group in enumerate(self.param_groups):
             by_step = {}
             for p in group["params"]:
                 place += 1
                 g = p.grad
                 if g is None or p.numel() == 0:
+                    records.append((p, None))
                     continue
                 st = self._init_state(p, group)
                 key = (float(st["step"]), p.get_device())
@@ -102,6 +106,9 @@ class AdamW8bit(torch.optim.Optimizer):
                 found[0].append(st)
                 found[1].append((p, g, ops, place - 1))
                 found[2].append((place, *[t if t is None else (t.data_ptr(), t.dtype, t.numel()) for t in (p, g, *ops)], g.stride(), p.stride()))
+                keys = ("exp_avg", "exp_avg_scale", "exp_avg_sq_root", "exp_avg_sq_root_scale") if ops[1] is not None else ("exp_avg", "exp_avg_sq")
+                records.append((p, st, found[0], p.data_ptr(), p.numel(), g.data_ptr(), [(k, st[k], st[k].data_ptr(), st[k].numel()) for k in keys]))
+                plain = plain and p.is_contiguous() and g.is_contiguous()
             for n, key in enumerate(sorted(by_step)):
                 states, params, now = by_step[key]
                 now.append(_raw_stream(key[1]) if key[1] >= 0 else None)
@@ -109,10 +116,39 @@ class AdamW8bit(torch.optim.Optimizer):
                 if ent is None or ent[0] != now:
                     fresh = True
                     items = [(p.data, self._check(p, g, ops), *ops, index) for p, g, ops, index in params]
-                    copies = [(i[1], g) for (_, g, _, _), i in zip(params, items) if i[1] is not g]
+                    copies = [(i[1], p) for (p, g, _, _), i in zip(params, items) if i[1] is not g]
                     ent = cache[gi, n] = (now, kernels.adam8_table(items), copies)
                 work.append((group, states, params[0][0].device, *ent[1:]))
+        devices = {w[2].index for w in work}
+        # (one device, dense tensors: what _as_seen looks at says that all is as it was)
+        self._seen = ((records, [len(g["params"]) for g in self.param_groups], devices.pop(), work and _raw_stream(work[0][2].index)), work) \
+            if plain and len(devices) == 1 else None
         return work, fresh
+
+    def _as_seen(self, records, counts, device, stream):
+        """Is every address where the last step's tables have it, and every count of steps still its group's?"""
+        if len(counts) != len(self.param_groups) or any(len(g["params"]) != n for g, n in zip(self.param_groups, counts)) or _raw_stream(device) != stream:
+            return False
+        at = iter(records)
+        state = self.state
+        for group in self.param_groups:
+            for p in group["params"]:
+                r = next(at)
+                g = p.grad
+                if r[0] is not p:
+                    return False
+                if r[1] is None:
+                    if g is not None and p.numel():
+                        return False
+                    continue
+                st = r[1]
+                if (g is None or state.get(p) is not st or st["step"] != r[2][0]["step"] or p.data_ptr() != r[3] or p.numel() != r[4]
+                        or g.data_ptr() != r[5] or not p.is_contiguous() or not g.is_contiguous()):
+                    return False
+                for key, t, where, n in r[6]:
+                    if st.get(key) is not t or t.data_ptr() != where or t.numel() != n:
+                        return False
+        return True
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -138,8 +174,8 @@ class AdamW8bit(torch.optim.Optimizer):
     def _launch(kernels, group, states, table, copies, stream, scaler_state=None):
         """One launch, on the current stream; with a loss scaler's state the count of steps is the device's, and the states' entries are not
         touched."""
-        for mine, g in copies:
-            mine.copy_(g)
+        for mine, p in copies:
+            mine.copy_(p.grad)
         b1, b2 = group["betas"]
         step = int(states[0]["step"]) + 1
         kernels.adam8_step(*table, float(group["lr"]), float(b1), float(b2), float(group["eps"]), float(group["weight_decay"]), step,

@@ -274,3 +274,67 @@ def test_many_tensors_in_two_groups():
         moved = old * (1 - lr * 1e-2) ** 2 - p.detach()
         assert ((moved - 2 * lr).abs() <= 2 * lr * 0.13 + 4 * 2.0 ** -24 * old.abs()).all(), k
         assert ("exp_avg_scale" in opt.state[p]) == (k >= 70 or p.numel() >= 4096)
+
+
+def test_what_changes_between_steps_is_seen():
+    """Gradients that come and go or move, state that is replaced, a parameter that is given other memory, a group that is added, another
+    stream: always the step that an optimizer made anew from the same state takes."""
+    from pfeife_amd.optim import AdamW8bit
+
+    g = torch.Generator().manual_seed(6)
+    params = [torch.nn.Parameter(torch.randn(n, generator=g).cuda()) for n in (5000, 300, 9000)]
+    opt = AdamW8bit(params, lr=LR)
+    side = torch.cuda.Stream()
+    late = torch.nn.Parameter(torch.randn(6000, generator=g).cuda())
+
+    def both(stream=None):
+        torch.cuda.synchronize()
+        twins = [[torch.nn.Parameter(p.detach().clone()) for p in grp["params"]] for grp in opt.param_groups]
+        other = AdamW8bit([{"params": t} for t in twins], lr=LR)
+        other.load_state_dict(opt.state_dict())
+        for grp, t in zip(opt.param_groups, twins):
+            for p, q in zip(grp["params"], t):
+                q.grad = None if p.grad is None else p.grad.clone()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            opt.step()
+        torch.cuda.synchronize()
+        other.step()
+        for grp, t in zip(opt.param_groups, twins):
+            for p, q in zip(grp["params"], t):
+                assert torch.equal(p, q)
+                for key, v in opt.state.get(p, {}).items():
+                    w = other.state[q][key]
+                    assert torch.equal(raw(v), raw(w)) if torch.is_tensor(v) and torch.is_tensor(w) else float(v) == float(w), key
+
+    rnd = lambda p: torch.randn(p.shape, generator=g).cuda()  # noqa: E731
+    for p in params:
+        p.grad = rnd(p)
+    both()
+    both()
+    params[0].grad.mul_(0.5)
+    both()
+    params[1].grad = None
+    both()
+    params[1].grad = rnd(params[1])      # one step behind the others from here on
+    both()
+    both()
+    params[2].grad = rnd(params[2])
+    both()
+    opt.state[params[0]]["exp_avg"] = opt.state[params[0]]["exp_avg"].clone()
+    both()
+    params[2].data = rnd(params[2])
+    both()
+    both(side)
+    both(side)
+    both()
+    opt.add_param_group({"params": [late]})
+    both()
+    late.grad = rnd(late)
+    both()
+    both()
+    late.grad = rnd(late).view(2, 3000).t().reshape(-1)[:6000].view(3000, 2).t().reshape(-1)
+    both()
+    opt.load_state_dict(copy.deepcopy(opt.state_dict()))
+    both()
+    both()
