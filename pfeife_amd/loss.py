@@ -99,6 +99,9 @@ _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_get
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _table(t, who):
     """The kernel table of the tensor's own device."""
     k = _tables.get(t.get_device())
@@ -115,7 +118,7 @@ def _table(t, who):
 def _issue(t, launch):
     """On the current stream of the tensor's device, whichever device is the current one."""
     index = t.get_device()
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         launch(_raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -194,13 +197,24 @@ class _NoContext:
 
 def _apply(fn, logits, *args):
     if torch.is_grad_enabled() and logits.requires_grad:
-        return fn.apply(logits, *args, True)
-    return fn.forward(_NoContext, logits, *args, False)
+        return fn.apply(logits, args)
+    return fn.forward(_NoContext, logits, args, False)
+
+
+def _once(backward):
+    """torch.autograd.function.once_differentiable where it matters: a backward pass that keeps no graph does not pay for it."""
+    wrapped = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (wrapped if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return staticmethod(run)
 
 
 class _TokenLogprobFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, labels, cfg, want):
+    def forward(ctx, logits, args, want=True):
+        labels, cfg = args
         B, T, _ = logits.shape
         out = _new(logits, B, max(0, T - cfg[0]))
         stats = _new(logits, *out.shape, 2) if want else None
@@ -210,17 +224,17 @@ class _TokenLogprobFn(torch.autograd.Function):
             ctx.cfg = cfg
         return out
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, grad):
         logits, labels, stats = ctx.saved_tensors
         grad = _as_scale(grad)      # (any strides: a sum's gradient is one number)
-        return _logits_gradient(logits, labels, ctx.cfg, stats, grad, grad.stride()), None, None, None
+        return _logits_gradient(logits, labels, ctx.cfg, stats, grad, grad.stride()), None
 
 
 class _PreferenceFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, labels, ref, cfg, beta, smoothing, average, want):
+    def forward(ctx, logits, args, want=True):
+        labels, ref, cfg, beta, smoothing, average = args
         B, T, _ = logits.shape
         k = _table(logits, "")
         n, rows = k.preference_workspace(B, T, cfg[0]), B * max(0, T - cfg[0])
@@ -237,12 +251,11 @@ class _PreferenceFn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return loss, rewards
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, grad, _):
         logits, labels, _ = ctx.saved_tensors
         d = None if grad is None else _logits_gradient(logits, labels, ctx.cfg, *ctx.at, (1, 0), _as_scale(grad))
-        return (d,) + (None,) * 7
+        return d, None
 
 
 class _PolicyFn(torch.autograd.Function):
@@ -251,7 +264,8 @@ class _PolicyFn(torch.autograd.Function):
     by, on the device: by one it has nothing to do, by anything else it computes the gradient from the logits."""
 
     @staticmethod
-    def forward(ctx, logits, labels, old, adv, a_strides, ref, cfg, clip, kl_coef, by_sequence, want):
+    def forward(ctx, logits, args, want=True):
+        labels, old, adv, a_strides, ref, cfg, clip, kl_coef, by_sequence = args
         B, T, _ = logits.shape
         k = _table(logits, "")
         R = max(0, T - cfg[0])
@@ -276,8 +290,7 @@ class _PolicyFn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return loss, logprobs, kl
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, grad, *_):
         logits, labels, _ = ctx.saved_tensors
         d = None
@@ -287,7 +300,7 @@ class _PolicyFn(torch.autograd.Function):
             d, ctx.d = ctx.d, None
             ready = d is not None and ctx.captured == torch.cuda.is_current_stream_capturing()
             d = _logits_gradient(logits, labels, ctx.cfg, *ctx.at, _as_scale(grad), d if ready else None, int(ready))
-        return (d,) + (None,) * 10
+        return d, None
 
 
 def token_logprobs(logits, labels, *, ignore_index=-100, temperature=1.0, shift=False):

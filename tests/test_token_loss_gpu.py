@@ -537,3 +537,16 @@ def test_gradients_that_go_past_the_caches(dtype, V):
         assert (total.abs() <= size * 2 * ((V / 64 + 96) * 2.0 ** -24 + U[dtype]) + V * LEAST[dtype]).all(), name
         assert (d[~seen] == 0).all() if name == "policy" else True
         del d
+
+
+def test_a_second_derivative_is_refused():
+    from pfeife_amd.loss import policy_loss, preference_loss, token_logprobs
+
+    x = torch.randn(2, 3, 7, device="cuda", requires_grad=True)
+    y = torch.ones(2, 3, dtype=torch.int64, device="cuda")
+    zero = torch.zeros(2, device="cuda")
+    for loss in (token_logprobs(x, y).sum(), preference_loss(x, y, zero)[0], policy_loss(x, y, torch.full((2, 3), -2.0, device="cuda"), zero + 1)[0]):
+        (d,) = torch.autograd.grad(loss, x, create_graph=True)
+        assert torch.isfinite(d).all()
+        with pytest.raises(RuntimeError, match="once_differentiable|differentiate twice|does not require grad"):
+            torch.autograd.grad(d.sum(), x)
