@@ -397,7 +397,7 @@ int pf_cross_entropy_gap_bwd(const void* logits, int l_dtype, const int64_t* tar
  *                          - label_smoothing ln sigma(-D); coef[b] = d loss / d logprob of each of b's tokens and stats
  *                          (optional) are what pf_token_logprob_bwd takes (g_sb = 1, g_st = 0).  workspace:
  *                          pf_preference_workspace(B, T, shift) doubles
- *   pf_policy_loss         r = exp(logprob - old), q = ref - logprob: loss[0] = sum of w (-min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A)
+ *   pf_policy_loss         r = exp(logprob - old), q = ref - logprob: loss[0] = scale times the sum of w (-min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A)
  *                          + kl_coef k), kl[0] = sum of w k with k = exp(q) - q - 1 (ref_logprobs null: 0); old / ref fp32 [B, R],
  *                          A = advantages[b * a_sb + t * a_st].  w = 1 / (tokens that count), by_sequence != 0: 1 / (such tokens of the
  *                          sequence * sequences that have any); with no such token loss and kl are 0.  stats and coef (optional,
@@ -419,7 +419,7 @@ int64_t pf_policy_workspace(int64_t B, int64_t T, int shift);
 int pf_policy_loss(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, int64_t sb, int64_t st,
                    const int64_t* labels, int shift, int64_t ignore_index, double temperature, const float* old_logprobs,
                    const float* advantages, int64_t a_sb, int64_t a_st, const float* ref_logprobs, double clip_low,
-                   double clip_high, double kl_coef, int by_sequence, float* loss, float* kl, float* logprobs, float* stats,
+                   double clip_high, double kl_coef, int by_sequence, double scale, float* loss, float* kl, float* logprobs, float* stats,
                    float* coef, void* dlogits, int64_t d_sb, int64_t d_st, double* workspace, void* stream);
 /* Mean squared error (F.mse_loss, bench_models/models/train_sdxl.py:1422-1424):
  * loss[0] = mean((a-b)^2) computed in fp32; partial: fp32 [pf_reduce_workspace(n)]. */

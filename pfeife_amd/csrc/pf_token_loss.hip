@@ -594,6 +594,7 @@ struct PolicyArgs {
   int64_t a_sb, a_st;
   double low, high;      // ln(1 - clip_low), ln(1 + clip_high)
   float low_ratio, high_ratio, kl_coef;
+  double scale;          // of the loss
 };
 
 // One token:  -min(r A, clip(r) A) + kl_coef (e^q - q - 1)  with r = e^d, d = logprob - old, q = ref - logprob; g is its derivative by the
@@ -665,10 +666,10 @@ __global__ __launch_bounds__(ONE ? 256 : 1024) void policy_kernel(const TokenRow
   const float xy = element<DT>(row.x, (int)y);
   const RowStats s = row_stats<false>(r, row, xy, slots, true);
   const TokenTerms o = policy_token(a, old, A, ref, s.logprob);
-  const float g = (float)(w * (double)o.g);
+  const float g = (float)(w * a.scale * (double)o.g);
   if (tid == 0) {
     logprobs[at] = (float)s.logprob;
-    terms[at] = w * (double)o.loss;
+    terms[at] = w * a.scale * (double)o.loss;
     terms[r.B * R + at] = w * (double)o.kl;
     if (coef) {
       coef[at] = g;
@@ -856,7 +857,7 @@ extern "C" int64_t pf_policy_workspace(int64_t B, int64_t T, int shift) { return
 
 extern "C" int pf_policy_loss(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, int64_t sb, int64_t st, const int64_t* labels, int shift,
                               int64_t ignore_index, double temperature, const float* old_logprobs, const float* advantages, int64_t a_sb, int64_t a_st,
-                              const float* ref_logprobs, double clip_low, double clip_high, double kl_coef, int by_sequence, float* loss, float* kl,
+                              const float* ref_logprobs, double clip_low, double clip_high, double kl_coef, int by_sequence, double scale, float* loss, float* kl,
                               float* logprobs, float* stats, float* coef, void* dlogits, int64_t d_sb, int64_t d_st, double* workspace, void* stream) {
   if (int rc = check_rows("pf_policy_loss", logits, dtype, B, T, V, sb, st, labels, shift, temperature)) return rc;
   PF_REQUIRE(a_sb >= 0 && a_st >= 0 && d_sb >= 0 && d_st >= 0, "pf_policy_loss: bad strides");
@@ -869,7 +870,7 @@ extern "C" int pf_policy_loss(const void* logits, int dtype, int64_t B, int64_t 
   const TokenRows r = token_rows(logits, B, T, V, sb, st, labels, shift, ignore_index, temperature);
   const GradRows d = {dlogits, d_sb, d_st};
   const PolicyArgs a = {old_logprobs, ref_logprobs, advantages, a_sb, a_st, clip_low < 1.0 ? log1p(-clip_low) : -INFINITY, log1p(clip_high),
-                        (float)(1.0 - clip_low), (float)(1.0 + clip_high), (float)kl_coef};
+                        (float)(1.0 - clip_low), (float)(1.0 + clip_high), (float)kl_coef, scale};
   const int64_t R = T > shift ? T - shift : 0;
   double* terms = workspace ? workspace + B : nullptr;
   if (B * T > 0 && (R > 0 || dlogits)) {

@@ -135,7 +135,7 @@ _SIGNATURES = {
     "pf_token_logprob_fwd": [_P, _I, _L, _L, _L, _L, _L, _P, _I, _L, _D, _P, _P, _P],
     "pf_token_logprob_bwd": [_P, _I, _L, _L, _L, _L, _L, _P, _I, _L, _D, _P, _P, _L, _L, _P, _I, _P, _L, _L, _P],
     "pf_preference_loss": [_P, _I, _L, _L, _L, _L, _L, _P, _I, _L, _P, _D, _D, _I, _P, _P, _P, _P, _P, _P],
-    "pf_policy_loss": [_P, _I, _L, _L, _L, _L, _L, _P, _I, _L, _D, _P, _P, _L, _L, _P, _D, _D, _D, _I, _P, _P, _P, _P, _P, _P, _L, _L, _P, _P],
+    "pf_policy_loss": [_P, _I, _L, _L, _L, _L, _L, _P, _I, _L, _D, _P, _P, _L, _L, _P, _D, _D, _D, _I, _D, _P, _P, _P, _P, _P, _P, _L, _L, _P, _P],
     "pf_mse_fwd": [_P, _I, _P, _I, _P, _P, _L, _P],
     "pf_mse_bwd": [_P, _I, _P, _I, _P, _P, _I, _L, _P],
     "pf_sum_fwd": [_P, _I, _P, _P, _L, _P],
@@ -667,9 +667,9 @@ class HipKernels:
     def policy_workspace(self, B, T, shift):
         return int(self.lib.pf_policy_workspace(B, T, int(shift)))
 
-    def policy_loss(self, rows, old, adv, a_strides, ref, clip_low, clip_high, kl_coef, by_sequence, loss, kl, logprobs, stats, coef,
+    def policy_loss(self, rows, old, adv, a_strides, ref, clip_low, clip_high, kl_coef, by_sequence, scale, loss, kl, logprobs, stats, coef,
                     dlogits, d_strides, ws):
-        args = self._token_rows(rows) + (_ptr(old), _ptr(adv), *a_strides, _ptr(ref), clip_low, clip_high, kl_coef, int(by_sequence),
+        args = self._token_rows(rows) + (_ptr(old), _ptr(adv), *a_strides, _ptr(ref), clip_low, clip_high, kl_coef, int(by_sequence), scale,
                                          _ptr(loss), _ptr(kl), _ptr(logprobs), _ptr(stats), _ptr(coef), _ptr(dlogits), *d_strides, _ptr(ws))
         return self._prep("pf_policy_loss", args, (rows, old, adv, ref, loss, kl, logprobs, stats, coef, dlogits, ws))
 

@@ -107,7 +107,7 @@ def _table(t, who):
     k = _tables.get(t.get_device())
     if k is None:
         if t.device.type != "cuda":
-            raise RuntimeError("%s: the HIP loss kernels need GPU tensors (got %s)" % (who, t.device))
+            raise RuntimeError("%s: the HIP kernels need GPU tensors (got %s)" % (who, t.device))
         from .hip import HipKernels
 
         with torch.cuda.device(t.device):
@@ -265,7 +265,7 @@ class _PolicyFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, args, want=True):
-        labels, old, adv, a_strides, ref, cfg, clip, kl_coef, by_sequence = args
+        labels, old, adv, a_strides, ref, cfg, clip, kl_coef, by_sequence, scale = args
         B, T, _ = logits.shape
         k = _table(logits, "")
         R = max(0, T - cfg[0])
@@ -281,7 +281,7 @@ class _PolicyFn(torch.autograd.Function):
             strides = d.stride()[:2]
         else:
             work = _new(logits, n, dtype=torch.float64)
-        _issue(logits, k.policy_loss(_rows(logits, labels, cfg), old, adv, a_strides, ref, *clip, kl_coef, by_sequence, loss, kl, logprobs, stats,
+        _issue(logits, k.policy_loss(_rows(logits, labels, cfg), old, adv, a_strides, ref, *clip, kl_coef, by_sequence, scale, loss, kl, logprobs, stats,
                                      coef, d, strides, work))
         if want:
             ctx.save_for_backward(logits, labels, work)
@@ -335,14 +335,15 @@ def preference_loss(logits, labels, ref_logprobs, *, beta=0.1, label_smoothing=0
 
 
 def policy_loss(logits, labels, old_logprobs, advantages, ref_logprobs=None, *, clip=0.2, clip_high=None, kl_coef=0.0, temperature=1.0,
-                reduction="tokens", ignore_index=-100, shift=False):
+                reduction="tokens", scale=1.0, ignore_index=-100, shift=False):
     """Clipped policy loss of sampled tokens with a KL term; -> (loss, logprobs, kl).
 
     logits [B, T, V], labels int64 [B, T] (the tokens that were sampled), old_logprobs [B, T'] under the policy that sampled them,
     advantages [B], [B, 1] or [B, T'], ref_logprobs [B, T'] under a reference model (T' = T - 1 with `shift`, else T).  With r =
     exp(logprob - old) a token's loss is -min(r A, clamp(r, 1 - clip, 1 + clip_high) A) + kl_coef (exp(ref - logprob) - (ref -
     logprob) - 1); clip_high defaults to clip.  reduction "tokens": the mean over all tokens that count; "sequences": the mean over
-    the sequences that have such tokens of their means; with none at all the loss is 0.  The gradient flows to the logits alone;
+    the sequences that have such tokens of their means; with none at all the loss is 0.  `scale` multiplies the loss (not `kl`): a factor given here is free, one that the loss is
+    multiplied by afterwards has the backward pass compute the gradient anew.  The gradient flows to the logits alone;
     `logprobs` [B, T'] and `kl` (the KL term's mean) are for the log.  `ignore_index`, `shift` and `temperature` as for
     `token_logprobs`; what the other operands hold at ignored tokens does not matter.  A backward pass captured into a graph of its own is
     replayed once for every replay of the forward pass's graph."""
@@ -351,7 +352,7 @@ def policy_loss(logits, labels, old_logprobs, advantages, ref_logprobs=None, *, 
     if logits.dim() != 3:
         raise RuntimeError("%s: logits are [sequences, tokens, classes] (got %s)" % (who, tuple(logits.shape)))
     clip_high = clip if clip_high is None else clip_high
-    if not (0.0 <= clip < math.inf and 0.0 <= clip_high < math.inf) or not math.isfinite(kl_coef):
+    if not (0.0 <= clip < math.inf and 0.0 <= clip_high < math.inf) or not math.isfinite(kl_coef) or not math.isfinite(scale):
         raise RuntimeError("%s: clip and clip_high must not be negative, and all coefficients finite" % who)
     if reduction not in ("tokens", "sequences"):
         raise RuntimeError("%s: reduction is 'tokens' or 'sequences' (got %r)" % (who, reduction))
@@ -364,7 +365,7 @@ def policy_loss(logits, labels, old_logprobs, advantages, ref_logprobs=None, *, 
     ref = None if ref_logprobs is None else _constant(who, "ref_logprobs", ref_logprobs, [(B, R)], logits).contiguous()
     a_strides = (adv.stride(0), adv.stride(1) if adv.dim() == 2 and adv.shape[1] > 1 else 0)
     return _apply(_PolicyFn, x, y, old, adv, a_strides, ref, (int(shift), ignore_index, float(temperature)), (float(clip), float(clip_high)),
-                  float(kl_coef), reduction == "sequences")
+                  float(kl_coef), reduction == "sequences", float(scale))
 
 
 class LossWrapper(nn.Module):

@@ -42,6 +42,7 @@ REFUSED = [
     ("policy_loss", (X, Y, torch.zeros(2, 3), torch.zeros(2), torch.zeros(2, 4)), {}, "ref_logprobs"),
     ("policy_loss", (X, Y, torch.zeros(2, 3), torch.zeros(2)), {"clip": -0.1}, "clip"), ("policy_loss", (X, Y, torch.zeros(2, 3), torch.zeros(2)), {"clip_high": float("nan")}, "clip"),
     ("policy_loss", (X, Y, torch.zeros(2, 3), torch.zeros(2)), {"reduction": "sum"}, "reduction"),
+    ("policy_loss", (X, Y, torch.zeros(2, 3), torch.zeros(2)), {"scale": float("inf")}, "finite"),
     ("policy_loss", (X, Y, torch.zeros(2, 3, requires_grad=True), torch.zeros(2)), {}, "no gradient"),
 ]
 
@@ -90,7 +91,7 @@ def test_the_c_entries_refuse_without_a_device():
     rc(pref(dt=4), b"fp32, fp16 or bf16")
     assert lib.pf_preference_workspace(4, 10, 1) == 2 + 4 * 9
     pol = lambda **k: lib.pf_policy_loss(*{**dict(x=one, dt=0, B=2, T=3, V=5, sb=15, st=5, y=one, shift=0, ig=-100, t=1.0, old=one, adv=one, asb=1, ast=0, ref=None, lo=0.2, hi=0.2,  # noqa: E731
-                                                  c=0.0, seq=0, loss=one, kl=one, lp=one, stats=None, coef=None, d=None, db=0, ds=0, ws=one, s=None), **k}.values())
+                                                  c=0.0, seq=0, scale=1.0, loss=one, kl=one, lp=one, stats=None, coef=None, d=None, db=0, ds=0, ws=one, s=None), **k}.values())
     rc(pol(lo=-1.0), b"clip")
     rc(pol(ws=None), b"workspace")
     rc(pol(old=None), b"null pointer")

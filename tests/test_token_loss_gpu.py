@@ -180,6 +180,13 @@ def test_policy_loss(dtype, B, T, V, shift, kl_coef, by_token, sequences):
     check_gradient(again[:, :T - shift], dz, g / temperature, *parts(z, temperature), rel, dtype, dg / temperature)
     (scaled,) = torch.autograd.grad(-3.0 * loss, leaf)
     check_gradient(scaled[:, :T - shift], -3.0 * dz, 3.0 * g / temperature, *parts(z, temperature), rel, dtype, 3.0 * dg / temperature + 2.0 ** -23 * g.abs())
+    # the factor as an argument: the same, and the KL term's mean is not touched by it
+    quarter, _, same_kl = policy_loss(leaf, y, old, adv, ref, clip=0.2, clip_high=0.28, kl_coef=kl_coef, temperature=temperature, scale=0.25,
+                                      reduction="sequences" if sequences else "tokens", shift=bool(shift))
+    assert torch.equal(quarter, 0.25 * loss) and torch.equal(same_kl, got_kl)
+    (less,) = torch.autograd.grad(quarter, leaf)
+    plain = first.abs() >= LEAST[dtype] * 2 ** 13      # (fp16: 2^-12, so that a quarter is 2^-14 or more, where subnormals end)
+    assert torch.equal(less[plain], (0.25 * first)[plain])
     with torch.no_grad():
         quiet, _, _ = policy_loss(leaf, y, old, adv, ref, clip=0.2, clip_high=0.28, kl_coef=kl_coef, temperature=temperature,
                                   reduction="sequences" if sequences else "tokens", shift=bool(shift))
