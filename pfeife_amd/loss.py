@@ -246,15 +246,16 @@ class _PreferenceFn(torch.autograd.Function):
         _issue(logits, k.preference_loss(_rows(logits, labels, cfg), ref, beta, smoothing, average, loss, rewards, stats if want else None, coef, work))
         if want:
             ctx.save_for_backward(logits, labels, work)
-            ctx.cfg, ctx.at = cfg, (stats, coef)
+            ctx.cfg, ctx.at = cfg, (8 * n, 8 * (n + rows))
         ctx.mark_non_differentiable(rewards)
         ctx.set_materialize_grads(False)
         return loss, rewards
 
     @_once
     def backward(ctx, grad, _):
-        logits, labels, _ = ctx.saved_tensors
-        d = None if grad is None else _logits_gradient(logits, labels, ctx.cfg, *ctx.at, (1, 0), _as_scale(grad))
+        logits, labels, work = ctx.saved_tensors      # (not always where it was: hooks may have moved it)
+        at = work.data_ptr()
+        d = None if grad is None else _logits_gradient(logits, labels, ctx.cfg, at + ctx.at[0], at + ctx.at[1], (1, 0), _as_scale(grad))
         return d, None
 
 
@@ -285,21 +286,23 @@ class _PolicyFn(torch.autograd.Function):
                                      coef, d, strides, work))
         if want:
             ctx.save_for_backward(logits, labels, work)
-            ctx.cfg, ctx.at, ctx.d, ctx.captured = cfg, (stats, coef, (R, 1)), d, torch.cuda.is_current_stream_capturing()
+            ctx.cfg, ctx.at, ctx.d, ctx.captured = cfg, (8 * n, 8 * (n + B * R)), d, torch.cuda.is_current_stream_capturing()
         ctx.mark_non_differentiable(logprobs, kl)
         ctx.set_materialize_grads(False)
         return loss, logprobs, kl
 
     @_once
     def backward(ctx, grad, *_):
-        logits, labels, _ = ctx.saved_tensors
+        logits, labels, work = ctx.saved_tensors
         d = None
         if grad is not None:
             # handed out once (what has it may change it), and not from an eager forward pass to a graph, whose
             # replays would find it changed
             d, ctx.d = ctx.d, None
             ready = d is not None and ctx.captured == torch.cuda.is_current_stream_capturing()
-            d = _logits_gradient(logits, labels, ctx.cfg, *ctx.at, _as_scale(grad), d if ready else None, int(ready))
+            at = work.data_ptr()
+            d = _logits_gradient(logits, labels, ctx.cfg, at + ctx.at[0], at + ctx.at[1], (max(0, logits.shape[1] - ctx.cfg[0]), 1), _as_scale(grad),
+                                 d if ready else None, int(ready))
         return d, None
 
 

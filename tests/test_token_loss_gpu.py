@@ -102,7 +102,7 @@ def test_preference_loss(dtype, B, T, V, shift, average):
     off = beta * ((rel + 2.0 ** -24 * (lp.detach().abs() + 4)) * seen).sum(1) / n
     assert ((got.double() - rewards).abs() <= off + 2.0 ** -24 * rewards.abs()).all()
     offD = off.view(-1, 2).sum(1)
-    assert abs(float(loss) - float(want.detach())) <= float(offD.mean()) + 2.0 ** -23 * float(want.detach())       # |d loss / dD| <= 1
+    assert abs(float(loss.detach()) - float(want.detach())) <= float(offD.mean()) + 2.0 ** -23 * float(want.detach())       # |d loss / dD| <= 1
     (dz,) = torch.autograd.grad(want, z)
     (d,) = torch.autograd.grad(loss, leaf, retain_graph=True)
     g = torch.sigmoid(D.detach()) - (1 - eps)
@@ -163,7 +163,7 @@ def test_policy_loss(dtype, B, T, V, shift, kl_coef, by_token, sequences):
     dlp = rel + 2.0 ** -24                             # (the kernel's own log-probability is in 64 bits, its sum is not)
     assert ((got.double() - lp).abs() <= dlp + 2.0 ** -24 * (lp.abs() + 4)).all()
     slope = ratio * a.abs() + (0 if back is None else kl_coef * (back + 1))
-    assert abs(float(loss) - float(want)) <= float((w * slope * dlp).sum()) * 2 + 2.0 ** -24 * abs(float(want)) + 1e-14
+    assert abs(float(loss.detach()) - float(want.detach())) <= float((w * slope * dlp).sum().detach()) * 2 + 2.0 ** -24 * abs(float(want.detach())) + 1e-14
     assert abs(float(got_kl) - float(kl)) <= (0 if back is None else float((w * (back + 1) * dlp).sum()) * 2) + 2.0 ** -24 * abs(float(kl)) + 1e-14
     (dz,) = torch.autograd.grad(want, z) if want.requires_grad else (torch.zeros_like(z),)
     (d,) = torch.autograd.grad(loss, leaf, retain_graph=True)
@@ -557,3 +557,26 @@ def test_a_second_derivative_is_refused():
         assert torch.isfinite(d).all()
         with pytest.raises(RuntimeError, match="once_differentiable|differentiate twice|does not require grad"):
             torch.autograd.grad(d.sum(), x)
+
+
+def test_saved_tensors_that_move():
+    """Hooks that keep what the backward pass needs on the host, and a forward pass that is run again for it."""
+    from torch.utils.checkpoint import checkpoint
+
+    from pfeife_amd.loss import policy_loss, preference_loss, token_logprobs
+
+    x, y = make(torch.bfloat16, 4, 9, 1003, 1, seed=50)
+    old, ref, adv = policy_operands(logprobs64(x, y, 1)[1].detach(), 51)
+    zero = torch.zeros(4, device="cuda")
+    for fn in (lambda t: token_logprobs(t, y, shift=True).sum(), lambda t: preference_loss(t, y, zero, shift=True)[0],
+               lambda t: policy_loss(t, y, old, adv, ref, kl_coef=0.1, shift=True)[0], lambda t: 3.0 * policy_loss(t, y, old, adv, ref, kl_coef=0.1, shift=True)[0]):
+        leaf = x.clone().requires_grad_()
+        (want,) = torch.autograd.grad(fn(leaf), leaf)
+        with torch.autograd.graph.save_on_cpu():
+            loss = fn(leaf)
+        junk = [torch.full((1 << k,), 1e30, device="cuda") for k in range(6, 18)]      # (where the scratch was)
+        (got,) = torch.autograd.grad(loss, leaf)
+        assert torch.equal(got, want)
+        (got,) = torch.autograd.grad(checkpoint(fn, leaf, use_reentrant=False), leaf)
+        assert torch.equal(got, want)
+        del junk
