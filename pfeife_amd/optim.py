@@ -66,8 +66,8 @@ class AdamW8bit(torch.optim.Optimizer):
         """The gradient as the kernel addresses it; errors where it, the parameter or the state is not what the kernel takes."""
         if p.device.type != "cuda":
             raise RuntimeError("AdamW8bit: the HIP step needs GPU parameters (got %s)" % p.device)
-        if g.is_sparse or g.dtype != torch.float32 or g.device != p.device:
-            raise RuntimeError("AdamW8bit: gradients are dense fp32 on the parameter's device (got %s %s on %s)" % (g.layout, g.dtype, g.device))
+        if g.dtype != torch.float32 or g.device != p.device:
+            raise RuntimeError("AdamW8bit: gradients are dense fp32 on the parameter's device (got %s on %s)" % (g.dtype, g.device))
         if not p.is_contiguous() and torch.empty_like(p, device="meta").stride() != p.stride():
             raise RuntimeError("AdamW8bit: a parameter's elements have to lie in memory without gaps (strides %s)" % (p.stride(),))
         n = p.numel()
@@ -80,6 +80,13 @@ class AdamW8bit(torch.optim.Optimizer):
         if not fits:
             raise RuntimeError("AdamW8bit: the optimizer's state does not fit its parameter of shape %s" % (tuple(p.shape),))
         return g if g.stride() == p.stride() or g.is_contiguous() and p.is_contiguous() else torch.empty_like(p)     # (of another layout: copied for each step)
+
+    @staticmethod
+    def _check_apart(params):
+        """One launch updates them all, in no order: none may be updated twice."""
+        spans = sorted((p.data_ptr(), p.data_ptr() + 4 * p.numel()) for p, *_ in params)
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise RuntimeError("AdamW8bit: parameters share memory, or one is in a group twice")
 
     def _prepare(self, kernels):
         """[(group, states, device, table, copies)] of what has a gradient, parameters at one step count together, and whether a table
@@ -97,6 +104,8 @@ class AdamW8bit(torch.optim.Optimizer):
                 if g is None or p.numel() == 0:
                     records.append((p, None))
                     continue
+                if g.layout is not torch.strided:
+                    raise RuntimeError("AdamW8bit: gradients are dense fp32 on the parameter's device (got %s)" % g.layout)
                 st = self._init_state(p, group)
                 key = (float(st["step"]), p.get_device())
                 found = by_step.get(key)
@@ -116,6 +125,7 @@ class AdamW8bit(torch.optim.Optimizer):
                 if ent is None or ent[0] != now:
                     fresh = True
                     items = [(p.data, self._check(p, g, ops), *ops, index) for p, g, ops, index in params]
+                    self._check_apart(params)
                     copies = [(i[1], p) for (p, g, _, _), i in zip(params, items) if i[1] is not g]
                     ent = cache[gi, n] = (now, kernels.adam8_table(items), copies)
                 work.append((group, states, params[0][0].device, *ent[1:]))

@@ -338,3 +338,32 @@ def test_what_changes_between_steps_is_seen():
     opt.load_state_dict(copy.deepcopy(opt.state_dict()))
     both()
     both()
+
+
+@pytest.mark.filterwarnings("ignore:.*duplicate parameters")
+def test_what_one_launch_cannot_update_is_refused():
+    """Parameters that share memory (in one launch, so in no order), one that is listed twice, a sparse gradient: nothing is changed."""
+    from pfeife_amd.optim import AdamW8bit
+
+    room = torch.randn(12_000, generator=torch.Generator().manual_seed(7)).cuda()
+    start = room.clone()
+    one = torch.nn.Parameter(room[:5000])
+    for params in ([one, one], [one, torch.nn.Parameter(room[:5000])], [torch.nn.Parameter(room[4999:9000]), one], [one, torch.nn.Parameter(room[100:101])]):
+        for p in params:
+            p.grad = torch.ones_like(p)
+        opt = AdamW8bit(params, lr=LR)
+        for _ in range(2):
+            with pytest.raises(RuntimeError, match="share memory"):
+                opt.step()
+    sparse = torch.nn.Parameter(room[6000:].view(100, 60))
+    sparse.grad = torch.ones(100, 60, device="cuda").to_sparse()
+    with pytest.raises(RuntimeError, match="dense"):
+        AdamW8bit([sparse], lr=LR).step()
+    torch.cuda.synchronize()
+    assert torch.equal(room, start)
+    # neighbours are fine, and so are groups, whose launches follow one another
+    opt = AdamW8bit([{"params": [one, torch.nn.Parameter(room[5000:9000])]}, {"params": [torch.nn.Parameter(room[:5000])]}], lr=LR)
+    for p in (p for grp in opt.param_groups for p in grp["params"]):
+        p.grad = torch.ones_like(p)
+    opt.step()
+    assert not torch.equal(room[:9000], start[:9000]) and torch.equal(room[9000:], start[9000:])
