@@ -481,7 +481,10 @@ __device__ double pair_terms(const PairArgs& a, int64_t i, const double (&total)
     a.rewards[2 * i + k] = (float)reward[k];
     a.coef[2 * i + k] = (float)((k ? -up : up) * a.beta * per_token[k] / (double)a.pairs);
   }
-  return (1.0 - a.smoothing) * softplus(-D) + a.smoothing * softplus(D);
+  double loss = 0.0;      // (a term of factor zero is none, where the other answer has a token of no probability too)
+  if (a.smoothing < 1.0) loss += (1.0 - a.smoothing) * softplus(-D);
+  if (a.smoothing > 0.0) loss += a.smoothing * softplus(D);
+  return loss;
 }
 
 __global__ __launch_bounds__(512) void preference_pair_kernel(const PairArgs a, double* pair_loss) {

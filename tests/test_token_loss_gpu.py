@@ -580,3 +580,27 @@ def test_saved_tensors_that_move():
         (got,) = torch.autograd.grad(checkpoint(fn, leaf, use_reentrant=False), leaf)
         assert torch.equal(got, want)
         del junk
+
+
+@pytest.mark.parametrize("smoothing", [0.0, 1.0, 0.25])
+def test_an_answer_of_no_probability(smoothing):
+    """One label's logit is -inf: the difference of the rewards is infinite, the loss so only where a term with a factor other than zero is; the pair's
+    gradient is the limit's."""
+    from pfeife_amd.loss import preference_loss
+
+    x, y = make(torch.bfloat16, 4, 9, 1003, 0, seed=60)
+    y[:, 3] = 5
+    ref = torch.zeros(4, device="cuda")
+    for gone in (0, 1):
+        z = x.clone()
+        z[gone, 3, 5] = -torch.inf
+        leaf = z.requires_grad_()
+        loss, rewards = preference_loss(leaf, y, ref, label_smoothing=smoothing)
+        alone, _ = preference_loss(x[2:], y[2:], ref[2:], label_smoothing=smoothing)
+        (d,) = torch.autograd.grad(loss, leaf)
+        assert rewards[gone] == -torch.inf and torch.isfinite(rewards[2:]).all() and torch.isfinite(d).all()
+        up = (0.0 if gone == 0 else 1.0) - (1 - smoothing)           # sigmoid(D) - (1 - smoothing)
+        if up == 0:
+            assert abs(float(loss.detach()) - 0.5 * float(alone)) <= 2.0 ** -22 * abs(float(alone)) and not d[:2].any()
+        else:
+            assert loss == torch.inf and d[:2].any()
