@@ -631,8 +631,10 @@ __device__ __forceinline__ TokenTerms policy_token(const PolicyArgs& a, float ol
       k = e - q;
     }
     o.kl = k;
-    o.loss = fmaf(a.kl_coef, k, o.loss);
-    o.g = fmaf(-a.kl_coef, e, o.g);
+    if (a.kl_coef != 0.f) {      // (else it is for the log alone, where it may be infinite)
+      o.loss = fmaf(a.kl_coef, k, o.loss);
+      o.g = fmaf(-a.kl_coef, e, o.g);
+    }
   }
   return o;
 }

@@ -604,3 +604,17 @@ def test_an_answer_of_no_probability(smoothing):
             assert abs(float(loss.detach()) - 0.5 * float(alone)) <= 2.0 ** -22 * abs(float(alone)) and not d[:2].any()
         else:
             assert loss == torch.inf and d[:2].any()
+
+
+def test_a_penalty_that_is_only_looked_at():
+    """kl_coef 0 with log-probabilities of a reference, some of them -inf: the loss and its gradient are those without it."""
+    from pfeife_amd.loss import policy_loss
+
+    x, y = make(torch.bfloat16, 3, 9, 1003, 1, seed=61)
+    old, ref, adv = policy_operands(logprobs64(x, y, 1)[1].detach(), 62)
+    ref[(y[:, 1:] != -100).nonzero(as_tuple=True)] = -torch.inf
+    leaf = x.clone().requires_grad_()
+    want, _, _ = policy_loss(leaf, y, old, adv, shift=True)
+    loss, _, kl = policy_loss(leaf, y, old, adv, ref, shift=True)
+    assert kl == torch.inf and torch.equal(loss, want) and torch.isfinite(loss)
+    assert torch.equal(torch.autograd.grad(loss, leaf)[0], torch.autograd.grad(want, leaf)[0])
