@@ -185,7 +185,10 @@ template <bool FULL> __device__ __forceinline__ void step_block(const Adam8Item&
   }
 }
 
-// A workgroup of four wavefronts to every 1024 elements, a wavefront to a block.
+// A workgroup of four wavefronts to every 1024 elements, a wavefront to a block: 16 bytes a lane of parameters and gradients, one word of each
+// code, the block's maximum by lane exchanges.  Bound by memory, 16.06 bytes a parameter: 117 M parameters in eight tensors 368 us, 5.1 TB/s (the
+// 32-bit step moves 28); 1.8 M in four 10.  Some 80 instructions an element (square root and quotient correctly rounded, the hash) keep the
+// arithmetic units busy two thirds of that time.
 __global__ __launch_bounds__(256) void adam8_kernel(const Adam8Item* items, const int64_t* ends, int64_t first, int n_items, Adam8Coef c,
                                                     const float* scaler_state) {
   if (scaler_state) {

@@ -311,7 +311,8 @@ def token_logprobs(logits, labels, *, ignore_index=-100, temperature=1.0, shift=
 
     logits [..., T, V] (fp32, fp16 or bf16), labels int64 [..., T].  shift: row t is scored against label t + 1 (labels as
     the model's own input), the result has T - 1 tokens.  Tokens whose label is `ignore_index` give 0 and take no part, whatever
-    their logits hold; labels outside the vocabulary give NaN."""
+    their logits hold; labels outside the vocabulary give NaN.  A backward pass is captured into a graph, as any of torch's, only
+    while no autograd graph made outside the capture holds the same leaves."""
     x, y = _check_rows("token_logprobs", logits, labels, ignore_index, temperature, shift)
     cfg = (int(shift), ignore_index, float(temperature))
     out = _apply(_TokenLogprobFn, x, y, cfg)

@@ -49,7 +49,7 @@ _VERBOSITY = {"error": logging.ERROR, "info": logging.INFO, "debug": logging.DEB
 class PipeOption:
     """
     compiler            dynamo backend for per-stage compilation (ignored: stages run on the HIP executor)
-    optimizer           dict(type=..., **kwargs of the torch optimizer)
+    optimizer           dict(type=..., **kwargs of the torch optimizer, or of optim.AdamW8bit for type "adamw8bit")
     device_cnt          number of pipeline ranks the schedule is drawn for (all run on one GPU here)
     batch_size          size of one micro-batch
     batch_cnt           number of micro-batches per step (default device_cnt)
