@@ -39,6 +39,9 @@ class AdamW8bit(torch.optim.Optimizer):
             for key, value in state_dict["state"].get(i, {}).items():
                 if torch.is_tensor(value):
                     self.state[p][key] = value.detach().clone() if key == "step" else value.detach().clone().to(p.device)
+        # new state may lie where the old one did, and the old one's memory is wanted back
+        for name in ("_seen", "_tables"):
+            self.__dict__.pop(name, None)
 
     def _init_state(self, p, group):
         st = self.state[p]

@@ -367,3 +367,25 @@ def test_what_one_launch_cannot_update_is_refused():
         p.grad = torch.ones_like(p)
     opt.step()
     assert not torch.equal(room[:9000], start[:9000]) and torch.equal(room[9000:], start[9000:])
+
+
+@pytest.mark.parametrize("layout", [torch.contiguous_format, torch.channels_last])
+def test_loaded_state_is_new(layout):
+    """Also where its memory is the old state's, which is given back: a loss scaler's count of steps starts from what was loaded."""
+    import weakref
+
+    from pfeife_amd.loss import _table
+    from pfeife_amd.optim import AdamW8bit
+
+    p = torch.nn.Parameter(torch.randn(16, 8, 8, 8, generator=torch.Generator().manual_seed(8)).cuda().to(memory_format=layout))
+    p.grad = torch.ones_like(p)
+    opt = AdamW8bit([p], lr=LR)
+    opt.step()
+    kernels = _table(p, "")
+    assert not opt._prepare(kernels)[1]
+    saved = copy.deepcopy(opt.state_dict())
+    old = weakref.ref(opt.state[p]["exp_avg"])
+    opt.load_state_dict(saved)
+    assert old() is None and opt._prepare(kernels)[1] and not opt._prepare(kernels)[1]
+    opt.step()
+    assert opt.state[p]["step"] == 2
