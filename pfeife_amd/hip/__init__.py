@@ -649,6 +649,17 @@ class HipKernels:
                           (logits, targets, row_lse, dloss, loss, dlogits), rows * classes * (_es(logits) + _es(dlogits)))
 
     # -- losses over token log-probabilities: `rows` is (logits, B, T, V, sb, st, labels, shift, ignore_index, temperature) -------
+    @staticmethod
+    def token_rows(logits, B, T, V, sb, st, labels, shift, ignore_index, temperature):
+        """`rows` as the entry points take them"""
+        return (_ptr(logits), _dt(logits), B, T, V, sb, st, _ptr(labels), int(shift), ignore_index, temperature)
+
+    def token_gradient(self, rows, stats, coef, g_strides, dlogits, scale, unless_one, stream):
+        """`token_logprob_bwd`, issued at once; rows of `token_rows`"""
+        rc = self.lib.pf_token_logprob_bwd(*rows, stats, coef, *g_strides, scale, unless_one, dlogits.data_ptr(), *dlogits.stride()[:2], stream)
+        if rc != 0:
+            raise RuntimeError("pf_token_logprob_bwd failed: %s" % self.lib.pf_last_error().decode())
+
     def token_logprob_fwd(self, rows, logprobs, stats=None):
         args = self._token_rows(rows) + (_ptr(logprobs), _ptr(stats))
         return self._prep("pf_token_logprob_fwd", args, (rows, logprobs, stats))
@@ -673,10 +684,8 @@ class HipKernels:
                                          _ptr(loss), _ptr(kl), _ptr(logprobs), _ptr(stats), _ptr(coef), _ptr(dlogits), *d_strides, _ptr(ws))
         return self._prep("pf_policy_loss", args, (rows, old, adv, ref, loss, kl, logprobs, stats, coef, dlogits, ws))
 
-    @staticmethod
-    def _token_rows(rows):
-        logits, B, T, V, sb, st, labels, shift, ignore_index, temperature = rows
-        return (_ptr(logits), _dt(logits), B, T, V, sb, st, _ptr(labels), int(shift), ignore_index, temperature)
+    def _token_rows(self, rows):
+        return self.token_rows(*rows) if len(rows) == 10 else rows
 
     def mse_fwd(self, a, b, partial, loss, n):
         args = (_ptr(a), _dt(a), _ptr(b), _dt(b), _ptr(partial), _ptr(loss), n)

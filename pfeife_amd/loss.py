@@ -166,16 +166,26 @@ def _constant(who, name, t, shapes, like):
 
 def _rows(logits, labels, cfg):
     """The kernels' description of the rows; cfg = (shift, ignore_index, temperature)."""
-    return (logits, *logits.shape, *logits.stride()[:2], labels, *cfg)
+    return _table(logits, "").token_rows(logits, *logits.shape, *logits.stride()[:2], labels, *cfg)
 
 
 def _new(like, *shape, dtype=torch.float32):
     return torch.empty(shape, dtype=dtype, device=like.device)
 
 
-def _logits_gradient(logits, labels, cfg, stats, coef, g_strides, scale=None, into=None, unless_one=0):
+def _logits_gradient(ctx, logits, labels, stats, coef, g_strides, scale=None, into=None, unless_one=0):
+    """stats, coef, scale: addresses.  Autograd calls this on a thread of its own, which finds little in its core's caches: it does no more
+    than it must, and takes the forward pass's description of the rows where they still lie there."""
+    rows, strides, k = ctx.rows
+    if logits.data_ptr() != rows[0] or labels.data_ptr() != rows[7] or logits.stride() != strides:      # (hooks may move what is saved)
+        rows = _rows(logits, labels, rows[8:])
     d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if into is None else into
-    _issue(logits, _table(logits, "").token_logprob_bwd(_rows(logits, labels, cfg), stats, coef, g_strides, d, d.stride()[:2], scale, unless_one))
+    index = logits.get_device()
+    if _current_device() == index:
+        k.token_gradient(rows, stats, coef, g_strides, d, scale, unless_one, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            k.token_gradient(rows, stats, coef, g_strides, d, scale, unless_one, _raw_stream(index))
     return d
 
 
@@ -218,17 +228,18 @@ class _TokenLogprobFn(torch.autograd.Function):
         B, T, _ = logits.shape
         out = _new(logits, B, max(0, T - cfg[0]))
         stats = _new(logits, *out.shape, 2) if want else None
-        _issue(logits, _table(logits, "").token_logprob_fwd(_rows(logits, labels, cfg), out, stats))
+        k, rows = _table(logits, ""), _rows(logits, labels, cfg)
+        _issue(logits, k.token_logprob_fwd(rows, out, stats))
         if want:
             ctx.save_for_backward(logits, labels, stats)
-            ctx.cfg = cfg
+            ctx.rows = rows, logits.stride(), k
         return out
 
     @_once
     def backward(ctx, grad):
         logits, labels, stats = ctx.saved_tensors
         grad = _as_scale(grad)      # (any strides: a sum's gradient is one number)
-        return _logits_gradient(logits, labels, ctx.cfg, stats, grad, grad.stride()), None
+        return _logits_gradient(ctx, logits, labels, stats.data_ptr(), grad.data_ptr(), grad.stride()), None
 
 
 class _PreferenceFn(torch.autograd.Function):
@@ -237,16 +248,17 @@ class _PreferenceFn(torch.autograd.Function):
         labels, ref, cfg, beta, smoothing, average = args
         B, T, _ = logits.shape
         k = _table(logits, "")
-        n, rows = k.preference_workspace(B, T, cfg[0]), B * max(0, T - cfg[0])
+        rows = _rows(logits, labels, cfg)
+        n, scored = k.preference_workspace(B, T, cfg[0]), B * max(0, T - cfg[0])
         # the kernels' scratch, and behind it what the backward pass takes: {reference, 1 / sum} of every row, a factor of every sequence
-        work = _new(logits, n + rows + (B + 1) // 2, dtype=torch.float64)
+        work = _new(logits, n + scored + (B + 1) // 2, dtype=torch.float64)
         at = work.data_ptr()
-        stats, coef = at + 8 * n, at + 8 * (n + rows)
+        stats, coef = at + 8 * n, at + 8 * (n + scored)
         loss, rewards = _new(logits), _new(logits, B)
-        _issue(logits, k.preference_loss(_rows(logits, labels, cfg), ref, beta, smoothing, average, loss, rewards, stats if want else None, coef, work))
+        _issue(logits, k.preference_loss(rows, ref, beta, smoothing, average, loss, rewards, stats if want else None, coef, work))
         if want:
             ctx.save_for_backward(logits, labels, work)
-            ctx.cfg, ctx.at = cfg, (8 * n, 8 * (n + rows))
+            ctx.rows, ctx.at = (rows, logits.stride(), k), (8 * n, 8 * (n + scored))
         ctx.mark_non_differentiable(rewards)
         ctx.set_materialize_grads(False)
         return loss, rewards
@@ -254,9 +266,10 @@ class _PreferenceFn(torch.autograd.Function):
     @_once
     def backward(ctx, grad, _):
         logits, labels, work = ctx.saved_tensors      # (not always where it was: hooks may have moved it)
-        at = work.data_ptr()
-        d = None if grad is None else _logits_gradient(logits, labels, ctx.cfg, at + ctx.at[0], at + ctx.at[1], (1, 0), _as_scale(grad))
-        return d, None
+        if grad is None:
+            return None, None
+        at, (stats, coef), grad = work.data_ptr(), ctx.at, _as_scale(grad)
+        return _logits_gradient(ctx, logits, labels, at + stats, at + coef, (1, 0), grad.data_ptr()), None
 
 
 class _PolicyFn(torch.autograd.Function):
@@ -268,7 +281,7 @@ class _PolicyFn(torch.autograd.Function):
     def forward(ctx, logits, args, want=True):
         labels, old, adv, a_strides, ref, cfg, clip, kl_coef, by_sequence, scale = args
         B, T, _ = logits.shape
-        k = _table(logits, "")
+        k, rows = _table(logits, ""), _rows(logits, labels, cfg)
         R = max(0, T - cfg[0])
         n = k.policy_workspace(B, T, cfg[0])
         loss, kl, logprobs = _new(logits), _new(logits), _new(logits, B, R)
@@ -282,11 +295,11 @@ class _PolicyFn(torch.autograd.Function):
             strides = d.stride()[:2]
         else:
             work = _new(logits, n, dtype=torch.float64)
-        _issue(logits, k.policy_loss(_rows(logits, labels, cfg), old, adv, a_strides, ref, *clip, kl_coef, by_sequence, scale, loss, kl, logprobs, stats,
-                                     coef, d, strides, work))
+        _issue(logits, k.policy_loss(rows, old, adv, a_strides, ref, *clip, kl_coef, by_sequence, scale, loss, kl, logprobs, stats, coef, d, strides, work))
         if want:
             ctx.save_for_backward(logits, labels, work)
-            ctx.cfg, ctx.at, ctx.d, ctx.captured = cfg, (8 * n, 8 * (n + B * R)), d, torch.cuda.is_current_stream_capturing()
+            ctx.rows, ctx.at = (rows, logits.stride(), k), (8 * n, 8 * (n + B * R), (R, 1))
+            ctx.d, ctx.captured = d, torch.cuda.is_current_stream_capturing()
         ctx.mark_non_differentiable(logprobs, kl)
         ctx.set_materialize_grads(False)
         return loss, logprobs, kl
@@ -294,16 +307,15 @@ class _PolicyFn(torch.autograd.Function):
     @_once
     def backward(ctx, grad, *_):
         logits, labels, work = ctx.saved_tensors
-        d = None
-        if grad is not None:
-            # handed out once (what has it may change it), and not from an eager forward pass to a graph, whose
-            # replays would find it changed
-            d, ctx.d = ctx.d, None
-            ready = d is not None and ctx.captured == torch.cuda.is_current_stream_capturing()
-            at = work.data_ptr()
-            d = _logits_gradient(logits, labels, ctx.cfg, at + ctx.at[0], at + ctx.at[1], (max(0, logits.shape[1] - ctx.cfg[0]), 1), _as_scale(grad),
-                                 d if ready else None, int(ready))
-        return d, None
+        if grad is None:
+            return None, None
+        # handed out once (what has it may change it), and not from an eager forward pass to a graph, whose replays would find it
+        # changed
+        d, ctx.d = ctx.d, None
+        if d is not None and ctx.captured != torch.cuda.is_current_stream_capturing():
+            d = None
+        at, (stats, coef, strides), grad = work.data_ptr(), ctx.at, _as_scale(grad)
+        return _logits_gradient(ctx, logits, labels, at + stats, at + coef, strides, grad.data_ptr(), d, 0 if d is None else 1), None
 
 
 def token_logprobs(logits, labels, *, ignore_index=-100, temperature=1.0, shift=False):

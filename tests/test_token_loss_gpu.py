@@ -618,3 +618,21 @@ def test_a_penalty_that_is_only_looked_at():
     loss, _, kl = policy_loss(leaf, y, old, adv, ref, shift=True)
     assert kl == torch.inf and torch.equal(loss, want) and torch.isfinite(loss)
     assert torch.equal(torch.autograd.grad(loss, leaf)[0], torch.autograd.grad(want, leaf)[0])
+
+
+def test_saved_tensors_of_another_layout():
+    """Hooks that hand back the saved logits without the gaps that they had."""
+    from pfeife_amd.loss import policy_loss, preference_loss, token_logprobs
+
+    wide, y = make(torch.bfloat16, 4, 9, 1100, 1, seed=52)
+    y = torch.where(y < 1003, y, IGNORE)
+    old, ref, adv = policy_operands(logprobs64(wide[..., :1003], y, 1)[1].detach(), 53)
+    zero = torch.zeros(4, device="cuda")
+    for fn in (lambda t: token_logprobs(t, y, shift=True).sum(), lambda t: preference_loss(t, y, zero, shift=True)[0],
+               lambda t: 3.0 * policy_loss(t, y, old, adv, ref, kl_coef=0.1, shift=True)[0]):
+        leaf = wide.clone().requires_grad_()
+        (want,) = torch.autograd.grad(fn(leaf[..., :1003]), leaf)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(memory_format=torch.contiguous_format), lambda t: t):
+            loss = fn(leaf[..., :1003])
+        (got,) = torch.autograd.grad(loss, leaf)
+        assert torch.equal(got, want)
