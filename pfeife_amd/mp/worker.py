@@ -843,7 +843,8 @@ class StageWorker:
         self._fused_adam_prepare(opt, scaled)()
 
     def _fused_adam_prepare(self, opt, scaled):
-        """The tables of the param groups, as their tensors are now; -> the call that makes the step."""
+        """The tables of the param groups' parameters, those at one step count together, as their tensors are now; -> the call that makes
+        the step."""
         cache = self.__dict__.setdefault("_adam_tables", {})
         rebuilt = False
         groups = []
@@ -864,17 +865,20 @@ class StageWorker:
                 continue
             ent = cache.get(gi)
             if ent is None or ent[0] != sig:    # (all that the table holds)
-                table = self.kernels.adam_table([p.data for p in params], [p.grad for p in params],
-                                                [st["exp_avg"] for st in state], [st["exp_avg_sq"] for st in state])
-                ent = cache[gi] = (sig, table)
+                by_step = {}      # (a parameter whose first gradient came later is at an earlier step than the others)
+                for i, st in enumerate(state):
+                    by_step.setdefault(float(st["step"]), []).append(i)
+                ent = cache[gi] = (sig, [(self.kernels.adam_table([params[i].data for i in at], [params[i].grad for i in at],
+                                                                  [state[i]["exp_avg"] for i in at], [state[i]["exp_avg_sq"] for i in at]), at)
+                                         for at in by_step.values()])
                 rebuilt = True
-            groups.append((g, params, state, ent[1]))
+            groups += [(g, [state[i] for i in at], table) for table, at in ent[1]]
 
         def step():
             s = self.stream()
             if scaled and rebuilt:
-                self._seed_device_step_count(opt, groups)
-            for g, params, state, (table, n_items, n_chunks) in groups:
+                self._seed_device_step_count(opt, [state for _, state, _ in groups])
+            for g, state, (table, n_items, n_chunks) in groups:
                 b1, b2 = g["betas"]
                 if scaled:
                     # skipped on overflow; the bias corrections use the device's count of completed steps.
@@ -904,7 +908,7 @@ class StageWorker:
 
         def step():
             if scaled and fresh:
-                self._seed_device_step_count(opt, [(w[0], None, w[1], None) for w in work])
+                self._seed_device_step_count(opt, [w[1] for w in work])
             with torch.cuda.stream(lane):
                 for g, states, _, table, copies in work:
                     opt._launch(self.kernels, g, states, table, copies, lane.cuda_stream, self.scaler_state if scaled else None)
@@ -912,7 +916,7 @@ class StageWorker:
 
         return step
 
-    def _seed_device_step_count(self, opt, groups):
+    def _seed_device_step_count(self, opt, served):
         """The fused step under dynamic loss scaling takes Adam's bias corrections from the device's
         count of completed steps (scaler_state[3]).  Whenever the optimizer's state tensors are new
         to this worker (first step, `load_state_dict`), that count is set from the optimizer's own
@@ -920,7 +924,7 @@ class StageWorker:
         One counter serves every parameter: an optimizer whose parameters disagree is refused."""
         if getattr(self, "_host_steps_stale", False) and getattr(self, "_steps_owner", None) is opt:
             self.sync_optimizer_steps()
-        steps = {int(float(st["step"])) for _, _, state, _ in groups for st in state}
+        steps = {int(float(st["step"])) for state in served for st in state}
         if len(steps) > 1:
             raise RuntimeError("fused Adam step with dynamic loss scaling: the optimizer's parameters are at "
                                "different step counts %s; one device-side counter serves them all" % sorted(steps))
