@@ -499,6 +499,7 @@ class StageWorker:
             self.issuer.close()
             self.issuer = None
         self._drain()
+        self.sync_optimizer_steps()      # (the optimizer may be the caller's, and go on without this worker)
         self._drop_jobs()
         for slot in self.mbs.values():
             self._drop_graphs(slot)
@@ -846,8 +847,7 @@ class StageWorker:
         """The tables of the param groups' parameters, those at one step count together, as their tensors are now; -> the call that makes
         the step."""
         cache = self.__dict__.setdefault("_adam_tables", {})
-        rebuilt = False
-        groups = []
+        looked_at = []
         for gi, g in enumerate(opt.param_groups):
             params, sig, state = [], [], []
             for p in g["params"]:
@@ -860,18 +860,26 @@ class StageWorker:
                     st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
                 params.append(p)
                 state.append(st)
-                sig.append((p.numel(), p.data_ptr(), p.grad.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr()))
-            if not params:
-                continue
+                sig.append((p.numel(), p.data_ptr(), p.grad.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(), id(st)))
+            if params:
+                looked_at.append((gi, g, params, state, sig))
+        # (all that the tables hold; a group may also have no gradient any more)
+        rebuilt = len(cache) != len(looked_at) or any(gi not in cache or cache[gi][0] != sig for gi, _, _, _, sig in looked_at)
+        if rebuilt:
+            if scaled:
+                self.sync_optimizer_steps()
+            for gi in set(cache) - {entry[0] for entry in looked_at}:
+                del cache[gi]
+        groups = []
+        for gi, g, params, state, sig in looked_at:
             ent = cache.get(gi)
-            if ent is None or ent[0] != sig:    # (all that the table holds)
+            if ent is None or ent[0] != sig:
                 by_step = {}      # (a parameter whose first gradient came later is at an earlier step than the others)
                 for i, st in enumerate(state):
                     by_step.setdefault(float(st["step"]), []).append(i)
                 ent = cache[gi] = (sig, [(self.kernels.adam_table([params[i].data for i in at], [params[i].grad for i in at],
                                                                   [state[i]["exp_avg"] for i in at], [state[i]["exp_avg_sq"] for i in at]), at)
                                          for at in by_step.values()])
-                rebuilt = True
             groups += [(g, [state[i] for i in at], table) for table, at in ent[1]]
 
         def step():
@@ -884,9 +892,9 @@ class StageWorker:
                     # skipped on overflow; the bias corrections use the device's count of completed steps.
                     # The host-side `step` entries are brought up to date from that count when somebody
                     # reads them (sync_optimizer_steps: optimizer.state_dict() calls it)
-                    self.kernels.adam_step_scaled(table, n_items, n_chunks, float(g["lr"]), float(b1), float(b2),
-                                                  float(g["eps"]), float(g["weight_decay"]),
-                                                  type(opt) is torch.optim.AdamW, self.scaler_state, s)
+                    self._launch_at_step(state[0], lambda: self.kernels.adam_step_scaled(
+                        table, n_items, n_chunks, float(g["lr"]), float(b1), float(b2), float(g["eps"]),
+                        float(g["weight_decay"]), type(opt) is torch.optim.AdamW, self.scaler_state, s))
                     self._host_steps_stale = True
                 else:
                     t = int(state[0]["step"].item()) + 1
@@ -902,57 +910,81 @@ class StageWorker:
 
     def _adam8_prepare(self, opt, scaled):
         """The same for AdamW8bit, whose own step() cannot know of an overflow without a read from the device."""
-        lane = self.stream_obj if self.stream_obj is not None else torch.cuda.default_stream(self.device)
+        lane = self.stream_obj if self.stream_obj is not None or self.device.type != "cuda" else torch.cuda.default_stream(self.device)
         with torch.cuda.stream(lane):
             work, fresh = opt._prepare(self.kernels)
+            if scaled and not fresh:      # (a group may have no gradient any more, or the optimizer be one that has stepped before)
+                fresh = {id(st) for w in work for st in w[1]} != self.__dict__.setdefault("_served", {}).keys()
+            if scaled and fresh and getattr(self, "_host_steps_stale", False):
+                self.sync_optimizer_steps()
+                work, _ = opt._prepare(self.kernels)      # (which puts parameters at one step count together)
+        stream = lane.cuda_stream if lane is not None else None
 
         def step():
             if scaled and fresh:
                 self._seed_device_step_count(opt, [w[1] for w in work])
             with torch.cuda.stream(lane):
                 for g, states, _, table, copies in work:
-                    opt._launch(self.kernels, g, states, table, copies, lane.cuda_stream, self.scaler_state if scaled else None)
+                    if scaled:
+                        self._launch_at_step(states[0], lambda: opt._launch(self.kernels, g, states, table, copies, stream, self.scaler_state))
+                    else:
+                        opt._launch(self.kernels, g, states, table, copies, stream)
                     self._host_steps_stale = scaled
 
         return step
 
     def _seed_device_step_count(self, opt, served):
         """The fused step under dynamic loss scaling takes Adam's bias corrections from the device's
-        count of completed steps (scaler_state[3]).  Whenever the optimizer's state tensors are new
-        to this worker (first step, `load_state_dict`), that count is set from the optimizer's own
+        count of completed steps (scaler_state[3]).  Whenever a table is new (first step,
+        `load_state_dict`, gradients that come or go), that count is set from the optimizer's own
         `step` entries, so a resumed optimizer continues at step k + 1 against its warm moments.
-        One counter serves every parameter: an optimizer whose parameters disagree is refused."""
-        if getattr(self, "_host_steps_stale", False) and getattr(self, "_steps_owner", None) is opt:
-            self.sync_optimizer_steps()
-        steps = {int(float(st["step"])) for state in served for st in state}
-        if len(steps) > 1:
-            raise RuntimeError("fused Adam step with dynamic loss scaling: the optimizer's parameters are at "
-                               "different step counts %s; one device-side counter serves them all" % sorted(steps))
-        k = float(steps.pop()) if steps else 0.0
+        One counter serves every parameter: it counts for those that have made most steps, and a
+        parameter that has made fewer is noted with what it lags behind.  served: lists of states,
+        each at one count."""
+        counts = [int(float(states[0]["step"])) for states in served]
+        k = max(counts, default=0)
         if float(self.scaler_state[3].item()) != k:
             self.scaler_state[3:4].fill_(k)
+        self._served = {id(st): (st, c - k) for states, c in zip(served, counts) for st in states}
         if getattr(self, "_steps_owner", None) is not opt:
             self._steps_owner = opt
             if hasattr(opt, "register_state_dict_pre_hook"):
                 opt.register_state_dict_pre_hook(lambda o: self.sync_optimizer_steps())
+                # (what is loaded may share its tensors with what was there, or may not know of the steps since it was saved)
+                opt.register_load_state_dict_pre_hook(lambda o, state_dict: self.sync_optimizer_steps())
+                opt.register_load_state_dict_post_hook(self._state_was_loaded)
+
+    def _launch_at_step(self, state, launch):
+        """`launch` where scaler_state[3] is the count of completed steps of this state's parameter."""
+        behind = self._served[id(state)][1]
+        if behind == 0:
+            return launch()
+        with torch.cuda.stream(self.stream_obj):      # (None: the current one)
+            self.scaler_state[3:4].add_(behind)
+            launch()
+            self.scaler_state[3:4].sub_(behind)
 
     def sync_optimizer_steps(self):
-        """Writes the device's count of completed optimizer steps into the optimizer's `step`
-        entries (one host read).  torch.amp.GradScaler leaves `step` untouched on a skipped step;
+        """Writes the device's count of completed optimizer steps into the `step` entries that it
+        counted for (one host read).  torch.amp.GradScaler leaves `step` untouched on a skipped step;
         so does this, which is why the entries cannot simply be bumped on the host."""
-        opt = getattr(self, "_steps_owner", None)
-        if opt is None or not self.dyn_scale or not getattr(self, "_host_steps_stale", False):
+        if not self.dyn_scale or not getattr(self, "_host_steps_stale", False):
             return
         done = float(self.scaler_state[3].item())
-        for g in opt.param_groups:
-            for p in g["params"]:
-                st = opt.state.get(p)
-                if st and "step" in st:
-                    if torch.is_tensor(st["step"]):
-                        st["step"].fill_(done)
-                    else:
-                        st["step"] = done
+        for st, behind in self._served.values():
+            if torch.is_tensor(st["step"]):
+                st["step"].fill_(done + behind)
+            else:
+                st["step"] = done + behind
         self._host_steps_stale = False
+
+    def _state_was_loaded(self, opt):
+        """The optimizer's entries are what was loaded: the device's count is set from them before the next step."""
+        if self._steps_owner is not opt:
+            return
+        self._served = {}
+        self._host_steps_stale = False
+        self.__dict__.pop("_adam_tables", None)
 
     def scaler_state_dict(self):
         """The dynamic loss scaler's state in torch.amp.GradScaler.state_dict()'s layout (empty

@@ -91,3 +91,95 @@ def test_a_late_gradient_starts_at_step_one(make, monkeypatch):
     assert step(a, late, b) == [6, 3, 5]
     assert step(a, late, b) == [7, 4, 6]
     assert counts(opt) == [7, 6, 4]
+
+
+def optimizers():
+    from pfeife_amd.optim import AdamW8bit
+
+    return [torch.optim.Adam, torch.optim.AdamW, AdamW8bit]
+
+
+@pytest.fixture(params=range(3), ids=["Adam", "AdamW", "AdamW8bit"])
+def make(request):
+    return optimizers()[request.param]
+
+
+def test_a_late_gradient_under_a_scaler(make, monkeypatch):
+    """The same where the device counts the steps, some of which an overflow skips."""
+    a, b, late = make_parameters(8, 5, 6)
+    opt = make([a, b, late], lr=0.1)
+    step = Steps(make_worker(True), opt, monkeypatch)
+    assert [step(a, b) for _ in range(3)] == [[1, 1], [2, 2], [3, 3]]
+    assert step(a, b, overflow=True) == [None, None]
+    assert step(a, late, b) == [4, 1, 4]
+    assert step(a, late, b, overflow=True) == [None] * 3
+    assert step(a, late, b) == [5, 2, 5]
+    assert counts(opt) == [5, 5, 2]
+    assert step(a, late) == [6, 3]
+    assert step(a, late) == [7, 4]
+    assert step(a, late, b) == [8, 5, 6]
+    assert step(late, a, b) == [6, 9, 7]
+    assert step(late) == [7]
+    assert step(late, a) == [8, 10]
+    assert counts(opt) == [10, 7, 8]
+
+
+def test_a_group_without_gradients(make, monkeypatch):
+    """All of a group's gradients gone for a while: the device's count goes on, the group's does not."""
+    a, b = make_parameters(8, 5)
+    opt = make([{"params": [a]}, {"params": [b], "lr": 0.2}], lr=0.1)
+    step = Steps(make_worker(True), opt, monkeypatch)
+    assert [step(a, b), step(a), step(a), step(a, b), step(a, b)] == [[1, 1], [2], [3], [4, 2], [5, 3]]
+    assert counts(opt) == [5, 3]
+    assert [step(b), step(b)] == [[4], [5]] and counts(opt) == [5, 5]
+
+
+def test_an_older_state_that_is_loaded(make, monkeypatch):
+    """Loaded after steps that nobody asked the counts of: the next step is the loaded state's next, not the device's."""
+    import copy
+
+    a, b = make_parameters(8, 5)
+    opt = make([a, b], lr=0.1)
+    step = Steps(make_worker(True), opt, monkeypatch)
+    assert [step(a, b) for _ in range(2)][-1] == [2, 2]
+    saved = copy.deepcopy(opt.state_dict())
+    assert [step(a, b) for _ in range(3)][-1] == [5, 5]
+    opt.load_state_dict(copy.deepcopy(saved))      # (torch's optimizers go on counting in the tensors that they are given)
+    assert counts(opt) == [2, 2]
+    assert [step(a, b), step(a, b, overflow=True), step(a, b)] == [[3, 3], [None, None], [4, 4]]
+    assert counts(opt) == [4, 4]
+    # a state that one parameter is not in
+    del saved["state"][1]
+    step(a, b)
+    opt.load_state_dict(saved)
+    assert [step(a, b), step(a, b)] == [[3, 1], [4, 2]] and counts(opt) == [4, 2]
+
+
+def test_its_own_state_that_is_loaded(make, monkeypatch):
+    """What state_dict() gives shares the optimizer's tensors, as torch's optimizers have it: it knows of the steps since."""
+    a, b = make_parameters(8, 5)
+    opt = make([a, b], lr=0.1)
+    step = Steps(make_worker(True), opt, monkeypatch)
+    step(a, b)
+    live = opt.state_dict()
+    step(a, b), step(a, b)
+    opt.load_state_dict(live)
+    assert step(a, b) == [4, 4] and counts(opt) == [4, 4]
+
+
+def test_an_optimizer_that_changes_workers(make, monkeypatch):
+    """One that has stepped before it is given to a worker, another in its place, and the counts that stay when the worker goes."""
+    a, b, c = make_parameters(8, 5, 3)
+    opt, other = make([a, b], lr=0.1), make([c], lr=0.1)
+    plain = Steps(make_worker(False), opt, monkeypatch)
+    assert [plain(a, b), plain(a, b)] == [[1, 1], [2, 2]]
+    w = make_worker(True)
+    step = Steps(w, opt, monkeypatch)
+    assert [step(a, b), step(a, b)] == [[3, 3], [4, 4]]
+    step = Steps(w, other, monkeypatch)
+    assert [step(c), step(c)] == [[1], [2]]
+    assert counts(opt) == [4, 4] and counts(other) == [2]
+    step = Steps(w, opt, monkeypatch)
+    assert step(a, b) == [5, 5]
+    w.sync_optimizer_steps()      # (as release() does)
+    assert [float(opt.state[p]["step"]) for p in (a, b)] == [5, 5] and counts(other) == [2]
