@@ -449,7 +449,8 @@ template <typename F> __device__ __forceinline__ double sum_in_eights(int64_t fi
 
 // ---- preference ------------------------------------------------------------------------------------------------------------
 // A workgroup to a pair, half of it to a sequence (2i, 2i + 1):  reward = beta (sum or mean of logprobs - ref),  D = reward_2i - reward_2i+1,
-//   loss_i = -(1 - e) ln sigma(D) - e ln sigma(-D),   d loss_i / dD = sigma(D) - (1 - e).
+//   loss_i = -(1 - e) ln sigma(D) - e ln sigma(-D),   d loss_i / dD = e sigma(D) - (1 - e) sigma(-D)
+// (= sigma(D) - (1 - e), which would cancel for a pair far apart).
 __device__ __forceinline__ double softplus(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }   // -ln sigma(-x)
 
 struct PairArgs {
@@ -478,7 +479,8 @@ __device__ double pair_terms(const PairArgs& a, int64_t i, const double (&total)
     per_token[k] = !a.average ? 1.0 : count[k] > 0.0 ? 1.0 / count[k] : 0.0;
     reward[k] = a.beta * (total[k] * per_token[k] - (double)a.ref[2 * i + k]);
   }
-  const double D = reward[0] - reward[1], up = 1.0 / (1.0 + exp(-D)) - (1.0 - a.smoothing);
+  const double D = reward[0] - reward[1], t = exp(-fabs(D)), most = 1.0 / (1.0 + t), least = t / (1.0 + t);      // sigma(|D|), sigma(-|D|)
+  const double up = a.smoothing * (D >= 0.0 ? most : least) - (1.0 - a.smoothing) * (D >= 0.0 ? least : most);
   for (int k = 0; k < 2; ++k) {
     a.rewards[2 * i + k] = (float)reward[k];
     a.coef[2 * i + k] = (float)((k ? -up : up) * a.beta * per_token[k] / (double)a.pairs);

@@ -1,0 +1,32 @@
+"""The token losses at the ends of what they accept, against the same in 64 bits."""
+import pytest
+import torch
+
+from test_token_loss_gpu import check_gradient, logprobs64, make, parts
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("smoothing", [0.0, 1.0, 1e-12])
+def test_pairs_far_apart(smoothing):
+    """The slope of a pair whose rewards differ by 30 and by 40, either way: what is left of it is small and has all its digits.  It is off by D's
+    error times itself (|d ln sigma / dD| <= 1), a gradient's entry by that, p's error and a few roundings."""
+    from pfeife_amd.loss import preference_loss
+
+    x, y = make(torch.float32, 8, 5, 37, 0, seed=70)
+    y[1, 2] = 3
+    z, lp, seen, rel = logprobs64(x, y, 0)
+    s = lp.detach().sum(1)
+    far = torch.tensor([30.0, -30.0, 40.0, -40.0], device="cuda", dtype=torch.float64)
+    ref = torch.stack((s[0::2] - far / 2, s[1::2] + far / 2), 1).reshape(-1).float()
+    rewards = s - ref.double()
+    D = rewards[0::2] - rewards[1::2]
+    up = (smoothing * torch.sigmoid(D) - (1 - smoothing) * torch.sigmoid(-D)) / 4
+    g = torch.stack((up, -up), 1).view(-1, 1) * seen
+    off = ((rel + 2.0 ** -24 * (lp.detach().abs() + 4)) * seen).sum(1).view(-1, 2).sum(1).repeat_interleave(2).unsqueeze(1)
+    leaf = x.clone().requires_grad_()
+    loss, _ = preference_loss(leaf, y, ref, beta=1.0, label_smoothing=smoothing)
+    (d,) = torch.autograd.grad(loss, leaf)
+    (dz,) = torch.autograd.grad(lp, z, g)
+    check_gradient(d, dz, g, *parts(z, 1.0), rel, torch.float32, g.abs() * (off + 2.0 ** -22))
+    assert (d[seen].abs().amax(-1) > 0).all() if smoothing else (d[:2][seen[:2]].abs().amax(-1) > 1e-15).all()
