@@ -13,6 +13,7 @@ ratio with a KL term), each straight from the logits, and `PreferenceLoss` / `Po
 import math
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 import torch.nn as nn
 
 
@@ -125,6 +126,11 @@ def _issue(t, launch):
             launch(_raw_stream(index))
 
 
+def _has_tangent(*tensors):
+    """Is one of them a dual number of forward-mode differentiation?  (Such a tensor need not require a gradient.)"""
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 _LOGITS = (torch.float32, torch.float16, torch.bfloat16)
 
 
@@ -145,6 +151,8 @@ def _check_rows(who, logits, labels, ignore_index, temperature, shift):
         raise RuntimeError("%s: ignore_index is a whole number and shift a truth value" % who)
     if not 1e-6 <= temperature <= 1e6:
         raise RuntimeError("%s: temperature must lie in [1e-6, 1e6] (got %s)" % (who, temperature))
+    if _has_tangent(logits):
+        raise RuntimeError("%s: there is no forward-mode derivative" % who)
     if len(shape) != 3:
         logits = logits.reshape((math.prod(shape[:-2]),) + shape[-2:])
         labels = labels.reshape(logits.shape[:-1])
@@ -159,7 +167,7 @@ def _constant(who, name, t, shapes, like):
         raise RuntimeError("%s: %s is a floating tensor of shape %s on %s (got %s)"
                            % (who, name, " or ".join(map(str, shapes)), like.device,
                               "%s %s on %s" % (t.dtype, tuple(t.shape), t.device) if torch.is_tensor(t) else type(t).__name__))
-    if t.requires_grad:
+    if t.requires_grad or _has_tangent(t):
         raise RuntimeError("%s: no gradient flows to %s: detach it" % (who, name))
     return t if t.dtype == torch.float32 else t.to(torch.float32)
 
@@ -216,6 +224,8 @@ def _once(backward):
     wrapped = torch.autograd.function.once_differentiable(backward)
 
     def run(ctx, *grads):
+        if _has_tangent(*grads):
+            raise RuntimeError("a backward pass of the token losses has no forward-mode derivative")
         return (wrapped if torch.is_grad_enabled() else backward)(ctx, *grads)
 
     return staticmethod(run)
@@ -323,8 +333,9 @@ def token_logprobs(logits, labels, *, ignore_index=-100, temperature=1.0, shift=
 
     logits [..., T, V] (fp32, fp16 or bf16), labels int64 [..., T].  shift: row t is scored against label t + 1 (labels as
     the model's own input), the result has T - 1 tokens.  Tokens whose label is `ignore_index` give 0 and take no part, whatever
-    their logits hold; labels outside the vocabulary give NaN.  A backward pass is captured into a graph, as any of torch's, only
-    while no autograd graph made outside the capture holds the same leaves."""
+    their logits hold; labels outside the vocabulary give NaN.  There are no second and no forward-mode derivatives.  A
+    backward pass is captured into a graph, as any of torch's, only while no autograd graph made outside the capture holds the same
+    leaves."""
     x, y = _check_rows("token_logprobs", logits, labels, ignore_index, temperature, shift)
     cfg = (int(shift), ignore_index, float(temperature))
     out = _apply(_TokenLogprobFn, x, y, cfg)
