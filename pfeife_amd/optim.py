@@ -10,12 +10,23 @@ from .hip import ADAM8_BLOCK
 from .loss import _raw_stream, _table
 
 
+def _layout(p):
+    """How a dense tensor's elements lie in memory: [(size, stride)] of its dimensions, those that follow one another taken as one."""
+    runs = []
+    for size, stride in zip(p.shape, p.stride()):
+        if size > 1 and runs and runs[-1][1] == size * stride:
+            runs[-1] = (runs[-1][0] * size, stride)
+        elif size > 1:
+            runs.append((size, stride))
+    return runs or [(1, 1)]
+
+
 class AdamW8bit(torch.optim.Optimizer):
     """torch.optim.AdamW's update on fp32 parameters and gradients, with 8-bit moments.
 
     state[p] of a large parameter, in the order of p's storage: `exp_avg` and `exp_avg_sq_root` (float8_e4m3fn codes [n]; the second is the
-    square root of AdamW's `exp_avg_sq`), `exp_avg_scale` and `exp_avg_sq_root_scale` (fp32 [ceil(n / 256)]); of a small one `exp_avg`
-    and `exp_avg_sq` in fp32; both `step`.  Codes are rounded so that their mean is kept, by bits that the element, the parameter's
+    square root of AdamW's `exp_avg_sq`), `exp_avg_scale` and `exp_avg_sq_root_scale` (fp32 [ceil(n / 256)]), `layout` (sizes and strides that
+    order is of: a parameter that lies in memory otherwise is refused); of a small one `exp_avg` and `exp_avg_sq` in fp32; both `step`.  Codes are rounded so that their mean is kept, by bits that the element, the parameter's
     place in the optimizer and the step give: a run repeats itself."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, min_8bit_size=4096):
@@ -38,7 +49,7 @@ class AdamW8bit(torch.optim.Optimizer):
         for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
             for key, value in state_dict["state"].get(i, {}).items():
                 if torch.is_tensor(value):
-                    self.state[p][key] = value.detach().clone() if key == "step" else value.detach().clone().to(p.device)
+                    self.state[p][key] = value.detach().clone() if key in ("step", "layout") else value.detach().clone().to(p.device)
         # new state may lie where the old one did, and the old one's memory is wanted back
         for name in ("_seen", "_tables"):
             self.__dict__.pop(name, None)
@@ -52,6 +63,7 @@ class AdamW8bit(torch.optim.Optimizer):
                 st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
                 st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
             else:
+                st["layout"] = torch.tensor(_layout(p))
                 for key in ("exp_avg", "exp_avg_sq_root"):
                     st[key] = torch.zeros(n, dtype=torch.uint8, device=p.device).view(torch.float8_e4m3fn)
                     st[key + "_scale"] = torch.zeros(-(-n // ADAM8_BLOCK), dtype=torch.float32, device=p.device)
@@ -65,7 +77,17 @@ class AdamW8bit(torch.optim.Optimizer):
         return st["exp_avg"], None, st["exp_avg_sq"], None
 
     @staticmethod
-    def _check(p, g, ops):
+    def _check_layout(p, st):
+        """Codes are in the order of a parameter's storage: that has to be the one they were made in."""
+        held, now = st.get("layout"), _layout(p)
+        if held is None:      # (not noted: taken as the parameter's)
+            st["layout"] = torch.tensor(now)
+        elif [tuple(run) for run in held.tolist()] != now:
+            raise RuntimeError("AdamW8bit: the optimizer's state does not fit its parameter of shape %s: its elements lie in memory by (size, stride) %s, "
+                               "the moments' by %s" % (tuple(p.shape), now, held.tolist()))
+
+    @staticmethod
+    def _check(p, g, ops, st):
         """The gradient as the kernel addresses it; errors where it, the parameter or the state is not what the kernel takes."""
         if p.device.type != "cuda":
             raise RuntimeError("AdamW8bit: the HIP step needs GPU parameters (got %s)" % p.device)
@@ -82,6 +104,8 @@ class AdamW8bit(torch.optim.Optimizer):
                        for t in ops[::2])
         if not fits:
             raise RuntimeError("AdamW8bit: the optimizer's state does not fit its parameter of shape %s" % (tuple(p.shape),))
+        if ops[1] is not None:
+            AdamW8bit._check_layout(p, st)
         return g if g.stride() == p.stride() or g.is_contiguous() and p.is_contiguous() else torch.empty_like(p)     # (of another layout: copied for each step)
 
     @staticmethod
@@ -127,7 +151,7 @@ class AdamW8bit(torch.optim.Optimizer):
                 ent = cache.get((gi, n))
                 if ent is None or ent[0] != now:
                     fresh = True
-                    items = [(p.data, self._check(p, g, ops), *ops, index) for p, g, ops, index in params]
+                    items = [(p.data, self._check(p, g, ops, st), *ops, index) for (p, g, ops, index), st in zip(params, states)]
                     self._check_apart(params)
                     copies = [(i[1], p) for (p, g, _, _), i in zip(params, items) if i[1] is not g]
                     ent = cache[gi, n] = (now, kernels.adam8_table(items), copies)
