@@ -89,6 +89,8 @@ class AdamW8bit(torch.optim.Optimizer):
     @staticmethod
     def _check(p, g, ops, st):
         """The gradient as the kernel addresses it; errors where it, the parameter or the state is not what the kernel takes."""
+        if p.dtype != torch.float32 or g.shape != p.shape:
+            raise RuntimeError("AdamW8bit: parameters are fp32, gradients of their shape (got %s %s and %s)" % (p.dtype, tuple(p.shape), tuple(g.shape)))
         if p.device.type != "cuda":
             raise RuntimeError("AdamW8bit: the HIP step needs GPU parameters (got %s)" % p.device)
         if g.dtype != torch.float32 or g.device != p.device:
@@ -143,7 +145,7 @@ class AdamW8bit(torch.optim.Optimizer):
                 found[1].append((p, g, ops, place - 1))
                 found[2].append((place, *[t if t is None else (t.data_ptr(), t.dtype, t.numel()) for t in (p, g, *ops)], g.stride(), p.stride()))
                 keys = ("exp_avg", "exp_avg_scale", "exp_avg_sq_root", "exp_avg_sq_root_scale") if ops[1] is not None else ("exp_avg", "exp_avg_sq")
-                records.append((p, st, found[0], p.data_ptr(), p.numel(), g.data_ptr(), [(k, st[k], st[k].data_ptr(), st[k].numel()) for k in keys]))
+                records.append((p, st, found[0], p.data_ptr(), 4 * p.numel(), g.data_ptr(), [(k, st[k], st[k].data_ptr(), st[k].numel()) for k in keys]))
                 plain = plain and p.is_contiguous() and g.is_contiguous()
             for n, key in enumerate(sorted(by_step)):
                 states, params, now = by_step[key]
@@ -179,8 +181,8 @@ class AdamW8bit(torch.optim.Optimizer):
                         return False
                     continue
                 st = r[1]
-                if (g is None or state.get(p) is not st or st["step"] != r[2][0]["step"] or p.data_ptr() != r[3] or p.numel() != r[4]
-                        or g.data_ptr() != r[5] or not p.is_contiguous() or not g.is_contiguous()):
+                if (g is None or state.get(p) is not st or st["step"] != r[2][0]["step"] or p.data_ptr() != r[3] or p.nbytes != r[4]
+                        or g.data_ptr() != r[5] or g.nbytes != r[4] or not p.is_contiguous() or not g.is_contiguous()):
                     return False
                 for key, t, where, n in r[6]:
                     if st.get(key) is not t or t.data_ptr() != where or t.numel() != n:
