@@ -40,7 +40,8 @@ __device__ __forceinline__ LabelKind label_kind(const TokenRows& r, int64_t y) {
 // A row is read once, 16 bytes to a lane and access, NV accesses of a lane in flight; the row stays in the registers that it was loaded to, so that a gradient of the same pass is formed from there.  Each lane sums 2^(x c - ref) against a
 // reference of its own, the whole number from its largest x c on: no exchange between lanes before the end, and one FMA and one exponential
 // to an element.  Sums of eight go into a double.  What such arithmetic cannot do (a row of nothing but the lowest values, where
-// x c overflows, infinities, NaN) shows as a sum that is not a positive number, and is done again as (x - m) c.
+// x c overflows, infinities, NaN, x c past 2^29, where a whole number near it is no longer within 32 of it) shows as a sum outside
+// (2^-32, 2^60), and is done again as (x - m) c.  (Below 2^24 the largest element's term lies between 1/4 and 2; there are 2^28 classes at most.)
 typedef uint32_t raw4 __attribute__((ext_vector_type(4)));
 typedef uint32_t raw4_any __attribute__((ext_vector_type(4), aligned(2)));      // (the memory unit takes any alignment)
 
@@ -280,7 +281,7 @@ __device__ __forceinline__ RowStats row_stats(const TokenRows& r, RowReader<DT, 
   }
   row.sum_loose(r.c, a);
   join_row<ONE, FIRST>(a, sm);
-  RowStats o = {a.ref, 0.f, !(a.s > 0.0 && a.s < INFINITY), 0.0};
+  RowStats o = {a.ref, 0.f, !(a.s > 0x1p-32 && a.s < 0x1p60), 0.0};      // (1 / s times a small gradient is then no subnormal number)
   if (o.slow) {
     a.s = slow_sums<DT, ONE>(row.x, (int)r.V, r.c, &o.ref, sm ? sm->s : nullptr);
     o.logprob = ((double)xy - (double)o.ref) * r.inv_temp - log(a.s);

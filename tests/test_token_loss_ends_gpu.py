@@ -1,4 +1,6 @@
 """The token losses at the ends of what they accept, against the same in 64 bits."""
+import math
+
 import pytest
 import torch
 
@@ -30,3 +32,25 @@ def test_pairs_far_apart(smoothing):
     (dz,) = torch.autograd.grad(lp, z, g)
     check_gradient(d, dz, g, *parts(z, 1.0), rel, torch.float32, g.abs() * (off + 2.0 ** -22))
     assert (d[seen].abs().amax(-1) > 0).all() if smoothing else (d[:2][seen[:2]].abs().amax(-1) > 1e-15).all()
+
+
+@pytest.mark.parametrize("temperature", [1.0, 1e-6])
+def test_huge_logits(temperature):
+    """Rows whose largest logits over the temperature lie between 2^30 and 2^34, where fp32 numbers are hundreds apart: two classes share a row's
+    probability to the last digit, however small the gradient that comes in."""
+    from pfeife_amd.loss import policy_loss, token_logprobs
+
+    n = 2000
+    g = torch.Generator().manual_seed(71)
+    top = (2.0 ** (30 + 4 * torch.rand(n, generator=g, dtype=torch.float64)) * temperature).float()
+    x = torch.stack((top / 2, top, -top, top, top * 0.75), 1).unsqueeze(0).cuda()
+    y = torch.full((1, n), 3, device="cuda")
+    for small in (1e-6, 1e-12):
+        leaf = x.clone().requires_grad_()
+        lp = token_logprobs(leaf, y, temperature=temperature)
+        assert ((lp + math.log(2)).abs() <= 4 * 2.0 ** -24).all()
+        for out, inflow in ((lp, torch.full_like(lp, small)),
+                            (policy_loss(leaf, y, lp.detach(), torch.full((1,), -small * n, device="cuda"), temperature=temperature)[0], None)):
+            (d,) = torch.autograd.grad(out, leaf, inflow)
+            want = 0.5 * small / temperature * torch.tensor([0.0, -1.0, 0.0, 1.0, 0.0], device="cuda", dtype=torch.float64)
+            assert ((d.double() - want).abs() <= 16 * 2.0 ** -24 * want.abs()).all()
