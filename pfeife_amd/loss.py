@@ -10,6 +10,7 @@ For fine-tuning a language model: `token_logprobs` (log-probabilities of given t
 `preference_loss` (paired log ratios against a reference model) and `policy_loss` (clipped
 ratio with a KL term), each straight from the logits, and `PreferenceLoss` / `PolicyLoss`.
 """
+import functools
 import math
 
 import torch
@@ -181,20 +182,50 @@ def _new(like, *shape, dtype=torch.float32):
     return torch.empty(shape, dtype=dtype, device=like.device)
 
 
-def _logits_gradient(ctx, logits, labels, stats, coef, g_strides, scale=None, into=None, unless_one=0):
-    """stats, coef, scale: addresses.  Autograd calls this on a thread of its own, which finds little in its core's caches: it does no more
-    than it must, and takes the forward pass's description of the rows where they still lie there."""
+def _logits_gradient(ctx, logits, labels, stats, coef, g_strides, keep, scale=None, into=None, unless_one=0):
+    """stats, coef: addresses within `keep`; scale: a tensor of one element.  Autograd calls this on a thread of its own, which finds little in its
+    core's caches: it does no more than it must, and takes the forward pass's description of the rows where they still lie there."""
     rows, strides, k = ctx.rows
     if logits.data_ptr() != rows[0] or labels.data_ptr() != rows[7] or logits.stride() != strides:      # (hooks may move what is saved)
         rows = _rows(logits, labels, rows[8:])
     d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if into is None else into
     index = logits.get_device()
+    at = None if scale is None else scale.data_ptr()
     if _current_device() == index:
-        k.token_gradient(rows, stats, coef, g_strides, d, scale, unless_one, _raw_stream(index))
+        k.token_gradient(rows, stats, coef, g_strides, d, at, unless_one, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            k.token_gradient(rows, stats, coef, g_strides, d, scale, unless_one, _raw_stream(index))
+            k.token_gradient(rows, stats, coef, g_strides, d, at, unless_one, _raw_stream(index))
+    if ctx.scaled:
+        d._pf_times = d._version, functools.partial(_gradient_times, k, rows, stats, coef, g_strides, scale, (logits, labels, keep))
     return d
+
+
+def _gradient_times(k, rows, stats, coef, g_strides, scale, keep, factor, out):
+    """The gradient times a loss scale, rounded once, where multiplying the fp16 gradient would find its small entries gone; -> is it written."""
+    like = keep[0]
+    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or out.stride(-1) != 1:
+        return False
+    by = factor if scale is None else scale * factor
+    k.token_gradient(rows, stats, coef, g_strides, out, by.data_ptr(), 0, _raw_stream(out.get_device()))
+    return True
+
+
+def mark_loss_scaled(output):
+    """Notes that the gradient of this output of a runner will be multiplied by a loss scale: a token loss of it, if it is in fp16, then leaves
+    with its gradient how to form the product itself (`scaled_gradient`)."""
+    output._pf_loss_scaled = True
+
+
+def scaled_gradient(grad, factor, out):
+    """`out` = grad times `factor` (fp32 on the device, of one element) from what a token loss left with it, on the current stream; -> is it written.
+    Not where the gradient is a sum of several or was changed."""
+    version, write = getattr(grad, "_pf_times", (None, None))
+    return write is not None and grad._version == version and write(factor, out)
+
+
+def _wants_scale(logits):
+    return logits.dtype == torch.float16 and getattr(logits, "_pf_loss_scaled", False)
 
 
 def _as_scale(g):
@@ -242,14 +273,14 @@ class _TokenLogprobFn(torch.autograd.Function):
         _issue(logits, k.token_logprob_fwd(rows, out, stats))
         if want:
             ctx.save_for_backward(logits, labels, stats)
-            ctx.rows = rows, logits.stride(), k
+            ctx.rows, ctx.scaled = (rows, logits.stride(), k), _wants_scale(logits)
         return out
 
     @_once
     def backward(ctx, grad):
         logits, labels, stats = ctx.saved_tensors
         grad = _as_scale(grad)      # (any strides: a sum's gradient is one number)
-        return _logits_gradient(ctx, logits, labels, stats.data_ptr(), grad.data_ptr(), grad.stride()), None
+        return _logits_gradient(ctx, logits, labels, stats.data_ptr(), grad.data_ptr(), grad.stride(), (stats, grad)), None
 
 
 class _PreferenceFn(torch.autograd.Function):
@@ -268,7 +299,7 @@ class _PreferenceFn(torch.autograd.Function):
         _issue(logits, k.preference_loss(rows, ref, beta, smoothing, average, loss, rewards, stats if want else None, coef, work))
         if want:
             ctx.save_for_backward(logits, labels, work)
-            ctx.rows, ctx.at = (rows, logits.stride(), k), (8 * n, 8 * (n + scored))
+            ctx.rows, ctx.at, ctx.scaled = (rows, logits.stride(), k), (8 * n, 8 * (n + scored)), _wants_scale(logits)
         ctx.mark_non_differentiable(rewards)
         ctx.set_materialize_grads(False)
         return loss, rewards
@@ -279,7 +310,7 @@ class _PreferenceFn(torch.autograd.Function):
         if grad is None:
             return None, None
         at, (stats, coef), grad = work.data_ptr(), ctx.at, _as_scale(grad)
-        return _logits_gradient(ctx, logits, labels, at + stats, at + coef, (1, 0), grad.data_ptr()), None
+        return _logits_gradient(ctx, logits, labels, at + stats, at + coef, (1, 0), work, grad), None
 
 
 class _PolicyFn(torch.autograd.Function):
@@ -308,7 +339,7 @@ class _PolicyFn(torch.autograd.Function):
         _issue(logits, k.policy_loss(rows, old, adv, a_strides, ref, *clip, kl_coef, by_sequence, scale, loss, kl, logprobs, stats, coef, d, strides, work))
         if want:
             ctx.save_for_backward(logits, labels, work)
-            ctx.rows, ctx.at = (rows, logits.stride(), k), (8 * n, 8 * (n + B * R), (R, 1))
+            ctx.rows, ctx.at, ctx.scaled = (rows, logits.stride(), k), (8 * n, 8 * (n + B * R), (R, 1)), _wants_scale(logits)
             ctx.d, ctx.captured = d, torch.cuda.is_current_stream_capturing()
         ctx.mark_non_differentiable(logprobs, kl)
         ctx.set_materialize_grads(False)
@@ -325,7 +356,7 @@ class _PolicyFn(torch.autograd.Function):
         if d is not None and ctx.captured != torch.cuda.is_current_stream_capturing():
             d = None
         at, (stats, coef, strides), grad = work.data_ptr(), ctx.at, _as_scale(grad)
-        return _logits_gradient(ctx, logits, labels, at + stats, at + coef, strides, grad.data_ptr(), d, 0 if d is None else 1), None
+        return _logits_gradient(ctx, logits, labels, at + stats, at + coef, strides, work, grad, d, 0 if d is None else 1), None
 
 
 def token_logprobs(logits, labels, *, ignore_index=-100, temperature=1.0, shift=False):

@@ -38,6 +38,7 @@ from ...executor.values import Val
 from ...graph.canonicalize import canonicalize
 from ...graph.partition_graph import compute_nodes, is_static_placeholder, partition_by_split_points
 from ...hip import Baton
+from ...loss import mark_loss_scaled
 from ...option import PipeOption
 from ...utils import get_logger, to_device
 from ..net_states import get_state
@@ -424,6 +425,8 @@ class PartialModule(nn.Module):
                     t.requires_grad_()
                     if not probe:
                         t.register_hook(partial(self._runner.backward_hook, mb, oi))
+                        if worker.scales_loss:
+                            mark_loss_scaled(t)
                 outs.append(t)
             else:
                 outs.append(v)

@@ -21,6 +21,7 @@ import torch
 from ..executor.lowering import BufferPool, Lowerer, ParamStore, Unsupported
 from ..executor.merge import MicroBatchLayout
 from ..executor.values import Val
+from ..loss import scaled_gradient
 from ..optim import AdamW8bit
 from ..option import get_optimizer_cls
 from ..schedule.scheduler import PipeSchedParams, SingleCommScheduler, StepWork, serialize_ranks
@@ -657,6 +658,8 @@ class StageWorker:
         if g.shape != buf.shape:
             raise RuntimeError("loss gradient of output %d has shape %s, expected %s"
                                % (out_idx, tuple(g.shape), tuple(buf.shape)))
+        if self._scaled_by_its_loss(grad, buf):
+            return
         if self.dyn_scale:
             if g.device == buf.device and g.dtype.is_floating_point and g.is_contiguous() and buf.is_contiguous():
                 self.kernels.scale_by_state(g, self.scaler_state, buf, g.numel())(self.stream())
@@ -675,6 +678,24 @@ class StageWorker:
                 self.kernels.cast(g, buf, g.numel())(self.stream())
         else:
             buf.copy_(g * scale if scale != 1.0 else g)
+
+    @property
+    def scales_loss(self):
+        return self.dyn_scale or self.option.loss_scale != 1.0
+
+    def _scaled_by_its_loss(self, grad, buf):
+        """A token loss's gradient in fp16, times the loss scale before its rounding: of entries below 2^-25 nothing is left to be
+        multiplied afterwards (97 % of a policy loss's over 5000 tokens of 32000 classes)."""
+        if not self.scales_loss or not hasattr(grad, "_pf_times"):
+            return False
+        if self.dyn_scale:
+            factor = self.scaler_state[0:1]
+        else:
+            factor = self.__dict__.get("_scale_on_device")
+            if factor is None:
+                factor = self._scale_on_device = torch.full((1,), self.option.loss_scale, dtype=torch.float32, device=buf.device)
+        with torch.cuda.stream(self.stream_obj):
+            return scaled_gradient(grad, factor, buf)
 
     def finish_micro_batch(self, mb):
         """Outputs whose hook never fired: zero gradient, except scalars which get 1
