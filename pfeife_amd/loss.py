@@ -313,10 +313,14 @@ class _PreferenceFn(torch.autograd.Function):
         return _logits_gradient(ctx, logits, labels, at + stats, at + coef, (1, 0), work, grad), None
 
 
+_saving_hooks = getattr(torch._C._autograd, "_top_saved_tensors_default_hooks", lambda ignore_is_tracing: None)
+
+
 class _PolicyFn(torch.autograd.Function):
     """The gradient of a loss that is itself the end (`loss.backward()`) is written by the forward pass, which has the row at
     hand: a token's part of it depends on its own row alone.  The backward pass looks at what it is asked to multiply it
-    by, on the device: by one it has nothing to do, by anything else it computes the gradient from the logits."""
+    by, on the device: by one it has nothing to do, by anything else it computes the gradient from the logits.  It does so too where
+    hooks take what is saved (off the device, or to forget it): they are there to save memory, and the gradient is as large as the logits."""
 
     @staticmethod
     def forward(ctx, logits, args, want=True):
@@ -332,8 +336,9 @@ class _PolicyFn(torch.autograd.Function):
             work = _new(logits, n + B * R + (B * R + 1) // 2, dtype=torch.float64)
             stats = work.data_ptr() + 8 * n
             coef = stats + 8 * B * R
-            d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-            strides = d.stride()[:2]
+            if _saving_hooks(False) is None:
+                d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+                strides = d.stride()[:2]
         else:
             work = _new(logits, n, dtype=torch.float64)
         _issue(logits, k.policy_loss(rows, old, adv, a_strides, ref, *clip, kl_coef, by_sequence, scale, loss, kl, logprobs, stats, coef, d, strides, work))

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from test_token_loss_gpu import check_gradient, logprobs64, make, parts
+from test_token_loss_gpu import LEAST, U, check_gradient, logprobs64, make, parts
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +54,35 @@ def test_huge_logits(temperature):
             (d,) = torch.autograd.grad(out, leaf, inflow)
             want = 0.5 * small / temperature * torch.tensor([0.0, -1.0, 0.0, 1.0, 0.0], device="cuda", dtype=torch.float64)
             assert ((d.double() - want).abs() <= 16 * 2.0 ** -24 * want.abs()).all()
+
+
+def test_hooks_get_all_of_the_policy_loss_memory():
+    """Where hooks take what the backward pass needs off the device, or a checkpoint forgets it, the loss leaves nothing as large as the logits behind.
+    The gradient may come from sums in another order (each off by (V / 64 + 96) 2^-24) and be rounded the other way."""
+    from torch.utils.checkpoint import checkpoint
+
+    from pfeife_amd.loss import policy_loss
+
+    x, y = make(torch.bfloat16, 2, 64, 65536, 0, seed=75, masked=0.0)
+    old, adv = torch.full((2, 64), -10.0, device="cuda"), torch.ones(2, device="cuda")
+    leaf = x.requires_grad_()
+    (want,) = torch.autograd.grad(policy_loss(leaf, y, old, adv)[0], leaf)
+    size = x.numel() * 2
+
+    def left(call):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        loss = call()
+        grown = torch.cuda.memory_allocated() - before
+        (d,) = torch.autograd.grad(loss, leaf)
+        step = 2 * (65536 / 64 + 96) * 2.0 ** -24 + 2 * U[torch.bfloat16]
+        assert ((d.double() - want.double()).abs() <= step * want.double().abs() + 2 * LEAST[torch.bfloat16]).all()
+        return grown
+
+    def on_cpu():
+        with torch.autograd.graph.save_on_cpu():
+            return policy_loss(leaf, y, old, adv)[0]
+
+    assert left(lambda: policy_loss(leaf, y, old, adv)[0]) >= size      # (the gradient, which the forward pass writes)
+    assert left(on_cpu) < size // 8
+    assert left(lambda: checkpoint(lambda t: policy_loss(t, y, old, adv)[0], leaf, use_reentrant=False)) < size // 8
