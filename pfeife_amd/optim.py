@@ -160,13 +160,13 @@ class AdamW8bit(torch.optim.Optimizer):
                 work.append((group, states, params[0][0].device, *ent[1:]))
         devices = {w[2].index for w in work}
         # (one device, dense tensors: what _as_seen looks at says that all is as it was)
-        self._seen = ((records, [len(g["params"]) for g in self.param_groups], devices.pop(), work and _raw_stream(work[0][2].index)), work) \
+        self._seen = ((records, [(g, len(g["params"])) for g in self.param_groups], devices.pop(), work and _raw_stream(work[0][2].index)), work) \
             if plain and len(devices) == 1 else None
         return work, fresh
 
     def _as_seen(self, records, counts, device, stream):
         """Is every address where the last step's tables have it, and every count of steps still its group's?"""
-        if len(counts) != len(self.param_groups) or any(len(g["params"]) != n for g, n in zip(self.param_groups, counts)) or _raw_stream(device) != stream:
+        if len(counts) != len(self.param_groups) or any(g is not h or len(g["params"]) != n for g, (h, n) in zip(self.param_groups, counts)) or _raw_stream(device) != stream:
             return False
         at = iter(records)
         state = self.state

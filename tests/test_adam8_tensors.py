@@ -37,3 +37,26 @@ def test_exchanged_memory(change, seen, monkeypatch):
     st = opt._init_state(p, opt.param_groups[0])
     with pytest.raises(RuntimeError, match="parameters are fp32, gradients of their shape"):
         opt._check(p, p.grad, opt._operands(p, st), st)
+
+
+def test_groups_that_are_made_anew(monkeypatch):
+    """The same parameters in a new group, with another learning rate: the next step is the new group's."""
+    from pfeife_amd import optim
+
+    monkeypatch.setattr(optim, "_raw_stream", lambda index: 0)
+    monkeypatch.setattr(optim.AdamW8bit, "_check", staticmethod(lambda p, g, *_: g))
+
+    class Kernels:
+        def adam8_table(self, items):
+            return items, 1, 1
+
+    p = torch.nn.Parameter(torch.zeros(6000))
+    p.grad = torch.ones(6000)
+    opt = optim.AdamW8bit([p], lr=0.5)
+    assert [w[0]["lr"] for w in opt._prepare(Kernels())[0]] == [0.5]
+    opt.param_groups.clear()
+    opt.add_param_group({"params": [p], "lr": 0.25})
+    work, fresh = opt._prepare(Kernels())
+    assert [w[0]["lr"] for w in work] == [0.25] and work[0][0] is opt.param_groups[0] and not fresh
+    opt.param_groups[0]["lr"] = 0.125
+    assert opt._prepare(Kernels())[0][0][0]["lr"] == 0.125
