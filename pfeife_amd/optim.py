@@ -44,6 +44,8 @@ class AdamW8bit(torch.optim.Optimizer):
                 raise RuntimeError("AdamW8bit: parameters are fp32 (got %s)" % p.dtype)
 
     def load_state_dict(self, state_dict):
+        if any(g.get(name) for g in state_dict["param_groups"] for name in ("amsgrad", "maximize")):
+            raise RuntimeError("AdamW8bit: state of an optimizer with amsgrad or maximize, of which there is neither here")
         super().load_state_dict(state_dict)      # gives every state tensor the parameter's type, and may share the dict's tensors
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
