@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from test_token_loss_gpu import LEAST, U, check_gradient, logprobs64, make, parts
+from test_token_loss_gpu import LEAST, U, check_gradient, logprobs64, make, parts, policy_operands
 
 pytestmark = pytest.mark.gpu
 
@@ -54,6 +54,62 @@ def test_huge_logits(temperature):
             (d,) = torch.autograd.grad(out, leaf, inflow)
             want = 0.5 * small / temperature * torch.tensor([0.0, -1.0, 0.0, 1.0, 0.0], device="cuda", dtype=torch.float64)
             assert ((d.double() - want).abs() <= 16 * 2.0 ** -24 * want.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("temperature", [1e-6, 1e6])
+def test_temperatures_at_the_ends(dtype, temperature):
+    """At 1e-6 a row's probability lies on its largest logits alone, at 1e6 on all alike; the labels of the first are the largest or near it."""
+    from pfeife_amd.loss import policy_loss, token_logprobs
+
+    x, y = make(dtype, 2, 40, 1003, 0, seed=72, masked=0.2)
+    if temperature < 1:
+        at = y.clamp_min(0).unsqueeze(-1)
+        x.scatter_(2, at, x.amax(-1, keepdim=True))      # (its equal, so half of the probability)
+        x[:, ::3] *= 1e-6                                # and rows whose logits over the temperature are ordinary
+    z, lp, seen, rel = logprobs64(x, y, 0, temperature)
+    assert torch.isfinite(lp).all()
+    leaf = x.clone().requires_grad_()
+    got = token_logprobs(leaf, y, temperature=temperature)
+    # (x - m) / temperature of the label is formed from fp32 factors where the sum is: some 2^-23 of it
+    far = ((z.amax(-1) - z.gather(-1, y.clamp_min(0).unsqueeze(-1)).squeeze(-1)) / temperature).detach()
+    tol = rel + 2.0 ** -24 * (lp.detach().abs() + 4) + 2.0 ** -22 * far
+    assert ((got.double() - lp).abs() <= tol)[seen].all()
+    inflow = torch.linspace(-2, 2, lp.numel(), device="cuda").view(lp.shape)
+    (d,), (dz,) = torch.autograd.grad(got, leaf, inflow), torch.autograd.grad(lp, z, inflow.double(), retain_graph=True)
+    check_gradient(d, dz, inflow.double() * seen / temperature, *parts(z, temperature), rel, dtype, torch.zeros_like(rel))
+    loss, logprobs, _ = policy_loss(leaf, y, got.detach() - 0.1, torch.ones(2, device="cuda"), temperature=temperature)
+    assert ((logprobs.double() - lp).abs() <= tol)[seen].all()
+    (d,) = torch.autograd.grad(loss, leaf)
+    ratio = torch.exp(lp.detach() - (got.detach() - 0.1).double())
+    gg = -ratio * seen / seen.sum()
+    (dz,) = torch.autograd.grad(lp, z, gg)
+    check_gradient(d, dz, gg / temperature, *parts(z, temperature), rel, dtype, gg.abs() / temperature * (2 * tol + 2.0 ** -22))
+
+
+@pytest.mark.parametrize("clip,clip_high", [(0.0, 0.0), (1.0, 0.28), (1.5, 3.0), (0.2, 1e30)])
+def test_wide_and_no_clips(clip, clip_high):
+    """A lower bound of one or more never holds (a ratio is positive), nor does an upper one that no ratio reaches; with none at all every ratio
+    but one is outside."""
+    from pfeife_amd.loss import policy_loss
+
+    x, y = make(torch.float32, 3, 30, 101, 0, seed=73)
+    z, lp, seen, rel = logprobs64(x, y, 0)
+    old, ref, adv = policy_operands(lp.detach(), 74)
+    old -= 0.01 * (old == lp.float())       # (no ratio at a border)
+    ratio = torch.exp(lp - old.double())
+    a = adv.double()
+    token = -torch.minimum(ratio * a, ratio.clamp(1 - clip, 1 + clip_high) * a)
+    want = torch.where(seen, token, 0.0).sum() / seen.sum()
+    leaf = x.clone().requires_grad_()
+    loss = policy_loss(leaf, y, old, adv, clip=clip, clip_high=clip_high)[0]
+    dlp = (rel + 2.0 ** -24) * seen
+    size = (ratio.detach() * a.abs() * seen / seen.sum())
+    assert abs(float(loss.detach()) - float(want.detach())) <= float((size * (dlp + 2.0 ** -23)).sum()) * 2 + 2.0 ** -24 * abs(float(want.detach())) + 1e-14
+    (d,), (dz,) = torch.autograd.grad(loss, leaf), torch.autograd.grad(want, z)
+    free = torch.where(a >= 0, ratio <= 1 + clip_high, ratio >= 1 - clip)
+    g = torch.where(free & seen, -a * ratio.detach() / seen.sum(), 0.0)
+    check_gradient(d, dz, g, *parts(z, 1.0), rel, torch.float32, 2 * size * dlp + 2.0 ** -23 * g.abs())
 
 
 def test_hooks_get_all_of_the_policy_loss_memory():
