@@ -12,6 +12,7 @@ ratio with a KL term), each straight from the logits, and `PreferenceLoss` / `Po
 """
 import functools
 import math
+from types import SimpleNamespace
 
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -127,9 +128,13 @@ def _issue(t, launch):
             launch(_raw_stream(index))
 
 
+# the level of forward-mode differentiation, -1 outside of it
+_dual = forward_ad if hasattr(forward_ad, "_current_level") else SimpleNamespace(_current_level=0)
+
+
 def _has_tangent(*tensors):
-    """Is one of them a dual number of forward-mode differentiation?  (Such a tensor need not require a gradient.)"""
-    return getattr(forward_ad, "_current_level", 0) >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    """Is one of them a dual number of forward-mode differentiation?  (Such a tensor need not require a gradient.)  Asked at a level of it."""
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 _LOGITS = (torch.float32, torch.float16, torch.bfloat16)
@@ -152,7 +157,7 @@ def _check_rows(who, logits, labels, ignore_index, temperature, shift):
         raise RuntimeError("%s: ignore_index is a whole number and shift a truth value" % who)
     if not 1e-6 <= temperature <= 1e6:
         raise RuntimeError("%s: temperature must lie in [1e-6, 1e6] (got %s)" % (who, temperature))
-    if _has_tangent(logits):
+    if _dual._current_level >= 0 and _has_tangent(logits):
         raise RuntimeError("%s: there is no forward-mode derivative" % who)
     if len(shape) != 3:
         logits = logits.reshape((math.prod(shape[:-2]),) + shape[-2:])
@@ -168,7 +173,7 @@ def _constant(who, name, t, shapes, like):
         raise RuntimeError("%s: %s is a floating tensor of shape %s on %s (got %s)"
                            % (who, name, " or ".join(map(str, shapes)), like.device,
                               "%s %s on %s" % (t.dtype, tuple(t.shape), t.device) if torch.is_tensor(t) else type(t).__name__))
-    if t.requires_grad or _has_tangent(t):
+    if t.requires_grad or _dual._current_level >= 0 and _has_tangent(t):
         raise RuntimeError("%s: no gradient flows to %s: detach it" % (who, name))
     return t if t.dtype == torch.float32 else t.to(torch.float32)
 
@@ -185,7 +190,7 @@ def _new(like, *shape, dtype=torch.float32):
 def _logits_gradient(ctx, logits, labels, stats, coef, g_strides, keep, scale=None, into=None, unless_one=0):
     """stats, coef: addresses within `keep`; scale: a tensor of one element.  Autograd calls this on a thread of its own, which finds little in its
     core's caches: it does no more than it must, and takes the forward pass's description of the rows where they still lie there."""
-    rows, strides, k = ctx.rows
+    rows, strides, k, scaled = ctx.rows
     if logits.data_ptr() != rows[0] or labels.data_ptr() != rows[7] or logits.stride() != strides:      # (hooks may move what is saved)
         rows = _rows(logits, labels, rows[8:])
     d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if into is None else into
@@ -196,7 +201,7 @@ def _logits_gradient(ctx, logits, labels, stats, coef, g_strides, keep, scale=No
     else:
         with torch.cuda.device(index):
             k.token_gradient(rows, stats, coef, g_strides, d, at, unless_one, _raw_stream(index))
-    if ctx.scaled:
+    if scaled:
         d._pf_times = d._version, functools.partial(_gradient_times, k, rows, stats, coef, g_strides, scale, (logits, labels, keep))
     return d
 
@@ -255,7 +260,7 @@ def _once(backward):
     wrapped = torch.autograd.function.once_differentiable(backward)
 
     def run(ctx, *grads):
-        if _has_tangent(*grads):
+        if _dual._current_level >= 0 and _has_tangent(*grads):
             raise RuntimeError("a backward pass of the token losses has no forward-mode derivative")
         return (wrapped if torch.is_grad_enabled() else backward)(ctx, *grads)
 
@@ -273,7 +278,7 @@ class _TokenLogprobFn(torch.autograd.Function):
         _issue(logits, k.token_logprob_fwd(rows, out, stats))
         if want:
             ctx.save_for_backward(logits, labels, stats)
-            ctx.rows, ctx.scaled = (rows, logits.stride(), k), _wants_scale(logits)
+            ctx.rows = rows, logits.stride(), k, _wants_scale(logits)
         return out
 
     @_once
@@ -299,7 +304,7 @@ class _PreferenceFn(torch.autograd.Function):
         _issue(logits, k.preference_loss(rows, ref, beta, smoothing, average, loss, rewards, stats if want else None, coef, work))
         if want:
             ctx.save_for_backward(logits, labels, work)
-            ctx.rows, ctx.at, ctx.scaled = (rows, logits.stride(), k), (8 * n, 8 * (n + scored)), _wants_scale(logits)
+            ctx.rows, ctx.at = (rows, logits.stride(), k, _wants_scale(logits)), (8 * n, 8 * (n + scored))
         ctx.mark_non_differentiable(rewards)
         ctx.set_materialize_grads(False)
         return loss, rewards
@@ -344,7 +349,7 @@ class _PolicyFn(torch.autograd.Function):
         _issue(logits, k.policy_loss(rows, old, adv, a_strides, ref, *clip, kl_coef, by_sequence, scale, loss, kl, logprobs, stats, coef, d, strides, work))
         if want:
             ctx.save_for_backward(logits, labels, work)
-            ctx.rows, ctx.at, ctx.scaled = (rows, logits.stride(), k), (8 * n, 8 * (n + B * R), (R, 1)), _wants_scale(logits)
+            ctx.rows, ctx.at = (rows, logits.stride(), k, _wants_scale(logits)), (8 * n, 8 * (n + B * R), (R, 1))
             ctx.d, ctx.captured = d, torch.cuda.is_current_stream_capturing()
         ctx.mark_non_differentiable(logprobs, kl)
         ctx.set_materialize_grads(False)

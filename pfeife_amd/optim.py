@@ -133,7 +133,7 @@ class AdamW8bit(torch.optim.Optimizer):
                 place += 1
                 g = p.grad
                 if g is None or p.numel() == 0:
-                    records.append((p, None))
+                    records.append((p, None, None, 0, 0, 0, ()))
                     continue
                 if g.layout is not torch.strided:
                     raise RuntimeError("AdamW8bit: gradients are dense fp32 on the parameter's device (got %s)" % g.layout)
@@ -174,20 +174,19 @@ class AdamW8bit(torch.optim.Optimizer):
         state = self.state
         for group in self.param_groups:
             for p in group["params"]:
-                r = next(at)
+                seen, st, first, where, size, g_where, held = next(at)
                 g = p.grad
-                if r[0] is not p:
+                if seen is not p:
                     return False
-                if r[1] is None:
+                if st is None:
                     if g is not None and p.numel():
                         return False
                     continue
-                st = r[1]
-                if (g is None or state.get(p) is not st or st["step"] != r[2][0]["step"] or p.data_ptr() != r[3] or p.nbytes != r[4]
-                        or g.data_ptr() != r[5] or g.nbytes != r[4] or not p.is_contiguous() or not g.is_contiguous()):
+                if (g is None or state.get(p) is not st or st["step"] != first[0]["step"] or p.data_ptr() != where or p.nbytes != size
+                        or g.data_ptr() != g_where or g.nbytes != size or not p.is_contiguous() or not g.is_contiguous()):
                     return False
-                for key, t, where, n in r[6]:
-                    if st.get(key) is not t or t.data_ptr() != where or t.numel() != n:
+                for key, t, t_where, n in held:
+                    if st.get(key) is not t or t.data_ptr() != t_where or t.numel() != n:
                         return False
         return True
 
