@@ -887,6 +887,7 @@ class StageWorker:
         # (all that the tables hold; a group may also have no gradient any more)
         rebuilt = len(cache) != len(looked_at) or any(gi not in cache or cache[gi][0] != sig for gi, _, _, _, sig in looked_at)
         if rebuilt:
+            self._count_unset = True      # (until a step is made: the one that this is for may fail before)
             if scaled:
                 self.sync_optimizer_steps()
             for gi in set(cache) - {entry[0] for entry in looked_at}:
@@ -905,7 +906,7 @@ class StageWorker:
 
         def step():
             s = self.stream()
-            if scaled and rebuilt:
+            if scaled and getattr(self, "_count_unset", False):
                 self._seed_device_step_count(opt, [state for _, state, _ in groups])
             for g, state, (table, n_items, n_chunks) in groups:
                 b1, b2 = g["betas"]
@@ -934,15 +935,19 @@ class StageWorker:
         lane = self.stream_obj if self.stream_obj is not None or self.device.type != "cuda" else torch.cuda.default_stream(self.device)
         with torch.cuda.stream(lane):
             work, fresh = opt._prepare(self.kernels)
-            if scaled and not fresh:      # (a group may have no gradient any more, or the optimizer be one that has stepped before)
+            if scaled and not fresh and work is not self.__dict__.get("_adam8_work"):
+                # (a group may have no gradient any more, or the optimizer be one that has stepped before)
                 fresh = {id(st) for w in work for st in w[1]} != self.__dict__.setdefault("_served", {}).keys()
             if scaled and fresh and getattr(self, "_host_steps_stale", False):
                 self.sync_optimizer_steps()
                 work, _ = opt._prepare(self.kernels)      # (which puts parameters at one step count together)
+            self._adam8_work = work
+            if fresh:
+                self._count_unset = True      # (until a step is made)
         stream = lane.cuda_stream if lane is not None else None
 
         def step():
-            if scaled and fresh:
+            if scaled and getattr(self, "_count_unset", False):
                 self._seed_device_step_count(opt, [w[1] for w in work])
             with torch.cuda.stream(lane):
                 for g, states, _, table, copies in work:
@@ -963,10 +968,11 @@ class StageWorker:
         parameter that has made fewer is noted with what it lags behind.  served: lists of states,
         each at one count."""
         counts = [int(float(states[0]["step"])) for states in served]
-        k = max(counts, default=0)
-        if float(self.scaler_state[3].item()) != k:
+        k = max(counts, default=None)
+        if k is not None and float(self.scaler_state[3].item()) != k:
             self.scaler_state[3:4].fill_(k)
         self._served = {id(st): (st, c - k) for states, c in zip(served, counts) for st in states}
+        self._count_unset = False
         if getattr(self, "_steps_owner", None) is not opt:
             self._steps_owner = opt
             if hasattr(opt, "register_state_dict_pre_hook"):

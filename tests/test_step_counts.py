@@ -183,3 +183,44 @@ def test_an_optimizer_that_changes_workers(make, monkeypatch):
     assert step(a, b) == [5, 5]
     w.sync_optimizer_steps()      # (as release() does)
     assert [float(opt.state[p]["step"]) for p in (a, b)] == [5, 5] and counts(other) == [2]
+
+
+def test_a_step_without_any_gradient(make, monkeypatch):
+    """It is nobody's; the device's count is the others' again afterwards."""
+    a, b = make_parameters(8, 5)
+    opt = make([a, b], lr=0.1)
+    w = make_worker(True)
+    step = Steps(w, opt, monkeypatch)
+    assert [step(a, b), step(a, b)] == [[1, 1], [2, 2]]
+    before = float(w.scaler_state[3])
+    assert step() == [] and float(w.scaler_state[3]) == before + 1 and counts(opt) == [2, 2]
+    assert [step(a, b), step(a, b)] == [[3, 3], [4, 4]] and counts(opt) == [4, 4]
+    # the same group in a new dict, which a table of addresses cannot tell from the old one
+    group = opt.param_groups[0]
+    opt.param_groups[0] = dict(group, lr=0.2)
+    assert step(a, b) == [5, 5] and counts(opt) == [5, 5]
+
+
+def test_a_step_that_fails_before_the_optimizers(make, monkeypatch):
+    """Its tables were made; the next step finds them as they are and knows the counts all the same."""
+    from pfeife_amd.optim import AdamW8bit
+
+    a, b, late = make_parameters(8, 5, 6)
+    opt = make([a, b, late], lr=0.1)
+    w = make_worker(True)
+    step = Steps(w, opt, monkeypatch)
+    prepare = w._adam8_prepare if make is AdamW8bit else w._fused_adam_prepare
+    a.grad, b.grad = torch.ones(8), torch.ones(5)
+    prepare(opt, True)
+    assert [step(a, b), step(a, b)] == [[1, 1], [2, 2]]
+    late.grad = torch.ones(6)
+    prepare(opt, True)
+    assert [step(a, b, late), step(a, b, late)] == [[3, 3, 1], [4, 4, 2]] and counts(opt) == [4, 4, 2]
+
+
+def test_the_first_gradients_come_late(make, monkeypatch):
+    a, b = make_parameters(8, 5)
+    opt = make([a, b], lr=0.1)
+    step = Steps(make_worker(True), opt, monkeypatch)
+    assert [step(), step()] == [[], []]
+    assert [step(a, b), step(a, b)] == [[1, 1], [2, 2]] and counts(opt) == [2, 2]
