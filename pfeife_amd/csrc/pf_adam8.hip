@@ -46,7 +46,8 @@ __device__ __forceinline__ float divide_by(float a, float b, float y) {
   return a < INFINITY ? r : a;
 }
 
-// 32 bits to 32 bits, one to one: shifts and products with odd constants
+// 32 bits to 32 bits, one to one: shifts and products with odd constants, 0x9E3779B1 the prime next to 2^32 over the golden ratio (the
+// multiplicative hash of D. Knuth), 0x93D765DD a multiplier of 32 bits from the tables of G. Steele and S. Vigna (2021)
 __device__ __forceinline__ uint32_t mix(uint32_t x) {
   x = (x ^ (x >> 16)) * 0x93D765DDu;
   x = (x ^ (x >> 15)) * 0x9E3779B1u;
