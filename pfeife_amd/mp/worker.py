@@ -520,7 +520,8 @@ class StageWorker:
         self.params = ParamStore(self.kernels, self.device)
         self.pool = BufferPool(self.device)
         self.lowerer = self._new_lowerer()
-        self.__dict__.pop("_adam_tables", None)
+        for name in ("_adam_tables", "_adam8_work", "_served"):      # (the last two hold the optimizer's state)
+            self.__dict__.pop(name, None)
 
     # -- per step --------------------------------------------------------------------
     def stream(self):
@@ -941,7 +942,8 @@ class StageWorker:
             if scaled and fresh and getattr(self, "_host_steps_stale", False):
                 self.sync_optimizer_steps()
                 work, _ = opt._prepare(self.kernels)      # (which puts parameters at one step count together)
-            self._adam8_work = work
+            if scaled:
+                self._adam8_work = work
             if fresh:
                 self._count_unset = True      # (until a step is made)
         stream = lane.cuda_stream if lane is not None else None
@@ -1009,9 +1011,9 @@ class StageWorker:
         """The optimizer's entries are what was loaded: the device's count is set from them before the next step."""
         if self._steps_owner is not opt:
             return
-        self._served = {}
         self._host_steps_stale = False
-        self.__dict__.pop("_adam_tables", None)
+        for name in ("_adam_tables", "_adam8_work", "_served"):      # (the last two hold the state that is gone)
+            self.__dict__.pop(name, None)
 
     def scaler_state_dict(self):
         """The dynamic loss scaler's state in torch.amp.GradScaler.state_dict()'s layout (empty

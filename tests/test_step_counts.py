@@ -224,3 +224,19 @@ def test_the_first_gradients_come_late(make, monkeypatch):
     step = Steps(make_worker(True), opt, monkeypatch)
     assert [step(), step()] == [[], []]
     assert [step(a, b), step(a, b)] == [[1, 1], [2, 2]] and counts(opt) == [2, 2]
+
+
+@pytest.mark.parametrize("scaled", [False, True])
+def test_loaded_state_lets_the_old_one_go(make, scaled, monkeypatch):
+    import copy
+    import weakref
+
+    a, b = make_parameters(8, 5000)
+    opt = make([a, b], lr=0.1)
+    step = Steps(make_worker(scaled), opt, monkeypatch)
+    step(a, b), step(a, b)
+    saved = copy.deepcopy(opt.state_dict())
+    old = [weakref.ref(st["exp_avg"]) for st in opt.state.values()]
+    opt.load_state_dict(saved)
+    assert all(t() is None for t in old)
+    assert step(a, b) == [3, 3]

@@ -77,3 +77,38 @@ def test_counts_that_differ(kind):
     late.grad = torch.ones_like(late)
     step()
     assert counts(opt) == counts(want) and counts(opt)[-2:] == [13, 1]
+
+
+@pytest.mark.parametrize("kind", ["adam", "adamw8bit"])
+def test_a_released_worker_keeps_no_moments(kind):
+    """The optimizer of the caller's own has its counts, and the one that the worker made goes away with its state."""
+    import gc
+    import weakref
+
+    from pfeife_amd.bench_models.vit import ViTConfig, VisionTransformer
+    from pfeife_amd.mp import partial_compiler
+    from pfeife_amd.option import PipeOption
+
+    g = torch.Generator().manual_seed(42)
+    x, y = torch.randn(8, 3, 32, 32, generator=g).cuda(), torch.randint(0, 10, (8,), generator=g).cuda()
+    model = VisionTransformer(ViTConfig(image_size=32, patch_size=16, dim=64, depth=2, heads=2, mlp_dim=128, num_classes=10)).cuda()
+    runner = _fresh_runner(PipeOption(device_cnt=2, batch_cnt=2, batch_size=4, split_points=["blocks.1"], loss_scale="dynamic", init_scale=1024.0,
+                                      optimizer=dict(type=kind, lr=1e-3)))
+    cmodel, crit = torch.compile(model, backend=partial_compiler), torch.nn.CrossEntropyLoss()
+
+    def fn(px, labels):
+        loss = crit(cmodel(px).float(), labels)
+        loss.backward()
+        return loss.detach()
+
+    runner.set_exec_fn(fn)
+    for _ in range(3):
+        runner.step(x, y)
+    worker, opt = runner.worker, runner.worker.optimizer
+    moments = [weakref.ref(st["exp_avg"]) for st in opt.state.values()]
+    worker.release()
+    assert {float(st["step"]) for st in opt.state.values()} == {3.0} and all(m() is not None for m in moments)
+    opt.state.clear()
+    del opt
+    gc.collect()
+    assert all(m() is None for m in moments)
