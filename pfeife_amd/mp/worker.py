@@ -990,8 +990,10 @@ class StageWorker:
             return launch()
         with torch.cuda.stream(self.stream_obj):      # (None: the current one)
             self.scaler_state[3:4].add_(behind)
-            launch()
-            self.scaler_state[3:4].sub_(behind)
+            try:
+                launch()
+            finally:
+                self.scaler_state[3:4].sub_(behind)
 
     def sync_optimizer_steps(self):
         """Writes the device's count of completed optimizer steps into the `step` entries that it

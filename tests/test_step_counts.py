@@ -240,3 +240,22 @@ def test_loaded_state_lets_the_old_one_go(make, scaled, monkeypatch):
     opt.load_state_dict(saved)
     assert all(t() is None for t in old)
     assert step(a, b) == [3, 3]
+
+
+def test_a_launch_that_is_refused_leaves_the_count(make, monkeypatch):
+    a, late = make_parameters(8, 6)
+    opt = make([a, late], lr=0.1)
+    w = make_worker(True)
+    step = Steps(w, opt, monkeypatch)
+    step(a), step(a), step(a, late)
+    count, refused = float(w.scaler_state[3]), []
+
+    def refuse(self, table, n_items, n_chunks, lr, b1, b2, eps, decay, adamw, state, stream):
+        if late.data_ptr() in table:
+            refused.append(float(state[3]))
+            raise RuntimeError("refused")
+
+    monkeypatch.setattr(Kernels, "adam_step_scaled", refuse)
+    with pytest.raises(RuntimeError, match="refused"):
+        step(a, late)
+    assert refused == [1.0] and float(w.scaler_state[3]) == count
