@@ -421,6 +421,27 @@ int pf_policy_loss(const void* logits, int dtype, int64_t B, int64_t T, int64_t 
                    const float* advantages, int64_t a_sb, int64_t a_st, const float* ref_logprobs, double clip_low,
                    double clip_high, double kl_coef, int by_sequence, double scale, float* loss, float* kl, float* logprobs, float* stats,
                    float* coef, void* dlogits, int64_t d_sb, int64_t d_st, double* workspace, void* stream);
+/* Cross entropy of a large vocabulary from the last hidden state, without the logits in memory: z = hidden weight^T in fp32, lse = ln sum exp z,
+ * a token's loss lse - z[label] + z_loss lse^2.  hidden [B, T, D] (fp32, fp16 or bf16; sb / st elements between sequences / tokens, unit stride
+ * over D, no alignment asked for), weight [V, D] of the same type, contiguous; labels, shift and ignore_index as above (a label outside
+ * the vocabulary gives NaN).  reduction 0: loss fp32 [B, T - shift], 0 where a token takes no part; 1: loss[0] = the mean over the tokens that
+ * take part; 2: their sum (of none: 0).  kept: pf_linear_ce_kept(B * T) bytes, written by the forward pass and read by the backward
+ * pass; workspace: pf_linear_ce_workspace bytes, on a boundary of 256 bytes (weight: its address decides whether a copy is needed; a negative status
+ * where the sizes are refused).  hidden and weight hold the same values in both passes.
+ *   pf_linear_ce_bwd          dhidden [B, T, D] and dweight [V, D] (either may be null), contiguous, in the operands' type; grad: of the loss,
+ *                             or (reduction 0) of every token's, grad[b * g_sb + t * g_st].  mean != 0: reduction 1
+ *   pf_linear_ce_hidden_grad  after pf_linear_ce_bwd, from what its workspace still holds: dhidden times a factor in device memory (null: 1), rounded once
+ * Stands in for the last stage's aten::linear followed by nn.CrossEntropyLoss (pfeife/loss.py:53-70). */
+int64_t pf_linear_ce_kept(int64_t tokens);
+int64_t pf_linear_ce_workspace(const void* weight, int dtype, int64_t tokens, int64_t D, int64_t V, int backward);
+int pf_linear_ce_fwd(const void* hidden, int dtype, int64_t B, int64_t T, int64_t D, int64_t sb, int64_t st, const void* weight, int64_t V,
+                     const int64_t* labels, int shift, int64_t ignore_index, double z_loss, int reduction, float* loss, void* kept,
+                     void* workspace, void* stream);
+int pf_linear_ce_bwd(const void* hidden, int dtype, int64_t B, int64_t T, int64_t D, int64_t sb, int64_t st, const void* weight, int64_t V,
+                     double z_loss, int mean, const void* kept, const float* grad, int64_t g_sb, int64_t g_st, void* dhidden, void* dweight,
+                     void* workspace, void* stream);
+int pf_linear_ce_hidden_grad(const void* weight, int dtype, int64_t tokens, int64_t D, int64_t V, const void* kept, const float* times, void* dhidden,
+                             const void* workspace, void* stream);
 /* Mean squared error (F.mse_loss, bench_models/models/train_sdxl.py:1422-1424):
  * loss[0] = mean((a-b)^2) computed in fp32; partial: fp32 [pf_reduce_workspace(n)]. */
 int64_t pf_reduce_workspace(int64_t n);

@@ -62,7 +62,9 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 // PW > 1 (right-hand operand of a row-major product): inside every 16*PW rows the tile holds row PW*i + t
 // as row i of MFMA tile t, so that the accumulators a lane keeps of PW tiles are PW CONSECUTIVE columns
 // of the result.
-template <int R, int BK, int NW, bool TRANS, int PW> struct DTile {
+// PAIR (with PW > 1): the operand is two matrices of `half` rows, one behind the other, and the tile holds R / 2 rows of each: MFMA
+// tiles 0 .. PW / 2 - 1 of every 16*PW rows are the first one's, the others the same rows of the second one.
+template <int R, int BK, int NW, bool TRANS, int PW, bool PAIR = false> struct DTile {
   static constexpr int BYTES = R * BK * 2;
   static constexpr int NI = BYTES / 1024;  // wavefront-wide load instructions per tile
   static constexpr int IPW = (NI + NW - 1) / NW;   // ... per wavefront
@@ -93,15 +95,21 @@ template <int R, int BK, int NW, bool TRANS, int PW> struct DTile {
   // byte offset (inside K-tile 0) of the chunk this lane fetches in its q-th instruction
   // tail[q]: all ones if that chunk lies past the `left` reduction elements of the last K-tile (RAG kernels)
   static __device__ __forceinline__ void init(uint32_t (&off)[IPW], uint32_t (&tail)[IPW], int64_t ld, int64_t r0, int left, int wave,
-                                              int lane) {
+                                              int lane, int64_t half = 0) {
 #pragma unroll
     for (int q = 0; q < IPW; ++q) {
       const int ii = instr(wave, q);
       if (!TRANS) {
         const int row = ii * RPI + lane / CPR;
         const int c = (lane % CPR) ^ swz_row(row);
-        const int src = PW > 1 ? row / (16 * PW) * (16 * PW) + (row & 15) * PW + (row >> 4) % PW : row;
-        off[q] = (uint32_t)(((r0 + src) * ld + c * 8) * 2);
+        if constexpr (PAIR) {
+          constexpr int P2 = PW / 2;
+          const int t = (row >> 4) % PW, src = row / (16 * PW) * (16 * P2) + (row & 15) * P2 + t % P2;
+          off[q] = (uint32_t)(((r0 + src + (t < P2 ? 0 : half)) * ld + c * 8) * 2);
+        } else {
+          const int src = PW > 1 ? row / (16 * PW) * (16 * PW) + (row & 15) * PW + (row >> 4) % PW : row;
+          off[q] = (uint32_t)(((r0 + src) * ld + c * 8) * 2);
+        }
         tail[q] = c * 8 >= left ? 0xffffffffu : 0u;
       } else {
         const int k = ii * KPI + lane / CPK;
@@ -234,10 +242,16 @@ template <bool AGPR, int TN> __device__ __forceinline__ void acc_read(float4_t (
   }
 }
 
+// A product whose results do not leave through the epilogue below: EC_OWN's last argument takes each wavefront's accumulators in
+// its place (an object of the caller's own, `run`, see the call).  PAIR: DTile's; p.N is then the rows of one half and every tile
+// covers BN / 2 of them.
+struct NoTail { static constexpr bool PAIR = false; };
+constexpr int EC_OWN = 100;
+
 // `pid`: index of this workgroup among the workgroups of its problem (the launch may hold several
 // problems, see gemm16x_group_kernel)
-template <int DT, int BM, int BN, int BK, int WGM, int WGN, int KS, int ST, bool AT, bool BT, int EC, bool RAG = false>
-__device__ __forceinline__ void gemm16x_body(const pf_gemm_desc& p, const GemmGrid& g, const int pid) {
+template <int DT, int BM, int BN, int BK, int WGM, int WGN, int KS, int ST, bool AT, bool BT, int EC, bool RAG = false, class Tail = NoTail>
+__device__ __forceinline__ void gemm16x_body(const pf_gemm_desc& p, const GemmGrid& g, const int pid, const Tail& tail = Tail()) {
   // KS = 2: the wavefronts form two WGM x WGN grids; grid h multiplies the h-th half of every
   // tile's 16-deep MFMA groups, and the two partial accumulator blocks are added through LDS
   // before the epilogue.  Eight wavefronts (two per SIMD, so that one's LDS reads and waits run
@@ -253,7 +267,9 @@ __device__ __forceinline__ void gemm16x_body(const pf_gemm_desc& p, const GemmGr
   static_assert((BK / 32) % KS == 0 && KK >= 1, "MFMA groups do not divide over the wavefront grids");
   constexpr bool C32 = EC == EC_STORE32 || EC == EC_RES32 || EC == EC_ACC32;
   using TA = DTile<BM, BK, NW, AT, 1>;
-  using TB = DTile<BN, BK, NW, BT, BT ? 1 : TN>;
+  constexpr bool PAIR = Tail::PAIR;
+  static_assert(!PAIR || (EC == EC_OWN && !BT), "pairs are a row-major product's");
+  using TB = DTile<BN, BK, NW, BT, BT ? 1 : TN, PAIR>;
   constexpr int STAGE = TA::BYTES + TB::BYTES;
   constexpr int LPW = TA::IPW + TB::IPW;  // load instructions per wavefront per tile
   static_assert((ST - 1) * LPW <= 63, "too many loads in flight for the 6-bit counter");
@@ -271,7 +287,7 @@ __device__ __forceinline__ void gemm16x_body(const pf_gemm_desc& p, const GemmGr
   int tm, tn;
   gemm_tile_rc(t, g.tiles_m, g.tiles_n, tm, tn);
   const int64_t M = p.M, N = p.N, K = p.K, lda = p.lda, ldb = p.ldb;
-  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * (PAIR ? BN / 2 : BN), rows_b = PAIR ? 2 * N : N;
   const int64_t z = blockIdx.y, z1 = z / p.batch2, z2 = z % p.batch2;
   const uint16_t* A = (const uint16_t*)p.A + z1 * p.a_stride1 + z2 * p.a_stride2;
   const uint16_t* B = (const uint16_t*)p.B + z1 * p.b_stride1 + z2 * p.b_stride2;
@@ -292,11 +308,11 @@ __device__ __forceinline__ void gemm16x_body(const pf_gemm_desc& p, const GemmGr
       for (int r = 0; r < 4; ++r) acc[i][j][r] = 0.f;
 
   const __amdgpu_buffer_rsrc_t rs_a = make_rsrc(A, TA::extent(M, K, lda));
-  const __amdgpu_buffer_rsrc_t rs_b = make_rsrc(B, TB::extent(N, K, ldb));
+  const __amdgpu_buffer_rsrc_t rs_b = make_rsrc(B, TB::extent(rows_b, K, ldb));
   uint32_t offa[TA::IPW], offb[TB::IPW], taila[TA::IPW], tailb[TB::IPW];
   const int nk = (int)((K + BK - 1) / BK);
   TA::init(offa, taila, lda, m0, (int)(K - (int64_t)(nk - 1) * BK), wave, lane);
-  TB::init(offb, tailb, ldb, n0, (int)(K - (int64_t)(nk - 1) * BK), wave, lane);
+  TB::init(offb, tailb, ldb, n0, (int)(K - (int64_t)(nk - 1) * BK), wave, lane, N);
   const uint32_t step_a = TA::tile_step(lda), step_b = TB::tile_step(ldb);
   uint32_t foa[NFA], fob[NFB];
   TA::template frag_init<NFA>(foa, wm0, lane, wave_k * KK);
@@ -310,7 +326,7 @@ __device__ __forceinline__ void gemm16x_body(const pf_gemm_desc& p, const GemmGr
   // again TN consecutive columns.)
   constexpr bool RUNS = !BT || TWO;        // a lane keeps runs of TN columns
   const int64_t row0 = m0 + wm0 + (lane >> 4) * (AT && TWO ? 32 : 4);
-  const int64_t c0 = n0 + wn0 + (lane & 15) * (RUNS ? TN : 1);
+  const int64_t c0 = PAIR ? n0 + wn0 / 2 + (lane & 15) * (TN / 2) : n0 + wn0 + (lane & 15) * (RUNS ? TN : 1);
   auto row_in = [](uint32_t h, uint32_t r) { return AT && TWO ? 8 * r + h : 16 * h + r; };
   float bias[TN];
   // One branch on the dtype around all of the bias loads; a missing bias, and columns past N, read as zeros
@@ -335,7 +351,7 @@ __device__ __forceinline__ void gemm16x_body(const pf_gemm_desc& p, const GemmGr
   };
   // Fetched before the K loop, which hides the latency; after it in the GELU' class, which hardly ever has a
   // bias and has no registers to spare for one.  (Weight-gradient products with a bias take the generic class.)
-  constexpr bool HAS_BIAS = EC != EC_GENERIC && !AT;
+  constexpr bool HAS_BIAS = EC != EC_GENERIC && EC != EC_OWN && !AT;
   constexpr bool BIAS_EARLY = HAS_BIAS && EC != EC_DACT16;
   if constexpr (BIAS_EARLY) load_bias();
 
@@ -449,7 +465,7 @@ __device__ __forceinline__ void gemm16x_body(const pf_gemm_desc& p, const GemmGr
       offa[q] += LEAD - (q & 3) * 1024;
       offb[q] += LEAD - (q & 3) * 1024;
     }
-    const uint32_t ext_a = TA::extent(M, K, lda), ext_b = TB::extent(N, K, ldb);
+    const uint32_t ext_a = TA::extent(M, K, lda), ext_b = TB::extent(rows_b, K, ldb);
     // (A row-major operand's extent goes on past the end of its rows, so whether there is a tile kt is asked of kt: the two tiles
     // past K that it would let through were 25 % of a launch's read requests to the L2 at K = 384, 11 % at 1024, 9 % at 1280.  Alone
     // the times are the same, within 0.5 %.)
@@ -689,7 +705,11 @@ __device__ __forceinline__ void gemm16x_body(const pf_gemm_desc& p, const GemmGr
   }
   if constexpr (HAS_BIAS && !BIAS_EARLY) load_bias();
   static_assert(BT || TN == 2 || TN == 4 || TN == 8, "whole vectors per lane and row");
-  if constexpr (EC == EC_GENERIC) {
+  if constexpr (EC == EC_OWN) {
+    static_assert(!AT, "rows row0 + 16 i + r");
+    tail.template run<TM, TN, TWO>(acc, row0, c0, M, N, lane, (int)((m0 + wm0) / WM));
+    return;
+  } else if constexpr (EC == EC_GENERIC) {
     // one rolled loop over 16-row blocks (unrolled, the run-time switches of this class fill the instruction cache)
     float worst = 0.f;   // sum of v * 0 over the values written: 0 if all are finite, NaN otherwise
 #pragma nounroll
@@ -721,7 +741,7 @@ __device__ __forceinline__ void gemm16x_body(const pf_gemm_desc& p, const GemmGr
     constexpr int NG = RUNS ? 1 : TN;      // runs of columns per lane and row
     constexpr int GW = RUNS ? TN : 1;      // columns per run
     constexpr int NV = GW * ESC / 4;       // 32-bit words per run
-    static_assert(!BT || C32, "reduction-strided products have fp32 results");
+    static_assert(!BT || C32 || (TWO && EC == EC_STORE16), "reduction-strided products have fp32 results, or whole runs of 16-bit ones");
     constexpr int DEPTH = !LOADS ? 1 : (TM * NG * NV <= 16 ? TM : (16 / (NG * NV) > 0 ? 16 / (NG * NV) : 1));
     const uint32_t OOB = 0x80000000u;
     const __amdgpu_buffer_rsrc_t rs_c = make_rsrc((const char*)epi.C + c_base * ESC, (uint32_t)(((M - 1) * epi.ldc + N) * ESC));

@@ -136,6 +136,9 @@ _SIGNATURES = {
     "pf_token_logprob_bwd": [_P, _I, _L, _L, _L, _L, _L, _P, _I, _L, _D, _P, _P, _L, _L, _P, _I, _P, _L, _L, _P],
     "pf_preference_loss": [_P, _I, _L, _L, _L, _L, _L, _P, _I, _L, _P, _D, _D, _I, _P, _P, _P, _P, _P, _P],
     "pf_policy_loss": [_P, _I, _L, _L, _L, _L, _L, _P, _I, _L, _D, _P, _P, _L, _L, _P, _D, _D, _D, _I, _D, _P, _P, _P, _P, _P, _P, _L, _L, _P, _P],
+    "pf_linear_ce_fwd": [_P, _I, _L, _L, _L, _L, _L, _P, _L, _P, _I, _L, _D, _I, _P, _P, _P, _P],
+    "pf_linear_ce_bwd": [_P, _I, _L, _L, _L, _L, _L, _P, _L, _D, _I, _P, _P, _L, _L, _P, _P, _P, _P],
+    "pf_linear_ce_hidden_grad": [_P, _I, _L, _L, _L, _P, _P, _P, _P, _P],
     "pf_mse_fwd": [_P, _I, _P, _I, _P, _P, _L, _P],
     "pf_mse_bwd": [_P, _I, _P, _I, _P, _P, _I, _L, _P],
     "pf_sum_fwd": [_P, _I, _P, _P, _L, _P],
@@ -175,7 +178,7 @@ _SIGNATURES = {
 }
 _RET_I64 = {"pf_gemm_colsum_rows": [POINTER(GemmDesc)], "pf_colreduce_workspace": [_L, _L], "pf_reduce_workspace": [_L],
             "pf_groupnorm_workspace": [_L, _L, _I], "pf_policy_workspace": [_L, _L, _I],
-            "pf_preference_workspace": [_L, _L, _I],
+            "pf_preference_workspace": [_L, _L, _I], "pf_linear_ce_kept": [_L], "pf_linear_ce_workspace": [_P, _I, _L, _L, _L, _I],
             "pf_colsum_static_capacity": []}
 EXPORTED_SYMBOLS = sorted(list(_SIGNATURES) + list(_RET_I64) + ["pf_version", "pf_last_error"])
 
@@ -686,6 +689,28 @@ class HipKernels:
 
     def _token_rows(self, rows):
         return self.token_rows(*rows) if len(rows) == 10 else rows
+
+    def linear_ce_bytes(self, weight, tokens, D, V, backward):
+        """(bytes that the forward pass leaves, bytes of workspace)"""
+        need = int(self.lib.pf_linear_ce_workspace(_ptr(weight), _dt(weight), tokens, D, V, int(backward)))
+        if need < 0:
+            raise RuntimeError(last_error())
+        return int(self.lib.pf_linear_ce_kept(tokens)), need
+
+    def linear_ce_fwd(self, hidden, sizes, weight, V, labels, shift, ignore_index, z_loss, reduction, loss, kept, ws):
+        """sizes: B, T, D and the strides of hidden's first two dimensions"""
+        args = (_ptr(hidden), _dt(hidden), *sizes, _ptr(weight), V, _ptr(labels), int(shift), ignore_index, z_loss, reduction, _ptr(loss), _ptr(kept),
+                _ptr(ws))
+        return self._prep("pf_linear_ce_fwd", args, (hidden, weight, labels, loss, kept, ws))
+
+    def linear_ce_bwd(self, hidden, sizes, weight, V, z_loss, mean, kept, grad, g_strides, dhidden, dweight, ws):
+        args = (_ptr(hidden), _dt(hidden), *sizes, _ptr(weight), V, z_loss, int(mean), _ptr(kept), _ptr(grad), *g_strides, _ptr(dhidden), _ptr(dweight),
+                _ptr(ws))
+        return self._prep("pf_linear_ce_bwd", args, (hidden, weight, kept, grad, dhidden, dweight, ws))
+
+    def linear_ce_hidden_grad(self, weight, tokens, D, V, kept, times, dhidden, ws):
+        args = (_ptr(weight), _dt(dhidden), tokens, D, V, _ptr(kept), _ptr(times), _ptr(dhidden), _ptr(ws))
+        return self._prep("pf_linear_ce_hidden_grad", args, (weight, kept, times, dhidden, ws))
 
     def mse_fwd(self, a, b, partial, loss, n):
         args = (_ptr(a), _dt(a), _ptr(b), _dt(b), _ptr(partial), _ptr(loss), n)

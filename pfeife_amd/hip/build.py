@@ -29,6 +29,7 @@ SOURCES = [
     "pf_elementwise.hip",
     "pf_softmax_loss.hip",
     "pf_token_loss.hip",
+    "pf_head.hip",
     "pf_adam8.hip",
     "pf_batch.hip",
     "pf_mfma_rate.hip",
@@ -38,6 +39,9 @@ SOURCES = [
 # (ids as in csrc/pf_gemm_common.h: dtypes PF_F16 = 1, PF_BF16 = 2; tiles PF_XT_* = 1..13)
 GEMM_X_SOURCE = "pf_gemm_x_inst.hip"
 GEMM_X_PAIRS = [(dt, xt) for xt in (12, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 13) for dt in (1, 2)]
+
+# further products on that kernel with epilogues of their own: one object per operand dtype id
+TAIL_SOURCES = ["pf_head_x.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
@@ -74,6 +78,7 @@ def build(verbose=True, jobs=None):
     os.makedirs(OBJ_DIR, exist_ok=True)
     work = [(GEMM_X_SOURCE, ["-DPF_X_DT=%d" % dt, "-DPF_X_TILE=%d" % xt], "pf_gemm_x_%d_%d" % (dt, xt))
             for dt, xt in GEMM_X_PAIRS]   # the long ones first
+    work += [(src, ["-DPF_X_DT=%d" % dt], "%s_%d" % (os.path.splitext(src)[0], dt)) for src in TAIL_SOURCES for dt in (1, 2)]
     work += [(src, [], os.path.splitext(src)[0]) for src in SOURCES]
     jobs = jobs or min(len(work), max(1, os.cpu_count() or 2))
     with ThreadPoolExecutor(max_workers=jobs) as pool:

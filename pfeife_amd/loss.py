@@ -6,6 +6,8 @@ nn.CrossEntropyLoss computed by the pf_cross_entropy_fwd/bwd kernels when the
 logits live on the GPU; `SumLoss` uses pf_sum_fwd.  The wrappers are ordinary
 autograd nodes, so user code keeps calling `loss.backward()`.
 
+`linear_cross_entropy` is the cross entropy of a decoder's head from the last hidden state, without the logits in memory.
+
 For fine-tuning a language model: `token_logprobs` (log-probabilities of given tokens),
 `preference_loss` (paired log ratios against a reference model) and `policy_loss` (clipped
 ratio with a KL term), each straight from the logits, and `PreferenceLoss` / `PolicyLoss`.
@@ -434,6 +436,100 @@ def policy_loss(logits, labels, old_logprobs, advantages, ref_logprobs=None, *, 
     a_strides = (adv.stride(0), adv.stride(1) if adv.dim() == 2 and adv.shape[1] > 1 else 0)
     return _apply(_PolicyFn, x, y, old, adv, a_strides, ref, (int(shift), ignore_index, float(temperature)), (float(clip), float(clip_high)),
                   float(kl_coef), reduction == "sequences", float(scale))
+
+
+class _LinearCrossEntropyFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, args, want=True):
+        labels, shift, ignore_index, z_loss, reduction = args
+        B, T, D = hidden.shape
+        V = weight.shape[0]
+        k = _table(hidden, "")
+        sizes = (B, T, D, *hidden.stride()[:2])
+        keeps, need = k.linear_ce_bytes(weight, B * T, D, V, False)
+        kept, work = _new(hidden, keeps, dtype=torch.uint8), _new(hidden, need, dtype=torch.uint8)
+        loss = _new(hidden, B, max(0, T - shift)) if reduction == 0 else _new(hidden)
+        _issue(hidden, k.linear_ce_fwd(hidden, sizes, weight, V, labels, shift, ignore_index, z_loss, reduction, loss, kept, work))
+        if want:
+            ctx.save_for_backward(hidden, weight, kept)
+            ctx.cfg = z_loss, reduction, _wants_scale(hidden)
+        return loss
+
+    @_once
+    def backward(ctx, grad):
+        hidden, weight, kept = ctx.saved_tensors
+        z_loss, reduction, scaled = ctx.cfg
+        B, T, D = hidden.shape
+        V = weight.shape[0]
+        k = _table(hidden, "")
+        work = _new(hidden, k.linear_ce_bytes(weight, B * T, D, V, True)[1], dtype=torch.uint8)
+        dh = _new(hidden, B, T, D, dtype=hidden.dtype) if ctx.needs_input_grad[0] else None
+        dw = _new(hidden, V, D, dtype=weight.dtype) if ctx.needs_input_grad[1] else None
+        grad = _as_scale(grad)      # (any strides: a sum's gradient is one number)
+        strides = grad.stride() if reduction == 0 else (0, 0)
+        _issue(hidden, k.linear_ce_bwd(hidden, (B, T, D, *hidden.stride()[:2]), weight, V, z_loss, reduction == 1, kept, grad, strides, dh, dw, work))
+        if scaled and dh is not None:
+            dh._pf_times = dh._version, functools.partial(_hidden_times, k, weight, kept, dh, work)
+        return dh, dw, None
+
+
+def _hidden_times(k, weight, kept, like, work, factor, out):
+    """The hidden state's gradient times a loss scale, rounded once, from the fp32 sums that the backward pass left; -> is it written."""
+    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or not out.is_contiguous():
+        return False
+    B, T, D = like.shape
+    _issue(out, k.linear_ce_hidden_grad(weight, B * T, D, weight.shape[0], kept, factor, out, work))
+    return True
+
+
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def linear_cross_entropy(hidden, weight, labels, *, ignore_index=-100, z_loss=0.0, reduction="mean", shift=False):
+    """Cross entropy of the classes' logits hidden @ weight.T, which are never in memory: they are formed in pieces of the vocabulary, in
+    fp32, and formed again by the backward pass.
+
+    hidden [..., T, D] and weight [V, D] (fp32, fp16 or bf16, the same type), labels int64 [..., T].  A token's loss is lse - logit[label] +
+    z_loss * lse^2, lse = log sum exp of its logits.  reduction "mean": over the tokens that count (with none of them 0), "sum", or "none": fp32
+    [..., T], 0 where a token does not count.  shift: token t is scored against label t + 1 (labels as the model's own input), the last
+    dimension of "none" is then T - 1.  Tokens whose label is `ignore_index` take no part, whatever their hidden state holds, and cost no
+    arithmetic; a label outside the vocabulary gives NaN.  The gradient flows to hidden and weight, in their types.  For a weight of
+    another type hand in `weight.to(hidden.dtype)`.  There are no second and no forward-mode derivatives.  A backward pass is captured
+    into a graph, as any of torch's, only while no autograd graph made outside the capture holds the same leaves."""
+    who = "linear_cross_entropy"
+    if not torch.is_tensor(hidden) or not torch.is_tensor(weight) or not torch.is_tensor(labels):
+        raise RuntimeError("%s: hidden, weight and labels are tensors" % who)
+    _table(hidden, who)
+    shape = hidden.shape
+    if hidden.dtype not in _LOGITS or weight.dtype != hidden.dtype:
+        raise RuntimeError("%s: hidden and weight are both fp32, fp16 or bf16 (got %s and %s)" % (who, hidden.dtype, weight.dtype))
+    if len(shape) < 2 or shape[-1] == 0:
+        raise RuntimeError("%s: hidden is [..., tokens, width] (got %s)" % (who, tuple(shape)))
+    if weight.dim() != 2 or weight.shape[1] != shape[-1] or weight.shape[0] == 0 or weight.get_device() != hidden.get_device():
+        raise RuntimeError("%s: weight is [classes, %d] on %s (got %s on %s)" % (who, shape[-1], hidden.device, tuple(weight.shape), weight.device))
+    if labels.dtype != torch.int64 or labels.get_device() != hidden.get_device() or labels.shape != shape[:-1]:
+        raise RuntimeError("%s: labels are int64 %s on %s (got %s %s on %s)"
+                           % (who, tuple(shape[:-1]), hidden.device, labels.dtype, tuple(labels.shape), labels.device))
+    if not isinstance(ignore_index, int) or not isinstance(shift, (bool, int)) or shift not in (0, 1):
+        raise RuntimeError("%s: ignore_index is a whole number and shift a truth value" % who)
+    if reduction not in _REDUCTIONS:
+        raise RuntimeError("%s: reduction is 'mean', 'sum' or 'none' (got %r)" % (who, reduction))
+    if not math.isfinite(z_loss):
+        raise RuntimeError("%s: z_loss must be finite" % who)
+    if _dual._current_level >= 0 and _has_tangent(hidden, weight):
+        raise RuntimeError("%s: there is no forward-mode derivative" % who)
+    x = hidden
+    if len(shape) != 3:
+        x = x.reshape((math.prod(shape[:-2]),) + shape[-2:])
+    if x.stride(-1) != 1 and shape[-1] > 1:
+        x = x.contiguous()
+    args = (labels.reshape(x.shape[:-1]).contiguous(), int(shift), ignore_index, float(z_loss), _REDUCTIONS[reduction])
+    weight = weight.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        out = _LinearCrossEntropyFn.apply(x, weight, args)
+    else:
+        out = _LinearCrossEntropyFn.forward(_NoContext, x, weight, args, False)
+    return out.reshape(shape[:-2] + out.shape[1:]) if reduction == "none" and len(shape) != 3 else out
 
 
 class LossWrapper(nn.Module):
