@@ -466,6 +466,18 @@ int pf_glu_fwd(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up,
 int pf_glu_bwd(const void* dy, int64_t ld_dy, const void* gate, int64_t ld_gate, const void* up, int64_t ld_up,
                void* dgate, int64_t ld_dgate, void* dup, int64_t ld_dup, int dtype, int act, int64_t rows,
                int64_t cols, void* stream);
+/* Gated projection with both of its products: y = act(x Wg^T) * (x Wu^T), weight [2 ffn, D] with the gate's rows first, x [rows, D], y
+ * [rows, ffn], all contiguous and of one type (fp32, fp16 or bf16; no alignment asked for).  keep: what the backward pass starts from
+ * and `kept` takes, 0 nothing (no backward pass), 1 both products in the operands' type, 2 (16-bit operands) both as e4m3 codes, 16
+ * neighbouring columns of a row under one power of two.  pf_gated_linear_bytes: bytes of workspace of either pass, on a boundary of 256 bytes,
+ * and of `kept` (the operands' addresses decide whether copies are needed; a negative status where the sizes are refused).  The
+ * backward pass takes x and weight as they were: dx [rows, D] and dweight [2 ffn, D], either may be null.  Replaces the aten::linear pair
+ * and the product behind it of a gated MLP, and their backward. */
+int64_t pf_gated_linear_bytes(const void* x, const void* weight, int dtype, int64_t rows, int64_t D, int64_t ffn, int keep, int backward, int64_t* kept);
+int pf_gated_linear_fwd(const void* x, int dtype, int64_t rows, int64_t D, const void* weight, int64_t ffn, int act, int keep, void* y, void* kept,
+                        void* workspace, void* stream);
+int pf_gated_linear_bwd(const void* x, int dtype, int64_t rows, int64_t D, const void* weight, int64_t ffn, int act, int keep, const void* kept,
+                        const void* dy, void* dx, void* dweight, void* workspace, void* stream);
 /* out = alpha*a + beta*b, each operand with its own dtype (residual add,
  * fan-out gradient sum `g.add_(lg)` of pfeife/mp/worker.py:1543). n elements. */
 int pf_axpby(const void* a, int a_dtype, float alpha, const void* b, int b_dtype, float beta, void* out,
@@ -623,6 +635,16 @@ int pf_embedding_fwd(const void* table, int t_dtype, const int64_t* ids, void* o
                      int64_t dim, int64_t vocab, void* stream);
 int pf_embedding_bwd(const void* dout, int d_dtype, const int64_t* ids, float* dtable_acc, int64_t n_ids,
                      int64_t dim, int64_t vocab, int64_t padding_idx, void* stream);
+/* The same with a factor, out[i, :] = scale * table[ids[i], :] (one type, no alignment asked for), and the gradient by sorted tokens: dtable[v, :] =
+ * scale * sum of dout[i, :] over ids[i] = v, summed in fp32 whatever the types (t_dtype: that of dout, or fp32), the same bits for the
+ * same ids.  Every row of dtable is written, zeros where no id names it; accumulate != 0: added to what is there, other rows are left
+ * alone.  Ids outside [0, vocab) give NaN rows and no gradient; padding_idx (-1: none) gets no gradient.  workspace:
+ * pf_embedding_sorted_workspace bytes, on a boundary of 256 bytes.  Replaces aten::embedding, the product behind it and
+ * embedding_dense_backward. */
+int pf_embedding_scaled_fwd(const void* table, int dtype, const int64_t* ids, void* out, int64_t n_ids, int64_t dim, int64_t vocab, double scale, void* stream);
+int64_t pf_embedding_sorted_workspace(int64_t n_ids, int64_t dim);
+int pf_embedding_sorted_bwd(const void* dout, int d_dtype, const int64_t* ids, void* dtable, int t_dtype, int64_t n_ids, int64_t dim, int64_t vocab,
+                            int64_t padding_idx, double scale, int accumulate, void* workspace, void* stream);
 
 #ifdef __cplusplus
 }

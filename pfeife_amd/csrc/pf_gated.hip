@@ -1,0 +1,344 @@
+// Gated projection y = act(x Wg^T) * (x Wu^T), weight [2 ffn, D] with the gate's rows first, and its backward pass.
+//
+//   g = x Wg^T, u = x Wu^T (fp32);  y = act(g) u
+//   dg = dy u act'(g);  du = dy act(g);  dx = [dg du] W;  dW = [dg du]^T x
+//
+// The backward pass starts from g and u as they were kept: in the operands' type, or (16-bit operands) as e4m3 codes, 16 neighbouring columns
+// of a row under one power of two, 17 instead of 32 bytes for 16 of them.  The power of two is the smallest that brings the
+// largest of the 16 to 448 or below, so that nothing saturates, and decoding is exact.  The pass over the elements that
+// makes dg and du reads the codes as they are: 4.1 bytes instead of 6 an element of y, and 4 written.
+#include "pf_gated.h"
+
+namespace {
+
+inline int64_t round_up(int64_t n, int64_t k) { return (n + k - 1) / k * k; }
+
+template <int ACT> __device__ __forceinline__ void act_and_slope(float g, float& value, float& slope) {
+  if constexpr (ACT == PF_ACT_SILU) {
+    const float p = pf_sigmoid_fast(g);
+    value = g * p;
+    slope = p * (1.f + g * (1.f - p));
+  } else {
+    value = ACT == PF_ACT_RELU && g != g ? g : pf_act(ACT, g);
+    slope = pf_act_grad(ACT, g);
+  }
+}
+
+// W neighbouring values of what was kept
+template <int DT, int KEEP, int W>
+__device__ __forceinline__ void kept_load(const void* kept, const uint8_t* exps, int64_t half, int64_t row, int64_t at, float (&v)[W]) {
+  if constexpr (KEEP == PF_KEEP_SAME) {
+    Vec8<DT>::load(kept, row * 2 * half + at, v);
+  } else {
+    const uint2 c = *(const uint2*)((const uint8_t*)kept + row * 2 * half + at);
+    const float by = pf_pow2(exps[(row * 2 * half + at) / PF_GATED_BLOCK]);
+    v[0] = __builtin_amdgcn_cvt_f32_fp8((int)c.x, 0) * by; v[1] = __builtin_amdgcn_cvt_f32_fp8((int)c.x, 1) * by;
+    v[2] = __builtin_amdgcn_cvt_f32_fp8((int)c.x, 2) * by; v[3] = __builtin_amdgcn_cvt_f32_fp8((int)c.x, 3) * by;
+    v[4] = __builtin_amdgcn_cvt_f32_fp8((int)c.y, 0) * by; v[5] = __builtin_amdgcn_cvt_f32_fp8((int)c.y, 1) * by;
+    v[6] = __builtin_amdgcn_cvt_f32_fp8((int)c.y, 2) * by; v[7] = __builtin_amdgcn_cvt_f32_fp8((int)c.y, 3) * by;
+  }
+}
+
+// dg and du side by side in rows of 2 wide columns (zeros past ffn), eight columns of a row to a thread; bound by memory
+template <int DT, int KEEP, int ACT>
+__global__ __launch_bounds__(256) void gated_backward_kernel(const void* dy, const void* kept, const uint8_t* exps, int64_t half, int64_t rows, int64_t ffn,
+                                                             void* dgu, int64_t wide, int vec) {
+  const int64_t per = wide / 8, total = rows * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / per, c = i % per * 8;
+    float d[8], g[8], u[8], dg[8], du[8];
+    if (vec) {
+      Vec8<DT>::load(dy, row * ffn + c, d);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) d[k] = c + k < ffn ? Codec<DT>::load(dy, row * ffn + c + k) : 0.f;
+    }
+    kept_load<DT, KEEP, 8>(kept, exps, half, row, c, g);
+    kept_load<DT, KEEP, 8>(kept, exps, half, row, half + c, u);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      float value, slope;
+      act_and_slope<ACT>(g[k], value, slope);
+      const bool in = vec || c + k < ffn;      // (what is kept past the last column may be anything)
+      dg[k] = in ? d[k] * u[k] * slope : 0.f;
+      du[k] = in ? d[k] * value : 0.f;
+    }
+    Vec8<DT>::store(dgu, row * 2 * wide + c, dg);
+    Vec8<DT>::store(dgu, row * 2 * wide + wide + c, du);
+  }
+}
+
+template <int DT, int KEEP>
+void backward_launch(const void* dy, const void* kept, const uint8_t* exps, int64_t half, int64_t rows, int64_t ffn, void* dgu, int64_t wide, int act, hipStream_t st) {
+  const int64_t blocks = (rows * (wide / 8) + 255) / 256;
+  const dim3 grid((unsigned)(blocks < 16384 ? blocks : 16384));
+  const int vec = ffn % 8 == 0 && pf_aligned(dy, 16);
+#define PF_GB(A) hipLaunchKernelGGL((gated_backward_kernel<DT, KEEP, A>), grid, dim3(256), 0, st, dy, kept, exps, half, rows, ffn, dgu, wide, vec)
+  switch (act) {
+    case PF_ACT_SILU: PF_GB(PF_ACT_SILU); break;
+    case PF_ACT_GELU: PF_GB(PF_ACT_GELU); break;
+    case PF_ACT_GELU_TANH: PF_GB(PF_ACT_GELU_TANH); break;
+    default: PF_GB(PF_ACT_RELU); break;
+  }
+#undef PF_GB
+}
+
+// a matrix with its rows' width raised (and of two halves each its number of rows), zeros in what is new
+__global__ __launch_bounds__(256) void gated_widen_kernel(const uint16_t* src, int64_t rows, int64_t width, uint16_t* dst, int64_t to_rows, int64_t to_width, int halves) {
+  const int64_t per = to_rows * to_width, total = per * halves;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t h = i / per, r = i % per / to_width, c = i % to_width;
+    dst[i] = r < rows && c < width ? src[(h * rows + r) * width + c] : (uint16_t)0;
+  }
+}
+void widen_rows(const void* src, int64_t rows, int64_t width, void* dst, int64_t to_rows, int64_t to_width, int halves, hipStream_t st) {
+  const int64_t blocks = (to_rows * to_width * halves + 255) / 256;
+  hipLaunchKernelGGL(gated_widen_kernel, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st, (const uint16_t*)src, rows, width, (uint16_t*)dst, to_rows,
+                     to_width, halves);
+}
+
+// A few rows: a wavefront takes a column of y, i.e. one row of either half of the weight, and R rows of x from LDS.  Bound by the
+// weight's way from memory: all of a wavefront's loads are independent, and ffn wavefronts are on their way at once.
+template <int DT, int R>
+__global__ __launch_bounds__(256) void gated_few_kernel(const void* x, const void* w, int64_t depth, int64_t rows, int64_t ffn, int act, void* y, void* kept, int64_t half) {
+  extern __shared__ __align__(16) char xs[];
+  typedef typename Codec<DT>::storage S;
+  for (int64_t i = (int64_t)threadIdx.x * 8; i < R * depth; i += 256 * 8) {
+    float v[8] = {};
+    if (i < rows * depth) Vec8<DT>::load(x, i, v);
+    Vec8<DT>::store(xs, i, v);
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 63;
+  const int64_t f = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (f >= ffn) return;
+  const S* wg = (const S*)w + f * depth;
+  const S* wu = (const S*)w + (ffn + f) * depth;
+  float g[R], u[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) g[r] = u[r] = 0.f;
+#pragma unroll 4
+  for (int64_t k = lane * 8; k < depth; k += 512) {
+    float a[8], b[8];
+    Vec8<DT>::load(wg, k, a);
+    Vec8<DT>::load(wu, k, b);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float v[8];
+      Vec8<DT>::load(xs, r * depth + k, v);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) { g[r] = fmaf(a[q], v[q], g[r]); u[r] = fmaf(b[q], v[q], u[r]); }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float gs = pf_wave_sum(g[r]), us = pf_wave_sum(u[r]);
+    if (lane == 0 && r < rows) {
+      const float v = act == PF_ACT_RELU && gs != gs ? gs : pf_act(act, gs);
+      Codec<DT>::store(y, r * ffn + f, v * us);
+      if (kept != nullptr) {
+        Codec<DT>::store(kept, r * 2 * half + f, gs);
+        Codec<DT>::store(kept, r * 2 * half + half + f, us);
+      }
+    }
+  }
+}
+template <int DT, int R>
+int few_launch(const void* x, const void* w, int64_t depth, int64_t rows, int64_t ffn, int act, void* y, void* kept, int64_t half, hipStream_t st) {
+  const size_t lds = (size_t)(R * depth * pf_dtype_size(DT));
+  hipLaunchKernelGGL((gated_few_kernel<DT, R>), dim3((unsigned)((ffn + 3) / 4)), dim3(256), lds, st, x, w, depth, rows, ffn, act, y, kept, half);
+  PF_CHECK_LAUNCH("pf_gated_linear_fwd");
+  return PF_OK;
+}
+// how many rows such a launch would hold in LDS, 0: it cannot run
+int few_rows(int64_t rows, int64_t depth, int64_t es) {
+  const int r = rows == 1 ? 1 : rows == 2 ? 2 : rows <= 4 ? 4 : rows <= 8 ? 8 : 0;
+  return depth % 8 == 0 && r * depth * es <= 64 * 1024 ? r : 0;
+}
+template <int DT>
+int few(int r, const void* x, const void* w, int64_t depth, int64_t rows, int64_t ffn, int act, void* y, void* kept, int64_t half, hipStream_t st) {
+  switch (r) {
+    case 1: return few_launch<DT, 1>(x, w, depth, rows, ffn, act, y, kept, half, st);
+    case 2: return few_launch<DT, 2>(x, w, depth, rows, ffn, act, y, kept, half, st);
+    case 4: return few_launch<DT, 4>(x, w, depth, rows, ffn, act, y, kept, half, st);
+    default: return few_launch<DT, 8>(x, w, depth, rows, ffn, act, y, kept, half, st);
+  }
+}
+
+// What lies where.  16 bits: depth is the width of the rows that the products read, of x and of the weight, which are copied where theirs
+// is another; wide that of one half of dg and du, with as many columns of the transposed weight.
+struct Plan {
+  int64_t es, depth, wide, half, kept, chunk;
+  bool copy_x, copy_w;
+  char* x; char* w; char* wt; char* dgu;
+  int64_t bytes;
+};
+bool plan_of(Plan& p, const void* x, const void* w, int dtype, int64_t rows, int64_t D, int64_t ffn, int keep, bool back, char* base) {
+  p.es = dtype == PF_F32 ? 4 : 2;
+  const bool f32 = dtype == PF_F32;
+  p.depth = f32 ? D : (D < 64 ? 64 : round_up(D, 8));
+  p.wide = f32 ? ffn : round_up(ffn, 8);
+  p.half = f32 ? ffn : keep == PF_KEEP_8BIT ? round_up(ffn, PF_GATED_BLOCK) : round_up(ffn, 8);
+  p.kept = keep == PF_KEEP_8BIT ? rows * 2 * p.half / PF_GATED_BLOCK * (PF_GATED_BLOCK + 1) : rows * 2 * p.half * p.es;
+  p.copy_x = !f32 && (p.depth != D || !pf_aligned(x, 16));
+  p.copy_w = !f32 && (p.depth != D || !pf_aligned(w, 16));
+  // rows of one launch: everything it addresses by 32-bit offsets stays below 2 GiB
+  const int64_t widest = p.depth > 2 * p.half ? p.depth : 2 * p.half;
+  p.chunk = ((1ll << 31) / (widest * p.es) - 512) / 256 * 256;
+  p.x = p.w = p.wt = p.dgu = nullptr;
+  int64_t used = 0;
+  auto take = [&](int64_t bytes) {
+    char* q = base == nullptr ? nullptr : base + used;
+    used += round_up(bytes, 256);
+    return q;
+  };
+  if (p.copy_x) p.x = take(rows * p.depth * 2);
+  if (p.copy_w) p.w = take(2 * ffn * p.depth * 2);
+  if (back) {
+    p.dgu = take(rows * 2 * p.wide * p.es);
+    if (!f32) p.wt = take(p.depth * 2 * p.wide * 2);
+  } else if (f32 && keep == PF_KEEP_NONE) {
+    p.dgu = take(rows * 2 * ffn * 4);
+  }
+  p.bytes = used;
+  return p.depth < (1ll << 19) && p.half < (1ll << 18) && p.chunk > 0 && (2 * ffn + 512) * p.depth * 2 < (1ll << 31) && (p.depth + 512) * 2 * p.wide * 2 < (1ll << 31) &&
+         (keep == PF_KEEP_NONE ? rows < (1ll << 31) : f32 || rows <= p.chunk);
+}
+
+int check(const char* who, int dtype, int64_t rows, int64_t D, int64_t ffn, int act, int keep) {
+  PF_REQUIRE(dtype == PF_F32 || dtype == PF_F16 || dtype == PF_BF16, "%s: bad dtype", who);
+  PF_REQUIRE(rows >= 0 && D > 0 && ffn > 0, "%s: bad sizes", who);
+  PF_REQUIRE(act >= PF_ACT_GELU && act <= PF_ACT_RELU, "%s: bad activation", who);
+  PF_REQUIRE(keep >= PF_KEEP_NONE && keep <= PF_KEEP_8BIT && (keep != PF_KEEP_8BIT || dtype != PF_F32), "%s: fp32 is not kept in 8 bits", who);
+  return PF_OK;
+}
+int too_large(const char* who) {
+  pf_set_error("%s: too large for one call: the weight, and with a gradient the kept rows and x, have to stay below 2 GiB each", who);
+  return PF_ERR_INVALID;
+}
+
+int product(int dtype, int a_trans, int b_trans, int64_t M, int64_t N, int64_t K, const void* A, int64_t lda, const void* B, int64_t ldb, void* C, int64_t ldc,
+            hipStream_t st) {
+  pf_gemm_desc d = {};
+  d.in_dtype = d.c_dtype = dtype;
+  d.a_trans = a_trans; d.b_trans = b_trans;
+  d.M = M; d.N = N; d.K = K;
+  d.A = A; d.lda = lda; d.B = B; d.ldb = ldb; d.C = C; d.ldc = ldc;
+  d.batch1 = d.batch2 = 1;
+  d.alpha = 1.f;
+  return pf_gemm(&d, st);
+}
+
+}  // namespace
+
+extern "C" int64_t pf_gated_linear_bytes(const void* x, const void* weight, int dtype, int64_t rows, int64_t D, int64_t ffn, int keep, int backward, int64_t* kept) {
+  const char* who = "pf_gated_linear_bytes";
+  int rc = check(who, dtype, rows, D, ffn, PF_ACT_SILU, keep);
+  if (rc != PF_OK) return rc;
+  Plan p;
+  if (!plan_of(p, x, weight, dtype, rows, D, ffn, keep, backward != 0, nullptr)) return too_large(who);
+  if (kept != nullptr) *kept = keep == PF_KEEP_NONE ? 0 : p.kept;
+  return p.bytes;
+}
+
+extern "C" int pf_gated_linear_fwd(const void* x, int dtype, int64_t rows, int64_t D, const void* weight, int64_t ffn, int act, int keep, void* y, void* kept,
+                                   void* workspace, void* stream) {
+  const char* who = "pf_gated_linear_fwd";
+  int rc = check(who, dtype, rows, D, ffn, act, keep);
+  if (rc != PF_OK || rows == 0) return rc;
+  Plan p;
+  if (!plan_of(p, x, weight, dtype, rows, D, ffn, keep, false, (char*)workspace)) return too_large(who);
+  PF_REQUIRE(x && weight && y && (keep == PF_KEEP_NONE || kept) && (p.bytes == 0 || workspace), "%s: null pointer", who);
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == PF_F32) {
+    const int r = D % 8 == 0 && pf_aligned(x, 16) && pf_aligned(weight, 16) ? few_rows(rows, D, 4) : 0;
+    if (r > 0) return few<PF_F32>(r, x, weight, D, rows, ffn, act, y, kept, ffn, st);
+    float* gu = keep == PF_KEEP_NONE ? (float*)p.dgu : (float*)kept;
+    rc = product(PF_F32, 0, 0, rows, 2 * ffn, D, x, D, weight, D, gu, 2 * ffn, st);
+    if (rc != PF_OK) return rc;
+    return pf_glu_fwd(gu, 2 * ffn, gu + ffn, 2 * ffn, y, ffn, PF_F32, act, rows, ffn, stream);
+  }
+  if (p.copy_x) widen_rows(x, rows, D, p.x, rows, p.depth, 1, st);
+  if (p.copy_w) widen_rows(weight, 2 * ffn, D, p.w, 2 * ffn, p.depth, 1, st);
+  PF_CHECK_LAUNCH(who);
+  const int r = keep == PF_KEEP_8BIT ? 0 : few_rows(rows, p.depth, 2);
+  if (r > 0) {
+    const void* xs = p.copy_x ? p.x : x;
+    const void* ws = p.copy_w ? p.w : weight;
+    return dtype == PF_F16 ? few<PF_F16>(r, xs, ws, p.depth, rows, ffn, act, y, kept, p.half, st) : few<PF_BF16>(r, xs, ws, p.depth, rows, ffn, act, y, kept, p.half, st);
+  }
+  const int64_t row_k = 2 * p.half * (keep == PF_KEEP_8BIT ? 1 : 2);
+  for (int64_t r = 0; r < rows; r += p.chunk) {
+    PfGatedProduct q = {};
+    q.rows = rows - r < p.chunk ? rows - r : p.chunk;
+    q.depth = p.depth; q.ffn = ffn;
+    q.x = (p.copy_x ? p.x : (const char*)x) + r * p.depth * 2; q.ldx = p.depth;
+    q.w = p.copy_w ? p.w : weight; q.ldw = p.depth;
+    q.act = act; q.keep = keep;
+    q.y = (char*)y + r * ffn * 2; q.ldy = ffn;
+    q.kept = keep == PF_KEEP_NONE ? nullptr : (char*)kept + r * row_k;
+    q.half = p.half;
+    q.exps = keep == PF_KEEP_8BIT ? (uint8_t*)kept + rows * 2 * p.half + r * (2 * p.half / PF_GATED_BLOCK) : nullptr;
+    rc = dtype == PF_F16 ? pf_gated_forward_1(q, st) : pf_gated_forward_2(q, st);
+    if (rc != PF_OK) return rc;
+  }
+  return PF_OK;
+}
+
+extern "C" int pf_gated_linear_bwd(const void* x, int dtype, int64_t rows, int64_t D, const void* weight, int64_t ffn, int act, int keep, const void* kept,
+                                   const void* dy, void* dx, void* dweight, void* workspace, void* stream) {
+  const char* who = "pf_gated_linear_bwd";
+  int rc = check(who, dtype, rows, D, ffn, act, keep);
+  if (rc != PF_OK) return rc;
+  PF_REQUIRE(keep != PF_KEEP_NONE, "%s: nothing was kept", who);
+  Plan p;
+  if (!plan_of(p, x, weight, dtype, rows, D, ffn, keep, true, (char*)workspace)) return too_large(who);
+  hipStream_t st = (hipStream_t)stream;
+  if (rows == 0) return dweight == nullptr ? PF_OK : pf_fill(dweight, dtype, 0.f, 2 * ffn * D, stream);
+  PF_REQUIRE(x && weight && kept && dy && workspace, "%s: null pointer", who);
+  if (dtype == PF_F32) {
+    const float* gu = (const float*)kept;
+    float* d = (float*)p.dgu;
+    rc = pf_glu_bwd(dy, ffn, gu, 2 * ffn, gu + ffn, 2 * ffn, d, 2 * ffn, d + ffn, 2 * ffn, PF_F32, act, rows, ffn, stream);
+    if (rc == PF_OK && dx) rc = product(PF_F32, 0, 1, rows, D, 2 * ffn, d, 2 * ffn, weight, D, dx, D, st);
+    if (rc == PF_OK && dweight) rc = product(PF_F32, 1, 1, 2 * ffn, D, rows, d, 2 * ffn, x, D, dweight, D, st);
+    return rc;
+  }
+  const uint8_t* exps = keep == PF_KEEP_8BIT ? (const uint8_t*)kept + rows * 2 * p.half : nullptr;
+  if (dtype == PF_F16) {
+    if (keep == PF_KEEP_SAME) backward_launch<PF_F16, PF_KEEP_SAME>(dy, kept, exps, p.half, rows, ffn, p.dgu, p.wide, act, st);
+    else backward_launch<PF_F16, PF_KEEP_8BIT>(dy, kept, exps, p.half, rows, ffn, p.dgu, p.wide, act, st);
+  } else {
+    if (keep == PF_KEEP_SAME) backward_launch<PF_BF16, PF_KEEP_SAME>(dy, kept, exps, p.half, rows, ffn, p.dgu, p.wide, act, st);
+    else backward_launch<PF_BF16, PF_KEEP_8BIT>(dy, kept, exps, p.half, rows, ffn, p.dgu, p.wide, act, st);
+  }
+  if (p.copy_x && dweight) widen_rows(x, rows, D, p.x, rows, p.depth, 1, st);
+  PF_CHECK_LAUNCH(who);
+  const char* xs = p.copy_x ? p.x : (const char*)x;
+  if (dx) {
+    // the reduction runs along the weight's rows, its transposed copy makes it contiguous: 6 % of the product at 8192 rows, where the
+    // product without it runs at half the rate
+    if (p.wide != ffn) {
+      rc = pf_fill(p.wt, dtype, 0.f, D * 2 * p.wide, stream);
+      if (rc != PF_OK) return rc;
+    }
+    for (int h = 0; h < 2; ++h) {
+      rc = pf_transpose_cast((const char*)weight + h * ffn * D * 2, dtype, D, p.wt + h * p.wide * 2, dtype, 2 * p.wide, ffn, D, stream);
+      if (rc != PF_OK) return rc;
+    }
+    for (int64_t r = 0; r < rows; r += p.chunk) {
+      const int64_t n = rows - r < p.chunk ? rows - r : p.chunk;
+      rc = product(dtype, 0, 0, n, D, 2 * p.wide, p.dgu + r * 2 * p.wide * 2, 2 * p.wide, p.wt, 2 * p.wide, (char*)dx + r * D * 2, D, st);
+      if (rc != PF_OK) return rc;
+    }
+  }
+  if (dweight) {
+    auto weight_product = dtype == PF_F16 ? pf_gated_weight_1 : pf_gated_weight_2;
+    if (p.wide == ffn) return weight_product(2 * ffn, D, rows, p.dgu, 2 * p.wide, xs, p.depth, dweight, D, st);
+    for (int h = 0; h < 2; ++h) {
+      rc = weight_product(ffn, D, rows, p.dgu + h * p.wide * 2, 2 * p.wide, xs, p.depth, (char*)dweight + h * ffn * D * 2, D, st);
+      if (rc != PF_OK) return rc;
+    }
+  }
+  return PF_OK;
+}

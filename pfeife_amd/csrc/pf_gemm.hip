@@ -839,6 +839,31 @@ int dispatch16(const pf_gemm_desc& d, hipStream_t st) {
 
 }  // namespace
 
+// The tile (PF_XT_*) that a product whose operands are stored alike would run on in one launch, 0: none
+int pf_gemm_best_tile(const pf_gemm_desc& d) {
+  double t = 0;
+  const int v = choose_tile(d, d.M, 0, t);
+  return v < 0 ? 0 : x_tile_of(v);
+}
+
+// A product of reduction-strided operands in two launches, as plan_split_of does for row-major ones: the rows that fill whole rounds of
+// 256 workgroups on the four-wavefront tile; d.M: one launch is not slower
+int64_t pf_gemm_strided_rows(const pf_gemm_desc& d) {
+  double best_t = 0;
+  choose_tile(d, d.M, 0, best_t);
+  best_t -= 3.0;      // (a launch, and what the rest's epilogue takes longer)
+  const int64_t tn = (d.N + 255) / 256;
+  int64_t found = d.M;
+  for (int64_t round = 1;; ++round) {
+    const int64_t blocks = 256 * round / tn, rows = blocks * 256;
+    if (rows >= d.M) return found;
+    double t2 = 0;
+    if (rows == 0 || choose_tile(d, d.M - rows, 0, t2) < 0) continue;
+    const double t = tile_cost(STRIDED[0], blocks * tn, d.K, true) + t2;
+    if (t < best_t) { best_t = t; found = rows; }
+  }
+}
+
 extern "C" int pf_gemm(const pf_gemm_desc* desc, void* stream) {
   PF_REQUIRE(desc != nullptr, "pf_gemm: null descriptor");
   pf_gemm_desc d = *desc;

@@ -274,6 +274,10 @@ inline int x_epi_class(const pf_gemm_desc& d, int vec_ok, int bm) {
 
 }  // namespace
 
+// pf_gemm.hip
+int pf_gemm_best_tile(const pf_gemm_desc& d);
+int64_t pf_gemm_strided_rows(const pf_gemm_desc& d);
+
 // pf_gemm_f32.hip: fp32 products straight from 16-byte-aligned operands
 bool pf_gemm_f32_direct_ok(const pf_gemm_desc& d);
 void pf_gemm_f32_direct_name(const pf_gemm_desc& d, char* out, size_t cap);   // the kernel, as the profiler prints it

@@ -258,10 +258,12 @@ int PF_H_CAT(pf_head_dh_, PF_X_DT)(const PfHeadProduct& p, hipStream_t st) {
   d.A = p.dz; d.lda = p.n_max; d.B = p.w; d.ldb = p.ldw; d.C = p.dh; d.ldc = p.depth;
   d.beta = p.add;
   d.unscale_by = p.unscale;
-  const int64_t tiles = ((p.n_max + 255) / 256) * ((p.depth + 255) / 256);
-  if (p.n_max <= 64) return hidden_launch<PF_XT_64x64>(d, p, st);
-  if (tiles <= 96) return hidden_launch<PF_XT_128x128w8>(d, p, st);
-  return hidden_launch<PF_XT_256x256w4>(d, p, st);
+  switch (pf_gemm_best_tile(d)) {
+    case PF_XT_64x64: return hidden_launch<PF_XT_64x64>(d, p, st);
+    case PF_XT_128x128w8: return hidden_launch<PF_XT_128x128w8>(d, p, st);
+    case PF_XT_256x128w8: return hidden_launch<PF_XT_256x128w8>(d, p, st);
+    default: return hidden_launch<PF_XT_256x256w4>(d, p, st);
+  }
 }
 
 int PF_H_CAT(pf_head_dw_, PF_X_DT)(const PfHeadProduct& p, hipStream_t st) {

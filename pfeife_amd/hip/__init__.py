@@ -146,6 +146,8 @@ _SIGNATURES = {
     "pf_act_bwd": [_P, _P, _P, _I, _I, _L, _P],
     "pf_glu_fwd": [_P, _L, _P, _L, _P, _L, _I, _I, _L, _L, _P],
     "pf_glu_bwd": [_P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _I, _I, _L, _L, _P],
+    "pf_gated_linear_fwd": [_P, _I, _L, _L, _P, _L, _I, _I, _P, _P, _P, _P],
+    "pf_gated_linear_bwd": [_P, _I, _L, _L, _P, _L, _I, _I, _P, _P, _P, _P, _P, _P],
     "pf_axpby": [_P, _I, _F, _P, _I, _F, _P, _I, _L, _P],
     "pf_bias_add": [_P, _I, _P, _I, _P, _I, _L, _L, _L, _P],
     "pf_groupnorm_fwd": [_P, _I, _P, _P, _P, _I, _P, _P, _L, _L, _L, _I, _F, _P],
@@ -173,12 +175,15 @@ _SIGNATURES = {
     "pf_merge_scatter": [_P, _P, _L, _L, _L, _P, _P],
     "pf_embedding_fwd": [_P, _I, _P, _P, _I, _L, _L, _L, _P],
     "pf_embedding_bwd": [_P, _I, _P, _P, _L, _L, _L, _L, _P],
+    "pf_embedding_scaled_fwd": [_P, _I, _P, _P, _L, _L, _L, _D, _P],
+    "pf_embedding_sorted_bwd": [_P, _I, _P, _P, _I, _L, _L, _L, _L, _D, _I, _P, _P],
     "pf_mfma_rate": [_I, _P, _L, _I, _P, _P],
     "pf_mfma16_rate": [_I, _P, _L, _I, _P, _P],
 }
 _RET_I64 = {"pf_gemm_colsum_rows": [POINTER(GemmDesc)], "pf_colreduce_workspace": [_L, _L], "pf_reduce_workspace": [_L],
             "pf_groupnorm_workspace": [_L, _L, _I], "pf_policy_workspace": [_L, _L, _I],
             "pf_preference_workspace": [_L, _L, _I], "pf_linear_ce_kept": [_L], "pf_linear_ce_workspace": [_P, _I, _L, _L, _L, _I],
+            "pf_embedding_sorted_workspace": [_L, _L], "pf_gated_linear_bytes": [_P, _P, _I, _L, _L, _L, _I, _I, POINTER(c_int64)],
             "pf_colsum_static_capacity": []}
 EXPORTED_SYMBOLS = sorted(list(_SIGNATURES) + list(_RET_I64) + ["pf_version", "pf_last_error"])
 
@@ -740,6 +745,22 @@ class HipKernels:
                 _dt(gate), int(act), rows, cols)
         return self._prep("pf_glu_bwd", args, (dy, gate, up, dgate, dup), 5 * rows * cols * _es(gate))
 
+    def gated_linear_bytes(self, x, weight, rows, D, ffn, keep, backward):
+        """(bytes that the forward pass leaves, bytes of workspace)"""
+        kept = c_int64(0)
+        need = int(self.lib.pf_gated_linear_bytes(_ptr(x), _ptr(weight), _dt(x), rows, D, ffn, keep, int(backward), byref(kept)))
+        if need < 0:
+            raise RuntimeError(last_error())
+        return kept.value, need
+
+    def gated_linear_fwd(self, x, rows, D, weight, ffn, act, keep, y, kept, ws):
+        args = (_ptr(x), _dt(x), rows, D, _ptr(weight), ffn, act, keep, _ptr(y), _ptr(kept), _ptr(ws))
+        return self._prep("pf_gated_linear_fwd", args, (x, weight, y, kept, ws))
+
+    def gated_linear_bwd(self, x, rows, D, weight, ffn, act, keep, kept, dy, dx, dweight, ws):
+        args = (_ptr(x), _dt(x), rows, D, _ptr(weight), ffn, act, keep, _ptr(kept), _ptr(dy), _ptr(dx), _ptr(dweight), _ptr(ws))
+        return self._prep("pf_gated_linear_bwd", args, (x, weight, kept, dy, dx, dweight, ws))
+
     def axpby(self, a, alpha, b, beta, out, n):
         args = (_ptr(a), _dt(a), alpha, _ptr(b), _dt(b), beta, _ptr(out), _dt(out), n)
         return self._prep("pf_axpby", args, (a, b, out), n * (_es(a) + _es(b) + _es(out)))
@@ -899,3 +920,14 @@ class HipKernels:
     def embedding_bwd(self, dout, ids, dtable, n_ids, dim, vocab, padding_idx=-1):
         args = (_ptr(dout), _dt(dout), _ptr(ids), _ptr(dtable), n_ids, dim, vocab, int(padding_idx))
         return self._prep("pf_embedding_bwd", args, (dout, ids, dtable))
+
+    def embedding_scaled_fwd(self, table, ids, out, n_ids, dim, vocab, scale):
+        args = (_ptr(table), _dt(table), _ptr(ids), _ptr(out), n_ids, dim, vocab, scale)
+        return self._prep("pf_embedding_scaled_fwd", args, (table, ids, out))
+
+    def embedding_sorted_workspace(self, n_ids, dim):
+        return int(self.lib.pf_embedding_sorted_workspace(n_ids, dim))
+
+    def embedding_sorted_bwd(self, dout, ids, dtable, n_ids, dim, vocab, padding_idx, scale, accumulate, ws):
+        args = (_ptr(dout), _dt(dout), _ptr(ids), _ptr(dtable), _dt(dtable), n_ids, dim, vocab, padding_idx, scale, int(accumulate), _ptr(ws))
+        return self._prep("pf_embedding_sorted_bwd", args, (dout, ids, dtable, ws))

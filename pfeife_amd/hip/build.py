@@ -30,6 +30,8 @@ SOURCES = [
     "pf_softmax_loss.hip",
     "pf_token_loss.hip",
     "pf_head.hip",
+    "pf_gated.hip",
+    "pf_table.hip",
     "pf_adam8.hip",
     "pf_batch.hip",
     "pf_mfma_rate.hip",
@@ -41,7 +43,7 @@ GEMM_X_SOURCE = "pf_gemm_x_inst.hip"
 GEMM_X_PAIRS = [(dt, xt) for xt in (12, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 13) for dt in (1, 2)]
 
 # further products on that kernel with epilogues of their own: one object per operand dtype id
-TAIL_SOURCES = ["pf_head_x.hip"]
+TAIL_SOURCES = ["pf_head_x.hip", "pf_gated_x.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
