@@ -428,7 +428,7 @@ int pf_policy_loss(const void* logits, int dtype, int64_t B, int64_t T, int64_t 
  * take part; 2: their sum (of none: 0).  kept: pf_linear_ce_kept(B * T) bytes, written by the forward pass and read by the backward
  * pass; workspace: pf_linear_ce_workspace bytes, on a boundary of 256 bytes (weight: its address decides whether a copy is needed; a negative status
  * where the sizes are refused).  hidden and weight hold the same values in both passes.
- *   pf_linear_ce_bwd          dhidden [B, T, D] and dweight [V, D] (either may be null), contiguous, in the operands' type; grad: of the loss,
+ *   pf_linear_ce_bwd          dhidden [B, T, D] and dweight [V, D] (either may be null), contiguous, in the operands' type, on boundaries of 16 bytes; grad: of the loss,
  *                             or (reduction 0) of every token's, grad[b * g_sb + t * g_st].  mean != 0: reduction 1
  *   pf_linear_ce_hidden_grad  after pf_linear_ce_bwd, from what its workspace still holds: dhidden times a factor in device memory (null: 1), rounded once
  * Stands in for the last stage's aten::linear followed by nn.CrossEntropyLoss (pfeife/loss.py:53-70). */
@@ -469,11 +469,12 @@ int pf_glu_bwd(const void* dy, int64_t ld_dy, const void* gate, int64_t ld_gate,
 /* Gated projection with both of its products: y = act(x Wg^T) * (x Wu^T), weight [2 ffn, D] with the gate's rows first, x [rows, D], y
  * [rows, ffn], all contiguous and of one type (fp32, fp16 or bf16; no alignment asked for).  keep: what the backward pass starts from
  * and `kept` takes, 0 nothing (no backward pass), 1 both products in the operands' type, 2 (16-bit operands) both as e4m3 codes, 16
- * neighbouring columns of a row under one power of two.  pf_gated_linear_bytes: bytes of workspace of either pass, on a boundary of 256 bytes,
- * and of `kept` (the operands' addresses decide whether copies are needed; a negative status where the sizes are refused).  The
- * backward pass takes x and weight as they were: dx [rows, D] and dweight [2 ffn, D], either may be null.  Replaces the aten::linear pair
- * and the product behind it of a gated MLP, and their backward. */
-int64_t pf_gated_linear_bytes(const void* x, const void* weight, int dtype, int64_t rows, int64_t D, int64_t ffn, int keep, int backward, int64_t* kept);
+ * neighbouring columns of a row under one power of two.  kept: pf_gated_linear_kept bytes, on a boundary of 16 bytes; workspace:
+ * pf_gated_linear_workspace bytes, on a boundary of 256 bytes (the operands' addresses decide whether copies are needed; a negative status
+ * where the sizes are refused).  The backward pass takes x and weight as they were: dx [rows, D] and dweight [2 ffn, D], either may be
+ * null, on boundaries of 16 bytes.  Replaces the aten::linear pair and the product behind it of a gated MLP, and their backward. */
+int64_t pf_gated_linear_kept(int dtype, int64_t rows, int64_t ffn, int keep);
+int64_t pf_gated_linear_workspace(const void* x, const void* weight, int dtype, int64_t rows, int64_t D, int64_t ffn, int keep, int backward);
 int pf_gated_linear_fwd(const void* x, int dtype, int64_t rows, int64_t D, const void* weight, int64_t ffn, int act, int keep, void* y, void* kept,
                         void* workspace, void* stream);
 int pf_gated_linear_bwd(const void* x, int dtype, int64_t rows, int64_t D, const void* weight, int64_t ffn, int act, int keep, const void* kept,
@@ -639,7 +640,7 @@ int pf_embedding_bwd(const void* dout, int d_dtype, const int64_t* ids, float* d
  * scale * sum of dout[i, :] over ids[i] = v, summed in fp32 whatever the types (t_dtype: that of dout, or fp32), the same bits for the
  * same ids.  Every row of dtable is written, zeros where no id names it; accumulate != 0: added to what is there, other rows are left
  * alone.  Ids outside [0, vocab) give NaN rows and no gradient; padding_idx (-1: none) gets no gradient.  workspace:
- * pf_embedding_sorted_workspace bytes, on a boundary of 256 bytes.  Replaces aten::embedding, the product behind it and
+ * pf_embedding_sorted_workspace bytes (none for a few ids), on a boundary of 256 bytes.  Replaces aten::embedding, the product behind it and
  * embedding_dense_backward. */
 int pf_embedding_scaled_fwd(const void* table, int dtype, const int64_t* ids, void* out, int64_t n_ids, int64_t dim, int64_t vocab, double scale, void* stream);
 int64_t pf_embedding_sorted_workspace(int64_t n_ids, int64_t dim);

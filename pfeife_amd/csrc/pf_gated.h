@@ -17,7 +17,7 @@ struct PfGatedProduct {
   int64_t ldy;
   void* kept;                  // the two halves of a row side by side, each `half` columns; with 8 bits codes
   int64_t half;                // a multiple of 8 (8 bits: of 16)
-  uint8_t* exps;               // 8 bits: exponents + 127, half / 16 of each half of a row
+  uint8_t* exps;               // 8 bits: exponents + 127, those of four rows' same columns side by side: [rows / 4][2 half / 16][4]
 };
 int pf_gated_forward_1(const PfGatedProduct& p, hipStream_t st);
 int pf_gated_forward_2(const PfGatedProduct& p, hipStream_t st);

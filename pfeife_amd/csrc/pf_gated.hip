@@ -8,6 +8,8 @@
 // largest of the 16 to 448 or below, so that nothing saturates, and decoding is exact.  The pass over the elements that
 // makes dg and du reads the codes as they are: 4.1 bytes instead of 6 an element of y, and 4 written.
 #include "pf_gated.h"
+#include "pf_gemm_common.h"
+#include "pf_rows.h"
 
 namespace {
 
@@ -31,7 +33,7 @@ __device__ __forceinline__ void kept_load(const void* kept, const uint8_t* exps,
     Vec8<DT>::load(kept, row * 2 * half + at, v);
   } else {
     const uint2 c = *(const uint2*)((const uint8_t*)kept + row * 2 * half + at);
-    const float by = pf_pow2(exps[(row * 2 * half + at) / PF_GATED_BLOCK]);
+    const float by = pf_pow2(exps[(row / 4 * 2 * half + at) / PF_GATED_BLOCK * 4 + row % 4]);
     v[0] = __builtin_amdgcn_cvt_f32_fp8((int)c.x, 0) * by; v[1] = __builtin_amdgcn_cvt_f32_fp8((int)c.x, 1) * by;
     v[2] = __builtin_amdgcn_cvt_f32_fp8((int)c.x, 2) * by; v[3] = __builtin_amdgcn_cvt_f32_fp8((int)c.x, 3) * by;
     v[4] = __builtin_amdgcn_cvt_f32_fp8((int)c.y, 0) * by; v[5] = __builtin_amdgcn_cvt_f32_fp8((int)c.y, 1) * by;
@@ -83,18 +85,25 @@ void backward_launch(const void* dy, const void* kept, const uint8_t* exps, int6
 #undef PF_GB
 }
 
-// a matrix with its rows' width raised (and of two halves each its number of rows), zeros in what is new
-__global__ __launch_bounds__(256) void gated_widen_kernel(const uint16_t* src, int64_t rows, int64_t width, uint16_t* dst, int64_t to_rows, int64_t to_width, int halves) {
-  const int64_t per = to_rows * to_width, total = per * halves;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t h = i / per, r = i % per / to_width, c = i % to_width;
-    dst[i] = r < rows && c < width ? src[(h * rows + r) * width + c] : (uint16_t)0;
+// dx from the sums of its shares, [splits][rows][ld] in fp32
+template <int W>
+__global__ __launch_bounds__(256) void gated_join_kernel(const float* acc, int64_t ld, int splits, int64_t rows, int64_t D, void* dx, int dt) {
+  const int64_t per = (D + 64 * W - 1) / (64 * W), total = rows * per;      // (a wavefront to 64 W columns of a row)
+  for (int64_t q = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); q < total; q += (int64_t)gridDim.x * 4) {
+    const int64_t r = q / per, i = q % per * 64 * W + (threadIdx.x & 63) * W;
+    if (i >= D) continue;
+    float v[W];
+#pragma unroll
+    for (int k = 0; k < W; ++k) v[k] = 0.f;
+#pragma unroll 4
+    for (int p = 0; p < splits; ++p) {
+      float w[W];
+      ld_vec<W>(acc, (p * rows + r) * ld + i, PF_F32, w);
+#pragma unroll
+      for (int k = 0; k < W; ++k) v[k] += w[k];
+    }
+    st_vec<W>(dx, r * D + i, dt, v);
   }
-}
-void widen_rows(const void* src, int64_t rows, int64_t width, void* dst, int64_t to_rows, int64_t to_width, int halves, hipStream_t st) {
-  const int64_t blocks = (to_rows * to_width * halves + 255) / 256;
-  hipLaunchKernelGGL(gated_widen_kernel, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st, (const uint16_t*)src, rows, width, (uint16_t*)dst, to_rows,
-                     to_width, halves);
 }
 
 // A few rows: a wavefront takes a column of y, i.e. one row of either half of the weight, and R rows of x from LDS.  Bound by the
@@ -165,45 +174,21 @@ int few(int r, const void* x, const void* w, int64_t depth, int64_t rows, int64_
   }
 }
 
-// What lies where.  16 bits: depth is the width of the rows that the products read, of x and of the weight, which are copied where theirs
-// is another; wide that of one half of dg and du, with as many columns of the transposed weight.
+// What lies where.  depth: the width of the rows that the products read, of x and of the weight, which are copied where theirs is
+// another (16 bytes have to lie at their front); wide: that of one half of dg and du, and with 16 bits of the transposed weight; half: that
+// of one half of what is kept.
+int64_t half_of(int dtype, int64_t ffn, int keep) { return round_up(ffn, keep == PF_KEEP_8BIT ? PF_GATED_BLOCK : dtype == PF_F32 ? 4 : 8); }
+int64_t kept_bytes(int dtype, int64_t rows, int64_t ffn, int keep) {
+  const int64_t half = half_of(dtype, ffn, keep);
+  return keep == PF_KEEP_8BIT ? rows * 2 * half + (rows + 3) / 4 * 4 * (2 * half / PF_GATED_BLOCK) : rows * 2 * half * (dtype == PF_F32 ? 4 : 2);
+}
 struct Plan {
-  int64_t es, depth, wide, half, kept, chunk;
-  bool copy_x, copy_w;
-  char* x; char* w; char* wt; char* dgu;
+  int64_t es, depth, wide, half, chunk;
+  bool copy_x, copy_w, narrow;
+  int splits;                  // of dx's sums (with `parts`)
+  char* x; char* w; char* wt; char* dgu; char* dw; float* parts;
   int64_t bytes;
 };
-bool plan_of(Plan& p, const void* x, const void* w, int dtype, int64_t rows, int64_t D, int64_t ffn, int keep, bool back, char* base) {
-  p.es = dtype == PF_F32 ? 4 : 2;
-  const bool f32 = dtype == PF_F32;
-  p.depth = f32 ? D : (D < 64 ? 64 : round_up(D, 8));
-  p.wide = f32 ? ffn : round_up(ffn, 8);
-  p.half = f32 ? ffn : keep == PF_KEEP_8BIT ? round_up(ffn, PF_GATED_BLOCK) : round_up(ffn, 8);
-  p.kept = keep == PF_KEEP_8BIT ? rows * 2 * p.half / PF_GATED_BLOCK * (PF_GATED_BLOCK + 1) : rows * 2 * p.half * p.es;
-  p.copy_x = !f32 && (p.depth != D || !pf_aligned(x, 16));
-  p.copy_w = !f32 && (p.depth != D || !pf_aligned(w, 16));
-  // rows of one launch: everything it addresses by 32-bit offsets stays below 2 GiB
-  const int64_t widest = p.depth > 2 * p.half ? p.depth : 2 * p.half;
-  p.chunk = ((1ll << 31) / (widest * p.es) - 512) / 256 * 256;
-  p.x = p.w = p.wt = p.dgu = nullptr;
-  int64_t used = 0;
-  auto take = [&](int64_t bytes) {
-    char* q = base == nullptr ? nullptr : base + used;
-    used += round_up(bytes, 256);
-    return q;
-  };
-  if (p.copy_x) p.x = take(rows * p.depth * 2);
-  if (p.copy_w) p.w = take(2 * ffn * p.depth * 2);
-  if (back) {
-    p.dgu = take(rows * 2 * p.wide * p.es);
-    if (!f32) p.wt = take(p.depth * 2 * p.wide * 2);
-  } else if (f32 && keep == PF_KEEP_NONE) {
-    p.dgu = take(rows * 2 * ffn * 4);
-  }
-  p.bytes = used;
-  return p.depth < (1ll << 19) && p.half < (1ll << 18) && p.chunk > 0 && (2 * ffn + 512) * p.depth * 2 < (1ll << 31) && (p.depth + 512) * 2 * p.wide * 2 < (1ll << 31) &&
-         (keep == PF_KEEP_NONE ? rows < (1ll << 31) : f32 || rows <= p.chunk);
-}
 
 int check(const char* who, int dtype, int64_t rows, int64_t D, int64_t ffn, int act, int keep) {
   PF_REQUIRE(dtype == PF_F32 || dtype == PF_F16 || dtype == PF_BF16, "%s: bad dtype", who);
@@ -217,27 +202,110 @@ int too_large(const char* who) {
   return PF_ERR_INVALID;
 }
 
-int product(int dtype, int a_trans, int b_trans, int64_t M, int64_t N, int64_t K, const void* A, int64_t lda, const void* B, int64_t ldb, void* C, int64_t ldc,
-            hipStream_t st) {
+// batch: shares of the depth, with results of their own; what does not divide is added to the first
+int product(int dtype, int c_dtype, int a_trans, int b_trans, int64_t M, int64_t N, int64_t K, const void* A, int64_t lda, const void* B, int64_t ldb, void* C,
+            int64_t ldc, int beta, hipStream_t st, int splits = 1) {
   pf_gemm_desc d = {};
-  d.in_dtype = d.c_dtype = dtype;
+  d.in_dtype = dtype;
+  d.c_dtype = c_dtype;
   d.a_trans = a_trans; d.b_trans = b_trans;
   d.M = M; d.N = N; d.K = K;
   d.A = A; d.lda = lda; d.B = B; d.ldb = ldb; d.C = C; d.ldc = ldc;
   d.batch1 = d.batch2 = 1;
   d.alpha = 1.f;
+  d.beta = beta;
+  const int64_t share = splits > 1 ? K / splits / 64 * 64 : 0;
+  if (share == 0) return pf_gemm(&d, st);
+  const int64_t es = dtype == PF_F32 ? 4 : 2;
+  d.K = share;
+  d.batch2 = splits;
+  d.a_stride2 = share * (a_trans ? lda : 1);
+  d.b_stride2 = share * (b_trans ? ldb : 1);
+  d.c_stride2 = M * ldc;
+  const int rc = pf_gemm(&d, st);
+  if (rc != PF_OK || share * splits == K) return rc;
+  d.K = K - share * splits;
+  d.batch2 = 1;
+  d.A = (const char*)A + splits * d.a_stride2 * es;
+  d.B = (const char*)B + splits * d.b_stride2 * es;
+  d.beta = 1;
   return pf_gemm(&d, st);
+}
+
+// In how many shares dx is best summed: few rows make few tiles, whose depth is both halves of the weight
+int splits_of(int dtype, int64_t rows, int64_t D, int64_t K) {
+  int best = 1;
+  double best_t = 0;
+  for (int s = 1; s <= 16 && (s == 1 || K / s >= 256); s *= 2) {
+    double t = 0;
+    if (dtype == PF_F32) {
+      const int64_t tiles = ((rows + 63) / 64) * ((D + 63) / 64) * s;      // (17 ns a unit of depth and 64x64 tile)
+      t = (double)((tiles + 255) / 256) * 0.0171 * (double)(K / s);
+    } else {
+      pf_gemm_desc d = {};
+      d.in_dtype = dtype;
+      d.c_dtype = PF_F32;
+      d.M = rows; d.N = D; d.K = K / s / 64 * 64 > 0 ? K / s / 64 * 64 : K;
+      d.batch1 = 1;
+      d.batch2 = s;
+      pf_gemm_best_tile(d, &t);
+    }
+    if (s > 1) t += 4.0 + (double)(rows * D) * s * 8.0 / 5.0e6;      // a launch, and the shares' way through memory at 5 TB/s
+    if (s == 1 || t < best_t) { best = s; best_t = t; }
+  }
+  return best;
+}
+
+bool plan_of(Plan& p, const void* x, const void* w, int dtype, int64_t rows, int64_t D, int64_t ffn, int keep, bool back, char* base) {
+  const bool f32 = dtype == PF_F32;
+  p.es = f32 ? 4 : 2;
+  p.depth = f32 ? round_up(D, 4) : (D < 64 ? 64 : round_up(D, 8));
+  p.wide = round_up(ffn, f32 ? 4 : 8);
+  p.half = half_of(dtype, ffn, keep);
+  p.copy_x = p.depth != D || !pf_aligned(x, 16);
+  p.copy_w = p.depth != D || !pf_aligned(w, 16);
+  p.narrow = !f32 && D % 8 != 0;
+  p.splits = back ? splits_of(dtype, rows, D, p.wide == ffn ? 2 * ffn : ffn) : 1;
+  // rows of one launch: everything it addresses by 32-bit offsets stays below 2 GiB
+  const int64_t widest = p.depth > 2 * p.half ? p.depth : 2 * p.half;
+  p.chunk = ((1ll << 31) / (widest * p.es) - 512) / 256 * 256;
+  p.x = p.w = p.wt = p.dgu = p.dw = nullptr;
+  p.parts = nullptr;
+  int64_t used = 0;
+  auto take = [&](int64_t bytes) {
+    char* q = base == nullptr ? nullptr : base + used;
+    used += round_up(bytes, 256);
+    return q;
+  };
+  if (p.copy_x) p.x = take(rows * p.depth * p.es);
+  if (p.copy_w) p.w = take(2 * ffn * p.depth * p.es);
+  if (back) {
+    p.dgu = take(rows * 2 * p.wide * p.es);
+    if (!f32) p.wt = take(p.depth * 2 * p.wide * 2);
+    if (p.narrow) p.dw = take(2 * ffn * p.depth * 2);
+    if (p.splits > 1 || p.narrow) p.parts = (float*)take(p.splits * rows * p.depth * 4);
+  } else if (f32 && keep == PF_KEEP_NONE) {
+    p.dgu = take(rows * 2 * p.wide * 4);
+  }
+  p.bytes = used;
+  return p.depth < (1ll << 19) && p.half < (1ll << 18) && p.chunk > 0 && (2 * ffn + 512) * p.depth * 2 < (1ll << 31) && (p.depth + 512) * 2 * p.wide * 2 < (1ll << 31) &&
+         (keep == PF_KEEP_NONE ? rows < (1ll << 31) : f32 || rows <= p.chunk);
 }
 
 }  // namespace
 
-extern "C" int64_t pf_gated_linear_bytes(const void* x, const void* weight, int dtype, int64_t rows, int64_t D, int64_t ffn, int keep, int backward, int64_t* kept) {
-  const char* who = "pf_gated_linear_bytes";
-  int rc = check(who, dtype, rows, D, ffn, PF_ACT_SILU, keep);
+extern "C" int64_t pf_gated_linear_kept(int dtype, int64_t rows, int64_t ffn, int keep) {
+  const int rc = check("pf_gated_linear_kept", dtype, rows, 1, ffn, PF_ACT_SILU, keep);
+  if (rc != PF_OK || keep == PF_KEEP_NONE) return rc;
+  return kept_bytes(dtype, rows, ffn, keep);
+}
+
+extern "C" int64_t pf_gated_linear_workspace(const void* x, const void* weight, int dtype, int64_t rows, int64_t D, int64_t ffn, int keep, int backward) {
+  const char* who = "pf_gated_linear_workspace";
+  const int rc = check(who, dtype, rows, D, ffn, PF_ACT_SILU, keep);
   if (rc != PF_OK) return rc;
   Plan p;
   if (!plan_of(p, x, weight, dtype, rows, D, ffn, keep, backward != 0, nullptr)) return too_large(who);
-  if (kept != nullptr) *kept = keep == PF_KEEP_NONE ? 0 : p.kept;
   return p.bytes;
 }
 
@@ -251,15 +319,24 @@ extern "C" int pf_gated_linear_fwd(const void* x, int dtype, int64_t rows, int64
   PF_REQUIRE(x && weight && y && (keep == PF_KEEP_NONE || kept) && (p.bytes == 0 || workspace), "%s: null pointer", who);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == PF_F32) {
-    const int r = D % 8 == 0 && pf_aligned(x, 16) && pf_aligned(weight, 16) ? few_rows(rows, D, 4) : 0;
-    if (r > 0) return few<PF_F32>(r, x, weight, D, rows, ffn, act, y, kept, ffn, st);
+    const int r = D % 8 == 0 && !p.copy_x && !p.copy_w ? few_rows(rows, D, 4) : 0;
+    if (r > 0) return few<PF_F32>(r, x, weight, D, rows, ffn, act, y, kept, p.half, st);
+    if (p.copy_x) pf_rows_widen(x, rows, D, p.x, rows, p.depth, 1, 4, st);
+    if (p.copy_w) pf_rows_widen(weight, 2 * ffn, D, p.w, 2 * ffn, p.depth, 1, 4, st);
+    const float* xs = p.copy_x ? (const float*)p.x : (const float*)x;
+    const float* ws = p.copy_w ? (const float*)p.w : (const float*)weight;
     float* gu = keep == PF_KEEP_NONE ? (float*)p.dgu : (float*)kept;
-    rc = product(PF_F32, 0, 0, rows, 2 * ffn, D, x, D, weight, D, gu, 2 * ffn, st);
+    if (p.wide == ffn) {
+      rc = product(PF_F32, PF_F32, 0, 0, rows, 2 * ffn, D, xs, p.depth, ws, p.depth, gu, 2 * ffn, 0, st);
+    } else {
+      for (int h = 0; h < 2 && rc == PF_OK; ++h)
+        rc = product(PF_F32, PF_F32, 0, 0, rows, ffn, D, xs, p.depth, ws + h * ffn * p.depth, p.depth, gu + h * p.wide, 2 * p.wide, 0, st);
+    }
     if (rc != PF_OK) return rc;
-    return pf_glu_fwd(gu, 2 * ffn, gu + ffn, 2 * ffn, y, ffn, PF_F32, act, rows, ffn, stream);
+    return pf_glu_fwd(gu, 2 * p.wide, gu + p.wide, 2 * p.wide, y, ffn, PF_F32, act, rows, ffn, stream);
   }
-  if (p.copy_x) widen_rows(x, rows, D, p.x, rows, p.depth, 1, st);
-  if (p.copy_w) widen_rows(weight, 2 * ffn, D, p.w, 2 * ffn, p.depth, 1, st);
+  if (p.copy_x) pf_rows_widen(x, rows, D, p.x, rows, p.depth, 1, 2, st);
+  if (p.copy_w) pf_rows_widen(weight, 2 * ffn, D, p.w, 2 * ffn, p.depth, 1, 2, st);
   PF_CHECK_LAUNCH(who);
   const int r = keep == PF_KEEP_8BIT ? 0 : few_rows(rows, p.depth, 2);
   if (r > 0) {
@@ -296,49 +373,73 @@ extern "C" int pf_gated_linear_bwd(const void* x, int dtype, int64_t rows, int64
   hipStream_t st = (hipStream_t)stream;
   if (rows == 0) return dweight == nullptr ? PF_OK : pf_fill(dweight, dtype, 0.f, 2 * ffn * D, stream);
   PF_REQUIRE(x && weight && kept && dy && workspace, "%s: null pointer", who);
-  if (dtype == PF_F32) {
+  PF_REQUIRE(dtype == PF_F32 || (pf_aligned(dx, 16) && pf_aligned(dweight, 16)), "%s: the gradients lie on boundaries of 16 bytes", who);
+  const bool f32 = dtype == PF_F32;
+  const int es = f32 ? 4 : 2;
+  const int halves = p.wide == ffn ? 1 : 2;      // products over both halves of the weight at once, or one by one
+  if (f32) {
     const float* gu = (const float*)kept;
     float* d = (float*)p.dgu;
-    rc = pf_glu_bwd(dy, ffn, gu, 2 * ffn, gu + ffn, 2 * ffn, d, 2 * ffn, d + ffn, 2 * ffn, PF_F32, act, rows, ffn, stream);
-    if (rc == PF_OK && dx) rc = product(PF_F32, 0, 1, rows, D, 2 * ffn, d, 2 * ffn, weight, D, dx, D, st);
-    if (rc == PF_OK && dweight) rc = product(PF_F32, 1, 1, 2 * ffn, D, rows, d, 2 * ffn, x, D, dweight, D, st);
-    return rc;
-  }
-  const uint8_t* exps = keep == PF_KEEP_8BIT ? (const uint8_t*)kept + rows * 2 * p.half : nullptr;
-  if (dtype == PF_F16) {
-    if (keep == PF_KEEP_SAME) backward_launch<PF_F16, PF_KEEP_SAME>(dy, kept, exps, p.half, rows, ffn, p.dgu, p.wide, act, st);
-    else backward_launch<PF_F16, PF_KEEP_8BIT>(dy, kept, exps, p.half, rows, ffn, p.dgu, p.wide, act, st);
+    rc = pf_glu_bwd(dy, ffn, gu, 2 * p.wide, gu + p.wide, 2 * p.wide, d, 2 * p.wide, d + p.wide, 2 * p.wide, PF_F32, act, rows, ffn, stream);
+    if (rc != PF_OK) return rc;
   } else {
-    if (keep == PF_KEEP_SAME) backward_launch<PF_BF16, PF_KEEP_SAME>(dy, kept, exps, p.half, rows, ffn, p.dgu, p.wide, act, st);
-    else backward_launch<PF_BF16, PF_KEEP_8BIT>(dy, kept, exps, p.half, rows, ffn, p.dgu, p.wide, act, st);
+    const uint8_t* exps = keep == PF_KEEP_8BIT ? (const uint8_t*)kept + rows * 2 * p.half : nullptr;
+    if (dtype == PF_F16) {
+      if (keep == PF_KEEP_SAME) backward_launch<PF_F16, PF_KEEP_SAME>(dy, kept, exps, p.half, rows, ffn, p.dgu, p.wide, act, st);
+      else backward_launch<PF_F16, PF_KEEP_8BIT>(dy, kept, exps, p.half, rows, ffn, p.dgu, p.wide, act, st);
+    } else {
+      if (keep == PF_KEEP_SAME) backward_launch<PF_BF16, PF_KEEP_SAME>(dy, kept, exps, p.half, rows, ffn, p.dgu, p.wide, act, st);
+      else backward_launch<PF_BF16, PF_KEEP_8BIT>(dy, kept, exps, p.half, rows, ffn, p.dgu, p.wide, act, st);
+    }
   }
-  if (p.copy_x && dweight) widen_rows(x, rows, D, p.x, rows, p.depth, 1, st);
+  if (p.copy_x && dweight) pf_rows_widen(x, rows, D, p.x, rows, p.depth, 1, es, st);
   PF_CHECK_LAUNCH(who);
   const char* xs = p.copy_x ? p.x : (const char*)x;
   if (dx) {
-    // the reduction runs along the weight's rows, its transposed copy makes it contiguous: 6 % of the product at 8192 rows, where the
-    // product without it runs at half the rate
-    if (p.wide != ffn) {
-      rc = pf_fill(p.wt, dtype, 0.f, D * 2 * p.wide, stream);
-      if (rc != PF_OK) return rc;
+    const bool parts = p.parts != nullptr;
+    void* c = parts ? (void*)p.parts : dx;
+    const int64_t ldc = parts ? p.depth : D, n = parts && !f32 ? round_up(D, 8) : D;
+    const int c_dtype = parts ? PF_F32 : dtype;
+    if (f32) {
+      if (p.copy_w) pf_rows_widen(weight, 2 * ffn, D, p.w, 2 * ffn, p.depth, 1, 4, st);
+      const float* ws = p.copy_w ? (const float*)p.w : (const float*)weight;
+      const float* d = (const float*)p.dgu;
+      for (int h = 0; h < halves && rc == PF_OK; ++h)
+        rc = product(dtype, c_dtype, 0, 1, rows, n, halves == 1 ? 2 * ffn : ffn, d + h * p.wide, 2 * p.wide, ws + h * ffn * p.depth, p.depth, c, ldc, h, st, p.splits);
+    } else {
+      // The reduction runs along the weight's rows, its transposed copy makes it contiguous: 3 % of the pass at 8192 rows, where the
+      // product without it runs at half the rate.  (Columns past ffn, of zeros in dg and du, are zeros here too.)
+      if (halves == 1) {
+        rc = pf_transpose_cast(weight, dtype, D, p.wt, dtype, 2 * ffn, 2 * ffn, D, stream);
+      } else {
+        rc = pf_fill(p.wt, dtype, 0.f, D * 2 * p.wide, stream);
+        for (int h = 0; h < 2 && rc == PF_OK; ++h)
+          rc = pf_transpose_cast((const char*)weight + h * ffn * D * 2, dtype, D, p.wt + h * p.wide * 2, dtype, 2 * p.wide, ffn, D, stream);
+      }
+      if (rc == PF_OK) rc = product(dtype, c_dtype, 0, 0, rows, n, 2 * p.wide, p.dgu, 2 * p.wide, p.wt, 2 * p.wide, c, ldc, 0, st, p.splits);
     }
-    for (int h = 0; h < 2; ++h) {
-      rc = pf_transpose_cast((const char*)weight + h * ffn * D * 2, dtype, D, p.wt + h * p.wide * 2, dtype, 2 * p.wide, ffn, D, stream);
-      if (rc != PF_OK) return rc;
-    }
-    for (int64_t r = 0; r < rows; r += p.chunk) {
-      const int64_t n = rows - r < p.chunk ? rows - r : p.chunk;
-      rc = product(dtype, 0, 0, n, D, 2 * p.wide, p.dgu + r * 2 * p.wide * 2, 2 * p.wide, p.wt, 2 * p.wide, (char*)dx + r * D * 2, D, st);
-      if (rc != PF_OK) return rc;
+    if (rc != PF_OK) return rc;
+    if (parts) {
+      const int64_t lanes = D % 8 == 0 ? 512 : 64, units = (rows * ((D + lanes - 1) / lanes) + 3) / 4;
+      const dim3 grid((unsigned)(units < 16384 ? units : 16384));
+      if (D % 8 == 0) hipLaunchKernelGGL(gated_join_kernel<8>, grid, dim3(256), 0, st, p.parts, p.depth, p.splits, rows, D, dx, dtype);
+      else hipLaunchKernelGGL(gated_join_kernel<1>, grid, dim3(256), 0, st, p.parts, p.depth, p.splits, rows, D, dx, dtype);
     }
   }
   if (dweight) {
-    auto weight_product = dtype == PF_F16 ? pf_gated_weight_1 : pf_gated_weight_2;
-    if (p.wide == ffn) return weight_product(2 * ffn, D, rows, p.dgu, 2 * p.wide, xs, p.depth, dweight, D, st);
-    for (int h = 0; h < 2; ++h) {
-      rc = weight_product(ffn, D, rows, p.dgu + h * p.wide * 2, 2 * p.wide, xs, p.depth, (char*)dweight + h * ffn * D * 2, D, st);
-      if (rc != PF_OK) return rc;
+    char* out = p.narrow ? p.dw : (char*)dweight;
+    const int64_t ldc = p.narrow ? p.depth : D, n = p.narrow ? round_up(D, 8) : D;
+    for (int h = 0; h < halves && rc == PF_OK; ++h) {
+      const int64_t m = halves == 1 ? 2 * ffn : ffn;
+      const char* d = p.dgu + h * p.wide * es;
+      char* c = out + h * ffn * ldc * es;
+      if (f32) rc = product(dtype, dtype, 1, 1, m, n, rows, d, 2 * p.wide, xs, p.depth, c, ldc, 0, st);
+      else if (dtype == PF_F16) rc = pf_gated_weight_1(m, n, rows, d, 2 * p.wide, xs, p.depth, c, ldc, st);
+      else rc = pf_gated_weight_2(m, n, rows, d, 2 * p.wide, xs, p.depth, c, ldc, st);
     }
+    if (rc != PF_OK) return rc;
+    if (p.narrow) pf_rows_narrow(p.dw, p.depth, dweight, 2 * ffn, D, st);
   }
+  PF_CHECK_LAUNCH(who);
   return PF_OK;
 }

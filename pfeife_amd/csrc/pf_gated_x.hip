@@ -40,6 +40,19 @@ __device__ __forceinline__ void store8(__amdgpu_buffer_rsrc_t rs, uint32_t at, c
   }
 }
 
+// The largest of N neighbouring lanes' values (N = 4, 8 or 16), which share a data-parallel row: no trip through LDS
+template <int N> __device__ __forceinline__ float largest(float v) {
+  auto with = [&](auto c) {
+    const int o = __builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(c)::value, 0xf, 0xf, true);
+    v = fmaxf(v, __int_as_float(o));
+  };
+  with(std::integral_constant<int, 0xB1>{});                            // lanes 1 0 3 2
+  with(std::integral_constant<int, 0x4E>{});                            // lanes 2 3 0 1
+  if constexpr (N >= 8) with(std::integral_constant<int, 0x141>{});     // mirrored in 8
+  if constexpr (N >= 16) with(std::integral_constant<int, 0x140>{});    // mirrored in 16
+  return v;
+}
+
 template <int KEEP> struct GatedTail {
   static constexpr bool PAIR = true;
   uint16_t* y;
@@ -56,11 +69,12 @@ template <int KEEP> struct GatedTail {
     constexpr uint32_t OOB = 0x80000000u;
     const __amdgpu_buffer_rsrc_t rs_y = make_rsrc(y, (uint32_t)(((M - 1) * ldy + N) * 2));
     const __amdgpu_buffer_rsrc_t rs_k = make_rsrc(KEEP ? kept : (void*)y, KEEP ? (uint32_t)(M * half * 2 * KS) : 0u);
-    const __amdgpu_buffer_rsrc_t rs_e = make_rsrc(KEEP == PF_KEEP_8BIT ? (void*)exps : (void*)y, KEEP == PF_KEEP_8BIT ? (uint32_t)(M * (half / PF_GATED_BLOCK) * 2) : 0u);
+    const __amdgpu_buffer_rsrc_t rs_e =
+        make_rsrc(KEEP == PF_KEEP_8BIT ? (void*)exps : (void*)y, KEEP == PF_KEEP_8BIT ? (uint32_t)((M + 3) / 4 * (half / PF_GATED_BLOCK) * 8) : 0u);
     const bool in = c0 < half;                      // (of what is kept; with 8 bits whole groups of lanes)
     uint32_t at_y = c0 < N ? (uint32_t)((row0 * ldy + c0) * 2) : OOB;
     uint32_t at_k = in ? (uint32_t)((row0 * half * 2 + c0) * KS) : OOB;
-    uint32_t at_e = in && lane % GROUP == 0 ? (uint32_t)(row0 * (half / PF_GATED_BLOCK) * 2 + c0 / PF_GATED_BLOCK) : OOB;
+    uint32_t at_e = in && lane % GROUP == 0 ? (uint32_t)(row0 * (half / PF_GATED_BLOCK) * 2 + c0 / PF_GATED_BLOCK * 4) : OOB;
     const uint32_t step_y = (uint32_t)(ldy * 2), step_k = (uint32_t)(half * 2 * KS), step_e = (uint32_t)(half / PF_GATED_BLOCK * 2);
 #pragma nounroll
     for (int h = 0; h < TM; ++h) {
@@ -87,6 +101,7 @@ template <int KEEP> struct GatedTail {
         case PF_ACT_GELU_TANH: gate([](float t) { return pf_gelu_tanh(t); }); break;
         default: gate([](float t) { return t > 0.f ? t : (t != t ? t : 0.f); }); break;
       }
+      uint32_t eg4 = 0, eu4 = 0;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         float o[P], g[P], u[P];
@@ -109,14 +124,16 @@ template <int KEEP> struct GatedTail {
           float tg = 0.f, tu = 0.f;
 #pragma unroll
           for (int k = 0; k < P; ++k) { tg = fmaxf(tg, fabsf(g[k])); tu = fmaxf(tu, fabsf(u[k])); }
-#pragma unroll
-          for (int o2 = 1; o2 < GROUP; o2 <<= 1) { tg = fmaxf(tg, __shfl_xor(tg, o2, 64)); tu = fmaxf(tu, __shfl_xor(tu, o2, 64)); }
-          const int eg = pf_e4m3_exponent(tg), eu = pf_e4m3_exponent(tu);
+          const int eg = pf_e4m3_exponent(largest<GROUP>(tg)), eu = pf_e4m3_exponent(largest<GROUP>(tu));
           store8<P>(rs_k, at_k + (uint32_t)r * step_k, g, pf_pow2(254 - eg));
           store8<P>(rs_k, at_k + (uint32_t)r * step_k + (uint32_t)half, u, pf_pow2(254 - eu));
-          __builtin_amdgcn_raw_buffer_store_b8((char)eg, rs_e, (int)(at_e + (uint32_t)r * step_e), 0, 0);
-          __builtin_amdgcn_raw_buffer_store_b8((char)eu, rs_e, (int)(at_e + (uint32_t)r * step_e + (uint32_t)(half / PF_GATED_BLOCK)), 0, 0);
+          eg4 |= (uint32_t)eg << (8 * r);
+          eu4 |= (uint32_t)eu << (8 * r);
         }
+      }
+      if constexpr (KEEP == PF_KEEP_8BIT) {
+        __builtin_amdgcn_raw_buffer_store_b32((int)eg4, rs_e, (int)at_e, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b32((int)eu4, rs_e, (int)(at_e + (uint32_t)(half / PF_GATED_BLOCK * 4)), 0, 0);
       }
       at_y += 16 * step_y;
       at_k += 16 * step_k;

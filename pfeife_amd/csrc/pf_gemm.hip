@@ -839,10 +839,11 @@ int dispatch16(const pf_gemm_desc& d, hipStream_t st) {
 
 }  // namespace
 
-// The tile (PF_XT_*) that a product whose operands are stored alike would run on in one launch, 0: none
-int pf_gemm_best_tile(const pf_gemm_desc& d) {
+// The tile (PF_XT_*) that a product whose operands are stored alike would run on in one launch, 0: none; us: what it would take
+int pf_gemm_best_tile(const pf_gemm_desc& d, double* us) {
   double t = 0;
   const int v = choose_tile(d, d.M, 0, t);
+  if (us != nullptr) *us = t;
   return v < 0 ? 0 : x_tile_of(v);
 }
 

@@ -275,7 +275,7 @@ inline int x_epi_class(const pf_gemm_desc& d, int vec_ok, int bm) {
 }  // namespace
 
 // pf_gemm.hip
-int pf_gemm_best_tile(const pf_gemm_desc& d);
+int pf_gemm_best_tile(const pf_gemm_desc& d, double* us = nullptr);
 int64_t pf_gemm_strided_rows(const pf_gemm_desc& d);
 
 // pf_gemm_f32.hip: fp32 products straight from 16-byte-aligned operands

@@ -22,10 +22,11 @@ struct PfHeadProduct {
   const PfHeadColumn* col;   // [n_max]
   void* dz;                  // [rows][n_max] gradient of the piece's logits
   const void* ht;            // [dim][n_max] the tokens' hidden state, transposed
-  int64_t dim;               // columns of dw
-  void* dw;                  // [rows][dim], contiguous, in the operands' type
-  float* dh;                 // [n_max][depth], accumulated where `add`
-  int add;
+  int64_t dim;               // columns of dw, the width of its rows a multiple of 8
+  int64_t ldw_out;
+  void* dw;                  // [rows][ldw_out] in the operands' type, on a boundary of 16 bytes
+  float* dh;                 // [splits][n_max][depth], accumulated where `add`
+  int add, splits;           // the piece's rows in so many shares, a sum for each
   const float* unscale;      // both gradients are divided by this
 };
 
@@ -45,3 +46,5 @@ int pf_head_stats(int dtype, const PfHeadProduct& p, hipStream_t st);
 int pf_head_dz(int dtype, const PfHeadProduct& p, hipStream_t st);
 int pf_head_dh(int dtype, const PfHeadProduct& p, hipStream_t st);
 int pf_head_dw(int dtype, const PfHeadProduct& p, hipStream_t st);
+// in how many shares the hidden state's gradient is best summed over `rows` vocabulary rows
+int pf_head_splits(int dtype, int64_t n_max, int64_t depth, int64_t rows);

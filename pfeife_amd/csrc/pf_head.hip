@@ -17,6 +17,7 @@
 // that, which keeps probabilities down to 2^-38.
 // fp32: the same through pf_gemm, with a piece's logits in memory.
 #include "pf_head.h"
+#include "pf_rows.h"
 
 #include <math.h>
 
@@ -53,27 +54,35 @@ inline Kept kept_of(void* p, int64_t n_max) {
 }
 
 struct Sizes {
-  int64_t n, n_max, depth, piece;
-  bool copy_w;
+  int64_t n, n_max, depth, piece, dim8;
+  int splits;
+  bool copy_w, narrow;
 };
 
-// tokens in groups of 1024, each of which counts for itself what lies before it: one launch, no order of arrival in the result
-__global__ __launch_bounds__(1024) void head_index_kernel(const int64_t* labels, int64_t n, int64_t T, int shift, int64_t ignore, int64_t V,
-                                                          int64_t n_max, Kept k, float* out) {
+struct Labels {
+  const int64_t* labels;
+  int64_t n, T, V, ignore, n_max;
+  int shift;
+  __device__ __forceinline__ int64_t at(int64_t r) const { return r >= n || (shift && r % T == T - 1) ? ignore : labels[r + shift]; }
+  __device__ __forceinline__ int64_t out(int64_t r) const { return r / T * (T - shift) + r % T; }
+  __device__ __forceinline__ bool scored(int64_t r) const { return r < n && !(shift && r % T == T - 1); }
+  __device__ __forceinline__ int label(int64_t l) const { return l >= 0 && l < V ? (int)l : -2; }
+};
+
+// Which tokens take part: groups of 1024, each of which counts for itself what lies before it: one launch, no order of arrival in the
+// result
+__global__ __launch_bounds__(1024) void head_index_kernel(const Labels y, Kept k, float* out) {
   __shared__ float sm[16];
   __shared__ int before[17];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  auto label = [&](int64_t r) -> int64_t {
-    if (r >= n || (shift && r % T == T - 1)) return ignore;
-    return labels[r + shift];
-  };
   int ahead = 0;
-  for (int64_t r = tid; r < (int64_t)blockIdx.x * 1024; r += 1024) ahead += label(r) != ignore;
+#pragma unroll 4
+  for (int64_t r = tid; r < (int64_t)blockIdx.x * 1024; r += 1024) ahead += y.at(r) != y.ignore;
   // (at most 2^24 tokens: exact in fp32)
   const int base = (int)pf_block_sum<16>((float)ahead, sm);
   const int64_t r = (int64_t)blockIdx.x * 1024 + tid;
-  const int64_t l = label(r);
-  const bool in = l != ignore;
+  const int64_t l = y.at(r);
+  const bool in = l != y.ignore;
   const unsigned long long mask = __ballot(in);
   if (lane == 0) before[wave + 1] = __popcll(mask);
   __syncthreads();
@@ -83,46 +92,89 @@ __global__ __launch_bounds__(1024) void head_index_kernel(const int64_t* labels,
   }
   __syncthreads();
   const int c = before[wave] + __popcll(mask & ((1ull << lane) - 1));
-  if (r < n) k.inv[r] = in ? c : -1;
+  if (r < y.n) k.inv[r] = in ? c : -1;
   if (in) {
     k.rows[c] = (int)r;
-    k.lab[c] = l >= 0 && l < V ? (int)l : -2;
-  } else if (out != nullptr && r < n && !(shift && r % T == T - 1)) {
-    out[r / T * (T - shift) + r % T] = 0.f;
+    k.lab[c] = y.label(l);
+  } else if (out != nullptr && y.scored(r)) {
+    out[y.out(r)] = 0.f;
   }
   if (blockIdx.x == gridDim.x - 1) {
     const int total = before[16];
     if (tid == 0) *k.count = total;
-    for (int64_t i = total + tid; i < n_max; i += 1024) k.lab[i] = -1;
+    for (int64_t i = total + tid; i < y.n_max; i += 1024) k.lab[i] = -1;
   }
 }
 
-// The tokens that take part, one behind the other, zeros behind them up to a multiple of 64 (all: up to n_max) and in columns D .. depth - 1.
-// One wavefront to a row.  U: 16 bytes, or one element where something is not aligned.
+__device__ __forceinline__ int64_t rows_needed(int n, int64_t n_max, int all) { return all ? n_max : (n > 64 ? (n + 63) / 64 * 64 : 64); }
+
+struct Hidden {
+  const char* h;
+  int64_t T, sb, st, D, depth;      // in units of the copy
+  char* hc;
+  int64_t n_max;
+  int all;                          // rows of zeros up to n_max, not just to the next multiple of 64
+};
+// One token's row by one wavefront, or zeros.  U: 16 bytes, or one element where something is not aligned.
 template <typename U>
-__global__ __launch_bounds__(256) void head_gather_kernel(const char* h, int64_t T, int64_t sb, int64_t st, int64_t D, int64_t depth, const int* count,
-                                                          const int* rows, char* hc, int64_t n_max, int all) {
-  const int n = *count;
-  const int64_t padded = all ? n_max : (n > 64 ? (n + 63) / 64 * 64 : 64);
-  const int64_t c = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (c >= padded) return;
-  U* dst = (U*)hc + c * depth;
-  const U* src = nullptr;
-  if (c < n) {
-    const int64_t r = rows[c];
-    src = (const U*)h + (r / T) * sb + (r % T) * st;
-  }
+__device__ __forceinline__ void gather_row(const Hidden& x, int64_t c, int64_t r) {
+  U* dst = (U*)x.hc + c * x.depth;
+  const U* src = r >= 0 ? (const U*)x.h + (r / x.T) * x.sb + (r % x.T) * x.st : nullptr;
   const U zero = {};
-  for (int64_t i = threadIdx.x & 63; i < depth; i += 64) dst[i] = src != nullptr && i < D ? src[i] : zero;
+#pragma unroll 8
+  for (int64_t i = threadIdx.x & 63; i < x.depth; i += 64) dst[i] = src != nullptr && i < x.D ? src[i] : zero;
 }
 
-// a matrix with its rows' width raised, zeros in the new columns
+// The tokens that take part, one behind the other, zeros behind them and in columns D .. depth - 1
 template <typename U>
-__global__ __launch_bounds__(256) void head_widen_kernel(const U* src, int64_t ld, int64_t D, U* dst, int64_t depth, int64_t rows) {
-  const int64_t total = rows * depth;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / depth, c = i % depth;
-    dst[i] = c < D ? src[r * ld + c] : (U)0;
+__global__ __launch_bounds__(256) void head_gather_kernel(const Hidden x, const Kept k) {
+  const int n = *k.count;
+  const int64_t c = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (c < rows_needed(n, x.n_max, x.all)) gather_row<U>(x, c, c < n ? k.rows[c] : -1);
+}
+
+// Both in one launch for up to 4096 tokens, where every workgroup can count all of them: four tokens to a workgroup, and the rows of
+// zeros behind the last one dealt out too
+template <typename U>
+__global__ __launch_bounds__(256) void head_index_gather_kernel(const Labels y, const Hidden x, Kept k, float* out) {
+  __shared__ int sm[4], sa[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t r0 = (int64_t)blockIdx.x * 4;
+  int ahead = 0, total = 0;
+#pragma unroll 4
+  for (int64_t r = tid; r < y.n; r += 256) {
+    const int in = y.at(r) != y.ignore;
+    total += in;
+    ahead += r < r0 ? in : 0;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    ahead += __shfl_xor(ahead, o, 64);
+    total += __shfl_xor(total, o, 64);
+  }
+  if (lane == 0) { sm[wave] = total; sa[wave] = ahead; }
+  __syncthreads();
+  total = sm[0] + sm[1] + sm[2] + sm[3];
+  int c = sa[0] + sa[1] + sa[2] + sa[3];
+  const int64_t r = r0 + wave;
+  for (int64_t q = r0; q < r; ++q) c += y.at(q) != y.ignore;
+  const int64_t l = y.at(r);
+  const bool in = l != y.ignore;
+  if (in) gather_row<U>(x, c, r);
+  if (lane == 0 && r < y.n) {
+    k.inv[r] = in ? c : -1;
+    if (in) {
+      k.rows[c] = (int)r;
+      k.lab[c] = y.label(l);
+    } else if (out != nullptr && y.scored(r)) {
+      out[y.out(r)] = 0.f;
+    }
+  }
+  const int64_t zeros = rows_needed(total, x.n_max, x.all);
+  for (int64_t z = total + (int64_t)blockIdx.x * 4 + wave; z < zeros; z += (int64_t)gridDim.x * 4) gather_row<U>(x, z, -1);
+  if (blockIdx.x == 0) {
+    if (tid == 0) *k.count = total;
+    for (int64_t i = total + tid; i < y.n_max; i += 256) k.lab[i] = -1;
   }
 }
 
@@ -199,53 +251,115 @@ __device__ __forceinline__ void factors(const Upstream& u, int n, int64_t c, flo
   g = u.k.lab[c] < 0 ? NAN : (float)up;
   f = u.k.lab[c] < 0 ? NAN : (float)(up * (1.0 + 2.0 * u.z_loss * lse));
 }
-// The number that brings the largest factor to `most`
-__global__ __launch_bounds__(1024) void head_scale_kernel(const Upstream u, float most, float* scale) {
-  __shared__ float sm[16];
-  const int n = *u.k.count;
+// The number that brings the largest factor to `most`; nothing to scale by where all factors are zero, one is infinite, or the
+// quotient would be
+__device__ __forceinline__ float scale_of(float top, float most) { return top > 1e-30f && top < INFINITY ? most / top : 1.f; }
+__device__ __forceinline__ float largest_factor(const Upstream& u, int n, int first, int step) {
   float top = 0.f;
-  for (int c = threadIdx.x; c < n; c += 1024) {
+  for (int c = first; c < n; c += step) {
     float f, g;
     factors(u, n, c, f, g);
     top = fmaxf(top, fmaxf(fabsf(f), fabsf(g)));
   }
-  top = pf_block_max<16>(top, sm);
-  // (nothing to scale by where all factors are zero, one is infinite, or the quotient would be)
-  if (threadIdx.x == 0) *scale = top > 1e-30f && top < INFINITY ? most / top : 1.f;
+  return top;
 }
-__global__ __launch_bounds__(256) void head_factor_kernel(const Upstream u, const float* scale, PfHeadColumn* col, int64_t n_max) {
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c >= n_max) return;
-  const int n = *u.k.count;
-  PfHeadColumn o = {0.f, 0.f, 0.f, 0.f};     // (behind the last token: zeros times exp(0))
-  if (c < n) {
-    const float s = scale != nullptr ? *scale : 1.f;
-    o.top = u.k.top[c];
-    o.bias = u.k.bias[c];
-    factors(u, n, c, o.f, o.g);
-    o.f *= s;
-    o.g *= s;
+__global__ __launch_bounds__(1024) void head_scale_kernel(const Upstream u, float most, float* scale) {
+  __shared__ float sm[16];
+  const float top = pf_block_max<16>(largest_factor(u, *u.k.count, threadIdx.x, 1024), sm);
+  if (threadIdx.x == 0) *scale = scale_of(top, most);
+}
+
+// What the backward pass's products read, in one launch: each token's factors (the first `factor` workgroups), the gathered rows (the
+// next `rows`) and their transpose (the others, 64 x 64 elements each).
+struct Ready {
+  Upstream u;
+  Hidden x;
+  PfHeadColumn* col;
+  float* scale;            // null: none
+  float most;
+  int known;               // the scale is there already
+  int factor, rows, tiles_n;
+  const char* h;           // as elements, for the transpose
+  int64_t sb, st, D, dim8;
+  uint16_t* ht;
+};
+template <typename U>
+__global__ __launch_bounds__(256) void head_ready_kernel(const Ready q) {
+  __shared__ uint16_t tile[64][66];
+  __shared__ float sm[4];
+  const Kept& k = q.u.k;
+  const int n = *k.count, t = threadIdx.x;
+  if ((int)blockIdx.x < q.factor) {
+    float s = 1.f;
+    if (q.scale != nullptr) {
+      s = q.known ? *q.scale : scale_of(pf_block_max<4>(largest_factor(q.u, n, t, 256), sm), q.most);
+      if (!q.known && blockIdx.x == 0 && t == 0) *q.scale = s;
+    }
+    const int64_t c = (int64_t)blockIdx.x * 256 + t;
+    if (c >= q.x.n_max) return;
+    PfHeadColumn o = {0.f, 0.f, 0.f, 0.f};     // (behind the last token: zeros times exp(0))
+    if (c < n) {
+      o.top = k.top[c];
+      o.bias = k.bias[c];
+      factors(q.u, n, c, o.f, o.g);
+      o.f *= s;
+      o.g *= s;
+    }
+    q.col[c] = o;
+    return;
   }
-  col[c] = o;
+  const int64_t padded = rows_needed(n, q.x.n_max, q.x.all);
+  const int block = (int)blockIdx.x - q.factor;
+  if (block < q.rows) {
+    const int64_t c = (int64_t)block * 4 + (t >> 6);
+    if (c < padded) gather_row<U>(q.x, c, c < n ? k.rows[c] : -1);
+    return;
+  }
+  const int64_t c0 = (int64_t)((block - q.rows) / q.tiles_n) * 64, d0 = (int64_t)((block - q.rows) % q.tiles_n) * 64;
+  if (c0 >= padded) return;
+  const int at = t & 63;
+#pragma unroll 4
+  for (int i = t >> 6; i < 64; i += 4) {
+    const int64_t c = c0 + i, d = d0 + at;
+    uint16_t v = 0;
+    if (c < n && d < q.D) {
+      const int64_t r = k.rows[c];
+      v = ((const uint16_t*)q.h)[(r / q.x.T) * q.sb + (r % q.x.T) * q.st + d];
+    }
+    tile[i][at] = v;
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int i = t >> 6; i < 64; i += 4) {
+    const int64_t d = d0 + i;
+    if (d < q.dim8) q.ht[d * q.x.n_max + c0 + at] = tile[at][i];
+  }
 }
 
 // The gradient of every row of the hidden state: a token's sum rounded once (times a loss scale first), zeros where it took no part
 template <int W>
-__global__ __launch_bounds__(256) void head_spread_kernel(const float* acc, int64_t ld, const int* inv, int64_t n, int64_t D, const float* times, void* dh, int dt) {
+__global__ __launch_bounds__(256) void head_spread_kernel(const float* acc, int64_t ld, int splits, int64_t n_max, const int* inv, int64_t n, int64_t D, const float* times, void* dh, int dt) {
   const float by = times != nullptr ? *times : 1.f;
-  for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < n; r += (int64_t)gridDim.x * 4) {
+  const int64_t per = (D + 64 * W - 1) / (64 * W), total = n * per;      // (a wavefront to 64 W columns of a row)
+  for (int64_t q = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); q < total; q += (int64_t)gridDim.x * 4) {
+    const int64_t r = q / per, i = q % per * 64 * W + (threadIdx.x & 63) * W;
+    if (i >= D) continue;
     const int c = inv[r];
-    for (int64_t i = (int64_t)(threadIdx.x & 63) * W; i < D; i += 64 * W) {
-      float v[W];
+    float v[W];
 #pragma unroll
-      for (int k = 0; k < W; ++k) v[k] = 0.f;
-      if (c >= 0) {
-        ld_vec<W>(acc, c * ld + i, PF_F32, v);
+    for (int k = 0; k < W; ++k) v[k] = 0.f;
+    if (c >= 0) {
+#pragma unroll 4
+      for (int p = 0; p < splits; ++p) {
+        float w[W];
+        ld_vec<W>(acc, (p * n_max + c) * ld + i, PF_F32, w);
 #pragma unroll
-        for (int k = 0; k < W; ++k) v[k] *= by;
+        for (int k = 0; k < W; ++k) v[k] += w[k];
       }
-      st_vec<W>(dh, r * D + i, dt, v);
+#pragma unroll
+      for (int k = 0; k < W; ++k) v[k] *= by;
     }
+    st_vec<W>(dh, r * D + i, dt, v);
   }
 }
 
@@ -308,10 +422,13 @@ bool sizes_of(const Call& c, Sizes& s) {
   s.n = c.B * c.T;
   s.n_max = round_up(s.n > 0 ? s.n : 1, 64);
   s.depth = c.dtype == PF_F32 ? round_up(c.D, 4) : (c.D < 64 ? 64 : round_up(c.D, 8));
-  s.copy_w = c.dtype != PF_F32 && (s.depth != c.D || !pf_aligned(c.w, 16));
+  s.copy_w = s.depth != c.D || !pf_aligned(c.w, 16);
+  s.dim8 = round_up(c.D, 8);
+  s.narrow = es == 2 && s.dim8 != c.D;
   s.piece = piece_rows(s.n_max, c.V, es);
   if (es == 2 && s.piece > reach_rows(s.depth)) s.piece = reach_rows(s.depth);
-  return s.n < (1ll << 24) && c.V < (1ll << 31) && s.n_max * s.depth * 4 < (1ll << 31) - 64 && s.piece * s.n_max * es < (1ll << 31) - 64 &&
+  s.splits = pf_head_splits(c.dtype, s.n_max, s.depth, s.piece);
+  return s.n < (1ll << 24) && c.V < (1ll << 31) && s.n_max * s.depth * 4 * s.splits < (1ll << 31) - 64 && s.piece * s.n_max * es < (1ll << 31) - 64 &&
          s.depth < (1ll << 19);
 }
 
@@ -327,23 +444,24 @@ struct Carve {
 };
 struct Work {
   char* hc; char* wide; PfHeadPart* part; float* zl; double* terms;             // forward (hc and wide: backward too)
-  char* dz; char* ht; float* acc; PfHeadColumn* col; float* scale;               // backward (dz: fp32's logits in both)
+  char* dz; char* ht; char* dw; float* acc; PfHeadColumn* col; float* scale;     // backward (dz: fp32's logits in both)
 };
 Work carve(Carve& a, const Call& c, const Sizes& s, bool back) {
   const int64_t es = c.dtype == PF_F32 ? 4 : 2;
   Work w = {};
   w.hc = (char*)a.take(s.n_max * s.depth * es);
-  if (s.copy_w) w.wide = (char*)a.take(c.V * s.depth * 2);
+  if (s.copy_w) w.wide = (char*)a.take(c.V * s.depth * es);
   if (back || es == 4) w.dz = (char*)a.take(s.piece * s.n_max * es);
   if (!back) {
     w.part = (PfHeadPart*)a.take((es == 4 ? (c.V + 127) / 128 : pf_head_blocks(c.V, s.n_max, s.depth)) * s.n_max * 8);
     w.zl = (float*)a.take(s.n_max * 4);
     w.terms = (double*)a.take(s.n_max * 8);
   } else {
-    if (es == 2) w.ht = (char*)a.take(c.D * s.n_max * 2);
+    if (es == 2) w.ht = (char*)a.take(s.dim8 * s.n_max * 2);
+    if (s.narrow) w.dw = (char*)a.take(s.piece * s.depth * 2);
     w.col = (PfHeadColumn*)a.take(s.n_max * 16);
     w.scale = (float*)a.take(4);
-    w.acc = (float*)a.take(s.n_max * s.depth * 4);
+    w.acc = (float*)a.take(s.n_max * s.depth * 4 * s.splits);
   }
   return w;
 }
@@ -359,26 +477,31 @@ int check_call(const Call& c, const Sizes& s, bool ok) {
   return PF_OK;
 }
 
-void gather(const Call& c, const Sizes& s, const Work& w, const Kept& k, hipStream_t st) {
-  const int64_t es = c.dtype == PF_F32 ? 4 : 2, per = 16 / es;
-  const int all = es == 4;
-  const dim3 grid((unsigned)((s.n_max + 3) / 4));
-  if (pf_aligned(c.h, 16) && c.D % per == 0 && s.depth % per == 0 && c.sb % per == 0 && c.st % per == 0)
-    hipLaunchKernelGGL(head_gather_kernel<uint4>, grid, dim3(256), 0, st, (const char*)c.h, c.T, c.sb / per, c.st / per, c.D / per, s.depth / per, k.count, k.rows, w.hc,
-                       s.n_max, all);
-  else if (es == 4)
-    hipLaunchKernelGGL(head_gather_kernel<uint32_t>, grid, dim3(256), 0, st, (const char*)c.h, c.T, c.sb, c.st, c.D, s.depth, k.count, k.rows, w.hc, s.n_max, all);
-  else
-    hipLaunchKernelGGL(head_gather_kernel<uint16_t>, grid, dim3(256), 0, st, (const char*)c.h, c.T, c.sb, c.st, c.D, s.depth, k.count, k.rows, w.hc, s.n_max, all);
+// the hidden state in units of 16 bytes or of one element
+int unit_of(const Call& c, const Sizes& s) {
+  const int es = c.dtype == PF_F32 ? 4 : 2, per = 16 / es;
+  return pf_aligned(c.h, 16) && c.D % per == 0 && s.depth % per == 0 && c.sb % per == 0 && c.st % per == 0 ? 16 : es;
 }
+Hidden hidden_of(const Call& c, const Sizes& s, const Work& w) {
+  const int64_t per = unit_of(c, s) / (c.dtype == PF_F32 ? 4 : 2);
+  return {(const char*)c.h, c.T > 0 ? c.T : 1, c.sb / per, c.st / per, c.D / per, s.depth / per, w.hc, s.n_max, c.dtype == PF_F32};
+}
+#define PF_BY_UNIT(KERNEL, ...)                                                          \
+  do {                                                                                   \
+    switch (unit_of(c, s)) {                                                             \
+      case 16: hipLaunchKernelGGL(KERNEL<uint4>, __VA_ARGS__); break;                    \
+      case 4: hipLaunchKernelGGL(KERNEL<uint32_t>, __VA_ARGS__); break;                  \
+      default: hipLaunchKernelGGL(KERNEL<uint16_t>, __VA_ARGS__); break;                 \
+    }                                                                                    \
+  } while (0)
+
 void widen(const Call& c, const Sizes& s, const Work& w, hipStream_t st) {
-  if (s.copy_w)
-    hipLaunchKernelGGL(head_widen_kernel<uint16_t>, dim3(4096), dim3(256), 0, st, (const uint16_t*)c.w, c.D, c.D, (uint16_t*)w.wide, s.depth, c.V);
+  if (s.copy_w) pf_rows_widen(c.w, c.V, c.D, w.wide, c.V, s.depth, 1, c.dtype == PF_F32 ? 4 : 2, st);
 }
 
-// a product over fp32 operands
-int product32(int a_trans, int b_trans, int64_t M, int64_t N, int64_t K, const void* A, int64_t lda, const void* B, int64_t ldb, void* C, int64_t ldc, int beta,
-              hipStream_t st) {
+// a product over fp32 operands; batch: shares of the depth, `share` of it each, with results of their own
+int product32(int a_trans, int b_trans, int64_t M, int64_t N, int64_t K, const float* A, int64_t lda, const float* B, int64_t ldb, float* C, int64_t ldc, int beta,
+              hipStream_t st, int splits = 1, int64_t c_stride = 0) {
   pf_gemm_desc d = {};
   d.in_dtype = d.c_dtype = PF_F32;
   d.a_trans = a_trans; d.b_trans = b_trans;
@@ -387,6 +510,20 @@ int product32(int a_trans, int b_trans, int64_t M, int64_t N, int64_t K, const v
   d.batch1 = d.batch2 = 1;
   d.alpha = 1.f;
   d.beta = beta;
+  const int64_t share = splits > 1 ? K / splits / 64 * 64 : 0;
+  if (share == 0) return pf_gemm(&d, st);
+  d.K = share;
+  d.batch2 = splits;
+  d.a_stride2 = share * lda;
+  d.b_stride2 = share * ldb;
+  d.c_stride2 = c_stride;
+  const int rc = pf_gemm(&d, st);
+  if (rc != PF_OK || share * splits == K) return rc;
+  d.K = K - share * splits;
+  d.batch2 = 1;
+  d.A = A + share * splits * lda;
+  d.B = B + share * splits * ldb;
+  d.beta = 1;
   return pf_gemm(&d, st);
 }
 
@@ -423,16 +560,22 @@ extern "C" int pf_linear_ce_fwd(const void* hidden, int dtype, int64_t B, int64_
   Carve a = {(char*)workspace};
   const Work w = carve(a, c, s, false);
   float* out = reduction == 0 ? loss : nullptr;
-  hipLaunchKernelGGL(head_index_kernel, dim3((unsigned)((s.n + 1023) / 1024 > 0 ? (s.n + 1023) / 1024 : 1)), dim3(1024), 0, st, labels, s.n, T > 0 ? T : 1, shift,
-                     ignore_index, V, s.n_max, k, out);
-  gather(c, s, w, k, st);
+  const Labels y = {labels, s.n, T > 0 ? T : 1, V, ignore_index, s.n_max, shift};
+  const Hidden x = hidden_of(c, s, w);
+  if (s.n <= 4096) {
+    PF_BY_UNIT(head_index_gather_kernel, dim3((unsigned)(s.n_max / 4)), dim3(256), 0, st, y, x, k, out);
+  } else {
+    hipLaunchKernelGGL(head_index_kernel, dim3((unsigned)((s.n + 1023) / 1024)), dim3(1024), 0, st, y, k, out);
+    PF_BY_UNIT(head_gather_kernel, dim3((unsigned)(s.n_max / 4)), dim3(256), 0, st, x, k);
+  }
   widen(c, s, w, st);
   PF_CHECK_LAUNCH(c.who);
+  const char* wide = s.copy_w ? w.wide : (const char*)weight;
   int64_t blocks = 0;
   if (dtype == PF_F32) {
     for (int64_t v0 = 0; v0 < V; v0 += s.piece) {
       const int64_t rows = V - v0 < s.piece ? V - v0 : s.piece;
-      rc = product32(0, 0, rows, s.n_max, D, (const float*)weight + v0 * D, D, w.hc, s.depth, w.dz, s.n_max, 0, st);
+      rc = product32(0, 0, rows, s.n_max, D, (const float*)wide + v0 * s.depth, s.depth, (const float*)w.hc, s.depth, (float*)w.dz, s.n_max, 0, st);
       if (rc != PF_OK) return rc;
       hipLaunchKernelGGL(head_stats32_kernel, dim3((unsigned)((s.n_max + 255) / 256), (unsigned)((rows + 127) / 128)), dim3(256), 0, st, (const float*)w.dz, rows,
                          s.n_max, v0, k.lab, k.count, w.part + blocks * s.n_max, w.zl);
@@ -447,7 +590,7 @@ extern "C" int pf_linear_ce_fwd(const void* hidden, int dtype, int64_t B, int64_
     for (int64_t v0 = 0; v0 < V; v0 += reach) {
       p.v0 = v0;
       p.rows = V - v0 < reach ? V - v0 : reach;
-      p.w = (s.copy_w ? w.wide : (const char*)weight) + v0 * s.depth * 2;
+      p.w = wide + v0 * s.depth * 2;
       p.part = w.part + blocks * s.n_max;
       rc = pf_head_stats(dtype, p, st);
       if (rc != PF_OK) return rc;
@@ -469,47 +612,64 @@ extern "C" int pf_linear_ce_bwd(const void* hidden, int dtype, int64_t B, int64_
   int rc = check_call(c, s, B < 0 || T < 0 || D <= 0 || V <= 0 || sizes_of(c, s));
   if (rc != PF_OK) return rc;
   PF_REQUIRE(kept && workspace && weight && grad && (s.n == 0 || hidden), "%s: null pointer", c.who);
+  PF_REQUIRE(dtype == PF_F32 || pf_aligned(dweight, 16), "%s: dweight lies on a boundary of 16 bytes", c.who);
   hipStream_t st = (hipStream_t)stream;
   const Kept k = kept_of((void*)kept, s.n_max);
   Carve a = {(char*)workspace};
   const Work w = carve(a, c, s, true);
   const Upstream u = {grad, g_sb, g_st, T > 0 ? T : 1, mean, z_loss, k};
-  const bool narrow = dtype != PF_F32;
-  if (narrow) hipLaunchKernelGGL(head_scale_kernel, dim3(1), dim3(1024), 0, st, u, dtype == PF_F16 ? 8192.f : 1.f, w.scale);
-  hipLaunchKernelGGL(head_factor_kernel, dim3((unsigned)((s.n_max + 255) / 256)), dim3(256), 0, st, u, (const float*)(narrow ? w.scale : nullptr), w.col, s.n_max);
-  gather(c, s, w, k, st);
+  const bool half = dtype != PF_F32;
+  Ready q = {};
+  q.u = u;
+  q.x = hidden_of(c, s, w);
+  q.col = w.col;
+  q.scale = half ? w.scale : nullptr;
+  q.most = dtype == PF_F16 ? 8192.f : 1.f;
+  if (half && s.n > 1024) {      // (fewer: every workgroup finds the largest factor for itself)
+    hipLaunchKernelGGL(head_scale_kernel, dim3(1), dim3(1024), 0, st, u, q.most, w.scale);
+    q.known = 1;
+  }
+  q.factor = (int)((s.n_max + 255) / 256);
+  q.rows = (int)(s.n_max / 4);
+  q.h = (const char*)c.h; q.sb = sb; q.st = st_; q.D = D; q.dim8 = s.dim8;
+  q.ht = (uint16_t*)w.ht;
+  q.tiles_n = (int)((s.dim8 + 63) / 64);
+  const int tiles = half && dweight ? (int)(s.n_max / 64) * q.tiles_n : 0;
+  PF_BY_UNIT(head_ready_kernel, dim3((unsigned)(q.factor + q.rows + tiles)), dim3(256), 0, st, q);
   widen(c, s, w, st);
   PF_CHECK_LAUNCH(c.who);
-  if (dtype != PF_F32 && dweight) {
-    rc = pf_transpose_cast(w.hc, dtype, s.depth, w.ht, dtype, s.n_max, s.n_max, D, stream);
-    if (rc != PF_OK) return rc;
-  }
+  const char* wide = s.copy_w ? w.wide : (const char*)weight;
   for (int64_t v0 = 0; v0 < V; v0 += s.piece) {
     const int64_t rows = V - v0 < s.piece ? V - v0 : s.piece;
-    if (dtype == PF_F32) {
-      const float* wp = (const float*)weight + v0 * D;
-      rc = product32(0, 0, rows, s.n_max, D, wp, D, w.hc, s.depth, w.dz, s.n_max, 0, st);
+    if (!half) {
+      const float* wp = (const float*)wide + v0 * s.depth;
+      float* dz = (float*)w.dz;
+      rc = product32(0, 0, rows, s.n_max, D, wp, s.depth, (const float*)w.hc, s.depth, dz, s.n_max, 0, st);
       if (rc != PF_OK) return rc;
-      hipLaunchKernelGGL(head_dz32_kernel, dim3((unsigned)((s.n_max + 255) / 256), (unsigned)((rows + 127) / 128)), dim3(256), 0, st, (float*)w.dz, rows, s.n_max, v0,
-                         k.lab, w.col);
-      if (dhidden) rc = product32(1, 1, s.n_max, D, rows, w.dz, s.n_max, wp, D, w.acc, s.depth, v0 > 0, st);
-      if (rc == PF_OK && dweight) rc = product32(0, 1, rows, D, s.n_max, w.dz, s.n_max, w.hc, s.depth, (float*)dweight + v0 * D, D, 0, st);
+      hipLaunchKernelGGL(head_dz32_kernel, dim3((unsigned)((s.n_max + 255) / 256), (unsigned)((rows + 127) / 128)), dim3(256), 0, st, dz, rows, s.n_max, v0, k.lab,
+                         w.col);
+      if (dhidden) rc = product32(1, 1, s.n_max, D, rows, dz, s.n_max, wp, s.depth, w.acc, s.depth, v0 > 0, st, s.splits, s.n_max * s.depth);
+      if (rc == PF_OK && dweight) rc = product32(0, 1, rows, D, s.n_max, dz, s.n_max, (const float*)w.hc, s.depth, (float*)dweight + v0 * D, D, 0, st);
       if (rc != PF_OK) return rc;
       continue;
     }
     PfHeadProduct p = {};
-    p.w = (s.copy_w ? w.wide : (const char*)weight) + v0 * s.depth * 2;
+    p.w = wide + v0 * s.depth * 2;
     p.ldw = s.depth; p.v0 = v0; p.rows = rows; p.depth = s.depth;
     p.hc = w.hc; p.ldh = s.depth; p.n_max = s.n_max;
-    p.count = k.count; p.lab = k.lab; p.col = w.col; p.dz = w.dz; p.ht = w.ht; p.dim = D;
-    p.dw = dweight ? (char*)dweight + v0 * D * 2 : nullptr;
-    p.dh = w.acc; p.add = v0 > 0;
+    p.count = k.count; p.lab = k.lab; p.col = w.col; p.dz = w.dz; p.ht = w.ht; p.dim = s.dim8;
+    char* dw = (char*)dweight + v0 * D * 2;
+    p.dw = s.narrow ? w.dw : dw;
+    p.ldw_out = s.narrow ? s.depth : D;
+    p.dh = w.acc; p.add = v0 > 0; p.splits = s.splits;
     p.unscale = w.scale;
     rc = pf_head_dz(dtype, p, st);
     if (rc == PF_OK && dhidden) rc = pf_head_dh(dtype, p, st);
     if (rc == PF_OK && dweight) rc = pf_head_dw(dtype, p, st);
     if (rc != PF_OK) return rc;
+    if (dweight && s.narrow) pf_rows_narrow(w.dw, s.depth, dw, rows, D, st);
   }
+  PF_CHECK_LAUNCH(c.who);
   if (!dhidden) return PF_OK;
   return pf_linear_ce_hidden_grad(weight, dtype, s.n, D, V, kept, nullptr, dhidden, workspace, stream);
 }
@@ -526,11 +686,13 @@ extern "C" int pf_linear_ce_hidden_grad(const void* weight, int dtype, int64_t t
   const Kept k = kept_of((void*)kept, s.n_max);
   Carve a = {(char*)workspace};
   const Work w = carve(a, c, s, true);
-  const dim3 grid((unsigned)((s.n + 3) / 4 < 8192 ? (s.n + 3) / 4 : 8192));
+  const int64_t lanes = D % 8 == 0 && pf_aligned(dhidden, 16) ? 512 : 64, units = (s.n * ((D + lanes - 1) / lanes) + 3) / 4;
+  const dim3 grid((unsigned)(units < 16384 ? units : 16384));
+  const int dhidden_splits = s.piece / s.splits >= 64 ? s.splits : 1;
   if (D % 8 == 0 && pf_aligned(dhidden, 16))
-    hipLaunchKernelGGL(head_spread_kernel<8>, grid, dim3(256), 0, st, w.acc, s.depth, k.inv, s.n, D, times, dhidden, dtype);
+    hipLaunchKernelGGL(head_spread_kernel<8>, grid, dim3(256), 0, st, w.acc, s.depth, dhidden_splits, s.n_max, k.inv, s.n, D, times, dhidden, dtype);
   else
-    hipLaunchKernelGGL(head_spread_kernel<1>, grid, dim3(256), 0, st, w.acc, s.depth, k.inv, s.n, D, times, dhidden, dtype);
+    hipLaunchKernelGGL(head_spread_kernel<1>, grid, dim3(256), 0, st, w.acc, s.depth, dhidden_splits, s.n_max, k.inv, s.n, D, times, dhidden, dtype);
   PF_CHECK_LAUNCH(c.who);
   return PF_OK;
 }

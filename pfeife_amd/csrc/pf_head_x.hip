@@ -198,12 +198,12 @@ template <int XT> constexpr size_t tile_lds() {
   return (size_t)T::ST * (T::BM + T::BN) * T::BK * 2 + (T::ST == 2 ? (size_t)T::BN * T::BK * 2 : 0);
 }
 template <int XT, class K, class... A>
-int launch(K kern, int64_t M, int64_t N, hipStream_t st, const A&... args) {
+int launch(K kern, int64_t M, int64_t N, int batch, hipStream_t st, const A&... args) {
   using T = XTile<XT>;
   const int rc = pf_allow_lds((const void*)kern, tile_lds<XT>(), "pf_linear_ce");
   if (rc != PF_OK) return rc;
   const int64_t tiles = ((M + T::BM - 1) / T::BM) * ((N + T::BN - 1) / T::BN);
-  hipLaunchKernelGGL(kern, dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(64 * T::WGM * T::WGN), tile_lds<XT>(), st, args...);
+  hipLaunchKernelGGL(kern, dim3((unsigned)((tiles + 7) / 8 * 8), (unsigned)batch), dim3(64 * T::WGM * T::WGN), tile_lds<XT>(), st, args...);
   PF_CHECK_LAUNCH("pf_linear_ce");
   return PF_OK;
 }
@@ -226,15 +226,23 @@ template <class Tail> int logits_launch(const PfHeadProduct& p, const Tail& tail
   static_assert(XTile<PF_XT_64x64>::BM / XTile<PF_XT_64x64>::WGM == 32 && XTile<PF_XT_256x128w8>::BM / XTile<PF_XT_256x128w8>::WGM == 64 &&
                 XTile<PF_XT_256x256w4>::BM / XTile<PF_XT_256x256w4>::WGM == 128, "pf_head_blocks");
   switch (pf_head_tile(p.n_max, p.depth)) {
-    case PF_HEAD_64x64: return launch<PF_XT_64x64>(head_logits_kernel<PF_XT_64x64, true, Tail>, p.rows, p.n_max, st, d, p.count, tail);
-    case PF_HEAD_256x128: return launch<PF_XT_256x128w8>(head_logits_kernel<PF_XT_256x128w8, true, Tail>, p.rows, p.n_max, st, d, p.count, tail);
-    default: return launch<PF_XT_256x256w4>(head_logits_kernel<PF_XT_256x256w4, false, Tail>, p.rows, p.n_max, st, d, p.count, tail);
+    case PF_HEAD_64x64: return launch<PF_XT_64x64>(head_logits_kernel<PF_XT_64x64, true, Tail>, p.rows, p.n_max, 1, st, d, p.count, tail);
+    case PF_HEAD_256x128: return launch<PF_XT_256x128w8>(head_logits_kernel<PF_XT_256x128w8, true, Tail>, p.rows, p.n_max, 1, st, d, p.count, tail);
+    default: return launch<PF_XT_256x256w4>(head_logits_kernel<PF_XT_256x256w4, false, Tail>, p.rows, p.n_max, 1, st, d, p.count, tail);
   }
 }
 
 template <int XT> int hidden_launch(const pf_gemm_desc& d, const PfHeadProduct& p, hipStream_t st) {
-  return p.add ? launch<XT>(head_hidden_grad_kernel<XT, EC_ACC32>, d.M, d.N, st, d, p.count)
-               : launch<XT>(head_hidden_grad_kernel<XT, EC_STORE32>, d.M, d.N, st, d, p.count);
+  return d.beta ? launch<XT>(head_hidden_grad_kernel<XT, EC_ACC32>, d.M, d.N, (int)d.batch2, st, d, p.count)
+                : launch<XT>(head_hidden_grad_kernel<XT, EC_STORE32>, d.M, d.N, (int)d.batch2, st, d, p.count);
+}
+int hidden_grad(const pf_gemm_desc& d, const PfHeadProduct& p, hipStream_t st) {
+  switch (pf_gemm_best_tile(d)) {
+    case PF_XT_64x64: return hidden_launch<PF_XT_64x64>(d, p, st);
+    case PF_XT_128x128w8: return hidden_launch<PF_XT_128x128w8>(d, p, st);
+    case PF_XT_256x128w8: return hidden_launch<PF_XT_256x128w8>(d, p, st);
+    default: return hidden_launch<PF_XT_256x256w4>(d, p, st);
+  }
 }
 
 }  // namespace
@@ -258,19 +266,29 @@ int PF_H_CAT(pf_head_dh_, PF_X_DT)(const PfHeadProduct& p, hipStream_t st) {
   d.A = p.dz; d.lda = p.n_max; d.B = p.w; d.ldb = p.ldw; d.C = p.dh; d.ldc = p.depth;
   d.beta = p.add;
   d.unscale_by = p.unscale;
-  switch (pf_gemm_best_tile(d)) {
-    case PF_XT_64x64: return hidden_launch<PF_XT_64x64>(d, p, st);
-    case PF_XT_128x128w8: return hidden_launch<PF_XT_128x128w8>(d, p, st);
-    case PF_XT_256x128w8: return hidden_launch<PF_XT_256x128w8>(d, p, st);
-    default: return hidden_launch<PF_XT_256x256w4>(d, p, st);
-  }
+  const int64_t share = p.splits > 1 ? p.rows / p.splits / 64 * 64 : 0;
+  if (share == 0) return hidden_grad(d, p, st);
+  d.K = share;
+  d.batch2 = p.splits;
+  d.a_stride2 = share * d.lda;
+  d.b_stride2 = share * d.ldb;
+  d.c_stride2 = p.n_max * p.depth;
+  int rc = hidden_grad(d, p, st);
+  const int64_t done = share * p.splits;
+  if (rc != PF_OK || done == p.rows) return rc;
+  d.K = p.rows - done;      // what does not divide goes to the first share
+  d.batch2 = 1;
+  d.A = (const uint16_t*)p.dz + done * d.lda;
+  d.B = (const uint16_t*)p.w + done * d.ldb;
+  d.beta = 1;
+  return hidden_grad(d, p, st);
 }
 
 int PF_H_CAT(pf_head_dw_, PF_X_DT)(const PfHeadProduct& p, hipStream_t st) {
   pf_gemm_desc d = plain_desc();
   d.c_dtype = PF_X_DT;
   d.M = p.rows; d.N = p.dim; d.K = p.n_max;
-  d.A = p.dz; d.lda = p.n_max; d.B = p.ht; d.ldb = p.n_max; d.C = p.dw; d.ldc = p.dim;
+  d.A = p.dz; d.lda = p.n_max; d.B = p.ht; d.ldb = p.n_max; d.C = p.dw; d.ldc = p.ldw_out;
   d.unscale_by = p.unscale;
   using T = XTile<PF_XT_256x256w4>;
   GemmGrid g;
@@ -278,7 +296,29 @@ int PF_H_CAT(pf_head_dw_, PF_X_DT)(const PfHeadProduct& p, hipStream_t st) {
   g.tiles_n = (int)((d.N + T::BN - 1) / T::BN);
   g.per_xcd = (int)(((int64_t)g.tiles_m * g.tiles_n + 7) / 8);
   g.vec_epi = epi_vec_ok(d);
-  if (x_epi_class(d, g.vec_epi, T::BM) == EC_STORE16)
-    return launch<PF_XT_256x256w4>(head_weight_grad_kernel<PF_XT_256x256w4, EC_STORE16>, d.M, d.N, st, d, g, p.count);
-  return launch<PF_XT_256x256w4>(head_weight_grad_kernel<PF_XT_256x256w4, EC_GENERIC>, d.M, d.N, st, d, g, p.count);
+  return launch<PF_XT_256x256w4>(head_weight_grad_kernel<PF_XT_256x256w4, EC_STORE16>, d.M, d.N, 1, st, d, g, p.count);
 }
+
+#if PF_X_DT == 1
+int pf_head_splits(int dtype, int64_t n_max, int64_t depth, int64_t rows) {
+  int best = 1;
+  double best_t = 0;
+  for (int s = 1; s <= 16 && (s == 1 || rows / s >= 256); s *= 2) {
+    double t = 0;
+    if (dtype == PF_F32) {
+      const int64_t tiles = ((n_max + 63) / 64) * ((depth + 63) / 64) * s;      // (17 ns a unit of depth and 64x64 tile)
+      t = (double)((tiles + 255) / 256) * 0.0171 * (double)(rows / s);
+    } else {
+      pf_gemm_desc d = plain_desc();
+      d.c_dtype = PF_F32;
+      d.a_trans = d.b_trans = 1;
+      d.M = n_max; d.N = depth; d.K = rows / s;
+      d.batch2 = s;
+      pf_gemm_best_tile(d, &t);
+    }
+    t += (double)(n_max * depth) * s * 8.0 / 5.0e6;      // the shares' way through memory, written and read at 5 TB/s
+    if (s == 1 || t < best_t) { best = s; best_t = t; }
+  }
+  return best;
+}
+#endif

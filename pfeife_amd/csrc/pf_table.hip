@@ -5,20 +5,23 @@
 // Text holds few tokens very often and most of the table not at all, so the gradient's work is dealt out by the tokens and not by
 // the table's rows: the places are sorted by token (a stable radix sort of two digits, 2^18 rows; three beyond), a
 // group of lanes adds up CHUNK neighbours of the sorted list, and a token whose run crosses chunks has its partial sums added
-// in order by a last kernel.  Which lane adds what follows from the ids alone: the same ids give the same bits.  Rows that no token
-// names are found by searching the sorted list and are zeroed by other workgroups of the same launch, so every byte of the
-// gradient is written once.
+// in order by a last kernel.  Which lane adds what follows from the ids alone: the same ids give the same bits.
 #include "pf_common.h"
 
 namespace {
 
 constexpr int BINS = 512;        // of one digit
-constexpr int SMALL = 4096;      // ids that one workgroup sorts by itself
+constexpr int FEW_IDS = 256;     // ids that every workgroup looks through by itself
+constexpr int PLACE_BITS = 11;
+constexpr int BLOCK = 1 << PLACE_BITS;      // ids that are sorted among themselves first, key and place in one word
+constexpr int MANY = 65536;                 // ids up to which that is faster than the radix sort
 
 __device__ __forceinline__ int key_of(int64_t id, int64_t vocab, int64_t padding) { return id >= 0 && id < vocab && id != padding ? (int)id : (int)vocab; }
 
-// One digit's stable ranks: `wc[digit]` is where the wavefront's next key of the digit goes; -> where this lane's goes
-__device__ __forceinline__ int rank_of(int digit, bool active, int bits, int* wc) {
+// One digit's stable ranks among the keys of a wavefront, which counts in `wc` (its own, zero before its first key): how many of the
+// digit came before this lane's.  No atomics: a token that fills half of the list would queue all lanes at one counter.
+template <typename C>
+__device__ __forceinline__ int rank_of(int digit, bool active, int bits, C* wc) {
   const int lane = threadIdx.x & 63;
   unsigned long long same = __ballot(active);
   for (int b = 0; b < bits; ++b) {
@@ -30,14 +33,16 @@ __device__ __forceinline__ int rank_of(int digit, bool active, int bits, int* wc
   if (active) at = wc[digit];
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
-  if (active && (same & ((1ull << lane) - 1)) == 0) wc[digit] = at + __popcll(same);
+  const int before = __popcll(same & ((1ull << lane) - 1));
+  if (active && before == 0) wc[digit] = (C)(at + __popcll(same));
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
-  return at + __popcll(same & ((1ull << lane) - 1));
+  return at + before;
 }
 
-// sums of BINS values before each, by the first BINS threads of a workgroup; every thread of it calls
-__device__ __forceinline__ int scan_bins(int v, int* sm) {
+// the sum of the values of the threads before this one, in workgroups of WAVES wavefronts
+template <int WAVES>
+__device__ __forceinline__ int sum_before(int v, int* sm) {
   const int t = threadIdx.x, lane = t & 63;
   int x = v;
 #pragma unroll
@@ -45,88 +50,128 @@ __device__ __forceinline__ int scan_bins(int v, int* sm) {
     const int y = __shfl_up(x, o, 64);
     if (lane >= o) x += y;
   }
-  if (lane == 63 && t < BINS) sm[t >> 6] = x;
+  if (lane == 63) sm[t >> 6] = x;
   __syncthreads();
   int before = 0;
-  for (int w = 0; w < (t >> 6) && w < BINS / 64; ++w) before += sm[w];
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) before += w < (t >> 6) ? sm[w] : 0;
   __syncthreads();
   return before + x - v;
 }
 
-// Up to SMALL ids sorted by one workgroup, in LDS
-__global__ __launch_bounds__(1024) void table_sort_small_kernel(const int64_t* ids, int n, int64_t vocab, int64_t padding, int bits, int digits, int* keys, int* places) {
-  extern __shared__ int lds[];
-  auto kb = [&](int k) { return lds + k * SMALL; };
-  auto pb = [&](int k) { return lds + (2 + k) * SMALL; };
-  int* counts = lds + 4 * SMALL;      // [16][BINS]
-  __shared__ int sm[BINS / 64];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int per = (n + 1023) / 1024 * 64;      // keys of a wavefront
-  for (int i = t; i < n; i += 1024) {
-    kb(0)[i] = key_of(ids[i], vocab, padding);
-    pb(0)[i] = i;
+// Zeros to the whole of the table's gradient, by workgroups that would otherwise wait for the sort: what the sums write later
+// they write over.  (Only the rows that no token names would be fewer bytes, but they are known when the sort is done:
+// 16384 ids, 32000 x 2048, bf16: 28 us of sort and then 63 of sums and zeros against 24 of both at once and then 25.)
+struct Zero { uint32_t* p; int64_t words, odd; };      // odd: a 16-bit value before / behind them, bits 0 and 1
+__device__ __forceinline__ void zero_part(const Zero& z, int64_t block, int64_t blocks, int threads) {
+  typedef uint32_t u4_t __attribute__((ext_vector_type(4), aligned(4)));
+  const u4_t none = {0, 0, 0, 0};
+  const int64_t n = z.words / 4;
+  for (int64_t i = block * threads + threadIdx.x; i < n; i += blocks * threads) ((u4_t*)z.p)[i] = none;
+  if (block == 0 && threadIdx.x < (z.words & 3)) z.p[n * 4 + threadIdx.x] = 0;
+  if (block == 0 && threadIdx.x == 0 && (z.odd & 1)) ((uint16_t*)z.p)[-1] = 0;
+  if (block == 0 && threadIdx.x == 0 && (z.odd & 2)) *(uint16_t*)(z.p + z.words) = 0;
+}
+
+// Up to MANY ids.  First BLOCK neighbours among themselves, by counting: a word's rank is the number of words below it (no two
+// are alike), found by 16 wavefronts that each compare 64 of them with an eighth of a thousand.  2048 compares an id, but spread over
+// the whole chip and without a dependence between them.  The other workgroups write zeros.
+__global__ __launch_bounds__(1024) void table_rank_kernel(const int64_t* ids, int n, int64_t vocab, int64_t padding, uint32_t* words, int* keys, int* places, int groups,
+                                                          const Zero zero) {
+  __shared__ __align__(16) uint32_t w[BLOCK];
+  __shared__ int parts[16][64];
+  if ((int)blockIdx.x >= groups) {
+    zero_part(zero, (int)blockIdx.x - groups, (int)gridDim.x - groups, 1024);
+    return;
   }
-  for (int d = 0; d < digits; ++d) {
-    const int *kin = kb(d & 1), *pin = pb(d & 1);
-    int *kout = kb((d & 1) ^ 1), *pout = pb((d & 1) ^ 1);
-    const int shift = d * bits, mask = (1 << bits) - 1;
-    for (int i = t; i < 16 * BINS; i += 1024) counts[i] = 0;
-    __syncthreads();
-    for (int i = lane; i < per; i += 64)
-      if (wave * per + i < n) atomicAdd(&counts[wave * BINS + ((kin[wave * per + i] >> shift) & mask)], 1);
-    __syncthreads();
-    int total = 0;
-    if (t < BINS)
-      for (int w = 0; w < 16; ++w) total += counts[w * BINS + t];
-    int at = scan_bins(total, sm);
-    if (t < BINS)
-      for (int w = 0; w < 16; ++w) {
-        const int c = counts[w * BINS + t];
-        counts[w * BINS + t] = at;
-        at += c;
-      }
-    __syncthreads();
-    for (int i = lane; i < per; i += 64) {
-      const bool active = wave * per + i < n;
-      const int key = active ? kin[wave * per + i] : 0, place = active ? pin[wave * per + i] : 0;
-      const int to = rank_of((key >> shift) & mask, active, bits, counts + wave * BINS);
-      if (active) {
-        kout[to] = key;
-        pout[to] = place;
-      }
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int base = (int)blockIdx.x * 64 / BLOCK * BLOCK, mine = (int)blockIdx.x * 64 % BLOCK + lane;
+#pragma unroll
+  for (int i = 0; i < BLOCK / 1024; ++i) {
+    const int at = base + i * 1024 + t;
+    w[i * 1024 + t] = at < n ? (uint32_t)key_of(ids[at], vocab, padding) << PLACE_BITS | (uint32_t)(i * 1024 + t) : ~0u;
+  }
+  __syncthreads();
+  const uint32_t word = w[mine];
+  int below = 0;
+#pragma unroll 8
+  for (int j = wave * (BLOCK / 16); j < (wave + 1) * (BLOCK / 16); j += 4) {
+    const uint4 o = *(const uint4*)(w + j);
+    below += (o.x < word) + (o.y < word) + (o.z < word) + (o.w < word);
+  }
+  parts[wave][lane] = below;
+  __syncthreads();
+  if (wave > 0 || base + mine >= n) return;
+  int rank = 0;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) rank += parts[k][lane];
+  if (n <= BLOCK) {
+    keys[rank] = (int)(word >> PLACE_BITS);
+    places[rank] = (int)(word & (BLOCK - 1));
+  } else {
+    words[base + rank] = word;
+  }
+}
+
+// Then every sorted block's words to their places among all: as many as in each block before are not above it, in each behind below
+// it.  Eight blocks at a time lie in LDS, and a thread's eight searches in them run side by side (in memory a search's twelve steps
+// are twelve round trips: 16384 ids 17 us, 50021 57).
+__global__ __launch_bounds__(256) void table_merge_kernel(const uint32_t* words, int n, int* keys, int* places) {
+  extern __shared__ __align__(16) uint32_t w[];      // [8][BLOCK]
+  const int t = threadIdx.x, i = (int)blockIdx.x * 256 + t;
+  const uint32_t word = i < n ? words[i] : 0;
+  const int key = (int)(word >> PLACE_BITS), own = i / BLOCK, blocks = (n + BLOCK - 1) / BLOCK;
+  int rank = i % BLOCK;
+  for (int b0 = 0; b0 < blocks; b0 += 8) {
+    uint4 v[8 * BLOCK / 1024];
+#pragma unroll
+    for (int k = 0; k < 8 * BLOCK / 1024; ++k) {
+      const int at = b0 * BLOCK + (k * 256 + t) * 4;      // (what lies behind the last word is not looked at)
+      v[k] = at < n ? *(const uint4*)(words + at) : make_uint4(~0u, ~0u, ~0u, ~0u);
     }
     __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 8 * BLOCK / 1024; ++k) *(uint4*)(w + (k * 256 + t) * 4) = v[k];
+    __syncthreads();
+    int pos[8], size[8], limit[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      pos[q] = 0;
+      const int left = n - (b0 + q) * BLOCK;
+      size[q] = left < 0 ? 0 : left < BLOCK ? left : BLOCK;
+      limit[q] = b0 + q < own ? key + 1 : key;
+    }
+#pragma unroll
+    for (int step = BLOCK / 2; step > 0; step >>= 1) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {      // (no branch: eight reads on their way, not one)
+        const int to = pos[q] + step, at = (int)(w[q * BLOCK + to - 1] >> PLACE_BITS);
+        pos[q] = ((to <= size[q]) & (at < limit[q])) ? to : pos[q];
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const int at = (int)(w[q * BLOCK + (pos[q] < BLOCK ? pos[q] : BLOCK - 1)] >> PLACE_BITS);
+      pos[q] += (pos[q] < size[q]) & (at < limit[q]);      // (all of a block)
+      if (b0 + q != own) rank += pos[q];
+    }
   }
-  for (int i = t; i < n; i += 1024) {
-    keys[i] = kb(digits & 1)[i];
-    places[i] = pb(digits & 1)[i];
+  if (i < n) {
+    keys[rank] = key;
+    places[rank] = own * BLOCK + (int)(word & (BLOCK - 1));
   }
 }
 
 // How often each value of a digit occurs among a block's keys
 template <int ITEMS>
-__global__ __launch_bounds__(256) void table_count_kernel(const int64_t* ids, const int* keys, int64_t n, int64_t vocab, int64_t padding, int shift, int bits, int* counts) {
-  __shared__ int c[BINS];
-  const int t = threadIdx.x;
-  for (int i = t; i < BINS; i += 256) c[i] = 0;
-  __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * 256 * ITEMS;
-#pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
-    const int64_t at = base + i * 256 + t;
-    if (at < n) atomicAdd(&c[((ids != nullptr ? key_of(ids[at], vocab, padding) : keys[at]) >> shift) & ((1 << bits) - 1)], 1);
-  }
-  __syncthreads();
-  for (int i = t; i < BINS; i += 256) counts[(int64_t)blockIdx.x * BINS + i] = c[i];
-}
-
-// ... and the keys to their places.  A block finds out from all blocks' counts where its own begin.
-template <int ITEMS>
-__global__ __launch_bounds__(256) void table_place_kernel(const int64_t* ids, const int* keys, const int* places, int64_t n, int64_t vocab, int64_t padding, int shift,
-                                                          int bits, const int* counts, int* keys_out, int* places_out) {
+__global__ __launch_bounds__(256) void table_count_kernel(const int64_t* ids, const int* keys, int64_t n, int64_t vocab, int64_t padding, int shift, int bits, int* counts,
+                                                          int blocks, const Zero zero) {
   __shared__ int wc[4][BINS];
-  __shared__ int sm[8];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, mask = (1 << bits) - 1;
+  if ((int)blockIdx.x >= blocks) {
+    zero_part(zero, (int)blockIdx.x - blocks, (int)gridDim.x - blocks, 256);
+    return;
+  }
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   for (int i = t; i < 4 * BINS; i += 256) (&wc[0][0])[i] = 0;
   __syncthreads();
   const int64_t base = (int64_t)blockIdx.x * 256 * ITEMS + wave * 64 * ITEMS;
@@ -135,8 +180,32 @@ __global__ __launch_bounds__(256) void table_place_kernel(const int64_t* ids, co
   for (int i = 0; i < ITEMS; ++i) {
     const int64_t at = base + i * 64 + lane;
     key[i] = at >= n ? 0 : ids != nullptr ? key_of(ids[at], vocab, padding) : keys[at];
-    if (at < n) atomicAdd(&wc[wave][(key[i] >> shift) & mask], 1);
   }
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) rank_of((key[i] >> shift) & ((1 << bits) - 1), base + i * 64 + lane < n, bits, wc[wave]);
+  __syncthreads();
+  for (int i = t; i < BINS; i += 256) counts[(int64_t)blockIdx.x * BINS + i] = wc[0][i] + wc[1][i] + wc[2][i] + wc[3][i];
+}
+
+// ... and the keys to their places.  A block finds out from all blocks' counts where its own begin.
+template <int ITEMS>
+__global__ __launch_bounds__(256) void table_place_kernel(const int64_t* ids, const int* keys, const int* places, int64_t n, int64_t vocab, int64_t padding, int shift,
+                                                          int bits, const int* counts, int* keys_out, int* places_out) {
+  __shared__ int wc[4][BINS];
+  __shared__ int sm[4];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, mask = (1 << bits) - 1;
+  for (int i = t; i < 4 * BINS; i += 256) (&wc[0][0])[i] = 0;
+  __syncthreads();
+  const int64_t base = (int64_t)blockIdx.x * 256 * ITEMS + wave * 64 * ITEMS;
+  int key[ITEMS], rank[ITEMS], place[ITEMS];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int64_t at = base + i * 64 + lane;
+    key[i] = at >= n ? 0 : ids != nullptr ? key_of(ids[at], vocab, padding) : keys[at];
+    place[i] = at >= n || places == nullptr ? (int)at : places[at];
+  }
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) rank[i] = rank_of((key[i] >> shift) & mask, base + i * 64 + lane < n, bits, wc[wave]);
   // thread t: digits 2 t and 2 t + 1
   int mine[2] = {0, 0}, all[2] = {0, 0};
   const int blocks = gridDim.x;
@@ -147,17 +216,7 @@ __global__ __launch_bounds__(256) void table_place_kernel(const int64_t* ids, co
     all[1] += c.y;
     if (b < (int)blockIdx.x) { mine[0] += c.x; mine[1] += c.y; }
   }
-  int x = all[0] + all[1];
-  const int own = x;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(x, o, 64);
-    if (lane >= o) x += y;
-  }
-  if (lane == 63) sm[wave] = x;
-  __syncthreads();
-  int before = x - own;
-  for (int w = 0; w < wave; ++w) before += sm[w];
+  const int before = sum_before<4>(all[0] + all[1], sm);      // (its barriers: all wavefronts have counted)
   mine[0] += before;
   mine[1] += before + all[0];
 #pragma unroll
@@ -173,12 +232,10 @@ __global__ __launch_bounds__(256) void table_place_kernel(const int64_t* ids, co
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
     const int64_t at = base + i * 64 + lane;
-    const bool active = at < n;
-    const int to = rank_of((key[i] >> shift) & mask, active, bits, wc[wave]);
-    if (active) {
-      keys_out[to] = key[i];
-      places_out[to] = places != nullptr ? places[at] : (int)at;
-    }
+    if (at >= n) continue;
+    const int to = wc[wave][(key[i] >> shift) & mask] + rank[i];
+    keys_out[to] = key[i];
+    places_out[to] = place[i];
   }
 }
 
@@ -259,6 +316,7 @@ struct Sum {
   const int* places;
   void* dtable;
   float* partial;      // [chunks][2][dim]: of a run that comes from the chunk before, of one that goes on into the next
+  float* blocks;       // [chunks / FEW][dim]
   int64_t n, dim, vocab, chunks;
   float scale;
   int lg, t_f32, accumulate;
@@ -280,36 +338,79 @@ __device__ __forceinline__ void put_row(const Sum& s, int64_t row, int64_t c, fl
   else store_row<DT, W>(s.dtable, at, left, v);
 }
 
-// Workgroups of the first `sums` columns of the grid: a group of lanes adds up one chunk of the sorted list in one slice of the columns;
-// runs that end inside it go to the table's gradient, the others' parts to `partial`.  The other workgroups: rows without a token.
-template <int DT, int W, int CHUNK>
-__global__ __launch_bounds__(256) void table_sum_kernel(const Sum s, int sums) {
-  const int lane = threadIdx.x & 63;
-  if ((int)blockIdx.x >= sums) {
-    // 64 rows to a wavefront, a lane looks for its own; then the rows that are not there, one by one
-    const int64_t v0 = ((int64_t)((int)blockIdx.x - sums) * 4 + (threadIdx.x >> 6)) * 64;
-    const int64_t v = v0 + lane;
-    int64_t lo = 0, hi = s.n;
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) >> 1;
-      if (s.keys[mid] < v) lo = mid + 1;
-      else hi = mid;
-    }
-    unsigned long long missing = __ballot(v < s.vocab && !(lo < s.n && s.keys[lo] == v));
-    const int64_t step = 64 * W;
+// Up to FEW_IDS ids, in one launch: a workgroup owns `own` rows of the table's gradient, writes zeros to them, finds the ids that name
+// one of them and adds up, a wavefront to a row, in the list's order.  (The sort takes two launches more; a token that is all of the list is
+// 32 round trips of eight rows here.)
+template <int DT, int W>
+__global__ __launch_bounds__(256) void table_few_kernel(const Sum s, const int64_t* ids, int64_t padding, int64_t own) {
+  __shared__ int rows[FEW_IDS], at[FEW_IDS];
+  __shared__ int before[5];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int64_t v0 = (int64_t)blockIdx.x * own, v1 = v0 + own < s.vocab ? v0 + own : s.vocab;
+  const int64_t id = t < s.n ? ids[t] : -1;
+  if (!s.accumulate) {
     float zero[W];
 #pragma unroll
     for (int k = 0; k < W; ++k) zero[k] = 0.f;
-    while (missing) {
-      const int b = __ffsll((long long)missing) - 1;
-      missing &= missing - 1;
-      for (int64_t c = lane * W; c < s.dim; c += step) {
-        if (s.t_f32) store_row<PF_F32, W>(s.dtable, (v0 + b) * s.dim + c, s.dim - c, zero);
-        else store_row<DT, W>(s.dtable, (v0 + b) * s.dim + c, s.dim - c, zero);
-      }
+    const int64_t end = v1 * s.dim;
+    for (int64_t i = v0 * s.dim + (int64_t)t * W; i < end; i += 256 * W) {
+      if (s.t_f32) store_row<PF_F32, W>(s.dtable, i, end - i, zero);
+      else store_row<DT, W>(s.dtable, i, end - i, zero);
     }
-    return;
   }
+  const bool hit = id >= v0 && id < v1 && id != padding;
+  const unsigned long long mask = __ballot(hit);
+  if (lane == 0) before[wave + 1] = __popcll(mask);
+  __syncthreads();
+  int first = 0;
+  for (int w = 0; w < wave; ++w) first += before[w + 1];
+  if (hit) {
+    const int j = first + __popcll(mask & ((1ull << lane) - 1));
+    rows[j] = (int)(id - v0);
+    at[j] = t;
+  }
+  const int hits = before[1] + before[2] + before[3] + before[4];
+  __syncthreads();      // (and the zeros are written)
+  for (int j = wave; j < hits; j += 4) {
+    const int row = rows[j];
+    bool earlier = false;
+    for (int q = lane; q < j; q += 64) earlier |= rows[q] == row;
+    if (__ballot(earlier) != 0) continue;
+    for (int64_t c = lane * W; c < s.dim; c += 64 * W) {
+      float acc[W];
+#pragma unroll
+      for (int k = 0; k < W; ++k) acc[k] = 0.f;
+      int q = j;
+      while (q < hits) {
+        int place[8];
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {      // the next eight of the row
+          while (q < hits && rows[q] != row) ++q;
+          place[k] = q < hits ? at[q] : 0;
+          n += q < hits;
+          ++q;
+        }
+        float v[8][W];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < n) load_row<DT, W>(s.dout, (int64_t)place[k] * s.dim + c, s.dim - c, v[k]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < n) {
+#pragma unroll
+            for (int e = 0; e < W; ++e) acc[e] += v[k][e];
+          }
+      }
+      put_row<DT, W>(s, v0 + row, c, acc);
+    }
+  }
+}
+
+// A group of lanes adds up one chunk of the sorted list in one slice of the columns; runs that end inside it go to the table's
+// gradient, the others' parts to `partial`
+template <int DT, int W, int CHUNK>
+__global__ __launch_bounds__(256) void table_sum_kernel(const Sum s) {
   const int G = 1 << s.lg;
   const int64_t slices = (s.dim + (int64_t)G * W - 1) / ((int64_t)G * W);
   const int64_t unit = (int64_t)blockIdx.x * (256 >> s.lg) + (threadIdx.x >> s.lg);
@@ -361,47 +462,116 @@ __global__ __launch_bounds__(256) void table_sum_kernel(const Sum s, int sums) {
   flush(run == first_after);
 }
 
-// A run that begins in this chunk and goes on into others: their parts, in the list's order, TEAMS of them at once
-template <int DT, int W, int CHUNK, int TEAMS>
-__global__ __launch_bounds__(64 * TEAMS) void table_join_kernel(const Sum s) {
-  __shared__ float part[TEAMS][64 * W];
-  const int64_t chunk = blockIdx.x;
-  const int lane = threadIdx.x & 63, team = threadIdx.x >> 6;
-  const int64_t next = (chunk + 1) * CHUNK;
+// Runs that cross chunks.  FEW neighbours from a multiple of FEW on are a block of chunks.
+constexpr int FEW = 64;
+
+// The first `waves` wavefronts of each slice, one to a chunk: a run that begins in it and goes on over less than FEW others, their parts in the
+// list's order.  The others, four to a block of chunks: where it lies inside one run, its parts' sum.
+template <int DT, int W, int CHUNK>
+__global__ __launch_bounds__(256) void table_join_kernel(const Sum s, int joins) {
+  __shared__ float part[4][64 * W];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t c = (int64_t)blockIdx.y * 64 * W + lane * W, left = s.dim - c;
+  float acc[W];
+#pragma unroll
+  for (int k = 0; k < W; ++k) acc[k] = 0.f;
+  if ((int)blockIdx.x >= joins) {
+    const int64_t block = (int)blockIdx.x - joins, first = block * FEW;
+    const int64_t end = (first + FEW - 1) * CHUNK;
+    if (first == 0 || end >= s.n) return;
+    const int run = s.keys[end];
+    if (run >= s.vocab || s.keys[first * CHUNK - 1] != run) return;
+    if (left > 0) {
+#pragma unroll
+      for (int p = 0; p < FEW / 4; ++p) {
+        float v[W];
+        load_row<PF_F32, W>(s.partial + (first + wave * (FEW / 4) + p) * 2 * s.dim, c, left, v);
+#pragma unroll
+        for (int k = 0; k < W; ++k) acc[k] += v[k];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < W; ++k) part[wave][lane * W + k] = acc[k];
+    __syncthreads();
+    if (wave > 0 || left <= 0) return;
+    for (int w = 1; w < 4; ++w) {
+#pragma unroll
+      for (int k = 0; k < W; ++k) acc[k] += part[w][lane * W + k];
+    }
+    store_row<PF_F32, W>(s.blocks + block * s.dim, c, left, acc);
+    return;
+  }
+  const int64_t chunk = (int64_t)blockIdx.x * 4 + wave, next = (chunk + 1) * CHUNK;
   if (next >= s.n) return;
   const int run = s.keys[next - 1];
   if (run >= s.vocab || s.keys[next] != run) return;
   if (s.keys[chunk * CHUNK] == run && chunk > 0 && s.keys[chunk * CHUNK - 1] == run) return;      // (it began before)
-  // the last chunk that begins with the run
-  int64_t lo = chunk + 1, hi = s.chunks - 1;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi + 1) >> 1;
-    if (s.keys[mid * CHUNK] == run) lo = mid;
-    else hi = mid - 1;
+  const int64_t mine = next + (int64_t)lane * CHUNK;
+  const unsigned long long on = __ballot(mine < s.n && s.keys[mine] == run);
+  if (on == ~0ull || left <= 0) return;                                                           // (of more chunks: below)
+  const int many = __ffsll((long long)~on) - 1;      // chunks that begin with the run
+  load_row<PF_F32, W>(s.partial + (chunk * 2 + 1) * s.dim, c, left, acc);
+#pragma unroll 4
+  for (int p = 1; p <= many; ++p) {
+    float v[W];
+    load_row<PF_F32, W>(s.partial + (chunk + p) * 2 * s.dim, c, left, v);
+#pragma unroll
+    for (int k = 0; k < W; ++k) acc[k] += v[k];
   }
-  const int64_t many = lo - chunk;        // parts besides this chunk's own
+  put_row<DT, W>(s, run, c, acc);
+}
+
+// The smallest i in [lo, hi] with f(i), hi if there is none below it, f being false first and then true; a wavefront looks at 64 at a time
+template <class F>
+__device__ __forceinline__ int64_t wave_find(int64_t lo, int64_t hi, F f) {
+  while (lo < hi) {
+    const int64_t step = (hi - lo + 63) / 64, at = lo + (threadIdx.x & 63) * step;
+    const unsigned long long yes = __ballot(at >= hi || f(at));
+    const int k = yes != 0 ? __ffsll((long long)yes) - 1 : 64;
+    const int64_t top = lo + k * step;
+    lo = k > 0 ? lo + (k - 1) * step + 1 : lo;
+    hi = top < hi ? top : hi;
+  }
+  return hi;
+}
+
+// Longer runs: each holds the first entry of a block of chunks.  The workgroup of the first such block finds the run's ends; its 16
+// wavefronts each add a share of the parts, in the list's order: chunks up to a block, whole blocks, chunks after them.
+template <int DT, int W, int CHUNK>
+__global__ __launch_bounds__(1024) void table_join_long_kernel(const Sum s) {
+  __shared__ float part[16][64 * W];
+  const int64_t mark = ((int64_t)blockIdx.x + 1) * FEW;
+  const int lane = threadIdx.x & 63, team = threadIdx.x >> 6;
+  if (mark >= s.chunks) return;
+  const int run = s.keys[mark * CHUNK];
+  if (run >= s.vocab || s.keys[mark * CHUNK - 1] != run) return;
+  if (mark > FEW && s.keys[(mark - FEW) * CHUNK] == run && s.keys[(mark - FEW) * CHUNK - 1] == run) return;      // (a block before this one's)
+  const int64_t first = wave_find(0, mark * CHUNK, [&](int64_t j) { return s.keys[j] >= run; }) / CHUNK;
+  const int64_t lo = wave_find(mark + 1, s.chunks, [&](int64_t m) { return s.keys[m * CHUNK] > run; }) - 1;      // the last chunk that begins with it
+  if (lo - first < FEW) return;
+  const int64_t blocks = (lo + 1 - mark) / FEW, head = mark - first, rest = lo + 1 - mark - blocks * FEW, many = head + blocks + rest;
   const int64_t c = (int64_t)blockIdx.y * 64 * W + lane * W, left = s.dim - c;
-  const int64_t per = (many + TEAMS - 1) / TEAMS, a = chunk + 1 + team * per, b = a + per < lo + 1 ? a + per : lo + 1;
+  const int64_t per = (many + 15) / 16, a = team * per, b = a + per < many ? a + per : many;
   float acc[W];
 #pragma unroll
   for (int k = 0; k < W; ++k) acc[k] = 0.f;
   if (left > 0) {
-    if (team == 0) load_row<PF_F32, W>(s.partial + (chunk * 2 + 1) * s.dim, c, left, acc);
-#pragma unroll 4
+#pragma unroll 8
     for (int64_t p = a; p < b; ++p) {
+      const float* from = p == 0 ? s.partial + (first * 2 + 1) * s.dim
+                          : p < head ? s.partial + (first + p) * 2 * s.dim
+                          : p < head + blocks ? s.blocks + (mark / FEW + p - head) * s.dim : s.partial + (mark + blocks * FEW + p - head - blocks) * 2 * s.dim;
       float v[W];
-      load_row<PF_F32, W>(s.partial + p * 2 * s.dim, c, left, v);
+      load_row<PF_F32, W>(from, c, left, v);
 #pragma unroll
       for (int k = 0; k < W; ++k) acc[k] += v[k];
     }
   }
-  if (team > 0) {
 #pragma unroll
-    for (int k = 0; k < W; ++k) part[team][lane * W + k] = acc[k];
-  }
+  for (int k = 0; k < W; ++k) part[team][lane * W + k] = acc[k];
   __syncthreads();
   if (team > 0 || left <= 0) return;
-  for (int w = 1; w < TEAMS && w * per < many; ++w) {
+  for (int w = 1; w < 16 && w * per < many; ++w) {
 #pragma unroll
     for (int k = 0; k < W; ++k) acc[k] += part[w][lane * W + k];
   }
@@ -409,10 +579,12 @@ __global__ __launch_bounds__(64 * TEAMS) void table_join_kernel(const Sum s) {
 }
 
 inline int64_t round_up(int64_t n, int64_t k) { return (n + k - 1) / k * k; }
-inline int chunk_of(int64_t n) { return n <= 8192 ? 8 : 32; }
+// Neighbours that a group of lanes adds up.  Few make more groups and more parts: 16384 ids, 2048 columns, bf16 27 us with 8, 49 with
+// 32; the parts of longer lists are worth more than their groups.
+inline int chunk_of(int64_t n) { return n <= MANY ? 8 : 32; }
 inline int items_of(int64_t n) { return n <= 65536 ? 8 : 16; }
 
-struct Layout { int64_t keys[2], places[2], counts, partial, bytes; };
+struct Layout { int64_t keys[2], places[2], counts, partial, blocks, bytes; };
 Layout layout_of(int64_t n, int64_t dim) {
   Layout l;
   int64_t at = 0;
@@ -420,6 +592,7 @@ Layout layout_of(int64_t n, int64_t dim) {
   for (int k = 0; k < 2; ++k) { l.keys[k] = take(n * 4); l.places[k] = take(n * 4); }
   l.counts = take((n + 256 * items_of(n) - 1) / (256 * items_of(n)) * BINS * 4);
   l.partial = take((n + chunk_of(n) - 1) / chunk_of(n) * 2 * dim * 4);
+  l.blocks = take((n + chunk_of(n) - 1) / chunk_of(n) / FEW * dim * 4);
   l.bytes = at;
   return l;
 }
@@ -428,10 +601,12 @@ template <int DT, int W, int CHUNK>
 void sum_launch(const Sum& s, hipStream_t st) {
   const int64_t slices = (s.dim + ((int64_t)W << s.lg) - 1) / ((int64_t)W << s.lg);
   const int64_t sums = (s.chunks * slices + (256 >> s.lg) - 1) / (256 >> s.lg);
-  const int64_t zeros = s.accumulate ? 0 : (s.vocab + 255) / 256;
-  if (sums + zeros > 0) hipLaunchKernelGGL((table_sum_kernel<DT, W, CHUNK>), dim3((unsigned)(sums + zeros)), dim3(256), 0, st, s, (int)sums);
-  if (s.chunks > 1)
-    hipLaunchKernelGGL((table_join_kernel<DT, W, CHUNK, 8>), dim3((unsigned)(s.chunks - 1), (unsigned)((s.dim + 64 * W - 1) / (64 * W))), dim3(512), 0, st, s);
+  hipLaunchKernelGGL((table_sum_kernel<DT, W, CHUNK>), dim3((unsigned)sums), dim3(256), 0, st, s);
+  if (s.chunks < 2) return;
+  const unsigned slices64 = (unsigned)((s.dim + 64 * W - 1) / (64 * W));
+  const int64_t joins = (s.chunks + 3) / 4, blocks = s.chunks / FEW;
+  hipLaunchKernelGGL((table_join_kernel<DT, W, CHUNK>), dim3((unsigned)(joins + blocks), slices64), dim3(256), 0, st, s, (int)joins);
+  if (blocks > 0) hipLaunchKernelGGL((table_join_long_kernel<DT, W, CHUNK>), dim3((unsigned)blocks, slices64), dim3(1024), 0, st, s);
 }
 template <int DT>
 void sum_dispatch(const Sum& s, bool wide, hipStream_t st) {
@@ -452,7 +627,8 @@ int lanes_of(int64_t dim, int W) {
 }
 
 template <int ITEMS>
-void sort_large(const int64_t* ids, int64_t n, int64_t vocab, int64_t padding, int bits, int digits, char* ws, const Layout& l, hipStream_t st) {
+void sort_large(const int64_t* ids, int64_t n, int64_t vocab, int64_t padding, int bits, int digits, char* ws, const Layout& l, const Zero& zero,
+                int zero_blocks, hipStream_t st) {
   const unsigned blocks = (unsigned)((n + 256 * ITEMS - 1) / (256 * ITEMS));
   int* counts = (int*)(ws + l.counts);
   for (int d = 0; d < digits; ++d) {
@@ -461,7 +637,8 @@ void sort_large(const int64_t* ids, int64_t n, int64_t vocab, int64_t padding, i
     const int* pin = d == 0 ? nullptr : (const int*)(ws + l.places[(d ^ digits) & 1]);
     int* kout = (int*)(ws + l.keys[(d + 1 + digits) & 1]);      // (the last digit's go to the first buffers)
     int* pout = (int*)(ws + l.places[(d + 1 + digits) & 1]);
-    hipLaunchKernelGGL(table_count_kernel<ITEMS>, dim3(blocks), dim3(256), 0, st, from, kin, n, vocab, padding, d * bits, bits, counts);
+    hipLaunchKernelGGL(table_count_kernel<ITEMS>, dim3(blocks + (d == 0 ? (unsigned)zero_blocks : 0u)), dim3(256), 0, st, from, kin, n, vocab, padding, d * bits, bits,
+                       counts, (int)blocks, zero);
     hipLaunchKernelGGL(table_place_kernel<ITEMS>, dim3(blocks), dim3(256), 0, st, from, kin, pin, n, vocab, padding, d * bits, bits, counts, kout, pout);
   }
 }
@@ -489,39 +666,68 @@ extern "C" int pf_embedding_scaled_fwd(const void* table, int dtype, const int64
   return PF_OK;
 }
 
-extern "C" int64_t pf_embedding_sorted_workspace(int64_t n_ids, int64_t dim) { return n_ids <= 0 || dim <= 0 ? 256 : layout_of(n_ids, dim).bytes; }
+extern "C" int64_t pf_embedding_sorted_workspace(int64_t n_ids, int64_t dim) { return n_ids <= FEW_IDS || dim <= 0 ? 0 : layout_of(n_ids, dim).bytes; }
 
 extern "C" int pf_embedding_sorted_bwd(const void* dout, int d_dtype, const int64_t* ids, void* dtable, int t_dtype, int64_t n_ids, int64_t dim, int64_t vocab,
                                        int64_t padding_idx, double scale, int accumulate, void* workspace, void* stream) {
   const char* who = "pf_embedding_sorted_bwd";
   PF_REQUIRE(n_ids >= 0 && dim > 0 && vocab > 0 && pf_is_float_dtype(d_dtype) && (t_dtype == d_dtype || t_dtype == PF_F32), "%s: bad arguments", who);
   PF_REQUIRE(padding_idx >= -1 && padding_idx < vocab, "%s: padding_idx must be -1 (none) or a row", who);
-  PF_REQUIRE(dtable && workspace && (n_ids == 0 || (dout && ids)), "%s: null pointer", who);
+  PF_REQUIRE(dtable && (n_ids <= FEW_IDS || workspace) && (n_ids == 0 || (dout && ids)), "%s: null pointer", who);
   PF_REQUIRE(n_ids <= (1ll << 27) && vocab < (1ll << 27) - 1 && dim < (1ll << 22), "%s: too many ids, rows or columns", who);
   hipStream_t st = (hipStream_t)stream;
   char* ws = (char*)workspace;
-  const Layout l = layout_of(n_ids > 0 ? n_ids : 1, dim);
-  Sum s = {dout, (const int*)(ws + l.keys[0]), (const int*)(ws + l.places[0]), dtable, (float*)(ws + l.partial), n_ids, dim, vocab,
+  const Layout l = layout_of(n_ids, dim);
+  Sum s = {dout, (const int*)(ws + l.keys[0]), (const int*)(ws + l.places[0]), dtable, (float*)(ws + l.partial), (float*)(ws + l.blocks), n_ids, dim, vocab,
            (n_ids + chunk_of(n_ids) - 1) / chunk_of(n_ids), (float)scale, 0, t_dtype == PF_F32, accumulate != 0};
-  if (n_ids > 0) {
-    int need = 1;
-    while ((vocab >> need) != 0) ++need;               // bits of the keys 0 .. vocab
-    const int digits = (need + 8) / 9, bits = (need + digits - 1) / digits;
-    if (n_ids <= SMALL) {
-      const size_t lds = (4 * SMALL + 16 * BINS) * sizeof(int);
-      const int rc = pf_allow_lds((const void*)table_sort_small_kernel, lds, who);
-      if (rc != PF_OK) return rc;
-      hipLaunchKernelGGL(table_sort_small_kernel, dim3(1), dim3(1024), lds, st, ids, (int)n_ids, vocab, padding_idx, bits, digits, (int*)(ws + l.keys[0]),
-                         (int*)(ws + l.places[0]));
-    } else if (items_of(n_ids) == 8) {
-      sort_large<8>(ids, n_ids, vocab, padding_idx, bits, digits, ws, l, st);
-    } else {
-      sort_large<16>(ids, n_ids, vocab, padding_idx, bits, digits, ws, l, st);
-    }
-  }
   const int size = pf_dtype_size(d_dtype);
   const bool wide = dim * size % 4 == 0 && pf_aligned(dout, 4) && pf_aligned(dtable, 4);
   s.lg = lanes_of(dim, wide ? 8 : 1);
+  if (n_ids <= FEW_IDS) {
+    int64_t own = 65536 / (dim * pf_dtype_size(t_dtype));
+    own = own < 1 ? 1 : own > 1024 ? 1024 : own;
+    const dim3 grid((unsigned)((vocab + own - 1) / own));
+#define PF_TF(DT) \
+    if (wide) hipLaunchKernelGGL((table_few_kernel<DT, 8>), grid, dim3(256), 0, st, s, ids, padding_idx, own); \
+    else hipLaunchKernelGGL((table_few_kernel<DT, 1>), grid, dim3(256), 0, st, s, ids, padding_idx, own);
+    if (d_dtype == PF_F32) { PF_TF(PF_F32) }
+    else if (d_dtype == PF_F16) { PF_TF(PF_F16) }
+    else { PF_TF(PF_BF16) }
+#undef PF_TF
+    PF_CHECK_LAUNCH(who);
+    return PF_OK;
+  }
+  // the gradient's bytes as words, and what is left of a 16-bit one at its ends
+  Zero zero = {nullptr, 0, 0};
+  int64_t zero_blocks = 0;
+  if (!accumulate) {
+    const int t_size = pf_dtype_size(t_dtype);
+    int64_t bytes = vocab * dim * t_size;
+    char* p = (char*)dtable;
+    if (t_size == 2 && !pf_aligned(p, 4)) { zero.odd |= 1; p += 2; bytes -= 2; }
+    if (bytes & 2) zero.odd |= 2;
+    zero.p = (uint32_t*)p;
+    zero.words = bytes / 4;
+    zero_blocks = (zero.words + 16383) / 16384 < 2048 ? (zero.words + 16383) / 16384 : 2048;
+    if (zero_blocks == 0) zero_blocks = 1;
+  }
+  int need = 1;
+  while ((vocab >> need) != 0) ++need;               // bits of the keys 0 .. vocab
+  const int digits = (need + 8) / 9, bits = (need + digits - 1) / digits;
+  if (n_ids <= MANY && need <= 32 - PLACE_BITS) {
+    const int groups = (int)((n_ids + 63) / 64);
+    uint32_t* words = (uint32_t*)(ws + l.keys[1]);
+    int *keys = (int*)(ws + l.keys[0]), *places = (int*)(ws + l.places[0]);
+    if (groups + zero_blocks > 0)
+      hipLaunchKernelGGL(table_rank_kernel, dim3((unsigned)(groups + zero_blocks)), dim3(1024), 0, st, ids, (int)n_ids, vocab, padding_idx, words, keys, places, groups, zero);
+    if (n_ids > BLOCK)
+      hipLaunchKernelGGL(table_merge_kernel, dim3((unsigned)((n_ids + 255) / 256)), dim3(256), 8 * BLOCK * 4, st, words, (int)n_ids, keys, places);
+  } else if (items_of(n_ids) == 8) {
+    sort_large<8>(ids, n_ids, vocab, padding_idx, bits, digits, ws, l, zero, (int)zero_blocks, st);
+  } else {
+    sort_large<16>(ids, n_ids, vocab, padding_idx, bits, digits, ws, l, zero, (int)zero_blocks, st);
+  }
+  PF_CHECK_LAUNCH(who);
   if (d_dtype == PF_F32) sum_dispatch<PF_F32>(s, wide, st);
   else if (d_dtype == PF_F16) sum_dispatch<PF_F16>(s, wide, st);
   else sum_dispatch<PF_BF16>(s, wide, st);

@@ -183,7 +183,8 @@ _SIGNATURES = {
 _RET_I64 = {"pf_gemm_colsum_rows": [POINTER(GemmDesc)], "pf_colreduce_workspace": [_L, _L], "pf_reduce_workspace": [_L],
             "pf_groupnorm_workspace": [_L, _L, _I], "pf_policy_workspace": [_L, _L, _I],
             "pf_preference_workspace": [_L, _L, _I], "pf_linear_ce_kept": [_L], "pf_linear_ce_workspace": [_P, _I, _L, _L, _L, _I],
-            "pf_embedding_sorted_workspace": [_L, _L], "pf_gated_linear_bytes": [_P, _P, _I, _L, _L, _L, _I, _I, POINTER(c_int64)],
+            "pf_embedding_sorted_workspace": [_L, _L], "pf_gated_linear_kept": [_I, _L, _L, _I],
+            "pf_gated_linear_workspace": [_P, _P, _I, _L, _L, _L, _I, _I],
             "pf_colsum_static_capacity": []}
 EXPORTED_SYMBOLS = sorted(list(_SIGNATURES) + list(_RET_I64) + ["pf_version", "pf_last_error"])
 
@@ -695,28 +696,6 @@ class HipKernels:
     def _token_rows(self, rows):
         return self.token_rows(*rows) if len(rows) == 10 else rows
 
-    def linear_ce_bytes(self, weight, tokens, D, V, backward):
-        """(bytes that the forward pass leaves, bytes of workspace)"""
-        need = int(self.lib.pf_linear_ce_workspace(_ptr(weight), _dt(weight), tokens, D, V, int(backward)))
-        if need < 0:
-            raise RuntimeError(last_error())
-        return int(self.lib.pf_linear_ce_kept(tokens)), need
-
-    def linear_ce_fwd(self, hidden, sizes, weight, V, labels, shift, ignore_index, z_loss, reduction, loss, kept, ws):
-        """sizes: B, T, D and the strides of hidden's first two dimensions"""
-        args = (_ptr(hidden), _dt(hidden), *sizes, _ptr(weight), V, _ptr(labels), int(shift), ignore_index, z_loss, reduction, _ptr(loss), _ptr(kept),
-                _ptr(ws))
-        return self._prep("pf_linear_ce_fwd", args, (hidden, weight, labels, loss, kept, ws))
-
-    def linear_ce_bwd(self, hidden, sizes, weight, V, z_loss, mean, kept, grad, g_strides, dhidden, dweight, ws):
-        args = (_ptr(hidden), _dt(hidden), *sizes, _ptr(weight), V, z_loss, int(mean), _ptr(kept), _ptr(grad), *g_strides, _ptr(dhidden), _ptr(dweight),
-                _ptr(ws))
-        return self._prep("pf_linear_ce_bwd", args, (hidden, weight, kept, grad, dhidden, dweight, ws))
-
-    def linear_ce_hidden_grad(self, weight, tokens, D, V, kept, times, dhidden, ws):
-        args = (_ptr(weight), _dt(dhidden), tokens, D, V, _ptr(kept), _ptr(times), _ptr(dhidden), _ptr(ws))
-        return self._prep("pf_linear_ce_hidden_grad", args, (weight, kept, times, dhidden, ws))
-
     def mse_fwd(self, a, b, partial, loss, n):
         args = (_ptr(a), _dt(a), _ptr(b), _dt(b), _ptr(partial), _ptr(loss), n)
         return self._prep("pf_mse_fwd", args, (a, b, partial, loss))
@@ -744,22 +723,6 @@ class HipKernels:
         args = (_ptr(dy), ld_dy, _ptr(gate), ld_gate, _ptr(up), ld_up, _ptr(dgate), ld_dgate, _ptr(dup), ld_dup,
                 _dt(gate), int(act), rows, cols)
         return self._prep("pf_glu_bwd", args, (dy, gate, up, dgate, dup), 5 * rows * cols * _es(gate))
-
-    def gated_linear_bytes(self, x, weight, rows, D, ffn, keep, backward):
-        """(bytes that the forward pass leaves, bytes of workspace)"""
-        kept = c_int64(0)
-        need = int(self.lib.pf_gated_linear_bytes(_ptr(x), _ptr(weight), _dt(x), rows, D, ffn, keep, int(backward), byref(kept)))
-        if need < 0:
-            raise RuntimeError(last_error())
-        return kept.value, need
-
-    def gated_linear_fwd(self, x, rows, D, weight, ffn, act, keep, y, kept, ws):
-        args = (_ptr(x), _dt(x), rows, D, _ptr(weight), ffn, act, keep, _ptr(y), _ptr(kept), _ptr(ws))
-        return self._prep("pf_gated_linear_fwd", args, (x, weight, y, kept, ws))
-
-    def gated_linear_bwd(self, x, rows, D, weight, ffn, act, keep, kept, dy, dx, dweight, ws):
-        args = (_ptr(x), _dt(x), rows, D, _ptr(weight), ffn, act, keep, _ptr(kept), _ptr(dy), _ptr(dx), _ptr(dweight), _ptr(ws))
-        return self._prep("pf_gated_linear_bwd", args, (x, weight, kept, dy, dx, dweight, ws))
 
     def axpby(self, a, alpha, b, beta, out, n):
         args = (_ptr(a), _dt(a), alpha, _ptr(b), _dt(b), beta, _ptr(out), _dt(out), n)
@@ -920,14 +883,3 @@ class HipKernels:
     def embedding_bwd(self, dout, ids, dtable, n_ids, dim, vocab, padding_idx=-1):
         args = (_ptr(dout), _dt(dout), _ptr(ids), _ptr(dtable), n_ids, dim, vocab, int(padding_idx))
         return self._prep("pf_embedding_bwd", args, (dout, ids, dtable))
-
-    def embedding_scaled_fwd(self, table, ids, out, n_ids, dim, vocab, scale):
-        args = (_ptr(table), _dt(table), _ptr(ids), _ptr(out), n_ids, dim, vocab, scale)
-        return self._prep("pf_embedding_scaled_fwd", args, (table, ids, out))
-
-    def embedding_sorted_workspace(self, n_ids, dim):
-        return int(self.lib.pf_embedding_sorted_workspace(n_ids, dim))
-
-    def embedding_sorted_bwd(self, dout, ids, dtable, n_ids, dim, vocab, padding_idx, scale, accumulate, ws):
-        args = (_ptr(dout), _dt(dout), _ptr(ids), _ptr(dtable), _dt(dtable), n_ids, dim, vocab, padding_idx, scale, int(accumulate), _ptr(ws))
-        return self._prep("pf_embedding_sorted_bwd", args, (dout, ids, dtable, ws))

@@ -29,6 +29,7 @@ SOURCES = [
     "pf_elementwise.hip",
     "pf_softmax_loss.hip",
     "pf_token_loss.hip",
+    "pf_rows.hip",
     "pf_head.hip",
     "pf_gated.hip",
     "pf_table.hip",

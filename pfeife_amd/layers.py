@@ -8,7 +8,7 @@ import math
 import torch
 
 from .hip import ACT_GELU, ACT_GELU_TANH, ACT_RELU, ACT_SILU
-from .loss import _LOGITS, _NoContext, _dual, _has_tangent, _issue, _new, _once, _table
+from .loss import _CODE, _LOGITS, _NoContext, _at, _call, _dual, _has_tangent, _need, _once, _table
 
 _ACTS = {"silu": ACT_SILU, "gelu": ACT_GELU, "gelu_tanh": ACT_GELU_TANH, "relu": ACT_RELU}
 _KEPT = {"16bit": 1, "8bit": 2}
@@ -19,8 +19,8 @@ class _EmbeddingFn(torch.autograd.Function):
     def forward(ctx, weight, args, want=True):
         ids, scale, padding = args
         vocab, dim = weight.shape
-        out = _new(weight, *ids.shape, dim, dtype=weight.dtype)
-        _issue(weight, _table(weight, "").embedding_scaled_fwd(weight, ids, out, ids.numel(), dim, vocab, scale))
+        out = torch.empty(ids.shape + (dim,), dtype=weight.dtype, device=weight.device)
+        _call(weight, "pf_embedding_scaled_fwd", weight.data_ptr(), _CODE[weight.dtype], ids.data_ptr(), out.data_ptr(), ids.numel(), dim, vocab, scale)
         if want:
             ctx.save_for_backward(ids)
             ctx.cfg = vocab, scale, padding
@@ -30,11 +30,12 @@ class _EmbeddingFn(torch.autograd.Function):
     def backward(ctx, dout):
         ids, = ctx.saved_tensors
         vocab, scale, padding = ctx.cfg
-        dim = dout.shape[-1]
-        k = _table(dout, "")
-        dw = _new(dout, vocab, dim, dtype=dout.dtype)
-        work = _new(dout, k.embedding_sorted_workspace(ids.numel(), dim), dtype=torch.uint8)
-        _issue(dout, k.embedding_sorted_bwd(dout.contiguous(), ids, dw, ids.numel(), dim, vocab, padding, scale, False, work))
+        dim, n, dtype = dout.shape[-1], ids.numel(), _CODE[dout.dtype]
+        dout = dout.contiguous()
+        dw = torch.empty((vocab, dim), dtype=dout.dtype, device=dout.device)
+        need = _need(dout, "pf_embedding_sorted_workspace", n, dim)
+        work = torch.empty((need,), dtype=torch.uint8, device=dout.device) if need else None
+        _call(dout, "pf_embedding_sorted_bwd", dout.data_ptr(), dtype, ids.data_ptr(), dw.data_ptr(), dtype, n, dim, vocab, padding, scale, 0, _at(work))
         return dw, None
 
 
@@ -74,13 +75,15 @@ class _GatedLinearFn(torch.autograd.Function):
         act, keep = args
         keep = keep if want else 0
         rows, D = x.shape
-        ffn = weight.shape[0] // 2
-        k = _table(x, "")
-        keeps, need = k.gated_linear_bytes(x, weight, rows, D, ffn, keep, False)
-        y = _new(x, rows, ffn, dtype=x.dtype)
-        kept = _new(x, keeps, dtype=torch.uint8) if want else None
-        work = _new(x, need, dtype=torch.uint8) if need else None
-        _issue(x, k.gated_linear_fwd(x, rows, D, weight, ffn, act, keep, y, kept, work))
+        ffn, dtype, dev = weight.shape[0] // 2, _CODE[x.dtype], x.device
+        at, w = x.data_ptr(), weight.data_ptr()
+        kept = None
+        if want:
+            kept = torch.empty((_need(x, "pf_gated_linear_kept", dtype, rows, ffn, keep),), dtype=torch.uint8, device=dev)
+        need = _need(x, "pf_gated_linear_workspace", at, w, dtype, rows, D, ffn, keep, 0)
+        work = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+        y = torch.empty((rows, ffn), dtype=x.dtype, device=dev)
+        _call(x, "pf_gated_linear_fwd", at, dtype, rows, D, w, ffn, act, keep, y.data_ptr(), _at(kept), _at(work))
         if want:
             ctx.save_for_backward(x, weight, kept)
             ctx.cfg = act, keep
@@ -91,13 +94,13 @@ class _GatedLinearFn(torch.autograd.Function):
         x, weight, kept = ctx.saved_tensors
         act, keep = ctx.cfg
         rows, D = x.shape
-        ffn = weight.shape[0] // 2
-        k = _table(x, "")
-        need = k.gated_linear_bytes(x, weight, rows, D, ffn, keep, True)[1]
-        work = _new(x, need, dtype=torch.uint8)
-        dx = _new(x, rows, D, dtype=x.dtype) if ctx.needs_input_grad[0] else None
-        dw = _new(x, 2 * ffn, D, dtype=x.dtype) if ctx.needs_input_grad[1] else None
-        _issue(x, k.gated_linear_bwd(x, rows, D, weight, ffn, act, keep, kept, dy.contiguous(), dx, dw, work))
+        ffn, dtype, dev = weight.shape[0] // 2, _CODE[x.dtype], x.device
+        at, w = x.data_ptr(), weight.data_ptr()
+        work = torch.empty((_need(x, "pf_gated_linear_workspace", at, w, dtype, rows, D, ffn, keep, 1),), dtype=torch.uint8, device=dev)
+        dx = torch.empty((rows, D), dtype=x.dtype, device=dev) if ctx.needs_input_grad[0] else None
+        dw = torch.empty((2 * ffn, D), dtype=x.dtype, device=dev) if ctx.needs_input_grad[1] else None
+        dy = dy.contiguous()
+        _call(x, "pf_gated_linear_bwd", at, dtype, rows, D, w, ffn, act, keep, kept.data_ptr(), dy.data_ptr(), _at(dx), _at(dw), work.data_ptr())
         return dx, dw, None
 
 

@@ -130,6 +130,32 @@ def _issue(t, launch):
             launch(_raw_stream(index))
 
 
+def _call(t, entry, *args):
+    """An entry point of the library at once, on the current stream of the tensor's device."""
+    index = t.get_device()
+    fn = getattr(_tables[index].lib, entry)
+    if _current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc != 0:
+        raise RuntimeError("%s failed: %s" % (entry, _tables[index].lib.pf_last_error().decode()))
+
+
+def _need(t, entry, *args):
+    """Bytes that an entry point asks for."""
+    lib = _tables[t.get_device()].lib
+    need = getattr(lib, entry)(*args)
+    if need < 0:
+        raise RuntimeError(lib.pf_last_error().decode())
+    return need
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
 # the level of forward-mode differentiation, -1 outside of it
 _dual = forward_ad if hasattr(forward_ad, "_current_level") else SimpleNamespace(_current_level=0)
 
@@ -140,6 +166,7 @@ def _has_tangent(*tensors):
 
 
 _LOGITS = (torch.float32, torch.float16, torch.bfloat16)
+_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}      # (PF_F32, PF_F16, PF_BF16)
 
 
 def _check_rows(who, logits, labels, ignore_index, temperature, shift):
@@ -443,13 +470,12 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
     def forward(ctx, hidden, weight, args, want=True):
         labels, shift, ignore_index, z_loss, reduction = args
         B, T, D = hidden.shape
-        V = weight.shape[0]
-        k = _table(hidden, "")
-        sizes = (B, T, D, *hidden.stride()[:2])
-        keeps, need = k.linear_ce_bytes(weight, B * T, D, V, False)
-        kept, work = _new(hidden, keeps, dtype=torch.uint8), _new(hidden, need, dtype=torch.uint8)
-        loss = _new(hidden, B, max(0, T - shift)) if reduction == 0 else _new(hidden)
-        _issue(hidden, k.linear_ce_fwd(hidden, sizes, weight, V, labels, shift, ignore_index, z_loss, reduction, loss, kept, work))
+        V, dtype, dev = weight.shape[0], _CODE[hidden.dtype], hidden.device
+        head = (hidden.data_ptr(), dtype, B, T, D, *hidden.stride()[:2], weight.data_ptr(), V)
+        kept = torch.empty((_need(hidden, "pf_linear_ce_kept", B * T),), dtype=torch.uint8, device=dev)
+        work = torch.empty((_need(hidden, "pf_linear_ce_workspace", head[7], dtype, B * T, D, V, 0),), dtype=torch.uint8, device=dev)
+        loss = torch.empty((B, max(0, T - shift)) if reduction == 0 else (), dtype=torch.float32, device=dev)
+        _call(hidden, "pf_linear_ce_fwd", *head, labels.data_ptr(), shift, ignore_index, z_loss, reduction, loss.data_ptr(), kept.data_ptr(), work.data_ptr())
         if want:
             ctx.save_for_backward(hidden, weight, kept)
             ctx.cfg = z_loss, reduction, _wants_scale(hidden)
@@ -460,25 +486,25 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
         hidden, weight, kept = ctx.saved_tensors
         z_loss, reduction, scaled = ctx.cfg
         B, T, D = hidden.shape
-        V = weight.shape[0]
-        k = _table(hidden, "")
-        work = _new(hidden, k.linear_ce_bytes(weight, B * T, D, V, True)[1], dtype=torch.uint8)
-        dh = _new(hidden, B, T, D, dtype=hidden.dtype) if ctx.needs_input_grad[0] else None
-        dw = _new(hidden, V, D, dtype=weight.dtype) if ctx.needs_input_grad[1] else None
+        V, dtype, dev = weight.shape[0], _CODE[hidden.dtype], hidden.device
+        head = (hidden.data_ptr(), dtype, B, T, D, *hidden.stride()[:2], weight.data_ptr(), V)
+        work = torch.empty((_need(hidden, "pf_linear_ce_workspace", head[7], dtype, B * T, D, V, 1),), dtype=torch.uint8, device=dev)
+        dh = torch.empty((B, T, D), dtype=hidden.dtype, device=dev) if ctx.needs_input_grad[0] else None
+        dw = torch.empty((V, D), dtype=weight.dtype, device=dev) if ctx.needs_input_grad[1] else None
         grad = _as_scale(grad)      # (any strides: a sum's gradient is one number)
         strides = grad.stride() if reduction == 0 else (0, 0)
-        _issue(hidden, k.linear_ce_bwd(hidden, (B, T, D, *hidden.stride()[:2]), weight, V, z_loss, reduction == 1, kept, grad, strides, dh, dw, work))
+        _call(hidden, "pf_linear_ce_bwd", *head, z_loss, int(reduction == 1), kept.data_ptr(), grad.data_ptr(), *strides, _at(dh), _at(dw), work.data_ptr())
         if scaled and dh is not None:
-            dh._pf_times = dh._version, functools.partial(_hidden_times, k, weight, kept, dh, work)
+            dh._pf_times = dh._version, functools.partial(_hidden_times, (head[7], dtype, B * T, D, V), dh, (weight, kept, work))
         return dh, dw, None
 
 
-def _hidden_times(k, weight, kept, like, work, factor, out):
+def _hidden_times(sizes, like, keep, factor, out):
     """The hidden state's gradient times a loss scale, rounded once, from the fp32 sums that the backward pass left; -> is it written."""
     if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or not out.is_contiguous():
         return False
-    B, T, D = like.shape
-    _issue(out, k.linear_ce_hidden_grad(weight, B * T, D, weight.shape[0], kept, factor, out, work))
+    _, kept, work = keep
+    _call(out, "pf_linear_ce_hidden_grad", *sizes, kept.data_ptr(), factor.data_ptr(), out.data_ptr(), work.data_ptr())
     return True
 
 
