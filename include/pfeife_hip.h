@@ -479,6 +479,9 @@ int pf_gated_linear_fwd(const void* x, int dtype, int64_t rows, int64_t D, const
                         void* workspace, void* stream);
 int pf_gated_linear_bwd(const void* x, int dtype, int64_t rows, int64_t D, const void* weight, int64_t ffn, int act, int keep, const void* kept,
                         const void* dy, void* dx, void* dweight, void* workspace, void* stream);
+/* The backward pass's first step alone, for a caller with products of its own: dgu [rows, 2 ffn] = the gradients of both products, side by
+ * side; ffn a multiple of 8, kept and dgu on boundaries of 16 bytes. */
+int pf_gated_linear_split(const void* dy, int dtype, int64_t rows, int64_t ffn, int act, int keep, const void* kept, void* dgu, void* stream);
 /* out = alpha*a + beta*b, each operand with its own dtype (residual add,
  * fan-out gradient sum `g.add_(lg)` of pfeife/mp/worker.py:1543). n elements. */
 int pf_axpby(const void* a, int a_dtype, float alpha, const void* b, int b_dtype, float beta, void* out,

@@ -443,6 +443,40 @@ class OracleKernels:
 
         return launch
 
+    # -- gated projection (what is kept stays with the oracle, as the values it stands for) ----------------------------------------
+    @staticmethod
+    def gated_linear_bytes(x, weight, rows, D, ffn, keep):
+        half = -(-ffn // 16) * 16
+        return (rows * 2 * half * 17 // 16 if keep == 2 else rows * 2 * ffn * x.element_size()), 0
+
+    @staticmethod
+    def _gated_hold(v, keep, dtype):
+        if keep != 2:
+            return v.to(dtype).float()
+        n, width = v.shape
+        b = F.pad(v, (0, -width % 16)).view(n, -1, 16)
+        m, e = torch.frexp(b.abs().amax(-1, keepdim=True) / 448)
+        e = torch.where(m == 0.5, e - 1, e).clamp(-126, 126)
+        return torch.ldexp(torch.ldexp(b, -e).to(torch.float8_e4m3fn).float(), e).view(n, -1)[:, :width]
+
+    def gated_linear_fwd(self, x, rows, D, weight, ffn, act, keep, y, kept, ws):
+        def launch(stream=None):
+            z = _rows(x, rows, D, D).float() @ _rows(weight, 2 * ffn, D, D).float().t()
+            _rows(y, rows, ffn, ffn).copy_((_act(act, z[:, :ffn]) * z[:, ffn:]).to(y.dtype))
+            self._gated[kept.data_ptr()] = torch.cat([self._gated_hold(v, keep, x.dtype) for v in (z[:, :ffn], z[:, ffn:])], 1)
+
+        return launch
+
+    def gated_linear_split(self, dy, rows, ffn, act, keep, kept, dgu):
+        def launch(stream=None):
+            z, d = self._gated[kept.data_ptr()], _rows(dy, rows, ffn, ffn).float()
+            g, u = z[:, :ffn], z[:, ffn:]
+            _rows(dgu, rows, 2 * ffn, 2 * ffn).copy_(torch.cat((d * u * _act_grad(act, g), d * _act(act, g)), 1).to(dgu.dtype))
+
+        return launch
+
+    _gated = {}      # what was kept, by its buffer
+
     def axpby(self, a, alpha, b, beta, out, n):
         def launch(stream=None):
             v = alpha * _flat(a, n).float()
@@ -624,5 +658,29 @@ class OracleKernels:
             if padding_idx >= 0:      # aten::embedding_dense_backward leaves the padding row at zero
                 g = g * (i != padding_idx).unsqueeze(1)
             _rows(dtable, vocab, dim, dim).index_add_(0, i, g)
+
+        return launch
+
+    def embedding_scaled_fwd(self, table, ids, out, n_ids, dim, vocab, scale):
+        def launch(stream=None):
+            t = _rows(table, vocab, dim, dim)
+            _rows(out, n_ids, dim, dim).copy_((t.index_select(0, _flat(ids, n_ids)).float() * scale).to(out.dtype))
+
+        return launch
+
+    @staticmethod
+    def embedding_sorted_workspace(n_ids, dim):
+        return 8
+
+    def embedding_sorted_bwd(self, dout, ids, dtable, n_ids, dim, vocab, padding_idx, scale, accumulate, ws):
+        def launch(stream=None):
+            i = _flat(ids, n_ids)
+            g = _rows(dout, n_ids, dim, dim).float() * scale
+            if padding_idx >= 0:
+                g = g * (i != padding_idx).unsqueeze(1)
+            t = _rows(dtable, vocab, dim, dim)
+            if not accumulate:
+                t.zero_()
+            t.index_add_(0, i, g.to(t.dtype))
 
         return launch

@@ -85,6 +85,17 @@ void backward_launch(const void* dy, const void* kept, const uint8_t* exps, int6
 #undef PF_GB
 }
 
+void split_launch(int dtype, int keep, const void* dy, const void* kept, int64_t half, int64_t rows, int64_t ffn, void* dgu, int64_t wide, int act, hipStream_t st) {
+  const uint8_t* exps = keep == PF_KEEP_8BIT ? (const uint8_t*)kept + rows * 2 * half : nullptr;
+  if (dtype == PF_F16) {
+    if (keep == PF_KEEP_SAME) backward_launch<PF_F16, PF_KEEP_SAME>(dy, kept, exps, half, rows, ffn, dgu, wide, act, st);
+    else backward_launch<PF_F16, PF_KEEP_8BIT>(dy, kept, exps, half, rows, ffn, dgu, wide, act, st);
+  } else {
+    if (keep == PF_KEEP_SAME) backward_launch<PF_BF16, PF_KEEP_SAME>(dy, kept, exps, half, rows, ffn, dgu, wide, act, st);
+    else backward_launch<PF_BF16, PF_KEEP_8BIT>(dy, kept, exps, half, rows, ffn, dgu, wide, act, st);
+  }
+}
+
 // dx from the sums of its shares, [splits][rows][ld] in fp32
 template <int W>
 __global__ __launch_bounds__(256) void gated_join_kernel(const float* acc, int64_t ld, int splits, int64_t rows, int64_t D, void* dx, int dt) {
@@ -106,10 +117,37 @@ __global__ __launch_bounds__(256) void gated_join_kernel(const float* acc, int64
   }
 }
 
+// What a few rows' kernel left in fp32 as it is kept: a thread to 16 columns of one half of a row
+__global__ __launch_bounds__(256) void gated_encode_kernel(const float* gu, int64_t rows, int64_t ffn, int64_t half, uint8_t* codes, uint8_t* exps) {
+  const int64_t per = half / PF_GATED_BLOCK, total = rows * 2 * per;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  const int64_t row = i / (2 * per), block = i % (2 * per), c = block % per * PF_GATED_BLOCK;
+  const float* from = gu + row * 2 * half + block * PF_GATED_BLOCK;
+  float v[PF_GATED_BLOCK], top = 0.f;
+#pragma unroll
+  for (int k = 0; k < PF_GATED_BLOCK; ++k) {
+    v[k] = c + k < ffn ? from[k] : 0.f;
+    top = fmaxf(top, fabsf(v[k]));
+  }
+  const int e = pf_e4m3_exponent(top);
+  const float by = pf_pow2(254 - e);
+  int w[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    w[k] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * k] * by, v[4 * k + 1] * by, 0, false);
+    w[k] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * k + 2] * by, v[4 * k + 3] * by, w[k], true);
+  }
+  *(int4*)(codes + row * 2 * half + block * PF_GATED_BLOCK) = make_int4(w[0], w[1], w[2], w[3]);
+  exps[(row / 4 * 2 * per + block) * 4 + row % 4] = (uint8_t)e;
+}
+
 // A few rows: a wavefront takes a column of y, i.e. one row of either half of the weight, and R rows of x from LDS.  Bound by the
 // weight's way from memory: all of a wavefront's loads are independent, and ffn wavefronts are on their way at once.
+// kept_f32: both products as they are, for the 8-bit codes.
 template <int DT, int R>
-__global__ __launch_bounds__(256) void gated_few_kernel(const void* x, const void* w, int64_t depth, int64_t rows, int64_t ffn, int act, void* y, void* kept, int64_t half) {
+__global__ __launch_bounds__(256) void gated_few_kernel(const void* x, const void* w, int64_t depth, int64_t rows, int64_t ffn, int act, void* y, void* kept, int64_t half,
+                                                        int kept_f32) {
   extern __shared__ __align__(16) char xs[];
   typedef typename Codec<DT>::storage S;
   for (int64_t i = (int64_t)threadIdx.x * 8; i < R * depth; i += 256 * 8) {
@@ -145,7 +183,10 @@ __global__ __launch_bounds__(256) void gated_few_kernel(const void* x, const voi
     if (lane == 0 && r < rows) {
       const float v = act == PF_ACT_RELU && gs != gs ? gs : pf_act(act, gs);
       Codec<DT>::store(y, r * ffn + f, v * us);
-      if (kept != nullptr) {
+      if (kept != nullptr && kept_f32) {
+        ((float*)kept)[r * 2 * half + f] = gs;
+        ((float*)kept)[r * 2 * half + half + f] = us;
+      } else if (kept != nullptr) {
         Codec<DT>::store(kept, r * 2 * half + f, gs);
         Codec<DT>::store(kept, r * 2 * half + half + f, us);
       }
@@ -153,9 +194,9 @@ __global__ __launch_bounds__(256) void gated_few_kernel(const void* x, const voi
   }
 }
 template <int DT, int R>
-int few_launch(const void* x, const void* w, int64_t depth, int64_t rows, int64_t ffn, int act, void* y, void* kept, int64_t half, hipStream_t st) {
+int few_launch(const void* x, const void* w, int64_t depth, int64_t rows, int64_t ffn, int act, void* y, void* kept, int64_t half, int kept_f32, hipStream_t st) {
   const size_t lds = (size_t)(R * depth * pf_dtype_size(DT));
-  hipLaunchKernelGGL((gated_few_kernel<DT, R>), dim3((unsigned)((ffn + 3) / 4)), dim3(256), lds, st, x, w, depth, rows, ffn, act, y, kept, half);
+  hipLaunchKernelGGL((gated_few_kernel<DT, R>), dim3((unsigned)((ffn + 3) / 4)), dim3(256), lds, st, x, w, depth, rows, ffn, act, y, kept, half, kept_f32);
   PF_CHECK_LAUNCH("pf_gated_linear_fwd");
   return PF_OK;
 }
@@ -165,12 +206,12 @@ int few_rows(int64_t rows, int64_t depth, int64_t es) {
   return depth % 8 == 0 && r * depth * es <= 64 * 1024 ? r : 0;
 }
 template <int DT>
-int few(int r, const void* x, const void* w, int64_t depth, int64_t rows, int64_t ffn, int act, void* y, void* kept, int64_t half, hipStream_t st) {
+int few(int r, const void* x, const void* w, int64_t depth, int64_t rows, int64_t ffn, int act, void* y, void* kept, int64_t half, int kept_f32, hipStream_t st) {
   switch (r) {
-    case 1: return few_launch<DT, 1>(x, w, depth, rows, ffn, act, y, kept, half, st);
-    case 2: return few_launch<DT, 2>(x, w, depth, rows, ffn, act, y, kept, half, st);
-    case 4: return few_launch<DT, 4>(x, w, depth, rows, ffn, act, y, kept, half, st);
-    default: return few_launch<DT, 8>(x, w, depth, rows, ffn, act, y, kept, half, st);
+    case 1: return few_launch<DT, 1>(x, w, depth, rows, ffn, act, y, kept, half, kept_f32, st);
+    case 2: return few_launch<DT, 2>(x, w, depth, rows, ffn, act, y, kept, half, kept_f32, st);
+    case 4: return few_launch<DT, 4>(x, w, depth, rows, ffn, act, y, kept, half, kept_f32, st);
+    default: return few_launch<DT, 8>(x, w, depth, rows, ffn, act, y, kept, half, kept_f32, st);
   }
 }
 
@@ -186,7 +227,7 @@ struct Plan {
   int64_t es, depth, wide, half, chunk;
   bool copy_x, copy_w, narrow;
   int splits;                  // of dx's sums (with `parts`)
-  char* x; char* w; char* wt; char* dgu; char* dw; float* parts;
+  char* x; char* w; char* wt; char* dgu; char* dw; float* parts; float* gu;
   int64_t bytes;
 };
 
@@ -270,7 +311,7 @@ bool plan_of(Plan& p, const void* x, const void* w, int dtype, int64_t rows, int
   const int64_t widest = p.depth > 2 * p.half ? p.depth : 2 * p.half;
   p.chunk = ((1ll << 31) / (widest * p.es) - 512) / 256 * 256;
   p.x = p.w = p.wt = p.dgu = p.dw = nullptr;
-  p.parts = nullptr;
+  p.parts = p.gu = nullptr;
   int64_t used = 0;
   auto take = [&](int64_t bytes) {
     char* q = base == nullptr ? nullptr : base + used;
@@ -284,6 +325,8 @@ bool plan_of(Plan& p, const void* x, const void* w, int dtype, int64_t rows, int
     if (!f32) p.wt = take(p.depth * 2 * p.wide * 2);
     if (p.narrow) p.dw = take(2 * ffn * p.depth * 2);
     if (p.splits > 1 || p.narrow) p.parts = (float*)take(p.splits * rows * p.depth * 4);
+  } else if (keep == PF_KEEP_8BIT && few_rows(rows, p.depth, 2) > 0) {
+    p.gu = (float*)take(rows * 2 * p.half * 4);
   } else if (f32 && keep == PF_KEEP_NONE) {
     p.dgu = take(rows * 2 * p.wide * 4);
   }
@@ -320,7 +363,7 @@ extern "C" int pf_gated_linear_fwd(const void* x, int dtype, int64_t rows, int64
   hipStream_t st = (hipStream_t)stream;
   if (dtype == PF_F32) {
     const int r = D % 8 == 0 && !p.copy_x && !p.copy_w ? few_rows(rows, D, 4) : 0;
-    if (r > 0) return few<PF_F32>(r, x, weight, D, rows, ffn, act, y, kept, p.half, st);
+    if (r > 0) return few<PF_F32>(r, x, weight, D, rows, ffn, act, y, kept, p.half, 0, st);
     if (p.copy_x) pf_rows_widen(x, rows, D, p.x, rows, p.depth, 1, 4, st);
     if (p.copy_w) pf_rows_widen(weight, 2 * ffn, D, p.w, 2 * ffn, p.depth, 1, 4, st);
     const float* xs = p.copy_x ? (const float*)p.x : (const float*)x;
@@ -338,11 +381,18 @@ extern "C" int pf_gated_linear_fwd(const void* x, int dtype, int64_t rows, int64
   if (p.copy_x) pf_rows_widen(x, rows, D, p.x, rows, p.depth, 1, 2, st);
   if (p.copy_w) pf_rows_widen(weight, 2 * ffn, D, p.w, 2 * ffn, p.depth, 1, 2, st);
   PF_CHECK_LAUNCH(who);
-  const int r = keep == PF_KEEP_8BIT ? 0 : few_rows(rows, p.depth, 2);
+  const int r = few_rows(rows, p.depth, 2);
   if (r > 0) {
     const void* xs = p.copy_x ? p.x : x;
     const void* ws = p.copy_w ? p.w : weight;
-    return dtype == PF_F16 ? few<PF_F16>(r, xs, ws, p.depth, rows, ffn, act, y, kept, p.half, st) : few<PF_BF16>(r, xs, ws, p.depth, rows, ffn, act, y, kept, p.half, st);
+    const int codes = keep == PF_KEEP_8BIT;
+    void* to = codes ? (void*)p.gu : kept;
+    rc = dtype == PF_F16 ? few<PF_F16>(r, xs, ws, p.depth, rows, ffn, act, y, to, p.half, codes, st) : few<PF_BF16>(r, xs, ws, p.depth, rows, ffn, act, y, to, p.half, codes, st);
+    if (rc != PF_OK || !codes) return rc;
+    hipLaunchKernelGGL(gated_encode_kernel, dim3((unsigned)((rows * 2 * p.half / PF_GATED_BLOCK + 255) / 256)), dim3(256), 0, st, p.gu, rows, ffn, p.half, (uint8_t*)kept,
+                       (uint8_t*)kept + rows * 2 * p.half);
+    PF_CHECK_LAUNCH(who);
+    return PF_OK;
   }
   const int64_t row_k = 2 * p.half * (keep == PF_KEEP_8BIT ? 1 : 2);
   for (int64_t r = 0; r < rows; r += p.chunk) {
@@ -359,6 +409,26 @@ extern "C" int pf_gated_linear_fwd(const void* x, int dtype, int64_t rows, int64
     rc = dtype == PF_F16 ? pf_gated_forward_1(q, st) : pf_gated_forward_2(q, st);
     if (rc != PF_OK) return rc;
   }
+  return PF_OK;
+}
+
+extern "C" int pf_gated_linear_split(const void* dy, int dtype, int64_t rows, int64_t ffn, int act, int keep, const void* kept, void* dgu, void* stream) {
+  const char* who = "pf_gated_linear_split";
+  const int rc = check(who, dtype, rows, 1, ffn, act, keep);
+  if (rc != PF_OK) return rc;
+  PF_REQUIRE(keep != PF_KEEP_NONE, "%s: nothing was kept", who);
+  PF_REQUIRE(ffn % 8 == 0, "%s: a multiple of 8 columns", who);
+  if (rows == 0) return PF_OK;
+  PF_REQUIRE(dy && kept && dgu, "%s: null pointer", who);
+  PF_REQUIRE(pf_aligned(kept, 16) && pf_aligned(dgu, 16), "%s: kept and dgu lie on boundaries of 16 bytes", who);
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == PF_F32) {
+    const float* gu = (const float*)kept;
+    float* d = (float*)dgu;
+    return pf_glu_bwd(dy, ffn, gu, 2 * ffn, gu + ffn, 2 * ffn, d, 2 * ffn, d + ffn, 2 * ffn, PF_F32, act, rows, ffn, stream);
+  }
+  split_launch(dtype, keep, dy, kept, half_of(dtype, ffn, keep), rows, ffn, dgu, ffn, act, st);
+  PF_CHECK_LAUNCH(who);
   return PF_OK;
 }
 
@@ -383,14 +453,7 @@ extern "C" int pf_gated_linear_bwd(const void* x, int dtype, int64_t rows, int64
     rc = pf_glu_bwd(dy, ffn, gu, 2 * p.wide, gu + p.wide, 2 * p.wide, d, 2 * p.wide, d + p.wide, 2 * p.wide, PF_F32, act, rows, ffn, stream);
     if (rc != PF_OK) return rc;
   } else {
-    const uint8_t* exps = keep == PF_KEEP_8BIT ? (const uint8_t*)kept + rows * 2 * p.half : nullptr;
-    if (dtype == PF_F16) {
-      if (keep == PF_KEEP_SAME) backward_launch<PF_F16, PF_KEEP_SAME>(dy, kept, exps, p.half, rows, ffn, p.dgu, p.wide, act, st);
-      else backward_launch<PF_F16, PF_KEEP_8BIT>(dy, kept, exps, p.half, rows, ffn, p.dgu, p.wide, act, st);
-    } else {
-      if (keep == PF_KEEP_SAME) backward_launch<PF_BF16, PF_KEEP_SAME>(dy, kept, exps, p.half, rows, ffn, p.dgu, p.wide, act, st);
-      else backward_launch<PF_BF16, PF_KEEP_8BIT>(dy, kept, exps, p.half, rows, ffn, p.dgu, p.wide, act, st);
-    }
+    split_launch(dtype, keep, dy, kept, p.half, rows, ffn, p.dgu, p.wide, act, st);
   }
   if (p.copy_x && dweight) pf_rows_widen(x, rows, D, p.x, rows, p.depth, 1, es, st);
   PF_CHECK_LAUNCH(who);

@@ -554,7 +554,7 @@ extern "C" int pf_linear_ce_fwd(const void* hidden, int dtype, int64_t B, int64_
   int rc = check_call(c, s, B < 0 || T < 0 || D <= 0 || V <= 0 || sizes_of(c, s));
   if (rc != PF_OK) return rc;
   PF_REQUIRE((shift == 0 || shift == 1) && reduction >= 0 && reduction <= 2, "%s: shift is 0 or 1, reduction 0, 1 or 2", c.who);
-  PF_REQUIRE(loss && kept && workspace && weight && (s.n == 0 || (hidden && labels)), "%s: null pointer", c.who);
+  PF_REQUIRE((loss || (reduction == 0 && B * (T - shift) <= 0)) && kept && workspace && weight && (s.n == 0 || (hidden && labels)), "%s: null pointer", c.who);
   hipStream_t st = (hipStream_t)stream;
   const Kept k = kept_of(kept, s.n_max);
   Carve a = {(char*)workspace};

@@ -27,6 +27,7 @@ import os
 import torch
 import torch.nn.functional as F
 
+from .. import layers
 from .merge import MAX_BYTES, CallRecorder, Merger
 from .values import Val, as_matrix, collapse_for_copy, dense_like, is_dense
 
@@ -2550,6 +2551,85 @@ def lower_embedding(L, node):
     return outv
 
 
+def lower_scaled_embedding(L, node):
+    """`layers.embedding` in a captured graph: as F.embedding, with a factor, and the gradient by sorted tokens."""
+    ids, table, scale, padding_idx = L.arg(node.args[0]), L.arg(node.args[1]), float(node.args[2]), int(node.args[3])
+    if ids.dtype != torch.int64 or not ids.buf.is_contiguous() or not table.buf.is_contiguous():
+        raise Unsupported("embedding expects contiguous int64 ids")
+    vocab, dim = table.shape
+    n = ids.buf.numel()
+    out = L.alloc(tuple(ids.shape) + (dim,), table.dtype)
+    L.emit(L.kernels.embedding_scaled_fwd(table.buf, ids.buf, out, n, dim, vocab, scale))
+    outv = Val(out, req_grad=table.req_grad)
+
+    def bwd(B):
+        g = B.grad_of(outv)
+        if g is None or table.param is None:
+            return
+        gc = g if g.is_contiguous() else _compact(B, g)
+        need = B.k.embedding_sorted_workspace(n, dim)
+        ws = L.pool.scratch("sorted_ids", (need,), torch.uint8) if need else None
+        B.emit(B.k.embedding_sorted_bwd(gc, ids.buf, L.params.grad(table.param), n, dim, vocab, padding_idx, scale, True, ws))
+
+    if table.req_grad:
+        L.add_backward(bwd)
+    return outv
+
+
+def lower_gated_linear(L, node):
+    """`layers.gated_linear` in a captured graph.  What its backward pass starts from is one buffer per micro-batch, with
+    kept="8bit" of half the size; both of its gradient products are a linear layer's, of the joint gradient."""
+    x, w, act, kept = L.arg(node.args[0]), L.arg(node.args[1]), layers.ACTS[node.args[2]], layers.KEPT[node.args[3]]
+    cd, K, N = L.cd, x.shape[-1], w.shape[0]
+    ffn = N // 2
+    if K % 8 or ffn % 8:
+        raise Unsupported("gated_linear of %d -> %d columns: both have to be multiples of 8" % (K, ffn))
+    if cd == torch.float32:
+        kept = layers.KEPT["16bit"]
+    w_cd = L.params.shadow(w.buf, cd) if w.param is not None or not w.req_grad else None
+    if w_cd is None or not w_cd.is_contiguous():
+        raise Unsupported("gated_linear with a weight that is no contiguous parameter")
+    xm = L.matrix_in(x.buf, cd)
+    M, _, lda = as_matrix(xm)
+    if lda != K:
+        xm, wide = L.alloc(x.shape, cd), xm
+        L.copy(wide, xm)
+    w_t = L.params.shadow_t(w.buf, cd) if (x.req_grad and w.param is not None and M >= 256) else None
+    keeps, need = L.kernels.gated_linear_bytes(xm, w_cd, M, K, ffn, kept)
+    y = L.alloc(tuple(x.shape[:-1]) + (ffn,), cd)
+    store = torch.empty(keeps, dtype=torch.uint8, device=L.device)      # (of no shape that lies beside another micro-batch's)
+    L.cur.fwd_bytes += keeps
+    ws = L.pool.scratch("gated_linear", (need,), torch.uint8) if need else None
+    L.emit(L.kernels.gated_linear_fwd(xm, M, K, w_cd, ffn, act, kept, y, store, ws))
+    defer_dw = L.defer_dw and w.req_grad and w.param is not None
+    if defer_dw:
+        L.cur.dw_sigs.add((M * N, cd))
+    outv = Val(y, req_grad=x.req_grad or w.req_grad, name=node.name)
+    x_users = len(node.args[0].users) if isinstance(node.args[0], torch.fx.Node) else 0
+
+    def bwd(B):
+        g = B.grad_of(outv)
+        if g is None:
+            return
+        dy = B.matrix_in(g, cd)
+        dy = dy if dy.is_contiguous() else _compact(B, dy)
+        dgu = B.temp(tuple(x.shape[:-1]) + (N,), cd)
+        B.emit(B.k.gated_linear_split(dy, M, ffn, act, kept, store, dgu))
+        if w.req_grad and w.param is not None:
+            wg = L.params.grad(w.param, (B.program.stage, node.name) if defer_dw else None)
+            if defer_dw:
+                B.program.dw_deferred.append(dict(name=node.name, dy=dgu, x=xm, wg=wg, param=w.param, rows=M, n_out=N, n_in=K, ld_dy=N, ld_x=K))
+            else:
+                B.emit_dw(B.k.gemm(dgu, xm, wg, M=N, N=K, K=M, lda=N, ldb=K, ldc=K, a_trans=1, b_trans=1, beta=1), wg)
+        if x.req_grad:
+            wb, kw = (w_t, dict(ldb=N, b_trans=0)) if w_t is not None else (w_cd, dict(ldb=K, b_trans=1))
+            _input_gradient(B, x, dgu, wb, K, dict(M=M, N=K, K=N, lda=N, **kw), x_users == 1)
+
+    if outv.req_grad:
+        L.add_backward(bwd)
+    return outv
+
+
 def lower_mul(L, node):
     a, b = L.arg(node.args[0]), L.arg(node.args[1])
     if isinstance(a, Val) and isinstance(b, Val):
@@ -2757,6 +2837,7 @@ FUNCTION_HANDLERS = {
     F.pad: lower_pad, torch._C._nn.pad: lower_pad,
     F.cross_entropy: lower_cross_entropy,
     F.embedding: lower_embedding,
+    torch.ops.pfeife_amd.embedding.default: lower_scaled_embedding, torch.ops.pfeife_amd.gated_linear.default: lower_gated_linear,
     operator.add: lower_add, operator.iadd: lower_add, torch.add: lower_add,
     operator.mul: lower_mul, torch.mul: lower_mul,
     operator.getitem: lower_getitem,
@@ -2772,4 +2853,5 @@ METHOD_HANDLERS = {
     "expand": lower_expand, "float": lower_float, "to": lower_to, "add": lower_add, "mul": lower_mul,
 }
 CAST_TO_CD_TARGETS = {F.linear, torch._C._nn.linear, F.conv2d, torch.conv2d,
-                      F.scaled_dot_product_attention, torch._C._nn.scaled_dot_product_attention, torch.matmul}
+                      F.scaled_dot_product_attention, torch._C._nn.scaled_dot_product_attention, torch.matmul,
+                      torch.ops.pfeife_amd.gated_linear.default}

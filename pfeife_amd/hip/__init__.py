@@ -148,6 +148,7 @@ _SIGNATURES = {
     "pf_glu_bwd": [_P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _I, _I, _L, _L, _P],
     "pf_gated_linear_fwd": [_P, _I, _L, _L, _P, _L, _I, _I, _P, _P, _P, _P],
     "pf_gated_linear_bwd": [_P, _I, _L, _L, _P, _L, _I, _I, _P, _P, _P, _P, _P, _P],
+    "pf_gated_linear_split": [_P, _I, _L, _L, _I, _I, _P, _P, _P],
     "pf_axpby": [_P, _I, _F, _P, _I, _F, _P, _I, _L, _P],
     "pf_bias_add": [_P, _I, _P, _I, _P, _I, _L, _L, _L, _P],
     "pf_groupnorm_fwd": [_P, _I, _P, _P, _P, _I, _P, _P, _L, _L, _L, _I, _F, _P],
@@ -724,6 +725,22 @@ class HipKernels:
                 _dt(gate), int(act), rows, cols)
         return self._prep("pf_glu_bwd", args, (dy, gate, up, dgate, dup), 5 * rows * cols * _es(gate))
 
+    def gated_linear_bytes(self, x, weight, rows, D, ffn, keep):
+        """(bytes that the forward pass leaves, bytes of its workspace)"""
+        sizes = (int(self.lib.pf_gated_linear_kept(_dt(x), rows, ffn, keep)),
+                 int(self.lib.pf_gated_linear_workspace(_ptr(x), _ptr(weight), _dt(x), rows, D, ffn, keep, 0)))
+        if min(sizes) < 0:
+            raise RuntimeError(last_error())
+        return sizes
+
+    def gated_linear_fwd(self, x, rows, D, weight, ffn, act, keep, y, kept, ws):
+        args = (_ptr(x), _dt(x), rows, D, _ptr(weight), ffn, act, keep, _ptr(y), _ptr(kept), _ptr(ws))
+        return self._prep("pf_gated_linear_fwd", args, (x, weight, y, kept, ws))
+
+    def gated_linear_split(self, dy, rows, ffn, act, keep, kept, dgu):
+        args = (_ptr(dy), _dt(dy), rows, ffn, act, keep, _ptr(kept), _ptr(dgu))
+        return self._prep("pf_gated_linear_split", args, (dy, kept, dgu))
+
     def axpby(self, a, alpha, b, beta, out, n):
         args = (_ptr(a), _dt(a), alpha, _ptr(b), _dt(b), beta, _ptr(out), _dt(out), n)
         return self._prep("pf_axpby", args, (a, b, out), n * (_es(a) + _es(b) + _es(out)))
@@ -883,3 +900,14 @@ class HipKernels:
     def embedding_bwd(self, dout, ids, dtable, n_ids, dim, vocab, padding_idx=-1):
         args = (_ptr(dout), _dt(dout), _ptr(ids), _ptr(dtable), n_ids, dim, vocab, int(padding_idx))
         return self._prep("pf_embedding_bwd", args, (dout, ids, dtable))
+
+    def embedding_scaled_fwd(self, table, ids, out, n_ids, dim, vocab, scale):
+        args = (_ptr(table), _dt(table), _ptr(ids), _ptr(out), n_ids, dim, vocab, scale)
+        return self._prep("pf_embedding_scaled_fwd", args, (table, ids, out))
+
+    def embedding_sorted_workspace(self, n_ids, dim):
+        return int(self.lib.pf_embedding_sorted_workspace(n_ids, dim))
+
+    def embedding_sorted_bwd(self, dout, ids, dtable, n_ids, dim, vocab, padding_idx, scale, accumulate, ws):
+        args = (_ptr(dout), _dt(dout), _ptr(ids), _ptr(dtable), _dt(dtable), n_ids, dim, vocab, padding_idx, scale, int(accumulate), _ptr(ws))
+        return self._prep("pf_embedding_sorted_bwd", args, (dout, ids, dtable, ws))

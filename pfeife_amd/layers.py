@@ -1,8 +1,9 @@
 """Layers of a decoder as functions: `embedding` (the token table's lookup with a factor, its gradient by sorted tokens) and
 `gated_linear` (both products of a gated feed-forward block, the activation and their product in one kernel).
 
-They are ordinary autograd nodes, for the parts of a model that run beside a runner's stages or without one; the stages' own are
-lowered from the captured graph (`executor/lowering.py`)."""
+They are ordinary autograd nodes, for the parts of a model that run beside a runner's stages or without one.  In a model that is
+compiled for a runner a call is one node of the captured graph (`torch.ops.pfeife_amd`), which the stages' lowering knows
+(`executor/lowering.py`)."""
 import math
 
 import torch
@@ -10,8 +11,8 @@ import torch
 from .hip import ACT_GELU, ACT_GELU_TANH, ACT_RELU, ACT_SILU
 from .loss import _CODE, _LOGITS, _NoContext, _at, _call, _dual, _has_tangent, _need, _once, _table
 
-_ACTS = {"silu": ACT_SILU, "gelu": ACT_GELU, "gelu_tanh": ACT_GELU_TANH, "relu": ACT_RELU}
-_KEPT = {"16bit": 1, "8bit": 2}
+ACTS = {"silu": ACT_SILU, "gelu": ACT_GELU, "gelu_tanh": ACT_GELU_TANH, "relu": ACT_RELU}
+KEPT = {"16bit": 1, "8bit": 2}
 
 
 class _EmbeddingFn(torch.autograd.Function):
@@ -47,26 +48,38 @@ def embedding(ids, weight, *, scale=1.0, padding_idx=None):
     out by the tokens, so a token that fills half of a batch costs no more than others.  There are no second and no forward-mode
     derivatives.  A backward pass is captured into a graph, as any of torch's, only while no autograd graph made outside the capture holds
     the same leaves."""
-    who = "embedding"
+    if torch.compiler.is_compiling():
+        return torch.ops.pfeife_amd.embedding.default(ids, weight, float(scale), _table_row(weight, padding_idx))
     if not torch.is_tensor(ids) or not torch.is_tensor(weight):
-        raise RuntimeError("%s: ids and weight are tensors" % who)
-    _table(weight, who)
-    if weight.dtype not in _LOGITS or weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
-        raise RuntimeError("%s: weight is [rows, width] in fp32, fp16 or bf16 (got %s %s)" % (who, weight.dtype, tuple(weight.shape)))
-    if ids.dtype != torch.int64 or ids.get_device() != weight.get_device():
-        raise RuntimeError("%s: ids are int64 on %s (got %s on %s)" % (who, weight.device, ids.dtype, ids.device))
-    if not isinstance(scale, (int, float)) or not math.isfinite(scale):
-        raise RuntimeError("%s: scale is a finite number" % who)
-    rows = weight.shape[0]
-    if padding_idx is not None and (not isinstance(padding_idx, int) or not -rows <= padding_idx < rows):
-        raise RuntimeError("%s: padding_idx is a row of the table (got %r)" % (who, padding_idx))
+        raise RuntimeError("embedding: ids and weight are tensors")
+    _table(weight, "embedding")
+    padding = _check_embedding(ids, weight, scale, padding_idx)
     if _dual._current_level >= 0 and _has_tangent(weight):
-        raise RuntimeError("%s: there is no forward-mode derivative" % who)
+        raise RuntimeError("embedding: there is no forward-mode derivative")
     weight = weight.contiguous()
-    args = (ids.contiguous(), float(scale), -1 if padding_idx is None else padding_idx % rows)
+    args = (ids.contiguous(), float(scale), padding)
     if torch.is_grad_enabled() and weight.requires_grad:
         return _EmbeddingFn.apply(weight, args)
     return _EmbeddingFn.forward(_NoContext, weight, args, False)
+
+
+def _table_row(weight, padding_idx):
+    """-1: none"""
+    rows = weight.shape[0]
+    if padding_idx is not None and (not isinstance(padding_idx, int) or not -rows <= padding_idx < rows):
+        raise RuntimeError("embedding: padding_idx is a row of the table (got %r)" % (padding_idx,))
+    return -1 if padding_idx is None else padding_idx % rows
+
+
+def _check_embedding(ids, weight, scale, padding_idx):
+    who = "embedding"
+    if weight.dtype not in _LOGITS or weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
+        raise RuntimeError("%s: weight is [rows, width] in fp32, fp16 or bf16 (got %s %s)" % (who, weight.dtype, tuple(weight.shape)))
+    if ids.dtype != torch.int64 or ids.device != weight.device:
+        raise RuntimeError("%s: ids are int64 on %s (got %s on %s)" % (who, weight.device, ids.dtype, ids.device))
+    if not isinstance(scale, (int, float)) or not math.isfinite(scale):
+        raise RuntimeError("%s: scale is a finite number" % who)
+    return _table_row(weight, padding_idx)
 
 
 class _GatedLinearFn(torch.autograd.Function):
@@ -113,27 +126,84 @@ def gated_linear(x, weight, *, act="silu", kept="16bit"):
     of two, in 17/32 of the memory; the result itself is the same.  The gradient flows to x and weight.  There are no second and no
     forward-mode derivatives.  A backward pass is captured into a graph, as any of torch's, only while no autograd graph made outside the
     capture holds the same leaves."""
-    who = "gated_linear"
+    if torch.compiler.is_compiling():
+        return torch.ops.pfeife_amd.gated_linear.default(x, weight, act, kept)
     if not torch.is_tensor(x) or not torch.is_tensor(weight):
-        raise RuntimeError("%s: x and weight are tensors" % who)
-    _table(x, who)
-    if x.dtype not in _LOGITS or weight.dtype != x.dtype:
-        raise RuntimeError("%s: x and weight are both fp32, fp16 or bf16 (got %s and %s)" % (who, x.dtype, weight.dtype))
-    if x.dim() < 1 or x.shape[-1] == 0:
-        raise RuntimeError("%s: x is [..., width] (got %s)" % (who, tuple(x.shape)))
-    if weight.dim() != 2 or weight.shape[1] != x.shape[-1] or weight.shape[0] == 0 or weight.shape[0] % 2 or weight.get_device() != x.get_device():
-        raise RuntimeError("%s: weight is [2 * columns, %d] on %s (got %s on %s)" % (who, x.shape[-1], x.device, tuple(weight.shape), weight.device))
-    if act not in _ACTS:
-        raise RuntimeError("%s: act is one of %s (got %r)" % (who, ", ".join(_ACTS), act))
-    if kept not in _KEPT or (kept == "8bit" and x.dtype == torch.float32):
-        raise RuntimeError("%s: kept is '16bit', or for 16-bit operands '8bit' (got %r for %s)" % (who, kept, x.dtype))
+        raise RuntimeError("gated_linear: x and weight are tensors")
+    _table(x, "gated_linear")
+    _check_gated(x, weight, act, kept)
     if _dual._current_level >= 0 and _has_tangent(x, weight):
-        raise RuntimeError("%s: there is no forward-mode derivative" % who)
+        raise RuntimeError("gated_linear: there is no forward-mode derivative")
+    if x.dtype == torch.float32 and kept == "8bit":
+        raise RuntimeError("gated_linear: kept is '16bit', or for 16-bit operands '8bit' (got %r for %s)" % (kept, x.dtype))
     rows = x.reshape(math.prod(x.shape[:-1]), x.shape[-1]).contiguous()
     weight = weight.contiguous()
-    args = (_ACTS[act], _KEPT[kept])
+    args = (ACTS[act], KEPT[kept])
     if torch.is_grad_enabled() and (rows.requires_grad or weight.requires_grad):
         y = _GatedLinearFn.apply(rows, weight, args)
     else:
         y = _GatedLinearFn.forward(_NoContext, rows, weight, args, False)
     return y.reshape(x.shape[:-1] + y.shape[1:])
+
+
+def _check_gated(x, weight, act, kept):
+    who = "gated_linear"
+    if x.dtype not in _LOGITS or weight.dtype != x.dtype:
+        raise RuntimeError("%s: x and weight are both fp32, fp16 or bf16 (got %s and %s)" % (who, x.dtype, weight.dtype))
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise RuntimeError("%s: x is [..., width] (got %s)" % (who, tuple(x.shape)))
+    if weight.dim() != 2 or weight.shape[1] != x.shape[-1] or weight.shape[0] == 0 or weight.shape[0] % 2 or weight.device != x.device:
+        raise RuntimeError("%s: weight is [2 * columns, %d] on %s (got %s on %s)" % (who, x.shape[-1], x.device, tuple(weight.shape), weight.device))
+    if act not in ACTS:
+        raise RuntimeError("%s: act is one of %s (got %r)" % (who, ", ".join(ACTS), act))
+    if kept not in KEPT:
+        raise RuntimeError("%s: kept is '16bit', or for 16-bit operands '8bit' (got %r for %s)" % (who, kept, x.dtype))
+
+
+# A call inside a graph that is being captured is a node of it.  What its result looks like is all that capturing asks; a runner's stages run the
+# nodes by their lowering, and whatever else runs a captured graph (the compiler's other backends) finds the functions above.
+@torch.library.custom_op("pfeife_amd::embedding", mutates_args=())
+def _embedding_op(ids: torch.Tensor, weight: torch.Tensor, scale: float, padding_idx: int) -> torch.Tensor:
+    return embedding(ids, weight.detach(), scale=scale, padding_idx=None if padding_idx < 0 else padding_idx)
+
+
+@_embedding_op.register_fake
+def _(ids, weight, scale, padding_idx):
+    _check_embedding(ids, weight, scale, None if padding_idx < 0 else padding_idx)
+    return weight.new_empty(tuple(ids.shape) + (weight.shape[1],))
+
+
+@torch.library.custom_op("pfeife_amd::gated_linear", mutates_args=())
+def _gated_linear_op(x: torch.Tensor, weight: torch.Tensor, act: str, kept: str) -> torch.Tensor:
+    return gated_linear(x.detach(), weight.detach(), act=act, kept="16bit")      # (nothing is kept: the backward pass comes here again)
+
+
+@_gated_linear_op.register_fake
+def _(x, weight, act, kept):
+    _check_gated(x, weight, act, kept)
+    return x.new_empty(tuple(x.shape[:-1]) + (weight.shape[0] // 2,))
+
+
+def _save(ctx, inputs, output):
+    ctx.save_for_backward(*inputs[:2])
+    ctx.rest = inputs[2:]
+
+
+def _embedding_backward(ctx, grad):
+    ids, weight = ctx.saved_tensors
+    scale, padding = ctx.rest
+    with torch.enable_grad():
+        w = weight.detach().requires_grad_()
+        out = embedding(ids, w, scale=scale, padding_idx=None if padding < 0 else padding)
+    return None, torch.autograd.grad(out, w, grad)[0], None, None
+
+
+def _gated_linear_backward(ctx, grad):
+    x, weight = (t.detach().requires_grad_() for t in ctx.saved_tensors)
+    with torch.enable_grad():
+        y = gated_linear(x, weight, act=ctx.rest[0], kept=ctx.rest[1])
+    return *torch.autograd.grad(y, (x, weight), grad), None, None
+
+
+_embedding_op.register_autograd(_embedding_backward, setup_context=_save)
+_gated_linear_op.register_autograd(_gated_linear_backward, setup_context=_save)
