@@ -305,6 +305,11 @@ bool plan_of(Plan& p, const void* x, const void* w, int dtype, int64_t rows, int
   p.half = half_of(dtype, ffn, keep);
   p.copy_x = p.depth != D || !pf_aligned(x, 16);
   p.copy_w = p.depth != D || !pf_aligned(w, 16);
+  // whole stages of the fastest tile, where both operands are copied anyway and where many rows pay for the copies (as in pf_head.hip)
+  if (!f32 && rows > 128 && ((p.copy_x && p.copy_w) || rows >= 4096) && p.depth % 64 != 0) {
+    p.depth = round_up(p.depth, 64);
+    p.copy_x = p.copy_w = true;
+  }
   p.narrow = !f32 && D % 8 != 0;
   p.splits = back ? splits_of(dtype, rows, D, p.wide == ffn ? 2 * ffn : ffn) : 1;
   // rows of one launch: everything it addresses by 32-bit offsets stays below 2 GiB
@@ -318,8 +323,10 @@ bool plan_of(Plan& p, const void* x, const void* w, int dtype, int64_t rows, int
     used += round_up(bytes, 256);
     return q;
   };
-  if (p.copy_x) p.x = take(rows * p.depth * p.es);
-  if (p.copy_w) p.w = take(2 * ffn * p.depth * p.es);
+  // (the 16-bit backward pass reads x as the right-hand operand of a reduction over its rows, and of the weight a transposed copy)
+  const bool x_as_is = back && !f32 && D % 8 == 0 && pf_aligned(x, 16);
+  if (p.copy_x && !x_as_is) p.x = take(rows * p.depth * p.es);
+  if (p.copy_w && (!back || f32)) p.w = take(2 * ffn * p.depth * p.es);
   if (back) {
     p.dgu = take(rows * 2 * p.wide * p.es);
     if (!f32) p.wt = take(p.depth * 2 * p.wide * 2);
@@ -455,9 +462,11 @@ extern "C" int pf_gated_linear_bwd(const void* x, int dtype, int64_t rows, int64
   } else {
     split_launch(dtype, keep, dy, kept, p.half, rows, ffn, p.dgu, p.wide, act, st);
   }
-  if (p.copy_x && dweight) pf_rows_widen(x, rows, D, p.x, rows, p.depth, 1, es, st);
+  const bool wide_x = p.x != nullptr && dweight != nullptr;
+  if (wide_x) pf_rows_widen(x, rows, D, p.x, rows, p.depth, 1, es, st);
   PF_CHECK_LAUNCH(who);
-  const char* xs = p.copy_x ? p.x : (const char*)x;
+  const char* xs = wide_x ? p.x : (const char*)x;
+  const int64_t ldx = wide_x ? p.depth : D;
   if (dx) {
     const bool parts = p.parts != nullptr;
     void* c = parts ? (void*)p.parts : dx;
@@ -496,9 +505,9 @@ extern "C" int pf_gated_linear_bwd(const void* x, int dtype, int64_t rows, int64
       const int64_t m = halves == 1 ? 2 * ffn : ffn;
       const char* d = p.dgu + h * p.wide * es;
       char* c = out + h * ffn * ldc * es;
-      if (f32) rc = product(dtype, dtype, 1, 1, m, n, rows, d, 2 * p.wide, xs, p.depth, c, ldc, 0, st);
-      else if (dtype == PF_F16) rc = pf_gated_weight_1(m, n, rows, d, 2 * p.wide, xs, p.depth, c, ldc, st);
-      else rc = pf_gated_weight_2(m, n, rows, d, 2 * p.wide, xs, p.depth, c, ldc, st);
+      if (f32) rc = product(dtype, dtype, 1, 1, m, n, rows, d, 2 * p.wide, xs, ldx, c, ldc, 0, st);
+      else if (dtype == PF_F16) rc = pf_gated_weight_1(m, n, rows, d, 2 * p.wide, xs, ldx, c, ldc, st);
+      else rc = pf_gated_weight_2(m, n, rows, d, 2 * p.wide, xs, ldx, c, ldc, st);
     }
     if (rc != PF_OK) return rc;
     if (p.narrow) pf_rows_narrow(p.dw, p.depth, dweight, 2 * ffn, D, st);

@@ -136,24 +136,26 @@ def gated_linear(x, weight, *, act="silu", kept="16bit"):
         raise RuntimeError("gated_linear: there is no forward-mode derivative")
     if x.dtype == torch.float32 and kept == "8bit":
         raise RuntimeError("gated_linear: kept is '16bit', or for 16-bit operands '8bit' (got %r for %s)" % (kept, x.dtype))
-    rows = x.reshape(math.prod(x.shape[:-1]), x.shape[-1]).contiguous()
+    shape = x.shape
+    rows = (x if len(shape) == 2 else x.reshape(math.prod(shape[:-1]), shape[-1])).contiguous()
     weight = weight.contiguous()
     args = (ACTS[act], KEPT[kept])
     if torch.is_grad_enabled() and (rows.requires_grad or weight.requires_grad):
         y = _GatedLinearFn.apply(rows, weight, args)
     else:
         y = _GatedLinearFn.forward(_NoContext, rows, weight, args, False)
-    return y.reshape(x.shape[:-1] + y.shape[1:])
+    return y if len(shape) == 2 else y.reshape(shape[:-1] + y.shape[1:])
 
 
 def _check_gated(x, weight, act, kept):
     who = "gated_linear"
     if x.dtype not in _LOGITS or weight.dtype != x.dtype:
         raise RuntimeError("%s: x and weight are both fp32, fp16 or bf16 (got %s and %s)" % (who, x.dtype, weight.dtype))
-    if x.dim() < 1 or x.shape[-1] == 0:
-        raise RuntimeError("%s: x is [..., width] (got %s)" % (who, tuple(x.shape)))
-    if weight.dim() != 2 or weight.shape[1] != x.shape[-1] or weight.shape[0] == 0 or weight.shape[0] % 2 or weight.device != x.device:
-        raise RuntimeError("%s: weight is [2 * columns, %d] on %s (got %s on %s)" % (who, x.shape[-1], x.device, tuple(weight.shape), weight.device))
+    shape, of = x.shape, weight.shape
+    if len(shape) < 1 or shape[-1] == 0:
+        raise RuntimeError("%s: x is [..., width] (got %s)" % (who, tuple(shape)))
+    if len(of) != 2 or of[1] != shape[-1] or of[0] == 0 or of[0] % 2 or weight.device != x.device:
+        raise RuntimeError("%s: weight is [2 * columns, %d] on %s (got %s on %s)" % (who, shape[-1], x.device, tuple(of), weight.device))
     if act not in ACTS:
         raise RuntimeError("%s: act is one of %s (got %r)" % (who, ", ".join(ACTS), act))
     if kept not in KEPT:
