@@ -479,8 +479,8 @@ __global__ __launch_bounds__(256) void table_join_kernel(const Sum s, int joins)
     const int64_t block = (int)blockIdx.x - joins, first = block * FEW;
     const int64_t end = (first + FEW - 1) * CHUNK;
     if (first == 0 || end >= s.n) return;
-    const int run = s.keys[end];
-    if (run >= s.vocab || s.keys[first * CHUNK - 1] != run) return;
+    const int run = s.keys[end], before = s.keys[first * CHUNK - 1];
+    if (run >= s.vocab || before != run) return;
     if (left > 0) {
 #pragma unroll
       for (int p = 0; p < FEW / 4; ++p) {
@@ -503,12 +503,13 @@ __global__ __launch_bounds__(256) void table_join_kernel(const Sum s, int joins)
   }
   const int64_t chunk = (int64_t)blockIdx.x * 4 + wave, next = (chunk + 1) * CHUNK;
   if (next >= s.n) return;
-  const int run = s.keys[next - 1];
-  if (run >= s.vocab || s.keys[next] != run) return;
-  if (s.keys[chunk * CHUNK] == run && chunk > 0 && s.keys[chunk * CHUNK - 1] == run) return;      // (it began before)
+  // (all that decides on the way at once)
   const int64_t mine = next + (int64_t)lane * CHUNK;
-  const unsigned long long on = __ballot(mine < s.n && s.keys[mine] == run);
-  if (on == ~0ull || left <= 0) return;                                                           // (of more chunks: below)
+  const int run = s.keys[next - 1], after = s.keys[next], first = s.keys[chunk * CHUNK], before = s.keys[chunk > 0 ? chunk * CHUNK - 1 : 0];
+  const int there = s.keys[mine < s.n ? mine : s.n - 1];
+  if (run >= s.vocab || after != run || (first == run && chunk > 0 && before == run)) return;      // (nothing goes on, or it began before)
+  const unsigned long long on = __ballot(mine < s.n && there == run);
+  if (on == ~0ull || left <= 0) return;                                                            // (of more chunks: below)
   const int many = __ffsll((long long)~on) - 1;      // chunks that begin with the run
   load_row<PF_F32, W>(s.partial + (chunk * 2 + 1) * s.dim, c, left, acc);
 #pragma unroll 4
@@ -543,9 +544,9 @@ __global__ __launch_bounds__(1024) void table_join_long_kernel(const Sum s) {
   const int64_t mark = ((int64_t)blockIdx.x + 1) * FEW;
   const int lane = threadIdx.x & 63, team = threadIdx.x >> 6;
   if (mark >= s.chunks) return;
-  const int run = s.keys[mark * CHUNK];
-  if (run >= s.vocab || s.keys[mark * CHUNK - 1] != run) return;
-  if (mark > FEW && s.keys[(mark - FEW) * CHUNK] == run && s.keys[(mark - FEW) * CHUNK - 1] == run) return;      // (a block before this one's)
+  const int run = s.keys[mark * CHUNK], before = s.keys[mark * CHUNK - 1];
+  const int last = s.keys[(mark - FEW) * CHUNK], last_before = s.keys[mark > FEW ? (mark - FEW) * CHUNK - 1 : 0];
+  if (run >= s.vocab || before != run || (mark > FEW && last == run && last_before == run)) return;      // (or a block before this one's)
   const int64_t first = wave_find(0, mark * CHUNK, [&](int64_t j) { return s.keys[j] >= run; }) / CHUNK;
   const int64_t lo = wave_find(mark + 1, s.chunks, [&](int64_t m) { return s.keys[m * CHUNK] > run; }) - 1;      // the last chunk that begins with it
   if (lo - first < FEW) return;
