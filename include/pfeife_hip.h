@@ -426,7 +426,7 @@ int pf_policy_loss(const void* logits, int dtype, int64_t B, int64_t T, int64_t 
  * over D, no alignment asked for), weight [V, D] of the same type, contiguous; labels, shift and ignore_index as above (a label outside
  * the vocabulary gives NaN).  reduction 0: loss fp32 [B, T - shift], 0 where a token takes no part; 1: loss[0] = the mean over the tokens that
  * take part; 2: their sum (of none: 0).  kept: pf_linear_ce_kept(B * T) bytes, written by the forward pass and read by the backward
- * pass; workspace: pf_linear_ce_workspace bytes, on a boundary of 256 bytes (weight: its address decides whether a copy is needed; a negative status
+ * pass; workspace: pf_linear_ce_workspace bytes; both on boundaries of 256 bytes (weight: its address decides whether a copy is needed; a negative status
  * where the sizes are refused).  hidden and weight hold the same values in both passes.
  *   pf_linear_ce_bwd          dhidden [B, T, D] and dweight [V, D] (either may be null), contiguous, in the operands' type, on boundaries of 16 bytes; grad: of the loss,
  *                             or (reduction 0) of every token's, grad[b * g_sb + t * g_st].  mean != 0: reduction 1

@@ -27,8 +27,8 @@ int pf_gated_weight_2(int64_t M, int64_t N, int64_t K, const void* A, int64_t ld
 
 #ifdef __HIPCC__
 // 1 / (1 + e^-x) by one exponential and one reciprocal of the hardware, each off by a unit in the last place: far below what
-// 16-bit results can hold (the library's exponential and division take four times as long, and the forward product's epilogue is
-// bound by them).  -inf and +inf give 0 and 1.
+// 16-bit results can hold.  (The forward product's epilogue waits for these: 8192 x 2048 x 5632 332 us with the library's exponential and
+// division, 313 with this.)  -inf and +inf give 0 and 1.
 __device__ __forceinline__ float pf_sigmoid_fast(float x) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x)); }
 __device__ __forceinline__ float pf_silu_fast(float x) { return x * pf_sigmoid_fast(x); }
 // 2^e for e + 127 in 1 .. 254

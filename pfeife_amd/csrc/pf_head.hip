@@ -430,7 +430,7 @@ bool sizes_of(const Call& c, Sizes& s) {
   s.depth = c.dtype == PF_F32 ? round_up(c.D, 4) : (c.D < 64 ? 64 : round_up(c.D, 8));
   s.copy_w = s.depth != c.D || !pf_aligned(c.w, 16);
   // Whole stages of the fastest tile: where the weight is copied anyway, and where many tokens pay for a copy.  4662 tokens, 1000 columns, 49999
-  // classes, fp16: the logits' product 446 us on the tile for any multiple of 8, 339 on the other behind 50 us of copy.
+  // classes, fp16: the logits' product 446 us on the tile for any multiple of 8, 336 on the other behind 55 us of copy.
   if (es == 2 && s.n_max > 128 && (s.copy_w || s.n_max >= 3000)) {
     s.depth = round_up(s.depth, 64);
     s.copy_w = s.copy_w || s.depth != c.D;
@@ -566,6 +566,7 @@ extern "C" int pf_linear_ce_fwd(const void* hidden, int dtype, int64_t B, int64_
   int rc = check_call(c, s, B < 0 || T < 0 || D <= 0 || V <= 0 || sizes_of(c, s));
   if (rc != PF_OK) return rc;
   PF_REQUIRE((shift == 0 || shift == 1) && reduction >= 0 && reduction <= 2, "%s: shift is 0 or 1, reduction 0, 1 or 2", c.who);
+  PF_REQUIRE(pf_aligned(kept, 16) && pf_aligned(workspace, 16), "%s: kept and the workspace lie on boundaries of 256 bytes", c.who);
   PF_REQUIRE((loss || (reduction == 0 && B * (T - shift) <= 0)) && kept && workspace && weight && (s.n == 0 || (hidden && labels)), "%s: null pointer", c.who);
   hipStream_t st = (hipStream_t)stream;
   const Kept k = kept_of(kept, s.n_max);
@@ -624,6 +625,7 @@ extern "C" int pf_linear_ce_bwd(const void* hidden, int dtype, int64_t B, int64_
   int rc = check_call(c, s, B < 0 || T < 0 || D <= 0 || V <= 0 || sizes_of(c, s));
   if (rc != PF_OK) return rc;
   PF_REQUIRE(kept && workspace && weight && grad && (s.n == 0 || hidden), "%s: null pointer", c.who);
+  PF_REQUIRE(pf_aligned(kept, 16) && pf_aligned(workspace, 16), "%s: kept and the workspace lie on boundaries of 256 bytes", c.who);
   PF_REQUIRE(dtype == PF_F32 || pf_aligned(dweight, 16), "%s: dweight lies on a boundary of 16 bytes", c.who);
   hipStream_t st = (hipStream_t)stream;
   const Kept k = kept_of((void*)kept, s.n_max);
@@ -694,6 +696,7 @@ extern "C" int pf_linear_ce_hidden_grad(const void* weight, int dtype, int64_t t
   if (rc != PF_OK) return rc;
   if (s.n == 0) return PF_OK;
   PF_REQUIRE(kept && dhidden && workspace, "%s: null pointer", c.who);
+  PF_REQUIRE(pf_aligned(kept, 16) && pf_aligned(workspace, 16), "%s: kept and the workspace lie on boundaries of 256 bytes", c.who);
   hipStream_t st = (hipStream_t)stream;
   const Kept k = kept_of((void*)kept, s.n_max);
   Carve a = {(char*)workspace};

@@ -60,8 +60,8 @@ __device__ __forceinline__ int sum_before(int v, int* sm) {
 }
 
 // Zeros to the whole of the table's gradient, by workgroups that would otherwise wait for the sort: what the sums write later
-// they write over.  (Only the rows that no token names would be fewer bytes, but they are known when the sort is done:
-// 16384 ids, 32000 x 2048, bf16: 28 us of sort and then 63 of sums and zeros against 24 of both at once and then 25.)
+// they write over.  (Only the rows that no token names would be fewer bytes, but they are known when the sort is done.  16384 ids, 32000 x
+// 2048, bf16: ranks and 131 MB of zeros take 20 us together, of which the ranks alone are 12.)
 struct Zero { uint32_t* p; int64_t words, odd; };      // odd: a 16-bit value before / behind them, bits 0 and 1
 __device__ __forceinline__ void zero_part(const Zero& z, int64_t block, int64_t blocks, int threads) {
   typedef uint32_t u4_t __attribute__((ext_vector_type(4), aligned(4)));
@@ -75,7 +75,7 @@ __device__ __forceinline__ void zero_part(const Zero& z, int64_t block, int64_t 
 
 // Up to MANY ids.  First BLOCK neighbours among themselves, by counting: a word's rank is the number of words below it (no two
 // are alike), found by 16 wavefronts that each compare 64 of them with an eighth of a thousand.  2048 compares an id, but spread over
-// the whole chip and without a dependence between them.  The other workgroups write zeros.
+// the whole chip and without a dependence between them (50021 ids: 12 us).  The other workgroups write zeros.
 __global__ __launch_bounds__(1024) void table_rank_kernel(const int64_t* ids, int n, int64_t vocab, int64_t padding, uint32_t* words, int* keys, int* places, int groups,
                                                           const Zero zero) {
   __shared__ __align__(16) uint32_t w[BLOCK];
@@ -114,8 +114,8 @@ __global__ __launch_bounds__(1024) void table_rank_kernel(const int64_t* ids, in
 }
 
 // Then every sorted block's words to their places among all: as many as in each block before are not above it, in each behind below
-// it.  Eight blocks at a time lie in LDS, and a thread's eight searches in them run side by side (in memory a search's twelve steps
-// are twelve round trips: 16384 ids 17 us, 50021 57).
+// it.  Eight blocks at a time lie in LDS, and a thread's eight searches in them run side by side: 16384 ids 5.7 us, 50021 16.  (In
+// memory a search's twelve steps are twelve round trips: 17 us and 57; in LDS with a branch at each step 9.6 and 28.)
 __global__ __launch_bounds__(256) void table_merge_kernel(const uint32_t* words, int n, int* keys, int* places) {
   extern __shared__ __align__(16) uint32_t w[];      // [8][BLOCK]
   const int t = threadIdx.x, i = (int)blockIdx.x * 256 + t;
@@ -290,7 +290,7 @@ template <int DT, int W> __device__ __forceinline__ void store_row(void* p, int6
   else if (left > 0) Codec<DT>::store(p, i, v[0]);
 }
 
-// out[i] = scale * W[ids[i]]; a group of 2^lg lanes takes a row
+// out[i] = scale * W[ids[i]]; a group of 2^lg lanes takes a row.  Bound by memory: 16384 x 2048, bf16: 27 us, 97 MB
 template <int DT, int W>
 __global__ __launch_bounds__(256) void table_lookup_kernel(const void* table, const int64_t* ids, void* out, int64_t n, int64_t dim, int64_t vocab, float scale, int lg) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> lg;
@@ -408,7 +408,8 @@ __global__ __launch_bounds__(256) void table_few_kernel(const Sum s, const int64
 }
 
 // A group of lanes adds up one chunk of the sorted list in one slice of the columns; runs that end inside it go to the table's
-// gradient, the others' parts to `partial`
+// gradient, the others' parts to `partial`.  Bound by memory, and by the places' loads before dout's: 16384 x 2048, bf16: 27 us with dout in
+// the last-level cache, 35 from memory, 82 MB
 template <int DT, int W, int CHUNK>
 __global__ __launch_bounds__(256) void table_sum_kernel(const Sum s) {
   const int G = 1 << s.lg;
@@ -462,7 +463,9 @@ __global__ __launch_bounds__(256) void table_sum_kernel(const Sum s) {
   flush(run == first_after);
 }
 
-// Runs that cross chunks.  FEW neighbours from a multiple of FEW on are a block of chunks.
+// Runs that cross chunks.  FEW neighbours from a multiple of FEW on are a block of chunks.  What is moved is small, each of the two
+// launches waits for a few round trips: 7 us each at 16384 ids; 50021 with one of them half of the list: 17 and 11 (50 without the
+// blocks' sums).
 constexpr int FEW = 64;
 
 // The first `waves` wavefronts of each slice, one to a chunk: a run that begins in it and goes on over less than FEW others, their parts in the
@@ -654,16 +657,22 @@ extern "C" int pf_embedding_scaled_fwd(const void* table, int dtype, const int64
   const int size = pf_dtype_size(dtype);
   const bool wide = dim * size % 4 == 0 && pf_aligned(table, 4) && pf_aligned(out, 4);
   const int lg = lanes_of(dim, wide ? 8 : 1);
-  const dim3 grid((unsigned)(((n_ids << lg) + 255) / 256));
   hipStream_t st = (hipStream_t)stream;
+  constexpr int64_t MOST = 1ll << 25;      // ids of a launch, 2^31 threads at most
+  for (int64_t i0 = 0; i0 < n_ids; i0 += MOST) {
+    const int64_t n = n_ids - i0 < MOST ? n_ids - i0 : MOST;
+    const int64_t* from = ids + i0;
+    void* to = (char*)out + i0 * dim * size;
+    const dim3 grid((unsigned)(((n << lg) + 255) / 256));
 #define PF_TL(DT) \
-  if (wide) hipLaunchKernelGGL((table_lookup_kernel<DT, 8>), grid, dim3(256), 0, st, table, ids, out, n_ids, dim, vocab, (float)scale, lg); \
-  else hipLaunchKernelGGL((table_lookup_kernel<DT, 1>), grid, dim3(256), 0, st, table, ids, out, n_ids, dim, vocab, (float)scale, lg);
-  if (dtype == PF_F32) { PF_TL(PF_F32) }
-  else if (dtype == PF_F16) { PF_TL(PF_F16) }
-  else { PF_TL(PF_BF16) }
+    if (wide) hipLaunchKernelGGL((table_lookup_kernel<DT, 8>), grid, dim3(256), 0, st, table, from, to, n, dim, vocab, (float)scale, lg); \
+    else hipLaunchKernelGGL((table_lookup_kernel<DT, 1>), grid, dim3(256), 0, st, table, from, to, n, dim, vocab, (float)scale, lg);
+    if (dtype == PF_F32) { PF_TL(PF_F32) }
+    else if (dtype == PF_F16) { PF_TL(PF_F16) }
+    else { PF_TL(PF_BF16) }
 #undef PF_TL
-  PF_CHECK_LAUNCH("pf_embedding_scaled_fwd");
+    PF_CHECK_LAUNCH("pf_embedding_scaled_fwd");
+  }
   return PF_OK;
 }
 
@@ -675,7 +684,8 @@ extern "C" int pf_embedding_sorted_bwd(const void* dout, int d_dtype, const int6
   PF_REQUIRE(n_ids >= 0 && dim > 0 && vocab > 0 && pf_is_float_dtype(d_dtype) && (t_dtype == d_dtype || t_dtype == PF_F32), "%s: bad arguments", who);
   PF_REQUIRE(padding_idx >= -1 && padding_idx < vocab, "%s: padding_idx must be -1 (none) or a row", who);
   PF_REQUIRE(dtable && (n_ids <= FEW_IDS || workspace) && (n_ids == 0 || (dout && ids)), "%s: null pointer", who);
-  PF_REQUIRE(n_ids <= (1ll << 27) && vocab < (1ll << 27) - 1 && dim < (1ll << 22), "%s: too many ids, rows or columns", who);
+  PF_REQUIRE(n_ids <= (1ll << 27) && vocab < (1ll << 27) - 1 && dim <= 65535 * 64, "%s: too many ids, rows or columns", who);
+  PF_REQUIRE(pf_aligned(workspace, 16), "%s: the workspace lies on a boundary of 256 bytes", who);
   hipStream_t st = (hipStream_t)stream;
   char* ws = (char*)workspace;
   const Layout l = layout_of(n_ids, dim);

@@ -130,3 +130,22 @@ def test_the_c_entries_refuse_without_a_device():
     for name in ("d", "ids", "out", "ws"):
         rc(grad(**{name: None}), b"null pointer")
     assert lib.pf_embedding_sorted_workspace(0, 8) == 0 and lib.pf_embedding_sorted_workspace(300, 8) > 0
+
+
+def test_the_c_entries_refuse_memory_that_their_wide_accesses_cannot_take():
+    from pfeife_amd import hip
+
+    lib = hip.load()
+    one = 1 << 20      # (an address that nothing reads)
+
+    def rc(call, says):
+        assert call == -1 and says in lib.pf_last_error(), (call, lib.pf_last_error())
+
+    for kept, ws in ((one + 4, one), (one, one + 4)):
+        rc(lib.pf_linear_ce_fwd(one, 2, 2, 3, 64, 192, 64, one, 100, one, 0, -100, 0.0, 1, one, kept, ws, None), b"boundaries")
+        rc(lib.pf_linear_ce_bwd(one, 2, 2, 3, 64, 192, 64, one, 100, 0.0, 1, kept, one, 0, 0, one, one, ws, None), b"boundaries")
+        rc(lib.pf_linear_ce_hidden_grad(one, 2, 6, 64, 100, kept, None, one, ws, None), b"boundaries")
+        rc(lib.pf_gated_linear_fwd(one, 2, 3, 64, one, 32, 3, 1, one, kept, ws, None), b"boundaries")
+        rc(lib.pf_gated_linear_bwd(one, 2, 3, 64, one, 32, 3, 1, kept, one, one, one, ws, None), b"boundaries")
+    rc(lib.pf_embedding_sorted_bwd(one, 2, one, one, 2, 300, 8, 5, -1, 1.0, 0, one + 4, None), b"boundary")
+    rc(lib.pf_embedding_sorted_bwd(one, 2, one, one, 2, 300, 65535 * 64 + 1, 5, -1, 1.0, 0, one, None), b"too many")
