@@ -21,9 +21,10 @@ struct PfGatedProduct {
 };
 int pf_gated_forward_1(const PfGatedProduct& p, hipStream_t st);
 int pf_gated_forward_2(const PfGatedProduct& p, hipStream_t st);
-// C[M][N] (16 bits, contiguous) = A^T B over K rows, A [K][lda], B [K][ldb]
-int pf_gated_weight_1(int64_t M, int64_t N, int64_t K, const void* A, int64_t lda, const void* B, int64_t ldb, void* C, int64_t ldc, hipStream_t st);
-int pf_gated_weight_2(int64_t M, int64_t N, int64_t K, const void* A, int64_t lda, const void* B, int64_t ldb, void* C, int64_t ldc, hipStream_t st);
+// C[M][N] (16 bits) = A^T B over K rows, A [K][lda], B [K][ldb]; batch: so many of them, `step` columns of A apart, their results one behind
+// the other
+int pf_gated_weight_1(int64_t M, int64_t N, int64_t K, const void* A, int64_t lda, const void* B, int64_t ldb, void* C, int64_t ldc, int batch, int64_t step, hipStream_t st);
+int pf_gated_weight_2(int64_t M, int64_t N, int64_t K, const void* A, int64_t lda, const void* B, int64_t ldb, void* C, int64_t ldc, int batch, int64_t step, hipStream_t st);
 
 #ifdef __HIPCC__
 // 1 / (1 + e^-x) by one exponential and one reciprocal of the hardware, each off by a unit in the last place: far below what

@@ -172,7 +172,7 @@ int launch(K kern, int64_t M, int64_t N, int bn, hipStream_t st, const pf_gemm_d
   g.tiles_n = (int)((N + bn - 1) / bn);
   g.per_xcd = (int)(((int64_t)g.tiles_m * g.tiles_n + 7) / 8);
   g.vec_epi = 1;
-  hipLaunchKernelGGL(kern, dim3((unsigned)(g.per_xcd * 8)), dim3(64 * T::WGM * T::WGN), lds, st, d, g, args...);
+  hipLaunchKernelGGL(kern, dim3((unsigned)(g.per_xcd * 8), (unsigned)d.batch2), dim3(64 * T::WGM * T::WGN), lds, st, d, g, args...);
   PF_CHECK_LAUNCH("pf_gated_linear");
   return PF_OK;
 }
@@ -209,17 +209,20 @@ int PF_T_CAT(pf_gated_forward_, PF_X_DT)(const PfGatedProduct& p, hipStream_t st
 }
 
 // A weight gradient in the operands' type.  pf_gemm has straight-line code for fp32 results of such products only (it accumulates
-// them); here the result is a tensor of its own, and 6 bytes an element less to move.
-int PF_T_CAT(pf_gated_weight_, PF_X_DT)(int64_t M, int64_t N, int64_t K, const void* A, int64_t lda, const void* B, int64_t ldb, void* C, int64_t ldc, hipStream_t st) {
+// them); here the result is a tensor of its own, and 6 bytes an element less to move.  Where columns lie between the halves (ffn no multiple of
+// 8) their products are one launch's two batches: 777 x 1000 x 2732, fp16: 33 us, one by one 2 x 19.5.
+int PF_T_CAT(pf_gated_weight_, PF_X_DT)(int64_t M, int64_t N, int64_t K, const void* A, int64_t lda, const void* B, int64_t ldb, void* C, int64_t ldc, int batch, int64_t step,
+                                     hipStream_t st) {
   pf_gemm_desc d = {};
   d.in_dtype = PF_X_DT; d.c_dtype = PF_X_DT;
   d.a_trans = d.b_trans = 1;
   d.M = M; d.N = N; d.K = K;
   d.A = A; d.lda = lda; d.B = B; d.ldb = ldb; d.C = C; d.ldc = ldc;
-  d.batch1 = d.batch2 = 1;
+  d.batch1 = 1; d.batch2 = batch;
+  d.a_stride2 = step; d.c_stride2 = M * ldc;
   d.alpha = 1.f;
   const bool runs = epi_class(d, epi_vec_ok(d)) == EC_STORE16 && (M + 255) / 256 * 256 * ldc * 2 < (1ll << 31);
-  const int64_t rows = runs ? pf_gemm_strided_rows(d) : M;
+  const int64_t rows = runs && batch == 1 ? pf_gemm_strided_rows(d) : M;
   const int best = pf_gemm_best_tile(d);
   if (!runs || (rows == M && best != PF_XT_256x256w4)) return pf_gemm(&d, st);
   d.M = rows;
