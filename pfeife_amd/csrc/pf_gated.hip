@@ -314,7 +314,7 @@ int product(int dtype, int c_dtype, int a_trans, int b_trans, int64_t M, int64_t
 int splits_of(int dtype, int64_t rows, int64_t D, int64_t K) {
   int best = 1;
   double best_t = 0;
-  for (int s = 1; s <= 16 && (s == 1 || K / s >= 256); s *= 2) {
+  for (int s = 1; s <= 16 && (s == 1 || K / s >= 256); ++s) {
     double t = 0;
     if (dtype == PF_F32) {
       const int64_t tiles = ((rows + 63) / 64) * ((D + 63) / 64) * s;      // (17 ns a unit of depth and 64x64 tile)

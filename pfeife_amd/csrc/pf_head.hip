@@ -731,11 +731,10 @@ extern "C" int pf_linear_ce_hidden_grad(const void* weight, int dtype, int64_t t
   const Work w = carve(a, c, s, true);
   const int64_t lanes = D % 8 == 0 && pf_aligned(dhidden, 16) ? 512 : 64, units = (s.n * ((D + lanes - 1) / lanes) + 3) / 4;
   const dim3 grid((unsigned)(units < 16384 ? units : 16384));
-  const int dhidden_splits = s.piece / s.splits >= 64 ? s.splits : 1;
   if (D % 8 == 0 && pf_aligned(dhidden, 16))
-    hipLaunchKernelGGL(head_spread_kernel<8>, grid, dim3(256), 0, st, w.acc, s.depth, dhidden_splits, s.n_max, k.inv, s.n, D, times, dhidden, dtype);
+    hipLaunchKernelGGL(head_spread_kernel<8>, grid, dim3(256), 0, st, w.acc, s.depth, s.splits, s.n_max, k.inv, s.n, D, times, dhidden, dtype);
   else
-    hipLaunchKernelGGL(head_spread_kernel<1>, grid, dim3(256), 0, st, w.acc, s.depth, dhidden_splits, s.n_max, k.inv, s.n, D, times, dhidden, dtype);
+    hipLaunchKernelGGL(head_spread_kernel<1>, grid, dim3(256), 0, st, w.acc, s.depth, s.splits, s.n_max, k.inv, s.n, D, times, dhidden, dtype);
   PF_CHECK_LAUNCH(c.who);
   return PF_OK;
 }

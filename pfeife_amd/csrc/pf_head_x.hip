@@ -179,12 +179,15 @@ __global__ PF_H_BOUNDS void head_logits_kernel(const pf_gemm_desc d, const int* 
   if (!shrink<T::BM, T::BN>(p, g)) return;
   gemm16x_body<PF_X_DT, PF_H_TILE, false, false, EC_OWN, RAG, Tail>(p, g, (int)blockIdx.x, tail);
 }
+// The piece's `rows` in shares of d.K, the last one shorter
 template <int XT, int EC>
-__global__ PF_H_BOUNDS void head_hidden_grad_kernel(const pf_gemm_desc d, const int* count) {
+__global__ PF_H_BOUNDS void head_hidden_grad_kernel(const pf_gemm_desc d, const int* count, int64_t rows) {
   using T = XTile<XT>;
   pf_gemm_desc p = d;
   GemmGrid g;
   p.M = *count;
+  const int64_t left = rows - (int64_t)blockIdx.y * d.K;
+  p.K = left < d.K ? left : d.K;
   g.vec_epi = 1;
   if (p.M == 0 || !shrink<T::BM, T::BN>(p, g)) return;
   gemm16x_body<PF_X_DT, PF_H_TILE, true, true, EC>(p, g, (int)blockIdx.x);
@@ -237,8 +240,8 @@ template <class Tail> int logits_launch(const PfHeadProduct& p, const Tail& tail
 }
 
 template <int XT> int hidden_launch(const pf_gemm_desc& d, const PfHeadProduct& p, hipStream_t st) {
-  return d.beta ? launch<XT>(head_hidden_grad_kernel<XT, EC_ACC32>, d.M, d.N, (int)d.batch2, st, d, p.count)
-                : launch<XT>(head_hidden_grad_kernel<XT, EC_STORE32>, d.M, d.N, (int)d.batch2, st, d, p.count);
+  return d.beta ? launch<XT>(head_hidden_grad_kernel<XT, EC_ACC32>, d.M, d.N, (int)d.batch2, st, d, p.count, p.rows)
+                : launch<XT>(head_hidden_grad_kernel<XT, EC_STORE32>, d.M, d.N, (int)d.batch2, st, d, p.count, p.rows);
 }
 int hidden_grad(const pf_gemm_desc& d, const PfHeadProduct& p, hipStream_t st) {
   switch (pf_gemm_best_tile(d)) {
@@ -266,25 +269,14 @@ int PF_H_CAT(pf_head_dh_, PF_X_DT)(const PfHeadProduct& p, hipStream_t st) {
   pf_gemm_desc d = plain_desc();
   d.c_dtype = PF_F32;
   d.a_trans = d.b_trans = 1;
-  d.M = p.n_max; d.N = p.depth; d.K = p.rows;
+  d.M = p.n_max; d.N = p.depth; d.K = pf_head_share(p.rows, p.splits);
   d.A = p.dz; d.lda = p.n_max; d.B = p.w; d.ldb = p.ldw; d.C = p.dh; d.ldc = p.depth;
   d.beta = p.add;
   d.unscale_by = p.unscale;
-  const int64_t share = p.splits > 1 ? p.rows / p.splits / 64 * 64 : 0;
-  if (share == 0) return hidden_grad(d, p, st);
-  d.K = share;
-  d.batch2 = p.splits;
-  d.a_stride2 = share * d.lda;
-  d.b_stride2 = share * d.ldb;
+  d.batch2 = (p.rows + d.K - 1) / d.K;
+  d.a_stride2 = d.K * d.lda;
+  d.b_stride2 = d.K * d.ldb;
   d.c_stride2 = p.n_max * p.depth;
-  int rc = hidden_grad(d, p, st);
-  const int64_t done = share * p.splits;
-  if (rc != PF_OK || done == p.rows) return rc;
-  d.K = p.rows - done;      // what does not divide goes to the first share
-  d.batch2 = 1;
-  d.A = (const uint16_t*)p.dz + done * d.lda;
-  d.B = (const uint16_t*)p.w + done * d.ldb;
-  d.beta = 1;
   return hidden_grad(d, p, st);
 }
 
@@ -307,7 +299,7 @@ int PF_H_CAT(pf_head_dw_, PF_X_DT)(const PfHeadProduct& p, hipStream_t st) {
 int pf_head_splits(int dtype, int64_t n_max, int64_t depth, int64_t rows) {
   int best = 1;
   double best_t = 0;
-  for (int s = 1; s <= 16 && (s == 1 || rows / s >= 256); s *= 2) {
+  for (int s = 1; s <= 16 && (s == 1 || rows / s >= 256); ++s) {
     double t = 0;
     if (dtype == PF_F32) {
       const int64_t tiles = ((n_max + 63) / 64) * ((depth + 63) / 64) * s;      // (17 ns a unit of depth and 64x64 tile)
@@ -316,13 +308,14 @@ int pf_head_splits(int dtype, int64_t n_max, int64_t depth, int64_t rows) {
       pf_gemm_desc d = plain_desc();
       d.c_dtype = PF_F32;
       d.a_trans = d.b_trans = 1;
-      d.M = n_max; d.N = depth; d.K = rows / s;
-      d.batch2 = s;
+      d.M = n_max; d.N = depth; d.K = pf_head_share(rows, s);
+      d.batch2 = (rows + d.K - 1) / d.K;
       pf_gemm_best_tile(d, &t);
     }
     t += (double)(n_max * depth) * s * 8.0 / 5.0e6;      // the shares' way through memory, written and read at 5 TB/s
     if (s == 1 || t < best_t) { best = s; best_t = t; }
   }
-  return best;
+  const int64_t share = pf_head_share(rows, best);
+  return dtype == PF_F32 ? best : (int)((rows + share - 1) / share);
 }
 #endif
