@@ -50,5 +50,5 @@ int pf_head_dw(int dtype, const PfHeadProduct& p, hipStream_t st);
 inline int64_t pf_head_share(int64_t rows, int splits) { return splits > 1 ? ((rows + splits - 1) / splits + 63) / 64 * 64 : rows; }
 // In how many shares the hidden state's gradient is best summed over `rows` vocabulary rows: few tokens make few tiles, and what a round of
 // 256 of them leaves over is idle.  So many are all used, by a piece of fewer rows no more.  (3163 of 4662 tokens, 1024 columns, 28672 rows, fp16:
-// two shares 286 us.)
+// two shares 282 us, three 208.)
 int pf_head_splits(int dtype, int64_t n_max, int64_t depth, int64_t rows);

@@ -449,7 +449,7 @@ struct Call {
   int64_t V;
 };
 
-bool sizes_of(const Call& c, Sizes& s) {
+bool sizes_of(const Call& c, Sizes& s, bool back) {
   const int64_t es = c.dtype == PF_F32 ? 4 : 2;
   s.n = c.B * c.T;
   s.n_max = round_up(s.n > 0 ? s.n : 1, 64);
@@ -465,8 +465,8 @@ bool sizes_of(const Call& c, Sizes& s) {
   s.narrow = es == 2 && s.dim8 != c.D;
   s.piece = piece_rows(s.n_max, c.V, es);
   if (es == 2 && s.piece > reach_rows(s.depth)) s.piece = reach_rows(s.depth);
-  s.splits = pf_head_splits(c.dtype, s.n_max, s.depth, s.piece);
-  return s.n < (1ll << 24) && c.V < (1ll << 31) && s.n_max * s.depth * 4 * s.splits < (1ll << 31) - 64 && s.piece * s.n_max * es < (1ll << 31) - 64 &&
+  s.splits = back ? pf_head_splits(c.dtype, s.n_max, s.depth, s.piece) : 1;
+  return s.n < (1ll << 24) && c.V < (1ll << 31) && s.n_max * s.depth * 4 < (1ll << 31) - 64 && s.piece * s.n_max * es < (1ll << 31) - 64 &&
          s.depth < (1ll << 19);
 }
 
@@ -577,7 +577,7 @@ extern "C" int64_t pf_linear_ce_kept(int64_t tokens) { return kept_bytes(round_u
 extern "C" int64_t pf_linear_ce_workspace(const void* weight, int dtype, int64_t tokens, int64_t D, int64_t V, int backward) {
   const Call c = {"pf_linear_ce_workspace", nullptr, dtype, 1, tokens, D, 0, D, weight, V};
   Sizes s = {};
-  const int rc = check_call(c, s, tokens < 0 || D <= 0 || V <= 0 || sizes_of(c, s));
+  const int rc = check_call(c, s, tokens < 0 || D <= 0 || V <= 0 || sizes_of(c, s, backward != 0));
   if (rc != PF_OK) return rc;
   Carve a = {nullptr};
   carve(a, c, s, backward != 0);
@@ -589,7 +589,7 @@ extern "C" int pf_linear_ce_fwd(const void* hidden, int dtype, int64_t B, int64_
                                 void* workspace, void* stream) {
   const Call c = {"pf_linear_ce_fwd", hidden, dtype, B, T, D, sb, st_, weight, V};
   Sizes s = {};
-  int rc = check_call(c, s, B < 0 || T < 0 || D <= 0 || V <= 0 || sizes_of(c, s));
+  int rc = check_call(c, s, B < 0 || T < 0 || D <= 0 || V <= 0 || sizes_of(c, s, false));
   if (rc != PF_OK) return rc;
   PF_REQUIRE((shift == 0 || shift == 1) && reduction >= 0 && reduction <= 2, "%s: shift is 0 or 1, reduction 0, 1 or 2", c.who);
   PF_REQUIRE(pf_aligned(kept, 16) && pf_aligned(workspace, 16), "%s: kept and the workspace lie on boundaries of 256 bytes", c.who);
@@ -648,7 +648,7 @@ extern "C" int pf_linear_ce_bwd(const void* hidden, int dtype, int64_t B, int64_
                                 void* workspace, void* stream) {
   const Call c = {"pf_linear_ce_bwd", hidden, dtype, B, T, D, sb, st_, weight, V};
   Sizes s = {};
-  int rc = check_call(c, s, B < 0 || T < 0 || D <= 0 || V <= 0 || sizes_of(c, s));
+  int rc = check_call(c, s, B < 0 || T < 0 || D <= 0 || V <= 0 || sizes_of(c, s, true));
   if (rc != PF_OK) return rc;
   PF_REQUIRE(kept && workspace && weight && grad && (s.n == 0 || hidden), "%s: null pointer", c.who);
   PF_REQUIRE(pf_aligned(kept, 16) && pf_aligned(workspace, 16), "%s: kept and the workspace lie on boundaries of 256 bytes", c.who);
@@ -720,7 +720,7 @@ extern "C" int pf_linear_ce_hidden_grad(const void* weight, int dtype, int64_t t
                                         const void* workspace, void* stream) {
   const Call c = {"pf_linear_ce_hidden_grad", nullptr, dtype, 1, tokens, D, 0, D, weight, V};
   Sizes s = {};
-  const int rc = check_call(c, s, tokens < 0 || D <= 0 || V <= 0 || sizes_of(c, s));
+  const int rc = check_call(c, s, tokens < 0 || D <= 0 || V <= 0 || sizes_of(c, s, true));
   if (rc != PF_OK) return rc;
   if (s.n == 0) return PF_OK;
   PF_REQUIRE(kept && dhidden && workspace, "%s: null pointer", c.who);

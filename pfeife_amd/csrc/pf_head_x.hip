@@ -299,7 +299,7 @@ int PF_H_CAT(pf_head_dw_, PF_X_DT)(const PfHeadProduct& p, hipStream_t st) {
 int pf_head_splits(int dtype, int64_t n_max, int64_t depth, int64_t rows) {
   int best = 1;
   double best_t = 0;
-  for (int s = 1; s <= 16 && (s == 1 || rows / s >= 256); ++s) {
+  for (int s = 1; s <= 16 && (s == 1 || (rows / s >= 256 && n_max * depth * 4 * s < (1ll << 31) - 64)); ++s) {
     double t = 0;
     if (dtype == PF_F32) {
       const int64_t tiles = ((n_max + 63) / 64) * ((depth + 63) / 64) * s;      // (17 ns a unit of depth and 64x64 tile)
