@@ -45,24 +45,20 @@ __device__ __forceinline__ void kept_load(const void* kept, const uint8_t* exps,
 // 79 us, 461 MB at 5.8 TB/s; from 8-bit codes 16384 rows in 128 us, 750 MB
 template <int DT, int KEEP, int ACT>
 __global__ __launch_bounds__(256) void gated_backward_kernel(const void* dy, const void* kept, const uint8_t* exps, int64_t half, int64_t rows, int64_t ffn,
-                                                             void* dgu, int64_t wide, int vec) {
+                                                             void* dgu, int64_t wide) {
   const int64_t per = wide / 8, total = rows * per;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int64_t row = i / per, c = i % per * 8;
     float d[8], g[8], u[8], dg[8], du[8];
-    if (vec) {
-      Vec8<DT>::load(dy, row * ffn + c, d);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) d[k] = c + k < ffn ? Codec<DT>::load(dy, row * ffn + c + k) : 0.f;
-    }
+    const uint4 bits = pf_load_loose((const uint16_t*)dy + row * ffn + c, ffn - c);
+    Vec8<DT>::load(&bits, 0, d);
     kept_load<DT, KEEP, 8>(kept, exps, half, row, c, g);
     kept_load<DT, KEEP, 8>(kept, exps, half, row, half + c, u);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       float value, slope;
       act_and_slope<ACT>(g[k], value, slope);
-      const bool in = vec || c + k < ffn;      // (what is kept past the last column may be anything)
+      const bool in = c + k < ffn;      // (what is kept past the last column may be anything)
       dg[k] = in ? d[k] * u[k] * slope : 0.f;
       du[k] = in ? d[k] * value : 0.f;
     }
@@ -75,8 +71,7 @@ template <int DT, int KEEP>
 void backward_launch(const void* dy, const void* kept, const uint8_t* exps, int64_t half, int64_t rows, int64_t ffn, void* dgu, int64_t wide, int act, hipStream_t st) {
   const int64_t blocks = (rows * (wide / 8) + 255) / 256;
   const dim3 grid((unsigned)(blocks < 16384 ? blocks : 16384));
-  const int vec = ffn % 8 == 0 && pf_aligned(dy, 16);
-#define PF_GB(A) hipLaunchKernelGGL((gated_backward_kernel<DT, KEEP, A>), grid, dim3(256), 0, st, dy, kept, exps, half, rows, ffn, dgu, wide, vec)
+#define PF_GB(A) hipLaunchKernelGGL((gated_backward_kernel<DT, KEEP, A>), grid, dim3(256), 0, st, dy, kept, exps, half, rows, ffn, dgu, wide)
   switch (act) {
     case PF_ACT_SILU: PF_GB(PF_ACT_SILU); break;
     case PF_ACT_GELU: PF_GB(PF_ACT_GELU); break;
@@ -99,7 +94,7 @@ void split_launch(int dtype, int keep, const void* dy, const void* kept, int64_t
 
 // Both halves of the weight transposed, 64 x 64 elements to a workgroup: wt[d][z * wide + f] = w[z * ffn + f][d], zeros for f from ffn to wide
 // (2 x 2732 x 1000: 6.4 us, where a fill and a transpose for each half took 13.6)
-__global__ __launch_bounds__(256) void gated_transpose_kernel(const uint16_t* w, int64_t ffn, int64_t D, uint16_t* wt, int64_t wide, int vec) {
+__global__ __launch_bounds__(256) void gated_transpose_kernel(const uint16_t* w, int64_t ffn, int64_t D, uint16_t* wt, int64_t wide) {
   __shared__ __align__(16) uint16_t tile[64][66];
   const int t = threadIdx.x;
   const int64_t d0 = (int64_t)blockIdx.x * 64, f0 = (int64_t)blockIdx.y * 64, z = blockIdx.z;
@@ -108,16 +103,7 @@ __global__ __launch_bounds__(256) void gated_transpose_kernel(const uint16_t* w,
     const int64_t f = f0 + i, d = d0 + (t & 7) * 8;
     const uint16_t* from = w + (z * ffn + f) * D + d;
     uint4 v = make_uint4(0, 0, 0, 0);
-    if (f < ffn && d < D) {
-      if (vec) {
-        v = *(const uint4*)from;
-      } else {
-        uint32_t e[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) e[k] = d + k < D ? from[k] : 0u;
-        v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
-      }
-    }
+    if (f < ffn && d < D) v = pf_load_loose(from, D - d);
     uint32_t* to = (uint32_t*)&tile[i][(t & 7) * 8];
     to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w;
   }
@@ -409,8 +395,8 @@ extern "C" int pf_gated_linear_fwd(const void* x, int dtype, int64_t rows, int64
   if (dtype == PF_F32) {
     const int r = D % 8 == 0 && !p.copy_x && !p.copy_w ? few_rows(rows, D, 4) : 0;
     if (r > 0) return few<PF_F32>(r, x, weight, D, rows, ffn, act, y, kept, p.half, 0, st);
-    if (p.copy_x) pf_rows_widen(x, rows, D, p.x, rows, p.depth, 1, 4, st);
-    if (p.copy_w) pf_rows_widen(weight, 2 * ffn, D, p.w, 2 * ffn, p.depth, 1, 4, st);
+    if (p.copy_x) pf_rows_widen(x, rows, D, p.x, p.depth, 4, st);
+    if (p.copy_w) pf_rows_widen(weight, 2 * ffn, D, p.w, p.depth, 4, st);
     const float* xs = p.copy_x ? (const float*)p.x : (const float*)x;
     const float* ws = p.copy_w ? (const float*)p.w : (const float*)weight;
     float* gu = keep == PF_KEEP_NONE ? (float*)p.dgu : (float*)kept;
@@ -423,8 +409,8 @@ extern "C" int pf_gated_linear_fwd(const void* x, int dtype, int64_t rows, int64
     if (rc != PF_OK) return rc;
     return pf_glu_fwd(gu, 2 * p.wide, gu + p.wide, 2 * p.wide, y, ffn, PF_F32, act, rows, ffn, stream);
   }
-  if (p.copy_x) pf_rows_widen(x, rows, D, p.x, rows, p.depth, 1, 2, st);
-  if (p.copy_w) pf_rows_widen(weight, 2 * ffn, D, p.w, 2 * ffn, p.depth, 1, 2, st);
+  if (p.copy_x) pf_rows_widen(x, rows, D, p.x, p.depth, 2, st);
+  if (p.copy_w) pf_rows_widen(weight, 2 * ffn, D, p.w, p.depth, 2, st);
   PF_CHECK_LAUNCH(who);
   const int r = few_rows(rows, p.depth, 2);
   if (r > 0) {
@@ -502,7 +488,7 @@ extern "C" int pf_gated_linear_bwd(const void* x, int dtype, int64_t rows, int64
     split_launch(dtype, keep, dy, kept, p.half, rows, ffn, p.dgu, p.wide, act, st);
   }
   const bool wide_x = p.x != nullptr && dweight != nullptr;
-  if (wide_x) pf_rows_widen(x, rows, D, p.x, rows, p.depth, 1, es, st);
+  if (wide_x) pf_rows_widen(x, rows, D, p.x, p.depth, es, st);
   PF_CHECK_LAUNCH(who);
   const char* xs = wide_x ? p.x : (const char*)x;
   const int64_t ldx = wide_x ? p.depth : D;
@@ -512,7 +498,7 @@ extern "C" int pf_gated_linear_bwd(const void* x, int dtype, int64_t rows, int64
     const int64_t ldc = parts ? p.depth : D, n = parts && !f32 ? round_up(D, 8) : D;
     const int c_dtype = parts ? PF_F32 : dtype;
     if (f32) {
-      if (p.copy_w) pf_rows_widen(weight, 2 * ffn, D, p.w, 2 * ffn, p.depth, 1, 4, st);
+      if (p.copy_w) pf_rows_widen(weight, 2 * ffn, D, p.w, p.depth, 4, st);
       const float* ws = p.copy_w ? (const float*)p.w : (const float*)weight;
       const float* d = (const float*)p.dgu;
       for (int h = 0; h < halves && rc == PF_OK; ++h)
@@ -524,7 +510,7 @@ extern "C" int pf_gated_linear_bwd(const void* x, int dtype, int64_t rows, int64
         rc = pf_transpose_cast(weight, dtype, D, p.wt, dtype, 2 * ffn, 2 * ffn, D, stream);
       } else {
         hipLaunchKernelGGL(gated_transpose_kernel, dim3((unsigned)((D + 63) / 64), (unsigned)((p.wide + 63) / 64), 2), dim3(256), 0, st, (const uint16_t*)weight, ffn, D,
-                           (uint16_t*)p.wt, p.wide, D % 8 == 0 && pf_aligned(weight, 16));
+                           (uint16_t*)p.wt, p.wide);
       }
       if (rc == PF_OK) rc = product(dtype, c_dtype, 0, 0, rows, n, 2 * p.wide, p.dgu, 2 * p.wide, p.wt, 2 * p.wide, c, ldc, 0, st, p.splits);
     }

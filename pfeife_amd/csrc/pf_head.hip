@@ -13,8 +13,9 @@
 // dz is rounded to the operands' type before the products, as the logits' gradient of any step in 16 bits is.  It is rounded as a
 // multiple of the largest factor c, which the products multiply by in fp32: the label's entry, 1 - p of it, is what weighs most in
 // both gradients, and is the more exact the less sure the model is (c (1 - p) would take over c's own rounding for all tokens
-// alike: 131072 classes, bf16, relative error of the gradients 2.8e-3 so, 1.7e-3 being the results' own rounding).  fp16: 2^13 times
-// that, which keeps probabilities down to 2^-38.
+// alike: 131072 classes, bf16, relative error of the gradients 2.8e-3 so, 1.9e-3 as it is, 1.7e-3 being the results' own rounding).  Where the
+// tokens' factors differ (a gradient for every token) the rounding of c is there.  fp16: 2^13 times that, which keeps probabilities down
+// to 2^-38.
 // fp32: the same through pf_gemm, with a piece's logits in memory.
 #include "pf_head.h"
 #include "pf_rows.h"
@@ -110,19 +111,20 @@ __device__ __forceinline__ int64_t rows_needed(int n, int64_t n_max, int all) { 
 
 struct Hidden {
   const char* h;
-  int64_t T, sb, st, D, depth;      // in units of the copy
+  int64_t T, sb, st, D, depth;
   char* hc;
   int64_t n_max;
   int all;                          // rows of zeros up to n_max, not just to the next multiple of 64
 };
-// One token's row by one wavefront, or zeros.  U: 16 bytes, or one element where something is not aligned.
+// One token's row by one wavefront, or zeros; U: an element, as bits
 template <typename U>
 __device__ __forceinline__ void gather_row(const Hidden& x, int64_t c, int64_t r) {
-  U* dst = (U*)x.hc + c * x.depth;
-  const U* src = r >= 0 ? (const U*)x.h + (r / x.T) * x.sb + (r % x.T) * x.st : nullptr;
-  const U zero = {};
+  constexpr int N = 16 / sizeof(U);
+  uint4* dst = (uint4*)((U*)x.hc + c * x.depth);
+  const U* src = (const U*)x.h + (r / x.T) * x.sb + (r % x.T) * x.st;
+  const int64_t width = r >= 0 ? x.D : 0;
 #pragma unroll 8
-  for (int64_t i = threadIdx.x & 63; i < x.depth; i += 64) dst[i] = src != nullptr && i < x.D ? src[i] : zero;
+  for (int64_t i = threadIdx.x & 63; i < x.depth / N; i += 64) dst[i] = i * N < width ? pf_load_loose(src + i * N, width - i * N) : make_uint4(0, 0, 0, 0);
 }
 
 // The tokens that take part, one behind the other, zeros behind them and in columns D .. depth - 1
@@ -285,8 +287,7 @@ struct Ready {
   float most;
   int known;               // 0: to be found; 1: there already; 2: all tokens' factors are alike
   int factor, rows, tiles_n;
-  const char* h;           // as elements, for the transpose
-  int64_t sb, st, D, dim8;
+  int64_t dim8;
   uint16_t* ht;
 };
 template <typename U>
@@ -325,45 +326,25 @@ __global__ __launch_bounds__(256) void head_ready_kernel(const Ready q) {
   }
   const int64_t c0 = (int64_t)((block - q.rows) / q.tiles_n) * 64, d0 = (int64_t)((block - q.rows) % q.tiles_n) * 64;
   if (c0 >= padded) return;
-  if constexpr (sizeof(U) == 16) {      // eight elements of a row to a thread, either way
 #pragma unroll
-    for (int i = t >> 3; i < 64; i += 32) {
-      const int64_t c = c0 + i, d = d0 + (t & 7) * 8;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (c < n && d < q.D) {
-        const int64_t r = k.rows[c];
-        v = *(const uint4*)((const uint16_t*)q.h + (r / q.x.T) * q.sb + (r % q.x.T) * q.st + d);
-      }
-      uint32_t* to = (uint32_t*)&tile[i][(t & 7) * 8];
-      to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = t >> 3; i < 64; i += 32) {
-      const int64_t d = d0 + i;
-      uint32_t o[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = (uint32_t)tile[(t & 7) * 8 + 2 * j][i] | (uint32_t)tile[(t & 7) * 8 + 2 * j + 1][i] << 16;
-      if (d < q.dim8) *(uint4*)(q.ht + d * q.x.n_max + c0 + (t & 7) * 8) = make_uint4(o[0], o[1], o[2], o[3]);
-    }
-    return;
-  }
-  const int at = t & 63;
-#pragma unroll 4
-  for (int i = t >> 6; i < 64; i += 4) {
-    const int64_t c = c0 + i, d = d0 + at;
-    uint16_t v = 0;
-    if (c < n && d < q.D) {
+  for (int i = t >> 3; i < 64; i += 32) {      // eight elements of a row to a thread, either way
+    const int64_t c = c0 + i, d = d0 + (t & 7) * 8;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (c < n && d < q.x.D) {
       const int64_t r = k.rows[c];
-      v = ((const uint16_t*)q.h)[(r / q.x.T) * q.sb + (r % q.x.T) * q.st + d];
+      v = pf_load_loose((const uint16_t*)q.x.h + (r / q.x.T) * q.x.sb + (r % q.x.T) * q.x.st + d, q.x.D - d);
     }
-    tile[i][at] = v;
+    uint32_t* to = (uint32_t*)&tile[i][(t & 7) * 8];
+    to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w;
   }
   __syncthreads();
-#pragma unroll 4
-  for (int i = t >> 6; i < 64; i += 4) {
+#pragma unroll
+  for (int i = t >> 3; i < 64; i += 32) {
     const int64_t d = d0 + i;
-    if (d < q.dim8) q.ht[d * q.x.n_max + c0 + at] = tile[at][i];
+    uint32_t o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = (uint32_t)tile[(t & 7) * 8 + 2 * j][i] | (uint32_t)tile[(t & 7) * 8 + 2 * j + 1][i] << 16;
+    if (d < q.dim8) *(uint4*)(q.ht + d * q.x.n_max + c0 + (t & 7) * 8) = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
@@ -456,7 +437,7 @@ bool sizes_of(const Call& c, Sizes& s, bool back) {
   s.depth = c.dtype == PF_F32 ? round_up(c.D, 4) : (c.D < 64 ? 64 : round_up(c.D, 8));
   s.copy_w = s.depth != c.D || !pf_aligned(c.w, 16);
   // Whole stages of the fastest tile: where the weight is copied anyway, and where many tokens pay for a copy.  4662 tokens, 1000 columns, 49999
-  // classes, fp16: the logits' product 446 us on the tile for any multiple of 8, 336 on the other behind 55 us of copy.
+  // classes, fp16: the logits' product 446 us on the tile for any multiple of 8, 336 on the other behind 31 us of copy.
   if (es == 2 && s.n_max > 128 && (s.copy_w || s.n_max >= 3000)) {
     s.depth = round_up(s.depth, 64);
     s.copy_w = s.copy_w || s.depth != c.D;
@@ -515,26 +496,17 @@ int check_call(const Call& c, const Sizes& s, bool ok) {
   return PF_OK;
 }
 
-// the hidden state in units of 16 bytes or of one element
-int unit_of(const Call& c, const Sizes& s) {
-  const int es = c.dtype == PF_F32 ? 4 : 2, per = 16 / es;
-  return pf_aligned(c.h, 16) && c.D % per == 0 && s.depth % per == 0 && c.sb % per == 0 && c.st % per == 0 ? 16 : es;
-}
 Hidden hidden_of(const Call& c, const Sizes& s, const Work& w) {
-  const int64_t per = unit_of(c, s) / (c.dtype == PF_F32 ? 4 : 2);
-  return {(const char*)c.h, c.T > 0 ? c.T : 1, c.sb / per, c.st / per, c.D / per, s.depth / per, w.hc, s.n_max, c.dtype == PF_F32};
+  return {(const char*)c.h, c.T > 0 ? c.T : 1, c.sb, c.st, c.D, s.depth, w.hc, s.n_max, c.dtype == PF_F32};
 }
-#define PF_BY_UNIT(KERNEL, ...)                                                          \
+#define PF_BY_SIZE(KERNEL, ...)                                                          \
   do {                                                                                   \
-    switch (unit_of(c, s)) {                                                             \
-      case 16: hipLaunchKernelGGL(KERNEL<uint4>, __VA_ARGS__); break;                    \
-      case 4: hipLaunchKernelGGL(KERNEL<uint32_t>, __VA_ARGS__); break;                  \
-      default: hipLaunchKernelGGL(KERNEL<uint16_t>, __VA_ARGS__); break;                 \
-    }                                                                                    \
+    if (c.dtype == PF_F32) hipLaunchKernelGGL(KERNEL<uint32_t>, __VA_ARGS__);            \
+    else hipLaunchKernelGGL(KERNEL<uint16_t>, __VA_ARGS__);                              \
   } while (0)
 
 void widen(const Call& c, const Sizes& s, const Work& w, hipStream_t st) {
-  if (s.copy_w) pf_rows_widen(c.w, c.V, c.D, w.wide, c.V, s.depth, 1, c.dtype == PF_F32 ? 4 : 2, st);
+  if (s.copy_w) pf_rows_widen(c.w, c.V, c.D, w.wide, s.depth, c.dtype == PF_F32 ? 4 : 2, st);
 }
 
 // a product over fp32 operands; batch: shares of the depth, `share` of it each, with results of their own
@@ -602,10 +574,10 @@ extern "C" int pf_linear_ce_fwd(const void* hidden, int dtype, int64_t B, int64_
   const Labels y = {labels, s.n, T > 0 ? T : 1, V, ignore_index, s.n_max, shift};
   const Hidden x = hidden_of(c, s, w);
   if (s.n <= 4096) {
-    PF_BY_UNIT(head_index_gather_kernel, dim3((unsigned)(s.n_max / 4)), dim3(256), 0, st, y, x, k, out);
+    PF_BY_SIZE(head_index_gather_kernel, dim3((unsigned)(s.n_max / 4)), dim3(256), 0, st, y, x, k, out);
   } else {
     hipLaunchKernelGGL(head_index_kernel, dim3((unsigned)((s.n + 1023) / 1024)), dim3(1024), 0, st, y, k, out);
-    PF_BY_UNIT(head_gather_kernel, dim3((unsigned)(s.n_max / 4)), dim3(256), 0, st, x, k);
+    PF_BY_SIZE(head_gather_kernel, dim3((unsigned)(s.n_max / 4)), dim3(256), 0, st, x, k);
   }
   widen(c, s, w, st);
   PF_CHECK_LAUNCH(c.who);
@@ -673,11 +645,11 @@ extern "C" int pf_linear_ce_bwd(const void* hidden, int dtype, int64_t B, int64_
   }
   q.factor = (int)((s.n_max + 255) / 256);
   q.rows = (int)(s.n_max / 4);
-  q.h = (const char*)c.h; q.sb = sb; q.st = st_; q.D = D; q.dim8 = s.dim8;
+  q.dim8 = s.dim8;
   q.ht = (uint16_t*)w.ht;
   q.tiles_n = (int)((s.dim8 + 63) / 64);
   const int tiles = half && dweight ? (int)(s.n_max / 64) * q.tiles_n : 0;
-  PF_BY_UNIT(head_ready_kernel, dim3((unsigned)(q.factor + q.rows + tiles)), dim3(256), 0, st, q);
+  PF_BY_SIZE(head_ready_kernel, dim3((unsigned)(q.factor + q.rows + tiles)), dim3(256), 0, st, q);
   widen(c, s, w, st);
   PF_CHECK_LAUNCH(c.who);
   const char* wide = s.copy_w ? w.wide : (const char*)weight;

@@ -239,29 +239,39 @@ __global__ __launch_bounds__(256) void table_place_kernel(const int64_t* ids, co
   }
 }
 
-// Eight neighbouring elements that lie on 4 bytes, `left` of them inside the row
+constexpr int W = 8;      // neighbouring elements of a lane
+
+// `left` of them inside the row, wherever that begins: 16 bytes at a time need no more than the element's own alignment
+// (What is left of a row is converted behind the branch with 16 bits, inside it with 32: the other way about 16384 x 2048 in bf16 are
+// summed in 35 us instead of 29, and 50021 x 769 in fp32 looked up in 57 instead of 47.)
 typedef uint32_t four_t __attribute__((ext_vector_type(4), aligned(4)));
-template <int DT> __device__ __forceinline__ void load8(const void* p, int64_t i, int64_t left, float (&v)[8]) {
-  if (left >= 8) {
-    if constexpr (DT == PF_F32) {
-      const four_t a = *(const four_t*)((const float*)p + i), b = *(const four_t*)((const float*)p + i + 4);
+template <int DT> __device__ __forceinline__ void load8(const void* p, int64_t i, int64_t left, float (&v)[W]) {
+  typedef typename Codec<DT>::storage S;
+  const S* from = (const S*)p + i;
+  if constexpr (DT == PF_F32) {
+    if (left >= W) {
+      const four_t a = *(const four_t*)from, b = *(const four_t*)(from + 4);
 #pragma unroll
       for (int k = 0; k < 4; ++k) { v[k] = __uint_as_float(a[k]); v[4 + k] = __uint_as_float(b[k]); }
     } else {
-      const four_t a = *(const four_t*)((const uint16_t*)p + i);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        v[2 * k] = DT == PF_BF16 ? __uint_as_float(a[k] << 16) : pf_f16_bits_to_f32((uint16_t)(a[k] & 0xffffu));
-        v[2 * k + 1] = DT == PF_BF16 ? __uint_as_float(a[k] & 0xffff0000u) : pf_f16_bits_to_f32((uint16_t)(a[k] >> 16));
-      }
+      for (int k = 0; k < W; ++k) v[k] = k < left ? from[k] : 0.f;
     }
   } else {
+    uint4 a;
+    if (left >= W) {
+      __builtin_memcpy(&a, from, sizeof(a));
+    } else {
+      S e[W];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = k < left ? Codec<DT>::load(p, i + k) : 0.f;
+      for (int k = 0; k < W; ++k) e[k] = k < left ? from[k] : (S)0;
+      __builtin_memcpy(&a, e, sizeof(a));
+    }
+    Vec8<DT>::load(&a, 0, v);
   }
 }
-template <int DT> __device__ __forceinline__ void store8(void* p, int64_t i, int64_t left, const float (&v)[8]) {
-  if (left >= 8) {
+template <int DT> __device__ __forceinline__ void store8(void* p, int64_t i, int64_t left, const float (&v)[W]) {
+  if (left >= W) {
     if constexpr (DT == PF_F32) {
       four_t a, b;
 #pragma unroll
@@ -269,29 +279,19 @@ template <int DT> __device__ __forceinline__ void store8(void* p, int64_t i, int
       *(four_t*)((float*)p + i) = a;
       *(four_t*)((float*)p + i + 4) = b;
     } else {
-      four_t a;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) a[k] = DT == PF_BF16 ? pf_pack2_bf16(v[2 * k], v[2 * k + 1]) : pf_pack2_f16(v[2 * k], v[2 * k + 1]);
-      *(four_t*)((uint16_t*)p + i) = a;
+      uint4 a;
+      Vec8<DT>::store(&a, 0, v);
+      __builtin_memcpy((uint16_t*)p + i, &a, sizeof(a));
     }
   } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
+    for (int k = 0; k < W; ++k)
       if (k < left) Codec<DT>::store(p, i + k, v[k]);
   }
 }
-// W = 8 where rows lie on 4 bytes, else 1
-template <int DT, int W> __device__ __forceinline__ void load_row(const void* p, int64_t i, int64_t left, float (&v)[W]) {
-  if constexpr (W == 8) load8<DT>(p, i, left, v);
-  else v[0] = left > 0 ? Codec<DT>::load(p, i) : 0.f;
-}
-template <int DT, int W> __device__ __forceinline__ void store_row(void* p, int64_t i, int64_t left, const float (&v)[W]) {
-  if constexpr (W == 8) store8<DT>(p, i, left, v);
-  else if (left > 0) Codec<DT>::store(p, i, v[0]);
-}
 
 // out[i] = scale * W[ids[i]]; a group of 2^lg lanes takes a row.  Bound by memory: 16384 x 2048, bf16: 27 us, 97 MB
-template <int DT, int W>
+template <int DT>
 __global__ __launch_bounds__(256) void table_lookup_kernel(const void* table, const int64_t* ids, void* out, int64_t n, int64_t dim, int64_t vocab, float scale, int lg) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> lg;
   if (i >= n) return;
@@ -303,10 +303,10 @@ __global__ __launch_bounds__(256) void table_lookup_kernel(const void* table, co
     float v[W];
 #pragma unroll
     for (int k = 0; k < W; ++k) v[k] = NAN;      // (an id outside the table is visible, never a wild read)
-    if (ok) load_row<DT, W>(table, id * dim + c, dim - c, v);
+    if (ok) load8<DT>(table, id * dim + c, dim - c, v);
 #pragma unroll
     for (int k = 0; k < W; ++k) v[k] *= scale;
-    store_row<DT, W>(out, i * dim + c, dim - c, v);
+    store8<DT>(out, i * dim + c, dim - c, v);
   }
 }
 
@@ -322,26 +322,26 @@ struct Sum {
   int lg, t_f32, accumulate;
 };
 
-template <int DT, int W>
+template <int DT>
 __device__ __forceinline__ void put_row(const Sum& s, int64_t row, int64_t c, float (&v)[W]) {
   const int64_t left = s.dim - c, at = row * s.dim + c;
 #pragma unroll
   for (int k = 0; k < W; ++k) v[k] *= s.scale;
   if (s.accumulate) {
     float old[W];
-    if (s.t_f32) load_row<PF_F32, W>(s.dtable, at, left, old);
-    else load_row<DT, W>(s.dtable, at, left, old);
+    if (s.t_f32) load8<PF_F32>(s.dtable, at, left, old);
+    else load8<DT>(s.dtable, at, left, old);
 #pragma unroll
     for (int k = 0; k < W; ++k) v[k] += old[k];
   }
-  if (s.t_f32) store_row<PF_F32, W>(s.dtable, at, left, v);
-  else store_row<DT, W>(s.dtable, at, left, v);
+  if (s.t_f32) store8<PF_F32>(s.dtable, at, left, v);
+  else store8<DT>(s.dtable, at, left, v);
 }
 
 // Up to FEW_IDS ids, in one launch: a workgroup owns `own` rows of the table's gradient, writes zeros to them, finds the ids that name
 // one of them and adds up, a wavefront to a row, in the list's order.  (The sort takes two launches more; a token that is all of the list is
 // 32 round trips of eight rows here.)
-template <int DT, int W>
+template <int DT>
 __global__ __launch_bounds__(256) void table_few_kernel(const Sum s, const int64_t* ids, int64_t padding, int64_t own) {
   __shared__ int rows[FEW_IDS], at[FEW_IDS];
   __shared__ int before[5];
@@ -354,8 +354,8 @@ __global__ __launch_bounds__(256) void table_few_kernel(const Sum s, const int64
     for (int k = 0; k < W; ++k) zero[k] = 0.f;
     const int64_t end = v1 * s.dim;
     for (int64_t i = v0 * s.dim + (int64_t)t * W; i < end; i += 256 * W) {
-      if (s.t_f32) store_row<PF_F32, W>(s.dtable, i, end - i, zero);
-      else store_row<DT, W>(s.dtable, i, end - i, zero);
+      if (s.t_f32) store8<PF_F32>(s.dtable, i, end - i, zero);
+      else store8<DT>(s.dtable, i, end - i, zero);
     }
   }
   const bool hit = id >= v0 && id < v1 && id != padding;
@@ -394,7 +394,7 @@ __global__ __launch_bounds__(256) void table_few_kernel(const Sum s, const int64
         float v[8][W];
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          if (k < n) load_row<DT, W>(s.dout, (int64_t)place[k] * s.dim + c, s.dim - c, v[k]);
+          if (k < n) load8<DT>(s.dout, (int64_t)place[k] * s.dim + c, s.dim - c, v[k]);
 #pragma unroll
         for (int k = 0; k < 8; ++k)
           if (k < n) {
@@ -402,15 +402,14 @@ __global__ __launch_bounds__(256) void table_few_kernel(const Sum s, const int64
             for (int e = 0; e < W; ++e) acc[e] += v[k][e];
           }
       }
-      put_row<DT, W>(s, v0 + row, c, acc);
+      put_row<DT>(s, v0 + row, c, acc);
     }
   }
 }
 
 // A group of lanes adds up one chunk of the sorted list in one slice of the columns; runs that end inside it go to the table's
-// gradient, the others' parts to `partial`.  Bound by memory, and by the places' loads before dout's: 16384 x 2048, bf16: 27 us with dout in
-// the last-level cache, 35 from memory, 82 MB
-template <int DT, int W, int CHUNK>
+// gradient, the others' parts to `partial`.  Bound by memory, and by the places' loads before dout's: 16384 x 2048, bf16: 29 us, 82 MB
+template <int DT, int CHUNK>
 __global__ __launch_bounds__(256) void table_sum_kernel(const Sum s) {
   const int G = 1 << s.lg;
   const int64_t slices = (s.dim + (int64_t)G * W - 1) / ((int64_t)G * W);
@@ -431,9 +430,9 @@ __global__ __launch_bounds__(256) void table_sum_kernel(const Sum s) {
     if (run < 0 || run >= s.vocab) return;
     if (from_before || goes_on) {
       float* to = s.partial + ((chunk * 2 + (from_before ? 0 : 1)) * s.dim);
-      store_row<PF_F32, W>(to, c, left, acc);
+      store8<PF_F32>(to, c, left, acc);
     } else {
-      put_row<DT, W>(s, run, c, acc);
+      put_row<DT>(s, run, c, acc);
     }
   };
   constexpr int AHEAD = 8;
@@ -444,7 +443,7 @@ __global__ __launch_bounds__(256) void table_sum_kernel(const Sum s) {
     for (int q = 0; q < AHEAD; ++q) {
       const int64_t j = j0 + (b + q < count ? b + q : count - 1);
       key[q] = b + q < count ? s.keys[j] : -1;
-      load_row<DT, W>(s.dout, (int64_t)s.places[j] * s.dim + c, left, v[q]);
+      load8<DT>(s.dout, (int64_t)s.places[j] * s.dim + c, left, v[q]);
     }
 #pragma unroll
     for (int q = 0; q < AHEAD; ++q) {
@@ -470,7 +469,7 @@ constexpr int FEW = 64;
 
 // The first `waves` wavefronts of each slice, one to a chunk: a run that begins in it and goes on over less than FEW others, their parts in the
 // list's order.  The others, four to a block of chunks: where it lies inside one run, its parts' sum.
-template <int DT, int W, int CHUNK>
+template <int DT, int CHUNK>
 __global__ __launch_bounds__(256) void table_join_kernel(const Sum s, int joins) {
   __shared__ float part[4][64 * W];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -488,7 +487,7 @@ __global__ __launch_bounds__(256) void table_join_kernel(const Sum s, int joins)
 #pragma unroll
       for (int p = 0; p < FEW / 4; ++p) {
         float v[W];
-        load_row<PF_F32, W>(s.partial + (first + wave * (FEW / 4) + p) * 2 * s.dim, c, left, v);
+        load8<PF_F32>(s.partial + (first + wave * (FEW / 4) + p) * 2 * s.dim, c, left, v);
 #pragma unroll
         for (int k = 0; k < W; ++k) acc[k] += v[k];
       }
@@ -501,7 +500,7 @@ __global__ __launch_bounds__(256) void table_join_kernel(const Sum s, int joins)
 #pragma unroll
       for (int k = 0; k < W; ++k) acc[k] += part[w][lane * W + k];
     }
-    store_row<PF_F32, W>(s.blocks + block * s.dim, c, left, acc);
+    store8<PF_F32>(s.blocks + block * s.dim, c, left, acc);
     return;
   }
   const int64_t chunk = (int64_t)blockIdx.x * 4 + wave, next = (chunk + 1) * CHUNK;
@@ -514,15 +513,15 @@ __global__ __launch_bounds__(256) void table_join_kernel(const Sum s, int joins)
   const unsigned long long on = __ballot(mine < s.n && there == run);
   if (on == ~0ull || left <= 0) return;                                                            // (of more chunks: below)
   const int many = __ffsll((long long)~on) - 1;      // chunks that begin with the run
-  load_row<PF_F32, W>(s.partial + (chunk * 2 + 1) * s.dim, c, left, acc);
+  load8<PF_F32>(s.partial + (chunk * 2 + 1) * s.dim, c, left, acc);
 #pragma unroll 4
   for (int p = 1; p <= many; ++p) {
     float v[W];
-    load_row<PF_F32, W>(s.partial + (chunk + p) * 2 * s.dim, c, left, v);
+    load8<PF_F32>(s.partial + (chunk + p) * 2 * s.dim, c, left, v);
 #pragma unroll
     for (int k = 0; k < W; ++k) acc[k] += v[k];
   }
-  put_row<DT, W>(s, run, c, acc);
+  put_row<DT>(s, run, c, acc);
 }
 
 // The smallest i in [lo, hi] with f(i), hi if there is none below it, f being false first and then true; a wavefront looks at 64 at a time
@@ -541,7 +540,7 @@ __device__ __forceinline__ int64_t wave_find(int64_t lo, int64_t hi, F f) {
 
 // Longer runs: each holds the first entry of a block of chunks.  The workgroup of the first such block finds the run's ends; its 16
 // wavefronts each add a share of the parts, in the list's order: chunks up to a block, whole blocks, chunks after them.
-template <int DT, int W, int CHUNK>
+template <int DT, int CHUNK>
 __global__ __launch_bounds__(1024) void table_join_long_kernel(const Sum s) {
   __shared__ float part[16][64 * W];
   const int64_t mark = ((int64_t)blockIdx.x + 1) * FEW;
@@ -566,7 +565,7 @@ __global__ __launch_bounds__(1024) void table_join_long_kernel(const Sum s) {
                           : p < head ? s.partial + (first + p) * 2 * s.dim
                           : p < head + blocks ? s.blocks + (mark / FEW + p - head) * s.dim : s.partial + (mark + blocks * FEW + p - head - blocks) * 2 * s.dim;
       float v[W];
-      load_row<PF_F32, W>(from, c, left, v);
+      load8<PF_F32>(from, c, left, v);
 #pragma unroll
       for (int k = 0; k < W; ++k) acc[k] += v[k];
     }
@@ -579,12 +578,12 @@ __global__ __launch_bounds__(1024) void table_join_long_kernel(const Sum s) {
 #pragma unroll
     for (int k = 0; k < W; ++k) acc[k] += part[w][lane * W + k];
   }
-  put_row<DT, W>(s, run, c, acc);
+  put_row<DT>(s, run, c, acc);
 }
 
 inline int64_t round_up(int64_t n, int64_t k) { return (n + k - 1) / k * k; }
-// Neighbours that a group of lanes adds up.  Few make more groups and more parts: 16384 ids, 2048 columns, bf16 27 us with 8, 49 with
-// 32; the parts of longer lists are worth more than their groups.
+// Neighbours that a group of lanes adds up.  Few make more groups and more parts: 16384 ids, 2048 columns, bf16, dout in the last-level cache: 27 us
+// with 8, 49 with 32; the parts of longer lists are worth more than their groups.
 inline int chunk_of(int64_t n) { return n <= MANY ? 8 : 32; }
 inline int items_of(int64_t n) { return n <= 65536 ? 8 : 16; }
 
@@ -601,30 +600,25 @@ Layout layout_of(int64_t n, int64_t dim) {
   return l;
 }
 
-template <int DT, int W, int CHUNK>
+template <int DT, int CHUNK>
 void sum_launch(const Sum& s, hipStream_t st) {
   const int64_t slices = (s.dim + ((int64_t)W << s.lg) - 1) / ((int64_t)W << s.lg);
   const int64_t sums = (s.chunks * slices + (256 >> s.lg) - 1) / (256 >> s.lg);
-  hipLaunchKernelGGL((table_sum_kernel<DT, W, CHUNK>), dim3((unsigned)sums), dim3(256), 0, st, s);
+  hipLaunchKernelGGL((table_sum_kernel<DT, CHUNK>), dim3((unsigned)sums), dim3(256), 0, st, s);
   if (s.chunks < 2) return;
   const unsigned slices64 = (unsigned)((s.dim + 64 * W - 1) / (64 * W));
   const int64_t joins = (s.chunks + 3) / 4, blocks = s.chunks / FEW;
-  hipLaunchKernelGGL((table_join_kernel<DT, W, CHUNK>), dim3((unsigned)(joins + blocks), slices64), dim3(256), 0, st, s, (int)joins);
-  if (blocks > 0) hipLaunchKernelGGL((table_join_long_kernel<DT, W, CHUNK>), dim3((unsigned)blocks, slices64), dim3(1024), 0, st, s);
+  hipLaunchKernelGGL((table_join_kernel<DT, CHUNK>), dim3((unsigned)(joins + blocks), slices64), dim3(256), 0, st, s, (int)joins);
+  if (blocks > 0) hipLaunchKernelGGL((table_join_long_kernel<DT, CHUNK>), dim3((unsigned)blocks, slices64), dim3(1024), 0, st, s);
 }
 template <int DT>
-void sum_dispatch(const Sum& s, bool wide, hipStream_t st) {
-  if (wide) {
-    if (chunk_of(s.n) == 8) sum_launch<DT, 8, 8>(s, st);
-    else sum_launch<DT, 8, 32>(s, st);
-  } else {
-    if (chunk_of(s.n) == 8) sum_launch<DT, 1, 8>(s, st);
-    else sum_launch<DT, 1, 32>(s, st);
-  }
+void sum_dispatch(const Sum& s, hipStream_t st) {
+  if (chunk_of(s.n) == 8) sum_launch<DT, 8>(s, st);
+  else sum_launch<DT, 32>(s, st);
 }
 
 // lanes that share a row: the power of two that covers it with W elements each, 64 at most
-int lanes_of(int64_t dim, int W) {
+int lanes_of(int64_t dim) {
   int lg = 0;
   while (lg < 6 && ((int64_t)W << lg) < dim) ++lg;
   return lg;
@@ -655,8 +649,7 @@ extern "C" int pf_embedding_scaled_fwd(const void* table, int dtype, const int64
   PF_REQUIRE(table && ids && out, "pf_embedding_scaled_fwd: null pointer");
   PF_REQUIRE(n_ids < (1ll << 31), "pf_embedding_scaled_fwd: too many ids");
   const int size = pf_dtype_size(dtype);
-  const bool wide = dim * size % 4 == 0 && pf_aligned(table, 4) && pf_aligned(out, 4);
-  const int lg = lanes_of(dim, wide ? 8 : 1);
+  const int lg = lanes_of(dim);
   hipStream_t st = (hipStream_t)stream;
   constexpr int64_t MOST = 1ll << 25;      // ids of a launch, 2^31 threads at most
   for (int64_t i0 = 0; i0 < n_ids; i0 += MOST) {
@@ -665,11 +658,10 @@ extern "C" int pf_embedding_scaled_fwd(const void* table, int dtype, const int64
     void* to = (char*)out + i0 * dim * size;
     const dim3 grid((unsigned)(((n << lg) + 255) / 256));
 #define PF_TL(DT) \
-    if (wide) hipLaunchKernelGGL((table_lookup_kernel<DT, 8>), grid, dim3(256), 0, st, table, from, to, n, dim, vocab, (float)scale, lg); \
-    else hipLaunchKernelGGL((table_lookup_kernel<DT, 1>), grid, dim3(256), 0, st, table, from, to, n, dim, vocab, (float)scale, lg);
-    if (dtype == PF_F32) { PF_TL(PF_F32) }
-    else if (dtype == PF_F16) { PF_TL(PF_F16) }
-    else { PF_TL(PF_BF16) }
+    hipLaunchKernelGGL(table_lookup_kernel<DT>, grid, dim3(256), 0, st, table, from, to, n, dim, vocab, (float)scale, lg)
+    if (dtype == PF_F32) PF_TL(PF_F32);
+    else if (dtype == PF_F16) PF_TL(PF_F16);
+    else PF_TL(PF_BF16);
 #undef PF_TL
     PF_CHECK_LAUNCH("pf_embedding_scaled_fwd");
   }
@@ -691,19 +683,16 @@ extern "C" int pf_embedding_sorted_bwd(const void* dout, int d_dtype, const int6
   const Layout l = layout_of(n_ids, dim);
   Sum s = {dout, (const int*)(ws + l.keys[0]), (const int*)(ws + l.places[0]), dtable, (float*)(ws + l.partial), (float*)(ws + l.blocks), n_ids, dim, vocab,
            (n_ids + chunk_of(n_ids) - 1) / chunk_of(n_ids), (float)scale, 0, t_dtype == PF_F32, accumulate != 0};
-  const int size = pf_dtype_size(d_dtype);
-  const bool wide = dim * size % 4 == 0 && pf_aligned(dout, 4) && pf_aligned(dtable, 4);
-  s.lg = lanes_of(dim, wide ? 8 : 1);
+  s.lg = lanes_of(dim);
   if (n_ids <= FEW_IDS) {
     int64_t own = 65536 / (dim * pf_dtype_size(t_dtype));
     own = own < 1 ? 1 : own > 1024 ? 1024 : own;
     const dim3 grid((unsigned)((vocab + own - 1) / own));
 #define PF_TF(DT) \
-    if (wide) hipLaunchKernelGGL((table_few_kernel<DT, 8>), grid, dim3(256), 0, st, s, ids, padding_idx, own); \
-    else hipLaunchKernelGGL((table_few_kernel<DT, 1>), grid, dim3(256), 0, st, s, ids, padding_idx, own);
-    if (d_dtype == PF_F32) { PF_TF(PF_F32) }
-    else if (d_dtype == PF_F16) { PF_TF(PF_F16) }
-    else { PF_TF(PF_BF16) }
+    hipLaunchKernelGGL(table_few_kernel<DT>, grid, dim3(256), 0, st, s, ids, padding_idx, own)
+    if (d_dtype == PF_F32) PF_TF(PF_F32);
+    else if (d_dtype == PF_F16) PF_TF(PF_F16);
+    else PF_TF(PF_BF16);
 #undef PF_TF
     PF_CHECK_LAUNCH(who);
     return PF_OK;
@@ -739,9 +728,9 @@ extern "C" int pf_embedding_sorted_bwd(const void* dout, int d_dtype, const int6
     sort_large<16>(ids, n_ids, vocab, padding_idx, bits, digits, ws, l, zero, (int)zero_blocks, st);
   }
   PF_CHECK_LAUNCH(who);
-  if (d_dtype == PF_F32) sum_dispatch<PF_F32>(s, wide, st);
-  else if (d_dtype == PF_F16) sum_dispatch<PF_F16>(s, wide, st);
-  else sum_dispatch<PF_BF16>(s, wide, st);
+  if (d_dtype == PF_F32) sum_dispatch<PF_F32>(s, st);
+  else if (d_dtype == PF_F16) sum_dispatch<PF_F16>(s, st);
+  else sum_dispatch<PF_BF16>(s, st);
   PF_CHECK_LAUNCH(who);
   return PF_OK;
 }
