@@ -302,16 +302,15 @@ int splits_of(int dtype, int64_t rows, int64_t D, int64_t K) {
   double best_t = 0;
   for (int s = 1; s <= 16 && (s == 1 || K / s >= 256); ++s) {
     double t = 0;
+    pf_gemm_desc d = {};
+    d.in_dtype = dtype;
+    d.c_dtype = PF_F32;
+    d.M = rows; d.N = D; d.K = K / s / 64 * 64 > 0 ? K / s / 64 * 64 : K;
+    d.batch1 = 1;
+    d.batch2 = s;
     if (dtype == PF_F32) {
-      const int64_t tiles = ((rows + 63) / 64) * ((D + 63) / 64) * s;      // (17 ns a unit of depth and 64x64 tile)
-      t = (double)((tiles + 255) / 256) * 0.0171 * (double)(K / s);
+      t = pf_gemm_f32_depth_us(d);
     } else {
-      pf_gemm_desc d = {};
-      d.in_dtype = dtype;
-      d.c_dtype = PF_F32;
-      d.M = rows; d.N = D; d.K = K / s / 64 * 64 > 0 ? K / s / 64 * 64 : K;
-      d.batch1 = 1;
-      d.batch2 = s;
       pf_gemm_best_tile(d, &t);
     }
     if (s > 1) t += 4.0 + (double)(rows * D) * s * 8.0 / 5.0e6;      // a launch, and the shares' way through memory at 5 TB/s

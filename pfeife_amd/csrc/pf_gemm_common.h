@@ -280,5 +280,8 @@ int64_t pf_gemm_strided_rows(const pf_gemm_desc& d);
 
 // pf_gemm_f32.hip: fp32 products straight from 16-byte-aligned operands
 bool pf_gemm_f32_direct_ok(const pf_gemm_desc& d);
+// pf_gemm_f32_depth.hip: such a product with a dimension that only the device knows (see gemm32k_counted_kernel), and what one without takes
+int pf_gemm_f32_counted(const pf_gemm_desc& d, const int* count, int64_t depth, hipStream_t st);
+double pf_gemm_f32_depth_us(const pf_gemm_desc& d);
 void pf_gemm_f32_direct_name(const pf_gemm_desc& d, char* out, size_t cap);   // the kernel, as the profiler prints it
 int pf_gemm_f32_direct(const pf_gemm_desc& d, hipStream_t st);

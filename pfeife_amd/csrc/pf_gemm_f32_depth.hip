@@ -84,7 +84,7 @@ template <int T, bool TRANS> struct FTile {
 };
 
 template <int TM, int TN, int ST, bool AT, bool BT>
-__global__ __launch_bounds__(64 * FNW) __attribute__((amdgpu_waves_per_eu(TM * TN >= 9 ? 2 : 4, TM * TN >= 9 ? 2 : 4))) void gemm32k_kernel(const pf_gemm_desc p, const GemmGrid g) {
+__device__ __forceinline__ void gemm32k_body(const pf_gemm_desc& p, const GemmGrid& g) {
   constexpr int BM = 16 * TM, BN = 16 * TN, NB = TM * TN;
   using TA = FTile<TM, AT>;
   using TB = FTile<TN, BT>;
@@ -222,20 +222,46 @@ __global__ __launch_bounds__(64 * FNW) __attribute__((amdgpu_waves_per_eu(TM * T
   epilogue_f32<BM>(p, g, v, m0, 4 * (lane >> 4) + wave, n0 + (lane & 15), c_base);
 }
 
+#define PF_FK_BOUNDS __launch_bounds__(64 * FNW) __attribute__((amdgpu_waves_per_eu(TM * TN >= 9 ? 2 : 4, TM * TN >= 9 ? 2 : 4)))
 template <int TM, int TN, int ST, bool AT, bool BT>
-int launch_one(const pf_gemm_desc& d, const GemmGrid& g, dim3 grid, hipStream_t st) {
+__global__ PF_FK_BOUNDS void gemm32k_kernel(const pf_gemm_desc p, const GemmGrid g) {
+  gemm32k_body<TM, TN, ST, AT, BT>(p, g);
+}
+// One dimension's length in device memory, at most what the descriptor says, which the grid covers: the columns of C where both operands
+// are stored along the reduction, its rows where neither is (`depth` then comes in shares of p.K, the last one shorter), else the depth
+template <int TM, int TN, int ST, bool AT, bool BT>
+__global__ PF_FK_BOUNDS void gemm32k_counted_kernel(const pf_gemm_desc d, const GemmGrid grid, const int* count, int64_t depth) {
+  pf_gemm_desc p = d;
+  GemmGrid g = grid;
+  const int n = *count;
+  if constexpr (!AT && !BT) {
+    p.N = n;
+  } else if constexpr (AT && BT) {
+    const int64_t left = depth - (int64_t)blockIdx.y * d.K;
+    p.M = n;
+    p.K = left < d.K ? left : d.K;
+  } else {
+    p.K = n;
+  }
+  g.tiles_m = (int)((p.M + 16 * TM - 1) / (16 * TM));
+  g.tiles_n = (int)((p.N + 16 * TN - 1) / (16 * TN));
+  g.per_xcd = (g.tiles_m * g.tiles_n + 7) / 8;
+  if ((int)(blockIdx.x >> 3) < g.per_xcd) gemm32k_body<TM, TN, ST, AT, BT>(p, g);
+}
+
+template <int TM, int TN, int ST, class K, class... A>
+int launch_one(K kern, const GemmGrid& g, dim3 grid, hipStream_t st, const pf_gemm_desc& d, const A&... more) {
   constexpr size_t lds = (size_t)ST * (TM + TN) * 16 * FK * 4;
   static_assert(lds >= (size_t)(FNW - 1) * TM * TN * 1024 && lds <= 160 * 1024, "the wavefronts' sums meet where the operands were");
-  auto kern = gemm32k_kernel<TM, TN, ST, AT, BT>;
   const int rc = pf_allow_lds((const void*)kern, lds, "pf_gemm(f32)");
   if (rc != PF_OK) return rc;
-  hipLaunchKernelGGL(kern, grid, dim3(64 * FNW), lds, st, d, g);
+  hipLaunchKernelGGL(kern, grid, dim3(64 * FNW), lds, st, d, g, more...);
   PF_CHECK_LAUNCH("pf_gemm(f32)");
   return PF_OK;
 }
 
 template <int TM, int TN, int ST>
-int launch(const pf_gemm_desc& d, hipStream_t st) {
+int launch(const pf_gemm_desc& d, const int* count, int64_t depth, hipStream_t st) {
   constexpr int BM = 16 * TM, BN = 16 * TN;
   GemmGrid g;
   g.tiles_m = (int)((d.M + BM - 1) / BM);
@@ -243,10 +269,15 @@ int launch(const pf_gemm_desc& d, hipStream_t st) {
   g.per_xcd = (int)(((int64_t)g.tiles_m * g.tiles_n + 7) / 8);
   g.vec_epi = epi_f32_vec_ok(d, BM);
   const dim3 grid((unsigned)(g.per_xcd * 8), (unsigned)(d.batch1 * d.batch2), 1);
-  if (d.a_trans && d.b_trans) return launch_one<TM, TN, ST, true, true>(d, g, grid, st);
-  if (d.a_trans) return launch_one<TM, TN, ST, true, false>(d, g, grid, st);
-  if (d.b_trans) return launch_one<TM, TN, ST, false, true>(d, g, grid, st);
-  return launch_one<TM, TN, ST, false, false>(d, g, grid, st);
+  if (count != nullptr) {
+    if (d.a_trans) return launch_one<TM, TN, ST>(gemm32k_counted_kernel<TM, TN, ST, true, true>, g, grid, st, d, count, depth);
+    if (d.b_trans) return launch_one<TM, TN, ST>(gemm32k_counted_kernel<TM, TN, ST, false, true>, g, grid, st, d, count, depth);
+    return launch_one<TM, TN, ST>(gemm32k_counted_kernel<TM, TN, ST, false, false>, g, grid, st, d, count, depth);
+  }
+  if (d.a_trans && d.b_trans) return launch_one<TM, TN, ST>(gemm32k_kernel<TM, TN, ST, true, true>, g, grid, st, d);
+  if (d.a_trans) return launch_one<TM, TN, ST>(gemm32k_kernel<TM, TN, ST, true, false>, g, grid, st, d);
+  if (d.b_trans) return launch_one<TM, TN, ST>(gemm32k_kernel<TM, TN, ST, false, true>, g, grid, st, d);
+  return launch_one<TM, TN, ST>(gemm32k_kernel<TM, TN, ST, false, false>, g, grid, st, d);
 }
 
 // Tiles: 16-row blocks, stages (two workgroups fit a CU's LDS but for the 64x80 tile with four stages, which is for one round), and
@@ -264,7 +295,7 @@ constexpr Tile TILES[] = {{16, 32, 3.17, 0.203, 0.043, 0.175, 0.97, "1, 2, 6"}, 
                           {48, 64, 3.68, 0.795, 0.293, 0.709, 1.36, "3, 4, 2"}, {64, 64, 3.96, 1.009, 0.339, 0.914, 1.55, "4, 4, 2"},
                           {64, 80, 4.99, 1.176, 0.161, 1.182, 3.35, "4, 5, 4"}, {64, 80, 4.35, 1.231, 0.266, 1.112, 1.85, "4, 5, 2"}};
 
-int choose(const pf_gemm_desc& d) {
+int choose(const pf_gemm_desc& d, double* us = nullptr) {
   const int64_t nb = (d.batch1 > 0 ? d.batch1 : 1) * (d.batch2 > 0 ? d.batch2 : 1);
   const double nk = (double)((d.K + FK - 1) / FK);
   int best = 0;
@@ -275,21 +306,34 @@ int choose(const pf_gemm_desc& d) {
     const double c = t.fixed + (rounds <= 1 ? nk * (t.t0 + t.t1 * (double)tiles / 256) : (double)rounds * (nk * t.sat + t.over));
     if (i == 0 || c < t_best) best = i, t_best = c;
   }
+  if (us != nullptr) *us = t_best;
   return best;
+}
+int on_best_tile(const pf_gemm_desc& d, const int* count, int64_t depth, hipStream_t st) {
+  switch (choose(d)) {
+    case 0: return launch<1, 2, 6>(d, count, depth, st);
+    case 1: return launch<2, 2, 4>(d, count, depth, st);
+    case 2: return launch<2, 3, 4>(d, count, depth, st);
+    case 3: return launch<3, 3, 3>(d, count, depth, st);
+    case 4: return launch<3, 4, 2>(d, count, depth, st);
+    case 5: return launch<4, 4, 2>(d, count, depth, st);
+    case 6: return launch<4, 5, 4>(d, count, depth, st);
+    default: return launch<4, 5, 2>(d, count, depth, st);
+  }
 }
 }  // namespace
 
 const char* pf_gemm_f32_depth_shape(const pf_gemm_desc& d) { return TILES[choose(d)].shape; }
 
-int pf_gemm_f32_depth(const pf_gemm_desc& d, hipStream_t st) {
-  switch (choose(d)) {
-    case 0: return launch<1, 2, 6>(d, st);
-    case 1: return launch<2, 2, 4>(d, st);
-    case 2: return launch<2, 3, 4>(d, st);
-    case 3: return launch<3, 3, 3>(d, st);
-    case 4: return launch<3, 4, 2>(d, st);
-    case 5: return launch<4, 4, 2>(d, st);
-    case 6: return launch<4, 5, 4>(d, st);
-    default: return launch<4, 5, 2>(d, st);
-  }
+double pf_gemm_f32_depth_us(const pf_gemm_desc& d) {
+  double us = 0;
+  choose(d, &us);
+  return us;
+}
+
+int pf_gemm_f32_depth(const pf_gemm_desc& d, hipStream_t st) { return on_best_tile(d, nullptr, 0, st); }
+
+int pf_gemm_f32_counted(const pf_gemm_desc& d, const int* count, int64_t depth, hipStream_t st) {
+  PF_REQUIRE(pf_gemm_f32_direct_ok(d) && (d.b_trans || !d.a_trans) && count != nullptr, "pf_gemm(f32): operands of a counted product");
+  return on_best_tile(d, count, depth, st);
 }

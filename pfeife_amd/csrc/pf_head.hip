@@ -16,7 +16,8 @@
 // alike: 131072 classes, bf16, relative error of the gradients 2.8e-3 so, 1.9e-3 as it is, 1.7e-3 being the results' own rounding).  Where the
 // tokens' factors differ (a gradient for every token) the rounding of c is there.  fp16: 2^13 times that, which keeps probabilities down
 // to 2^-38.
-// fp32: the same through pf_gemm, with a piece's logits in memory.
+// fp32: the same through the fp32 products, with a piece's logits in memory.
+#include "pf_gemm_common.h"
 #include "pf_head.h"
 #include "pf_rows.h"
 
@@ -107,14 +108,12 @@ __global__ __launch_bounds__(1024) void head_index_kernel(const Labels y, Kept k
   }
 }
 
-__device__ __forceinline__ int64_t rows_needed(int n, int64_t n_max, int all) { return all ? n_max : (n > 64 ? (n + 63) / 64 * 64 : 64); }
+__device__ __forceinline__ int64_t rows_needed(int n) { return n > 64 ? (n + 63) / 64 * 64 : 64; }
 
 struct Hidden {
   const char* h;
   int64_t T, sb, st, D, depth;
   char* hc;
-  int64_t n_max;
-  int all;                          // rows of zeros up to n_max, not just to the next multiple of 64
 };
 // One token's row by one wavefront, or zeros; U: an element, as bits
 template <typename U>
@@ -132,7 +131,7 @@ template <typename U>
 __global__ __launch_bounds__(256) void head_gather_kernel(const Hidden x, const Kept k) {
   const int n = *k.count;
   const int64_t c = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (c < rows_needed(n, x.n_max, x.all)) gather_row<U>(x, c, c < n ? k.rows[c] : -1);
+  if (c < rows_needed(n)) gather_row<U>(x, c, c < n ? k.rows[c] : -1);
 }
 
 // Both in one launch for up to 4096 tokens, where every workgroup can count all of them: four tokens to a workgroup, and the rows of
@@ -172,7 +171,7 @@ __global__ __launch_bounds__(256) void head_index_gather_kernel(const Labels y, 
       out[y.out(r)] = 0.f;
     }
   }
-  const int64_t zeros = rows_needed(total, x.n_max, x.all);
+  const int64_t zeros = rows_needed(total);
   for (int64_t z = total + (int64_t)blockIdx.x * 4 + wave; z < zeros; z += (int64_t)gridDim.x * 4) gather_row<U>(x, z, -1);
   if (blockIdx.x == 0) {
     if (tid == 0) *k.count = total;
@@ -287,7 +286,7 @@ struct Ready {
   float most;
   int known;               // 0: to be found; 1: there already; 2: all tokens' factors are alike
   int factor, rows, tiles_n;
-  int64_t dim8;
+  int64_t n_max, dim8;
   uint16_t* ht;
 };
 template <typename U>
@@ -305,7 +304,7 @@ __global__ __launch_bounds__(256) void head_ready_kernel(const Ready q) {
       if (q.known != 1 && blockIdx.x == 0 && t == 0) *q.scale = s;
     }
     const int64_t c = (int64_t)blockIdx.x * 256 + t;
-    if (c >= q.x.n_max) return;
+    if (c >= q.n_max) return;
     PfHeadColumn o = {0.f, 0.f, 0.f, 0.f};     // (behind the last token: zeros times exp(0))
     if (c < n) {
       o.top = k.top[c];
@@ -317,7 +316,7 @@ __global__ __launch_bounds__(256) void head_ready_kernel(const Ready q) {
     q.col[c] = o;
     return;
   }
-  const int64_t padded = rows_needed(n, q.x.n_max, q.x.all);
+  const int64_t padded = rows_needed(n);
   const int block = (int)blockIdx.x - q.factor;
   if (block < q.rows) {
     const int64_t c = (int64_t)block * 4 + (t >> 6);
@@ -344,7 +343,7 @@ __global__ __launch_bounds__(256) void head_ready_kernel(const Ready q) {
     uint32_t o[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] = (uint32_t)tile[(t & 7) * 8 + 2 * j][i] | (uint32_t)tile[(t & 7) * 8 + 2 * j + 1][i] << 16;
-    if (d < q.dim8) *(uint4*)(q.ht + d * q.x.n_max + c0 + (t & 7) * 8) = make_uint4(o[0], o[1], o[2], o[3]);
+    if (d < q.dim8) *(uint4*)(q.ht + d * q.n_max + c0 + (t & 7) * 8) = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
@@ -394,9 +393,9 @@ __global__ __launch_bounds__(256) void head_stats32_kernel(const float* z, int64
   }
   part[(int64_t)blockIdx.y * n_max + c] = {m, s};
 }
-__global__ __launch_bounds__(256) void head_dz32_kernel(float* z, int64_t rows, int64_t n_max, int64_t v0, const int* lab, const PfHeadColumn* col) {
+__global__ __launch_bounds__(256) void head_dz32_kernel(float* z, int64_t rows, int64_t n_max, int64_t v0, const int* lab, const int* count, const PfHeadColumn* col) {
   const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x, r0 = (int64_t)blockIdx.y * ROWS32;
-  if (c >= n_max) return;
+  if (c >= *count) return;
   const int64_t r1 = r0 + ROWS32 < rows ? r0 + ROWS32 : rows;
   const int64_t at = lab[c] >= 0 ? (int64_t)lab[c] - v0 : -1;
   const PfHeadColumn k = col[c];
@@ -497,7 +496,7 @@ int check_call(const Call& c, const Sizes& s, bool ok) {
 }
 
 Hidden hidden_of(const Call& c, const Sizes& s, const Work& w) {
-  return {(const char*)c.h, c.T > 0 ? c.T : 1, c.sb, c.st, c.D, s.depth, w.hc, s.n_max, c.dtype == PF_F32};
+  return {(const char*)c.h, c.T > 0 ? c.T : 1, c.sb, c.st, c.D, s.depth, w.hc};
 }
 #define PF_BY_SIZE(KERNEL, ...)                                                          \
   do {                                                                                   \
@@ -509,32 +508,22 @@ void widen(const Call& c, const Sizes& s, const Work& w, hipStream_t st) {
   if (s.copy_w) pf_rows_widen(c.w, c.V, c.D, w.wide, s.depth, c.dtype == PF_F32 ? 4 : 2, st);
 }
 
-// a product over fp32 operands; batch: shares of the depth, `share` of it each, with results of their own
+// A product over fp32 operands of the tokens that take part, n_max at most (N, M or K of it, see pf_gemm_f32_counted); splits: shares of the
+// depth, with results of their own
 int product32(int a_trans, int b_trans, int64_t M, int64_t N, int64_t K, const float* A, int64_t lda, const float* B, int64_t ldb, float* C, int64_t ldc, int beta,
-              hipStream_t st, int splits = 1, int64_t c_stride = 0) {
+              const int* count, hipStream_t st, int splits = 1, int64_t c_stride = 0) {
   pf_gemm_desc d = {};
   d.in_dtype = d.c_dtype = PF_F32;
   d.a_trans = a_trans; d.b_trans = b_trans;
-  d.M = M; d.N = N; d.K = K;
+  d.M = M; d.N = N; d.K = pf_head_share(K, splits);
   d.A = A; d.lda = lda; d.B = B; d.ldb = ldb; d.C = C; d.ldc = ldc;
-  d.batch1 = d.batch2 = 1;
+  d.batch1 = 1; d.batch2 = (K + d.K - 1) / d.K;
+  d.a_stride2 = d.K * lda;
+  d.b_stride2 = d.K * ldb;
+  d.c_stride2 = c_stride;
   d.alpha = 1.f;
   d.beta = beta;
-  const int64_t share = splits > 1 ? K / splits / 64 * 64 : 0;
-  if (share == 0) return pf_gemm(&d, st);
-  d.K = share;
-  d.batch2 = splits;
-  d.a_stride2 = share * lda;
-  d.b_stride2 = share * ldb;
-  d.c_stride2 = c_stride;
-  const int rc = pf_gemm(&d, st);
-  if (rc != PF_OK || share * splits == K) return rc;
-  d.K = K - share * splits;
-  d.batch2 = 1;
-  d.A = A + share * splits * lda;
-  d.B = B + share * splits * ldb;
-  d.beta = 1;
-  return pf_gemm(&d, st);
+  return pf_gemm_f32_counted(d, count, K, st);
 }
 
 }  // namespace
@@ -586,7 +575,7 @@ extern "C" int pf_linear_ce_fwd(const void* hidden, int dtype, int64_t B, int64_
   if (dtype == PF_F32) {
     for (int64_t v0 = 0; v0 < V; v0 += s.piece) {
       const int64_t rows = V - v0 < s.piece ? V - v0 : s.piece;
-      rc = product32(0, 0, rows, s.n_max, D, (const float*)wide + v0 * s.depth, s.depth, (const float*)w.hc, s.depth, (float*)w.dz, s.n_max, 0, st);
+      rc = product32(0, 0, rows, s.n_max, D, (const float*)wide + v0 * s.depth, s.depth, (const float*)w.hc, s.depth, (float*)w.dz, s.n_max, 0, k.count, st);
       if (rc != PF_OK) return rc;
       hipLaunchKernelGGL(head_stats32_kernel, dim3((unsigned)((s.n_max + 255) / 256), (unsigned)((rows + ROWS32 - 1) / ROWS32)), dim3(256), 0, st, (const float*)w.dz, rows,
                          s.n_max, v0, k.lab, k.count, w.part + blocks * s.n_max, w.zl);
@@ -645,7 +634,7 @@ extern "C" int pf_linear_ce_bwd(const void* hidden, int dtype, int64_t B, int64_
   }
   q.factor = (int)((s.n_max + 255) / 256);
   q.rows = (int)(s.n_max / 4);
-  q.dim8 = s.dim8;
+  q.n_max = s.n_max; q.dim8 = s.dim8;
   q.ht = (uint16_t*)w.ht;
   q.tiles_n = (int)((s.dim8 + 63) / 64);
   const int tiles = half && dweight ? (int)(s.n_max / 64) * q.tiles_n : 0;
@@ -658,12 +647,12 @@ extern "C" int pf_linear_ce_bwd(const void* hidden, int dtype, int64_t B, int64_
     if (!half) {
       const float* wp = (const float*)wide + v0 * s.depth;
       float* dz = (float*)w.dz;
-      rc = product32(0, 0, rows, s.n_max, D, wp, s.depth, (const float*)w.hc, s.depth, dz, s.n_max, 0, st);
+      rc = product32(0, 0, rows, s.n_max, D, wp, s.depth, (const float*)w.hc, s.depth, dz, s.n_max, 0, k.count, st);
       if (rc != PF_OK) return rc;
       hipLaunchKernelGGL(head_dz32_kernel, dim3((unsigned)((s.n_max + 255) / 256), (unsigned)((rows + ROWS32 - 1) / ROWS32)), dim3(256), 0, st, dz, rows, s.n_max, v0, k.lab,
-                         w.col);
-      if (dhidden) rc = product32(1, 1, s.n_max, D, rows, dz, s.n_max, wp, s.depth, w.acc, s.depth, v0 > 0, st, s.splits, s.n_max * s.depth);
-      if (rc == PF_OK && dweight) rc = product32(0, 1, rows, D, s.n_max, dz, s.n_max, (const float*)w.hc, s.depth, (float*)dweight + v0 * D, D, 0, st);
+                         k.count, w.col);
+      if (dhidden) rc = product32(1, 1, s.n_max, D, rows, dz, s.n_max, wp, s.depth, w.acc, s.depth, v0 > 0, k.count, st, s.splits, s.n_max * s.depth);
+      if (rc == PF_OK && dweight) rc = product32(0, 1, rows, D, s.n_max, dz, s.n_max, (const float*)w.hc, s.depth, (float*)dweight + v0 * D, D, 0, k.count, st);
       if (rc != PF_OK) return rc;
       continue;
     }

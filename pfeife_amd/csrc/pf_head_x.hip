@@ -301,21 +301,17 @@ int pf_head_splits(int dtype, int64_t n_max, int64_t depth, int64_t rows) {
   double best_t = 0;
   for (int s = 1; s <= 16 && (s == 1 || (rows / s >= 256 && n_max * depth * 4 * s < (1ll << 31) - 64)); ++s) {
     double t = 0;
-    if (dtype == PF_F32) {
-      const int64_t tiles = ((n_max + 63) / 64) * ((depth + 63) / 64) * s;      // (17 ns a unit of depth and 64x64 tile)
-      t = (double)((tiles + 255) / 256) * 0.0171 * (double)(rows / s);
-    } else {
-      pf_gemm_desc d = plain_desc();
-      d.c_dtype = PF_F32;
-      d.a_trans = d.b_trans = 1;
-      d.M = n_max; d.N = depth; d.K = pf_head_share(rows, s);
-      d.batch2 = (rows + d.K - 1) / d.K;
-      pf_gemm_best_tile(d, &t);
-    }
+    pf_gemm_desc d = plain_desc();
+    d.c_dtype = PF_F32;
+    d.a_trans = d.b_trans = 1;
+    d.M = n_max; d.N = depth; d.K = pf_head_share(rows, s);
+    d.batch2 = (rows + d.K - 1) / d.K;
+    if (dtype == PF_F32) t = pf_gemm_f32_depth_us(d);
+    else pf_gemm_best_tile(d, &t);
     t += (double)(n_max * depth) * s * 8.0 / 5.0e6;      // the shares' way through memory, written and read at 5 TB/s
     if (s == 1 || t < best_t) { best = s; best_t = t; }
   }
   const int64_t share = pf_head_share(rows, best);
-  return dtype == PF_F32 ? best : (int)((rows + share - 1) / share);
+  return (int)((rows + share - 1) / share);
 }
 #endif
