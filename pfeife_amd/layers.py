@@ -56,9 +56,12 @@ def embedding(ids, weight, *, scale=1.0, padding_idx=None):
     padding = _check_embedding(ids, weight, scale, padding_idx)
     if _dual._current_level >= 0 and _has_tangent(weight):
         raise RuntimeError("embedding: there is no forward-mode derivative")
+    wants = torch.is_grad_enabled() and weight.requires_grad
+    if wants and (ids.numel() > 1 << 27 or weight.shape[0] >= (1 << 27) - 1 or weight.shape[1] > 65535 * 64):
+        raise RuntimeError("embedding: too many ids, rows or columns for a gradient")
     weight = weight.contiguous()
     args = (ids.contiguous(), float(scale), padding)
-    if torch.is_grad_enabled() and weight.requires_grad:
+    if wants:
         return _EmbeddingFn.apply(weight, args)
     return _EmbeddingFn.forward(_NoContext, weight, args, False)
 

@@ -149,3 +149,11 @@ def test_the_c_entries_refuse_memory_that_their_wide_accesses_cannot_take():
         rc(lib.pf_gated_linear_bwd(one, 2, 3, 64, one, 32, 3, 1, kept, one, one, one, ws, None), b"boundaries")
     rc(lib.pf_embedding_sorted_bwd(one, 2, one, one, 2, 300, 8, 5, -1, 1.0, 0, one + 4, None), b"boundary")
     rc(lib.pf_embedding_sorted_bwd(one, 2, one, one, 2, 300, 65535 * 64 + 1, 5, -1, 1.0, 0, one, None), b"too many")
+
+
+def test_an_embedding_without_a_possible_gradient_is_refused_before_it_runs(on_any_device):
+    many = torch.zeros(1, dtype=torch.int64).expand((1 << 27) + 1)
+    with pytest.raises(RuntimeError, match="too many ids"):
+        on_any_device["embedding"](many, W.clone().requires_grad_())
+    with pytest.raises(RuntimeError, match="too many ids"):
+        on_any_device["embedding"](Y, torch.zeros(1).expand(2, 65535 * 64 + 1).requires_grad_())

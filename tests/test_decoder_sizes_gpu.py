@@ -1,0 +1,84 @@
+"""The decoder operators where one launch is not enough: a vocabulary in pieces, sums in shares, rows and ids of several launches."""
+import pytest
+import torch
+import torch.nn.functional as F
+
+from test_decoder_ops_gpu import IGNORE, TYPES, U32, head_inputs, head_reference, within
+
+pytestmark = pytest.mark.gpu
+
+
+# 1000 tokens: pieces of 131072 classes in 16 bits, 65536 in fp32.  The last piece is of fewer rows than it would have shares, or a few of its shares'
+PIECES = [(1, 1000, 64, 131072 + 300), (4, 250, 33, 131072 + 1), (1, 990, 72, 65536 * 2 + 5000)]
+
+
+@pytest.mark.parametrize("B,T,D,V", PIECES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_cross_entropy_in_pieces_of_the_vocabulary(dtype, B, T, D, V):
+    from pfeife_amd.loss import linear_cross_entropy
+
+    h, w, y = head_inputs(dtype, B, T, D, V)
+    y[0, 5], y[0, 6], y[0, 7] = V - 1, 65536, 131071      # labels at the pieces' ends
+    h.requires_grad_()
+    w.requires_grad_()
+    loss = linear_cross_entropy(h, w, y)
+    dh, dw = torch.autograd.grad(loss, (h, w))
+    term, bound, rh, eh, rw, ew = head_reference(h.detach(), w.detach(), y, 0, "mean", 0.0, torch.ones((), device="cuda"))
+    within(loss.detach(), term, bound, torch.float32)
+    within(dh, rh, eh, dtype)
+    within(dw, rw, ew, dtype)
+    again = torch.autograd.grad(linear_cross_entropy(h, w, y), (h, w))
+    assert torch.equal(again[0], dh) and torch.equal(again[1], dw)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scored", [0, 1, 2, 3, 65, 255, 256, 257])
+def test_linear_cross_entropy_counts_on_the_device(dtype, scored):
+    """Grids cover 700 tokens, `scored` take part: the counted dimension ends anywhere in a tile, a stage or a vector."""
+    from pfeife_amd.loss import linear_cross_entropy
+
+    h, w, y = head_inputs(dtype, 1, 700, 132, 1003, masked=0.0)
+    order = torch.randperm(700, generator=torch.Generator().manual_seed(scored)).cuda()
+    y[0, order[scored:]] = IGNORE
+    h[0, order[scored:]] = float("nan")
+    h.requires_grad_()
+    w.requires_grad_()
+    loss = linear_cross_entropy(h, w, y, reduction="sum")
+    dh, dw = torch.autograd.grad(loss, (h, w))
+    clean = torch.where((y == IGNORE).unsqueeze(-1), torch.zeros_like(h.detach()), h.detach())
+    term, bound, rh, eh, rw, ew = head_reference(clean, w.detach(), y, 0, "sum", 0.0, torch.ones((), device="cuda"))
+    within(loss.detach(), term, bound, torch.float32)
+    within(dh, rh, eh, dtype)
+    within(dw, rw, ew, dtype)
+
+
+def test_embedding_of_more_ids_than_a_launch_takes():
+    from pfeife_amd.layers import embedding
+
+    n = (1 << 25) + 77
+    ids = torch.randint(0, 100, (n,), device="cuda", generator=torch.Generator("cuda").manual_seed(0))
+    w = torch.randn(100, 3, device="cuda").half()
+    out = embedding(ids, w)
+    for at in (slice(0, 1000), slice((1 << 25) - 500, n)):
+        assert torch.equal(out[at], w[ids[at]])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_gated_linear_of_more_rows_than_a_launch_takes(dtype):
+    """Without a backward pass rows come in launches of 65024 here; with one they are refused, in words."""
+    from pfeife_amd.layers import gated_linear
+
+    g = torch.Generator("cuda").manual_seed(0)
+    rows, D, ffn = 65024 + 333, 64, 8192
+    x = torch.randn(rows, D, device="cuda", generator=g).to(dtype)
+    w = (torch.randn(2 * ffn, D, device="cuda", generator=g) * D ** -0.5).to(dtype)
+    y = gated_linear(x, w)
+    for at in (slice(0, 64), slice(65024 - 40, 65024 + 40), slice(rows - 40, rows)):
+        x64, w64 = x[at].double(), w.double()
+        z, off = x64 @ w64.t(), (D + 8) * U32 * (x64.abs() @ w64.abs().t())
+        a, b, ea, eb = z[:, :ffn], z[:, ffn:], off[:, :ffn], off[:, ffn:]
+        v = F.silu(a)
+        # an activation's slope is at most 1.1, its own arithmetic off by 2e-6 or 8 units of 2^-24
+        within(y[at], v * b, (1.2 * ea + 2e-6 * a.abs().clamp_max(1.0) + 8 * U32 * a.abs()) * (b.abs() + eb) + v.abs() * eb, dtype)
+    with pytest.raises(RuntimeError, match="too large for one call"):
+        gated_linear(x, w.requires_grad_())
