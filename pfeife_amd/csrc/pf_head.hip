@@ -57,7 +57,7 @@ inline Kept kept_of(void* p, int64_t n_max) {
 
 struct Sizes {
   int64_t n, n_max, depth, piece, dim8;
-  int splits;
+  PfHeadShares shares;
   bool copy_w, narrow;
 };
 
@@ -349,8 +349,11 @@ __global__ __launch_bounds__(256) void head_ready_kernel(const Ready q) {
 
 // The gradient of every row of the hidden state: a token's sum rounded once (times a loss scale first), zeros where it took no part
 template <int W>
-__global__ __launch_bounds__(256) void head_spread_kernel(const float* acc, int64_t ld, int splits, int64_t n_max, const int* inv, int64_t n, int64_t D, const float* times, void* dh, int dt) {
+__global__ __launch_bounds__(256) void head_spread_kernel(const float* acc, int64_t ld, const PfHeadShares shares, int64_t n_max, const int* count, const int* inv, int64_t n,
+                                                          int64_t D, const float* times, void* dh, int dt) {
   const float by = times != nullptr ? *times : 1.f;
+  const int splits = shares.of(*count, ld);
+  const int64_t step = shares.by_count ? *count : n_max;
   const int64_t per = (D + 64 * W - 1) / (64 * W), total = n * per;      // (a wavefront to 64 W columns of a row)
   for (int64_t q = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); q < total; q += (int64_t)gridDim.x * 4) {
     const int64_t r = q / per, i = q % per * 64 * W + (threadIdx.x & 63) * W;
@@ -363,7 +366,7 @@ __global__ __launch_bounds__(256) void head_spread_kernel(const float* acc, int6
 #pragma unroll 4
       for (int p = 0; p < splits; ++p) {
         float w[W];
-        ld_vec<W>(acc, (p * n_max + c) * ld + i, PF_F32, w);
+        ld_vec<W>(acc, (p * step + c) * ld + i, PF_F32, w);
 #pragma unroll
         for (int k = 0; k < W; ++k) v[k] += w[k];
       }
@@ -445,7 +448,7 @@ bool sizes_of(const Call& c, Sizes& s, bool back) {
   s.narrow = es == 2 && s.dim8 != c.D;
   s.piece = piece_rows(s.n_max, c.V, es);
   if (es == 2 && s.piece > reach_rows(s.depth)) s.piece = reach_rows(s.depth);
-  s.splits = back ? pf_head_splits(c.dtype, s.n_max, s.depth, s.piece) : 1;
+  if (back) s.shares = pf_head_shares(c.dtype, s.n_max, s.depth, s.piece);
   return s.n < (1ll << 24) && c.V < (1ll << 31) && s.n_max * s.depth * 4 < (1ll << 31) - 64 && s.piece * s.n_max * es < (1ll << 31) - 64 &&
          s.depth < (1ll << 19);
 }
@@ -479,7 +482,7 @@ Work carve(Carve& a, const Call& c, const Sizes& s, bool back) {
     if (s.narrow) w.dw = (char*)a.take(s.piece * s.depth * 2);
     w.col = (PfHeadColumn*)a.take(s.n_max * 16);
     w.scale = (float*)a.take(4);
-    w.acc = (float*)a.take(s.n_max * s.depth * 4 * s.splits);
+    w.acc = (float*)a.take(s.shares.bytes(s.n_max, s.depth));
   }
   return w;
 }
@@ -651,7 +654,7 @@ extern "C" int pf_linear_ce_bwd(const void* hidden, int dtype, int64_t B, int64_
       if (rc != PF_OK) return rc;
       hipLaunchKernelGGL(head_dz32_kernel, dim3((unsigned)((s.n_max + 255) / 256), (unsigned)((rows + ROWS32 - 1) / ROWS32)), dim3(256), 0, st, dz, rows, s.n_max, v0, k.lab,
                          k.count, w.col);
-      if (dhidden) rc = product32(1, 1, s.n_max, D, rows, dz, s.n_max, wp, s.depth, w.acc, s.depth, v0 > 0, k.count, st, s.splits, s.n_max * s.depth);
+      if (dhidden) rc = product32(1, 1, s.n_max, D, rows, dz, s.n_max, wp, s.depth, w.acc, s.depth, v0 > 0, k.count, st, s.shares.most, s.n_max * s.depth);
       if (rc == PF_OK && dweight) rc = product32(0, 1, rows, D, s.n_max, dz, s.n_max, (const float*)w.hc, s.depth, (float*)dweight + v0 * D, D, 0, k.count, st);
       if (rc != PF_OK) return rc;
       continue;
@@ -664,7 +667,7 @@ extern "C" int pf_linear_ce_bwd(const void* hidden, int dtype, int64_t B, int64_
     char* dw = (char*)dweight + v0 * D * 2;
     p.dw = s.narrow ? w.dw : dw;
     p.ldw_out = s.narrow ? s.depth : D;
-    p.dh = w.acc; p.add = v0 > 0; p.splits = s.splits;
+    p.dh = w.acc; p.add = v0 > 0; p.shares = s.shares;
     p.unscale = w.scale;
     rc = pf_head_dz(dtype, p, st);
     if (rc == PF_OK && dhidden) rc = pf_head_dh(dtype, p, st);
@@ -693,9 +696,9 @@ extern "C" int pf_linear_ce_hidden_grad(const void* weight, int dtype, int64_t t
   const int64_t lanes = D % 8 == 0 && pf_aligned(dhidden, 16) ? 512 : 64, units = (s.n * ((D + lanes - 1) / lanes) + 3) / 4;
   const dim3 grid((unsigned)(units < 16384 ? units : 16384));
   if (D % 8 == 0 && pf_aligned(dhidden, 16))
-    hipLaunchKernelGGL(head_spread_kernel<8>, grid, dim3(256), 0, st, w.acc, s.depth, s.splits, s.n_max, k.inv, s.n, D, times, dhidden, dtype);
+    hipLaunchKernelGGL(head_spread_kernel<8>, grid, dim3(256), 0, st, w.acc, s.depth, s.shares, s.n_max, k.count, k.inv, s.n, D, times, dhidden, dtype);
   else
-    hipLaunchKernelGGL(head_spread_kernel<1>, grid, dim3(256), 0, st, w.acc, s.depth, s.splits, s.n_max, k.inv, s.n, D, times, dhidden, dtype);
+    hipLaunchKernelGGL(head_spread_kernel<1>, grid, dim3(256), 0, st, w.acc, s.depth, s.shares, s.n_max, k.count, k.inv, s.n, D, times, dhidden, dtype);
   PF_CHECK_LAUNCH(c.who);
   return PF_OK;
 }

@@ -179,15 +179,19 @@ __global__ PF_H_BOUNDS void head_logits_kernel(const pf_gemm_desc d, const int* 
   if (!shrink<T::BM, T::BN>(p, g)) return;
   gemm16x_body<PF_X_DT, PF_H_TILE, false, false, EC_OWN, RAG, Tail>(p, g, (int)blockIdx.x, tail);
 }
-// The piece's `rows` in shares of d.K, the last one shorter
+// The piece's `rows` in shares, the last one shorter
 template <int XT, int EC>
-__global__ PF_H_BOUNDS void head_hidden_grad_kernel(const pf_gemm_desc d, const int* count, int64_t rows) {
+__global__ PF_H_BOUNDS void head_hidden_grad_kernel(const pf_gemm_desc d, const int* count, int64_t rows, const PfHeadShares shares) {
   using T = XTile<XT>;
   pf_gemm_desc p = d;
   GemmGrid g;
   p.M = *count;
-  const int64_t left = rows - (int64_t)blockIdx.y * d.K;
-  p.K = left < d.K ? left : d.K;
+  const int64_t share = pf_head_share(rows, shares.of(p.M, p.N)), left = rows - (int64_t)blockIdx.y * share;
+  if (left <= 0) return;
+  p.K = left < share ? left : share;
+  p.a_stride2 = share * p.lda;
+  p.b_stride2 = share * p.ldb;
+  p.c_stride2 = (shares.by_count ? p.M : d.M) * p.N;
   g.vec_epi = 1;
   if (p.M == 0 || !shrink<T::BM, T::BN>(p, g)) return;
   gemm16x_body<PF_X_DT, PF_H_TILE, true, true, EC>(p, g, (int)blockIdx.x);
@@ -240,11 +244,11 @@ template <class Tail> int logits_launch(const PfHeadProduct& p, const Tail& tail
 }
 
 template <int XT> int hidden_launch(const pf_gemm_desc& d, const PfHeadProduct& p, hipStream_t st) {
-  return d.beta ? launch<XT>(head_hidden_grad_kernel<XT, EC_ACC32>, d.M, d.N, (int)d.batch2, st, d, p.count, p.rows)
-                : launch<XT>(head_hidden_grad_kernel<XT, EC_STORE32>, d.M, d.N, (int)d.batch2, st, d, p.count, p.rows);
+  return d.beta ? launch<XT>(head_hidden_grad_kernel<XT, EC_ACC32>, d.M, d.N, (int)d.batch2, st, d, p.count, p.rows, p.shares)
+                : launch<XT>(head_hidden_grad_kernel<XT, EC_STORE32>, d.M, d.N, (int)d.batch2, st, d, p.count, p.rows, p.shares);
 }
 int hidden_grad(const pf_gemm_desc& d, const PfHeadProduct& p, hipStream_t st) {
-  switch (pf_gemm_best_tile(d)) {
+  switch (p.shares.by_count ? PF_XT_256x256w4 : pf_gemm_best_tile(d)) {
     case PF_XT_64x64: return hidden_launch<PF_XT_64x64>(d, p, st);
     case PF_XT_128x128w8: return hidden_launch<PF_XT_128x128w8>(d, p, st);
     case PF_XT_256x128w8: return hidden_launch<PF_XT_256x128w8>(d, p, st);
@@ -269,14 +273,11 @@ int PF_H_CAT(pf_head_dh_, PF_X_DT)(const PfHeadProduct& p, hipStream_t st) {
   pf_gemm_desc d = plain_desc();
   d.c_dtype = PF_F32;
   d.a_trans = d.b_trans = 1;
-  d.M = p.n_max; d.N = p.depth; d.K = pf_head_share(p.rows, p.splits);
+  d.M = p.n_max; d.N = p.depth; d.K = pf_head_share(p.rows, p.shares.most);
   d.A = p.dz; d.lda = p.n_max; d.B = p.w; d.ldb = p.ldw; d.C = p.dh; d.ldc = p.depth;
   d.beta = p.add;
   d.unscale_by = p.unscale;
-  d.batch2 = (p.rows + d.K - 1) / d.K;
-  d.a_stride2 = d.K * d.lda;
-  d.b_stride2 = d.K * d.ldb;
-  d.c_stride2 = p.n_max * p.depth;
+  d.batch2 = p.shares.most;
   return hidden_grad(d, p, st);
 }
 
@@ -296,8 +297,9 @@ int PF_H_CAT(pf_head_dw_, PF_X_DT)(const PfHeadProduct& p, hipStream_t st) {
 }
 
 #if PF_X_DT == 1
-int pf_head_splits(int dtype, int64_t n_max, int64_t depth, int64_t rows) {
-  int best = 1;
+PfHeadShares pf_head_shares(int dtype, int64_t n_max, int64_t depth, int64_t rows) {
+  PfHeadShares best = {1, 0, rows};
+  int tile = 0;
   double best_t = 0;
   for (int s = 1; s <= 16 && (s == 1 || (rows / s >= 256 && n_max * depth * 4 * s < (1ll << 31) - 64)); ++s) {
     double t = 0;
@@ -306,12 +308,17 @@ int pf_head_splits(int dtype, int64_t n_max, int64_t depth, int64_t rows) {
     d.a_trans = d.b_trans = 1;
     d.M = n_max; d.N = depth; d.K = pf_head_share(rows, s);
     d.batch2 = (rows + d.K - 1) / d.K;
+    const int on = dtype == PF_F32 ? 0 : pf_gemm_best_tile(d, &t);
     if (dtype == PF_F32) t = pf_gemm_f32_depth_us(d);
-    else pf_gemm_best_tile(d, &t);
     t += (double)(n_max * depth) * s * 8.0 / 5.0e6;      // the shares' way through memory, written and read at 5 TB/s
-    if (s == 1 || t < best_t) { best = s; best_t = t; }
+    if (s == 1 || t < best_t) { best.most = (int)d.batch2; best_t = t; tile = on; }
   }
-  const int64_t share = pf_head_share(rows, best);
-  return (int)((rows + share - 1) / share);
+  if (tile == PF_XT_256x256w4) {      // (half again as many as fill a round with all tokens: the workgroups that find nothing to do wait for a CU all the same)
+    int64_t most = 384 / ((n_max + 255) / 256 * ((depth + 255) / 256));
+    if (most > rows / 256) most = rows / 256;
+    if (most > 16) most = 16;
+    if (most > 1) best = {(int)most, 1, rows};
+  }
+  return best;
 }
 #endif

@@ -82,3 +82,22 @@ def test_gated_linear_of_more_rows_than_a_launch_takes(dtype):
         within(y[at], v * b, (1.2 * ea + 2e-6 * a.abs().clamp_max(1.0) + 8 * U32 * a.abs()) * (b.abs() + eb) + v.abs() * eb, dtype)
     with pytest.raises(RuntimeError, match="too large for one call"):
         gated_linear(x, w.requires_grad_())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("scored", [0, 1, 300, 700, 1025, 1300, 2048])
+def test_linear_cross_entropy_in_shares_by_the_count(dtype, scored):
+    """2048 tokens by 1024 columns: 32 tiles of 256, and with fewer tokens more shares of the vocabulary, whose number the device finds."""
+    from pfeife_amd.loss import linear_cross_entropy
+
+    h, w, y = head_inputs(dtype, 2, 1024, 1024, 70001, masked=0.0)
+    order = torch.randperm(2048, generator=torch.Generator().manual_seed(scored)).cuda()
+    y.view(-1)[order[scored:]] = IGNORE
+    h.requires_grad_()
+    w.requires_grad_()
+    loss = linear_cross_entropy(h, w, y, reduction="sum")
+    dh, dw = torch.autograd.grad(loss, (h, w))
+    term, bound, rh, eh, rw, ew = head_reference(h.detach(), w.detach(), y, 0, "sum", 0.0, torch.ones((), device="cuda"))
+    within(loss.detach(), term, bound, torch.float32)
+    within(dh, rh, eh, dtype)
+    within(dw, rw, ew, dtype)
