@@ -135,7 +135,8 @@ __global__ __launch_bounds__(256) void head_gather_kernel(const Hidden x, const 
 }
 
 // Both in one launch for up to 4096 tokens, where every workgroup can count all of them: four tokens to a workgroup, and the rows of
-// zeros behind the last one dealt out too
+// zeros behind the last one dealt out too.  (us of a forward pass with 512 classes of 512 columns, one launch and two: 1024 tokens 38 and 40, 4096 42.4 and 43.1, 8192
+// 55 and 47)
 template <typename U>
 __global__ __launch_bounds__(256) void head_index_gather_kernel(const Labels y, const Hidden x, Kept k, float* out) {
   __shared__ int sm[4], sa[4];
@@ -414,7 +415,8 @@ int bad(const char* who, const char* what) {
   return PF_ERR_INVALID;
 }
 
-// Vocabulary rows of a piece: its dz (fp32: its logits) in 256 MB, in whole tiles
+// Vocabulary rows of a piece: its dz (fp32: its logits) in 256 MB, in whole tiles.  (16384 tokens, 2048 columns, 32000 classes, bf16: 6.62 ms; with 512 MB 6.60, with
+// 128 7.35)
 int64_t piece_rows(int64_t n_max, int64_t V, int64_t size) {
   int64_t rows = (256ll << 20) / (n_max * size) / 256 * 256;
   if (rows < 256) rows = 256;
@@ -438,9 +440,9 @@ bool sizes_of(const Call& c, Sizes& s, bool back) {
   s.n_max = round_up(s.n > 0 ? s.n : 1, 64);
   s.depth = c.dtype == PF_F32 ? round_up(c.D, 4) : (c.D < 64 ? 64 : round_up(c.D, 8));
   s.copy_w = s.depth != c.D || !pf_aligned(c.w, 16);
-  // Whole stages of the fastest tile: where the weight is copied anyway, and where many tokens pay for a copy.  4662 tokens, 1000 columns, 49999
-  // classes, fp16: the logits' product 446 us on the tile for any multiple of 8, 336 on the other behind 31 us of copy.
-  if (es == 2 && s.n_max > 128 && (s.copy_w || s.n_max >= 3000)) {
+  // Whole stages of the fastest tile: where the weight is copied anyway, and where many tokens pay for a copy.  us of a step, 1000 columns, 50000 classes, bf16,
+  // on the tile for any multiple of 8 and on the other behind copies: 1024 tokens 567 and 589, 2048 937 and 875, 4096 1780 and 1546.
+  if (es == 2 && s.n_max > 128 && (s.copy_w || s.n_max >= 2048)) {
     s.depth = round_up(s.depth, 64);
     s.copy_w = s.copy_w || s.depth != c.D;
   }
@@ -631,7 +633,7 @@ extern "C" int pf_linear_ce_bwd(const void* hidden, int dtype, int64_t B, int64_
   q.most = dtype == PF_F16 ? 8192.f : 1.f;
   if (g_sb == 0 && g_st == 0 && z_loss == 0) {
     q.known = 2;
-  } else if (half && s.n > 1024) {      // (fewer: every workgroup finds the largest factor for itself; 8192: 13 us)
+  } else if (half && s.n > 1024) {      // (fewer: every workgroup finds the largest factor for itself; at 1024 the same, at 8192 10 us longer)
     hipLaunchKernelGGL(head_scale_kernel, dim3(1), dim3(1024), 0, st, u, q.most, w.scale);
     q.known = 1;
   }

@@ -14,7 +14,9 @@ constexpr int BINS = 512;        // of one digit
 constexpr int FEW_IDS = 256;     // ids that every workgroup looks through by itself
 constexpr int PLACE_BITS = 11;
 constexpr int BLOCK = 1 << PLACE_BITS;      // ids that are sorted among themselves first, key and place in one word
-constexpr int MANY = 65536;                 // ids up to which that is faster than the radix sort
+// ids up to which that is no slower than the radix sort (us of both sorts with sums of 256 columns: 1000 ids 20 / 39, 16384 30 / 49, 65536 56 / 63, 131072
+// 92 / 80, 262144 213 / 92)
+constexpr int MANY = 65536;
 
 __device__ __forceinline__ int key_of(int64_t id, int64_t vocab, int64_t padding) { return id >= 0 && id < vocab && id != padding ? (int)id : (int)vocab; }
 
@@ -339,8 +341,8 @@ __device__ __forceinline__ void put_row(const Sum& s, int64_t row, int64_t c, fl
 }
 
 // Up to FEW_IDS ids, in one launch: a workgroup owns `own` rows of the table's gradient, writes zeros to them, finds the ids that name
-// one of them and adds up, a wavefront to a row, in the list's order.  (The sort takes two launches more; a token that is all of the list is
-// 32 round trips of eight rows here.)
+// one of them and adds up in the list's order, wide rows by its wavefronts side by side, else a wavefront to a row.  (The sort takes two launches
+// more: 16 ids, 32000 x 2048, bf16: 24 us, most of them for the zeros, against 31.)
 template <int DT>
 __global__ __launch_bounds__(256) void table_few_kernel(const Sum s, const int64_t* ids, int64_t padding, int64_t own) {
   __shared__ int rows[FEW_IDS], at[FEW_IDS];
@@ -371,36 +373,40 @@ __global__ __launch_bounds__(256) void table_few_kernel(const Sum s, const int64
   }
   const int hits = before[1] + before[2] + before[3] + before[4];
   __syncthreads();      // (and the zeros are written)
-  for (int j = wave; j < hits; j += 4) {
+  const int across = s.dim > 64 * W ? (s.dim > 2 * 64 * W ? 4 : 2) : 1;      // wavefronts to a row
+  for (int j = wave / across; j < hits; j += 4 / across) {
     const int row = rows[j];
     bool earlier = false;
     for (int q = lane; q < j; q += 64) earlier |= rows[q] == row;
     if (__ballot(earlier) != 0) continue;
-    for (int64_t c = lane * W; c < s.dim; c += 64 * W) {
+    for (int64_t c0 = wave % across * 64 * W; c0 < s.dim; c0 += across * 64 * W) {      // (no lane leaves before the others)
+      const int64_t c = c0 + lane * W, left = s.dim - c;
       float acc[W];
 #pragma unroll
       for (int k = 0; k < W; ++k) acc[k] = 0.f;
-      int q = j;
-      while (q < hits) {
-        int place[8];
-        int n = 0;
+      for (int q0 = j & ~63; q0 < hits; q0 += 64) {
+        const int q = q0 + lane;
+        const int place = q < hits ? at[q] : 0;
+        unsigned long long mine = __ballot(q < hits && rows[q < hits ? q : 0] == row);
+        while (mine != 0) {      // the next eight of the row
+          int n = 0, from[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {      // the next eight of the row
-          while (q < hits && rows[q] != row) ++q;
-          place[k] = q < hits ? at[q] : 0;
-          n += q < hits;
-          ++q;
-        }
-        float v[8][W];
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (k < n) load8<DT>(s.dout, (int64_t)place[k] * s.dim + c, s.dim - c, v[k]);
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (k < n) {
-#pragma unroll
-            for (int e = 0; e < W; ++e) acc[e] += v[k][e];
+          for (int k = 0; k < 8; ++k) {
+            from[k] = mine != 0 ? __builtin_amdgcn_readlane(place, __ffsll((long long)mine) - 1) : 0;
+            n += mine != 0;
+            mine &= mine - 1;
           }
+          float v[8][W];
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (k < n) load8<DT>(s.dout, (int64_t)from[k] * s.dim + c, left, v[k]);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (k < n) {
+#pragma unroll
+              for (int e = 0; e < W; ++e) acc[e] += v[k][e];
+            }
+        }
       }
       put_row<DT>(s, v0 + row, c, acc);
     }
@@ -463,7 +469,7 @@ __global__ __launch_bounds__(256) void table_sum_kernel(const Sum s) {
 }
 
 // Runs that cross chunks.  FEW neighbours from a multiple of FEW on are a block of chunks.  What is moved is small, each of the two
-// launches waits for a few round trips: 7 us each at 16384 ids; 50021 with one of them half of the list: 17 and 11 (50 without the
+// launches waits for a few round trips: 7 us each at 16384 ids; 50021 with one of them a third of the list: 12 and 9 (50 without the
 // blocks' sums).
 constexpr int FEW = 64;
 
@@ -582,10 +588,11 @@ __global__ __launch_bounds__(1024) void table_join_long_kernel(const Sum s) {
 }
 
 inline int64_t round_up(int64_t n, int64_t k) { return (n + k - 1) / k * k; }
-// Neighbours that a group of lanes adds up.  Few make more groups and more parts: 16384 ids, 2048 columns, bf16, dout in the last-level cache: 27 us
-// with 8, 49 with 32; the parts of longer lists are worth more than their groups.
-inline int chunk_of(int64_t n) { return n <= MANY ? 8 : 32; }
-inline int items_of(int64_t n) { return n <= 65536 ? 8 : 16; }
+// Neighbours that a group of lanes adds up.  Few make more groups and more parts.  us of a gradient with 8 / 32, uniform ids, 32000 rows, bf16: 16384 x 128
+// 28 / 36, 16384 x 2048 59 / 59, 65536 x 512 66 / 65, 131072 x 1024 189 / 160, 262144 x 2048 559 / 405
+inline int chunk_of(int64_t n, int64_t dim) { return n * dim <= (1 << 25) ? 8 : 32; }
+// Keys of a thread of the radix sort: 70000 ids 61 us with 8, 78 with 16, 262144 86 / 98, 1048576 169 / 155
+inline int items_of(int64_t n) { return n <= (1 << 19) ? 8 : 16; }
 
 struct Layout { int64_t keys[2], places[2], counts, partial, blocks, bytes; };
 Layout layout_of(int64_t n, int64_t dim) {
@@ -594,8 +601,8 @@ Layout layout_of(int64_t n, int64_t dim) {
   auto take = [&](int64_t bytes) { const int64_t p = at; at += round_up(bytes, 256); return p; };
   for (int k = 0; k < 2; ++k) { l.keys[k] = take(n * 4); l.places[k] = take(n * 4); }
   l.counts = take((n + 256 * items_of(n) - 1) / (256 * items_of(n)) * BINS * 4);
-  l.partial = take((n + chunk_of(n) - 1) / chunk_of(n) * 2 * dim * 4);
-  l.blocks = take((n + chunk_of(n) - 1) / chunk_of(n) / FEW * dim * 4);
+  l.partial = take((n + chunk_of(n, dim) - 1) / chunk_of(n, dim) * 2 * dim * 4);
+  l.blocks = take((n + chunk_of(n, dim) - 1) / chunk_of(n, dim) / FEW * dim * 4);
   l.bytes = at;
   return l;
 }
@@ -613,7 +620,7 @@ void sum_launch(const Sum& s, hipStream_t st) {
 }
 template <int DT>
 void sum_dispatch(const Sum& s, hipStream_t st) {
-  if (chunk_of(s.n) == 8) sum_launch<DT, 8>(s, st);
+  if (chunk_of(s.n, s.dim) == 8) sum_launch<DT, 8>(s, st);
   else sum_launch<DT, 32>(s, st);
 }
 
@@ -682,10 +689,12 @@ extern "C" int pf_embedding_sorted_bwd(const void* dout, int d_dtype, const int6
   char* ws = (char*)workspace;
   const Layout l = layout_of(n_ids, dim);
   Sum s = {dout, (const int*)(ws + l.keys[0]), (const int*)(ws + l.places[0]), dtable, (float*)(ws + l.partial), (float*)(ws + l.blocks), n_ids, dim, vocab,
-           (n_ids + chunk_of(n_ids) - 1) / chunk_of(n_ids), (float)scale, 0, t_dtype == PF_F32, accumulate != 0};
+           (n_ids + chunk_of(n_ids, dim) - 1) / chunk_of(n_ids, dim), (float)scale, 0, t_dtype == PF_F32, accumulate != 0};
   s.lg = lanes_of(dim);
   if (n_ids <= FEW_IDS) {
+    // (64 KB of zeros, and a thousand workgroups: 1000 x 128, bf16, 256 ids 89 us on four of them)
     int64_t own = 65536 / (dim * pf_dtype_size(t_dtype));
+    own = own < vocab / 1024 ? own : vocab / 1024;
     own = own < 1 ? 1 : own > 1024 ? 1024 : own;
     const dim3 grid((unsigned)((vocab + own - 1) / own));
 #define PF_TF(DT) \

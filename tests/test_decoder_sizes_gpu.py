@@ -3,7 +3,7 @@ import pytest
 import torch
 import torch.nn.functional as F
 
-from test_decoder_ops_gpu import IGNORE, TYPES, U32, head_inputs, head_reference, within
+from test_decoder_ops_gpu import IGNORE, TYPES, U32, head_inputs, head_reference, table_reference, within
 
 pytestmark = pytest.mark.gpu
 
@@ -100,4 +100,21 @@ def test_linear_cross_entropy_in_shares_by_the_count(dtype, scored):
     term, bound, rh, eh, rw, ew = head_reference(h.detach(), w.detach(), y, 0, "sum", 0.0, torch.ones((), device="cuda"))
     within(loss.detach(), term, bound, torch.float32)
     within(dh, rh, eh, dtype)
+    within(dw, rw, ew, dtype)
+
+
+@pytest.mark.parametrize("n,V,D", [(256, 1, 2100), (256, 3, 600), (70, 5000, 1100), (65, 2, 513), (256, 1500, 1024), (1, 7, 4000), (200, 2, 30)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_embedding_gradient_of_a_few_ids_in_wide_rows(dtype, n, V, D):
+    """One launch does it all: rows that several wavefronts share, tokens that most of the list is, one row to a workgroup or many."""
+    from pfeife_amd.layers import embedding
+
+    g = torch.Generator().manual_seed(n + D)
+    ids = torch.randint(0, V, (n,), generator=g)
+    ids[n // 4: n // 2] = V - 1
+    ids = ids.cuda()
+    w = torch.randn(V, D, generator=g).to(dtype).cuda().requires_grad_()
+    up = torch.randn(n, D, generator=g).to(dtype).cuda()
+    dw, = torch.autograd.grad(embedding(ids, w, scale=1.5), w, up)
+    rw, ew = table_reference(ids, w, 1.5, None, up)
     within(dw, rw, ew, dtype)
