@@ -180,22 +180,25 @@ __global__ __launch_bounds__(256) void head_index_gather_kernel(const Labels y, 
   }
 }
 
-// Every token's statistics of all blocks merged, its loss; 32 tokens to a workgroup, 32 threads to a token.  The sum in 64 bits: a
-// loss near zero is the logarithm of a sum near one.
+// Every token's statistics of all blocks merged, its loss; TOKENS to a workgroup, 1024 / TOKENS threads to a token.  The sum in 64 bits: a
+// loss near zero is the logarithm of a sum near one.  A chain of latencies; us with 8 and 32 tokens to a workgroup: 16 of them with 1000 blocks each 4.4 / 7.5, 2048 with
+// 1024 9.8 / 10.7, 4662 with 391 7.6 / 6.6, 8192 with 250 11.8 / 7.0.
+template <int TOKENS>
 __global__ __launch_bounds__(1024) void head_merge_kernel(const PfHeadPart* part, int64_t blocks, int64_t n_max, const float* zl, Kept k, double z_loss,
                                                           int64_t T, int shift, double* terms, float* out) {
-  __shared__ float tops[32][33];
-  __shared__ double sums[32][33];
-  const int t = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  constexpr int SLICES = 1024 / TOKENS;
+  __shared__ float tops[16][TOKENS];
+  __shared__ double sums[16][TOKENS];
+  const int t = threadIdx.x % TOKENS, slice = threadIdx.x / TOKENS;
   const int n = *k.count;
-  const int64_t c = (int64_t)blockIdx.x * 32 + t;
+  const int64_t c = (int64_t)blockIdx.x * TOKENS + t;
   float m = LOWEST;
   double s = 0;
   if (c < n) {
-    for (int64_t i0 = slice; i0 < blocks; i0 += 32 * 8) {      // (eight loads on their way at once)
+    for (int64_t i0 = slice; i0 < blocks; i0 += SLICES * 8) {      // (eight loads on their way at once)
       PfHeadPart p[8];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) p[q] = i0 + 32 * q < blocks ? part[(i0 + 32 * q) * n_max + c] : PfHeadPart{LOWEST, 0.f};
+      for (int q = 0; q < 8; ++q) p[q] = i0 + SLICES * q < blocks ? part[(i0 + SLICES * q) * n_max + c] : PfHeadPart{LOWEST, 0.f};
       float x = m;
 #pragma unroll
       for (int q = 0; q < 8; ++q) x = fmaxf(x, p[q].top);
@@ -205,16 +208,28 @@ __global__ __launch_bounds__(1024) void head_merge_kernel(const PfHeadPart* part
       m = x;
     }
   }
-  tops[slice][t] = m;
-  sums[slice][t] = s;
+#pragma unroll
+  for (int o = TOKENS; o < 64; o <<= 1) {
+    const float om = __shfl_xor(m, o, 64);
+    const double os = __shfl_xor(s, o, 64);
+    const float x = fmaxf(m, om);
+    s = s * (double)__builtin_amdgcn_exp2f((m - x) * LOG2E) + os * (double)__builtin_amdgcn_exp2f((om - x) * LOG2E);
+    m = x;
+  }
+  if ((int)(threadIdx.x & 63) < TOKENS) {
+    tops[threadIdx.x >> 6][t] = m;
+    sums[threadIdx.x >> 6][t] = s;
+  }
   __syncthreads();
-  if (threadIdx.x >= 32) return;
+  if (threadIdx.x >= TOKENS) return;
   double term = 0;
   if (c < n) {
     float top = LOWEST;
-    for (int i = 0; i < 32; ++i) top = fmaxf(top, tops[i][t]);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, tops[i][t]);
     double total = 0;
-    for (int i = 0; i < 32; ++i) total += sums[i][t] * (double)__builtin_amdgcn_exp2f((tops[i][t] - top) * LOG2E);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) total += sums[i][t] * (double)__builtin_amdgcn_exp2f((tops[i][t] - top) * LOG2E);
     const double ls = log(total), lse = (double)top + ls;
     const int l = k.lab[c];
     term = l < 0 ? (double)NAN : ((double)top - (double)zl[c]) + ls + z_loss * lse * lse;
@@ -602,8 +617,12 @@ extern "C" int pf_linear_ce_fwd(const void* hidden, int dtype, int64_t B, int64_
       blocks += pf_head_blocks(p.rows, s.n_max, s.depth);
     }
   }
-  hipLaunchKernelGGL(head_merge_kernel, dim3((unsigned)((s.n_max + 31) / 32)), dim3(1024), 0, st, w.part, blocks, s.n_max, w.zl, k, z_loss, T > 0 ? T : 1, shift,
-                     reduction == 0 ? nullptr : w.terms, out);
+#define PF_HM(TOKENS) \
+  hipLaunchKernelGGL(head_merge_kernel<TOKENS>, dim3((unsigned)(s.n_max / TOKENS)), dim3(1024), 0, st, w.part, blocks, s.n_max, w.zl, k, z_loss, T > 0 ? T : 1, shift, \
+                     reduction == 0 ? nullptr : w.terms, out)
+  if (s.n_max <= 2048) PF_HM(8);
+  else PF_HM(32);
+#undef PF_HM
   if (reduction != 0) hipLaunchKernelGGL(head_reduce_kernel, dim3(1), dim3(1024), 0, st, w.terms, k.count, reduction == 1, loss);
   PF_CHECK_LAUNCH(c.who);
   return PF_OK;
