@@ -57,10 +57,11 @@ struct PfHeadProduct {
   const float* unscale;      // both gradients are divided by this
 };
 
-// Tile of the logits' product (vocabulary rows x tokens) and the rows of one wavefront's block in it, which leaves one partial statistic
+// Tile of the logits' product (vocabulary rows x tokens) and the rows of one wavefront's block in it, which leaves one partial statistic.
+// us of a forward pass, 2048 columns, 32000 classes, bf16, on 64x64 / 256x128 / 256x256: 64 tokens 39.7 / 42 / -, 128 48 / 43 / -, 256 73 / 48 / 61, 512 123 / 77 / 70
 enum { PF_HEAD_64x64, PF_HEAD_256x128, PF_HEAD_256x256 };
 inline int pf_head_tile(int64_t n_max, int64_t depth) {
-  return n_max <= 64 ? PF_HEAD_64x64 : depth % 64 == 0 && n_max > 128 ? PF_HEAD_256x256 : PF_HEAD_256x128;
+  return n_max <= 64 ? PF_HEAD_64x64 : depth % 64 == 0 && n_max > 256 ? PF_HEAD_256x256 : PF_HEAD_256x128;
 }
 inline int64_t pf_head_blocks(int64_t rows, int64_t n_max, int64_t depth) {
   switch (pf_head_tile(n_max, depth)) {

@@ -457,7 +457,7 @@ bool sizes_of(const Call& c, Sizes& s, bool back) {
   s.copy_w = s.depth != c.D || !pf_aligned(c.w, 16);
   // Whole stages of the fastest tile: where the weight is copied anyway, and where many tokens pay for a copy.  us of a step, 1000 columns, 50000 classes, bf16,
   // on the tile for any multiple of 8 and on the other behind copies: 1024 tokens 567 and 589, 2048 937 and 875, 4096 1780 and 1546.
-  if (es == 2 && s.n_max > 128 && (s.copy_w || s.n_max >= 2048)) {
+  if (es == 2 && s.n_max > 256 && (s.copy_w || s.n_max >= 2048)) {
     s.depth = round_up(s.depth, 64);
     s.copy_w = s.copy_w || s.depth != c.D;
   }
