@@ -287,6 +287,8 @@ int PF_H_CAT(pf_head_dw_, PF_X_DT)(const PfHeadProduct& p, hipStream_t st) {
   d.M = p.rows; d.N = p.dim; d.K = p.n_max;
   d.A = p.dz; d.lda = p.n_max; d.B = p.ht; d.ldb = p.n_max; d.C = p.dw; d.ldc = p.ldw_out;
   d.unscale_by = p.unscale;
+  // (one tile for all sizes, the widest runs of a row's stores: a step of the weight alone with 64 tokens, 2048 columns, 32000 classes, bf16 100 us, on 256x128
+  // 104, 128x128 113, 64x64 137; with 2048 tokens 653, 682, 726, 838)
   using T = XTile<PF_XT_256x256w4>;
   GemmGrid g;
   g.tiles_m = (int)((d.M + T::BM - 1) / T::BM);
