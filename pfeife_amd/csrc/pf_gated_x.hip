@@ -187,7 +187,8 @@ template <int KEEP> int forward(const PfGatedProduct& p, hipStream_t st) {
   const int best = pf_gemm_best_tile(d);
   d.N = p.ffn;
   const GatedTail<KEEP> tail = {(uint16_t*)p.y, p.ldy, p.kept, p.half, p.exps, p.act, p.ldy % 8 == 0 && pf_aligned(p.y, 16)};
-  // (Where pf_gemm would take a tile of 192 rows the four-wavefront one runs, or the next larger of its kind: three kernels an instantiation.)
+  // The plain product's choice, at most 4 % off the fastest of the four for 16 to 4096 rows of 1024, 2048 and 4096 columns.  (Where pf_gemm would take a
+  // tile of 192 rows the next larger of its kind runs, or the four-wavefront one: three kernels an instantiation.)
   switch (best) {
     case PF_XT_64x64: return launch<PF_XT_64x64>(gated_forward_kernel<PF_XT_64x64, true, KEEP>, d.M, d.N, 32, st, d, tail);
     case PF_XT_128x128w8: return launch<PF_XT_128x128w8>(gated_forward_kernel<PF_XT_128x128w8, true, KEEP>, d.M, d.N, 64, st, d, tail);
