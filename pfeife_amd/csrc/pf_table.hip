@@ -3,9 +3,9 @@
 //   out[i] = scale W[id_i];   dW[v] = scale * sum of dout_i over the i with id_i = v, in 32 bits, rounded once
 //
 // Text holds few tokens very often and most of the table not at all, so the gradient's work is dealt out by the tokens and not by
-// the table's rows: the places are sorted by token (a stable radix sort of two digits, 2^18 rows; three beyond), a
-// group of lanes adds up CHUNK neighbours of the sorted list, and a token whose run crosses chunks has its partial sums added
-// in order by a last kernel.  Which lane adds what follows from the ids alone: the same ids give the same bits.
+// the table's rows: the places are sorted by token (up to MANY by counting what is smaller, beyond by a stable radix sort of two or three
+// digits), a group of lanes adds up CHUNK neighbours of the sorted list, and a token whose run crosses chunks has its partial sums added
+// in order by two last kernels.  Which lane adds what follows from the ids alone: the same ids give the same bits.
 #include "pf_common.h"
 
 namespace {
