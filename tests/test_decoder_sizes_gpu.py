@@ -52,6 +52,23 @@ def test_linear_cross_entropy_counts_on_the_device(dtype, scored):
     within(dw, rw, ew, dtype)
 
 
+@pytest.mark.parametrize("n,D,V", [(48, 257, 1000), (47, 1030, 65), (49, 130, 300), (1, 4, 17), (9, 2051, 1)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_cross_entropy_of_a_few_tokens(dtype, n, D, V):
+    from pfeife_amd.loss import linear_cross_entropy
+
+    h, w, y = head_inputs(dtype, 1, n, D, V, masked=0.2)
+    h.requires_grad_()
+    w.requires_grad_()
+    loss = linear_cross_entropy(h, w, y, reduction="none")
+    up = 0.5 + torch.rand(loss.shape, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    dh, dw = torch.autograd.grad(loss, (h, w), up)
+    term, bound, rh, eh, rw, ew = head_reference(h.detach(), w.detach(), y, 0, "none", 0.0, up)
+    within(loss.detach(), term, bound, torch.float32)
+    within(dh, rh, eh, dtype)
+    within(dw, rw, ew, dtype)
+
+
 def test_embedding_of_more_ids_than_a_launch_takes():
     from pfeife_amd.layers import embedding
 
