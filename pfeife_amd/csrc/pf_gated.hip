@@ -234,6 +234,114 @@ int few(int r, const void* x, const void* w, int64_t depth, int64_t rows, int64_
   return r == 1 ? few_launch<DT, 1>(x, w, depth, rows, ffn, act, y, kept, half, kept_f32, st) : few_launch<DT, 2>(x, w, depth, rows, ffn, act, y, kept, half, kept_f32, st);
 }
 
+// A few rows' backward pass in 16 bits, without a transposed weight and without copies of odd widths: bound by the weight's way from memory and its gradient's
+// way there.  us, 2048 to 5632, bf16: dx with its join 21 for one row, 26 for four, 35 for eight, where transpose, product and join take 31; the weight's
+// gradient 10, 11 and 15, 22 for sixteen, and as a matrix product 36.
+constexpr int FEW_DX = 4, FEW_DW = 16, FEW_PARTS = 64;
+
+// dx's shares: a wavefront takes 512 columns and every so many 32 rows of the weight, a workgroup's four wavefronts add up in LDS; part [share][row][ld]
+template <int DT, int R>
+__global__ __launch_bounds__(256) void gated_few_dx_kernel(const uint16_t* __restrict__ dgu, int64_t wide, const uint16_t* __restrict__ w, int64_t rows, int64_t ffn, int64_t D, float* __restrict__ part,
+                                                           int64_t ld) {
+  __shared__ float sums[3][R][512];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t c = (int64_t)blockIdx.x * 512 + lane * 8, left = D - c, blocks = (ffn + 31) / 32;
+  float acc[R][8];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc[r][k] = 0.f;
+  for (int64_t q = (int64_t)blockIdx.y * 4 + wave; q < 2 * blocks; q += (int64_t)gridDim.y * 4) {
+    const int64_t z = q / blocks, k0 = q % blocks * 32, k1 = k0 + 32 < ffn ? k0 + 32 : ffn;
+    for (int64_t k = k0; k < k1; k += 8) {      // (columns of dg and du past ffn are zeros up to a multiple of 8)
+      float v[8][8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint4 bits = left > 0 ? pf_load_loose(w + (z * ffn + (k + j < ffn ? k + j : ffn - 1)) * D + c, left) : make_uint4(0, 0, 0, 0);
+        Vec8<DT>::load(&bits, 0, v[j]);
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float d[8];
+        Vec8<DT>::load(dgu, (r < rows ? r : rows - 1) * 2 * wide + z * wide + k, d);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[r][e] = fmaf(d[j], v[j][e], acc[r][e]);
+      }
+    }
+  }
+  if (wave > 0) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sums[wave - 1][r][e * 64 + lane] = acc[r][e];
+  }
+  __syncthreads();
+  if (wave > 0 || left <= 0) return;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (r >= rows) break;
+#pragma unroll
+    for (int s = 0; s < 3; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[r][e] += sums[s][r][e * 64 + lane];
+    Vec8<PF_F32>::store(part, (blockIdx.y * rows + r) * ld + c, acc[r]);
+  }
+}
+
+// The weight's gradient: a wavefront takes 16 of its rows and 512 columns
+template <int DT>
+__global__ __launch_bounds__(256) void gated_few_dw_kernel(const uint16_t* __restrict__ dgu, int64_t wide, const uint16_t* __restrict__ x, int64_t rows, int64_t ffn, int64_t D,
+                                                           uint16_t* __restrict__ dw) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t f0 = ((int64_t)blockIdx.x * 4 + wave) * 16, c = (int64_t)blockIdx.y * 512 + (threadIdx.x & 63) * 8, z = blockIdx.z;
+  if (f0 >= ffn || c >= D) return;
+  float acc[16][8];
+#pragma unroll
+  for (int f = 0; f < 16; ++f)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[f][e] = 0.f;
+#pragma unroll 2
+  for (int64_t r = 0; r < rows; ++r) {
+    float v[8], d[16];
+    const uint4 bits = pf_load_loose(x + r * D + c, D - c);
+    Vec8<DT>::load(&bits, 0, v);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float half[8];
+      Vec8<DT>::load(dgu, r * 2 * wide + z * wide + (f0 + 8 * h < wide ? f0 + 8 * h : f0), half);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) d[8 * h + k] = half[k];
+    }
+#pragma unroll
+    for (int f = 0; f < 16; ++f)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[f][e] = fmaf(d[f], v[e], acc[f][e]);
+  }
+#pragma unroll
+  for (int f = 0; f < 16; ++f)
+    if (f0 + f < ffn) {
+      uint4 o;
+      Vec8<DT>::store(&o, 0, acc[f]);
+      pf_store_loose(dw + (z * ffn + f0 + f) * D + c, D - c, o);
+    }
+}
+
+template <int DT>
+void few_dx(const void* dgu, int64_t wide, const void* w, int64_t rows, int64_t ffn, int64_t D, float* part, int64_t ld, int parts, hipStream_t st) {
+  const dim3 grid((unsigned)((D + 511) / 512), (unsigned)parts);
+  if (rows == 1)
+    hipLaunchKernelGGL((gated_few_dx_kernel<DT, 1>), grid, dim3(256), 0, st, (const uint16_t*)dgu, wide, (const uint16_t*)w, rows, ffn, D, part, ld);
+  else
+    hipLaunchKernelGGL((gated_few_dx_kernel<DT, FEW_DX>), grid, dim3(256), 0, st, (const uint16_t*)dgu, wide, (const uint16_t*)w, rows, ffn, D, part, ld);
+}
+template <int DT>
+void few_dw(const void* dgu, int64_t wide, const void* x, int64_t rows, int64_t ffn, int64_t D, void* dw, hipStream_t st) {
+  hipLaunchKernelGGL(gated_few_dw_kernel<DT>, dim3((unsigned)((ffn + 63) / 64), (unsigned)((D + 511) / 512), 2), dim3(256), 0, st, (const uint16_t*)dgu, wide,
+                     (const uint16_t*)x, rows, ffn, D, (uint16_t*)dw);
+}
+
 // What lies where.  depth: the width of the rows that the products read, of x and of the weight, which are copied where theirs is
 // another (16 bytes have to lie at their front); wide: that of one half of dg and du, and with 16 bits of the transposed weight; half: that
 // of one half of what is kept.
@@ -245,6 +353,7 @@ int64_t kept_bytes(int dtype, int64_t rows, int64_t ffn, int keep) {
 struct Plan {
   int64_t es, depth, wide, half, chunk;
   bool copy_x, copy_w, narrow;
+  bool few_dx, few_dw;         // kernels of a few rows
   int splits;                  // of dx's sums (with `parts`)
   char* x; char* w; char* wt; char* dgu; char* dw; float* parts; float* gu;
   int64_t bytes;
@@ -310,6 +419,7 @@ int splits_of(int dtype, int64_t rows, int64_t D, int64_t K) {
       pf_gemm_best_tile(d, &t);
     }
     if (s > 1) t += 4.0 + (double)(rows * D) * s * 8.0 / 5.0e6;      // a launch, and the shares' way through memory at 5 TB/s
+    if (s > 1 && K / s / 64 * 64 * s != K) t += 5.0;                 // another for what does not divide
     if (s == 1 || t < best_t) { best = s; best_t = t; }
   }
   return best;
@@ -329,8 +439,11 @@ bool plan_of(Plan& p, const void* x, const void* w, int dtype, int64_t rows, int
     p.depth = round_up(p.depth, 64);
     p.copy_x = p.copy_w = true;
   }
+  p.few_dx = back && !f32 && rows <= FEW_DX;
+  p.few_dw = back && !f32 && rows <= FEW_DW;
   p.narrow = !f32 && D % 8 != 0;
-  p.splits = back ? splits_of(dtype, rows, D, p.wide == ffn ? 2 * ffn : ffn) : 1;
+  const int64_t blocks = (ffn + 31) / 32 * 2;      // (of the weight's rows, to four wavefronts each)
+  p.splits = !back ? 1 : p.few_dx ? (int)(blocks < 4 * FEW_PARTS ? (blocks + 3) / 4 : FEW_PARTS) : splits_of(dtype, rows, D, p.wide == ffn ? 2 * ffn : ffn);
   // rows of one launch: everything it addresses by 32-bit offsets stays below 2 GiB
   const int64_t widest = p.depth > 2 * p.half ? p.depth : 2 * p.half;
   p.chunk = ((1ll << 31) / (widest * p.es) - 512) / 256 * 256;
@@ -344,13 +457,13 @@ bool plan_of(Plan& p, const void* x, const void* w, int dtype, int64_t rows, int
   };
   // (the 16-bit backward pass reads x as the right-hand operand of a reduction over its rows, and of the weight a transposed copy)
   const bool x_as_is = back && !f32 && D % 8 == 0 && pf_aligned(x, 16);
-  if (p.copy_x && !x_as_is) p.x = take(rows * p.depth * p.es);
+  if (p.copy_x && !x_as_is && !p.few_dw) p.x = take(rows * p.depth * p.es);
   if (p.copy_w && (!back || f32)) p.w = take(2 * ffn * p.depth * p.es);
   if (back) {
     p.dgu = take(rows * 2 * p.wide * p.es);
-    if (!f32) p.wt = take(p.depth * 2 * p.wide * 2);
-    if (p.narrow) p.dw = take(2 * ffn * p.depth * 2);
-    if (p.splits > 1 || p.narrow) p.parts = (float*)take(p.splits * rows * p.depth * 4);
+    if (!f32 && !p.few_dx) p.wt = take(p.depth * 2 * p.wide * 2);
+    if (p.narrow && !p.few_dw) p.dw = take(2 * ffn * p.depth * 2);
+    if (p.splits > 1 || p.narrow || p.few_dx) p.parts = (float*)take(p.splits * rows * p.depth * 4);
   } else if (keep == PF_KEEP_8BIT && few_rows(rows, p.depth, 2) > 0) {
     p.gu = (float*)take(rows * 2 * p.half * 4);
   } else if (f32 && keep == PF_KEEP_NONE) {
@@ -483,12 +596,22 @@ extern "C" int pf_gated_linear_bwd(const void* x, int dtype, int64_t rows, int64
   } else {
     split_launch(dtype, keep, dy, kept, p.half, rows, ffn, p.dgu, p.wide, act, st);
   }
+  auto join = [&] {
+    const int64_t lanes = D % 8 == 0 ? 512 : 64, units = (rows * ((D + lanes - 1) / lanes) + 3) / 4;
+    const dim3 grid((unsigned)(units < 16384 ? units : 16384));
+    if (D % 8 == 0) hipLaunchKernelGGL(gated_join_kernel<8>, grid, dim3(256), 0, st, p.parts, p.depth, p.splits, rows, D, dx, dtype);
+    else hipLaunchKernelGGL(gated_join_kernel<1>, grid, dim3(256), 0, st, p.parts, p.depth, p.splits, rows, D, dx, dtype);
+  };
   const bool wide_x = p.x != nullptr && dweight != nullptr;
   if (wide_x) pf_rows_widen(x, rows, D, p.x, p.depth, es, st);
   PF_CHECK_LAUNCH(who);
   const char* xs = wide_x ? p.x : (const char*)x;
   const int64_t ldx = wide_x ? p.depth : D;
-  if (dx) {
+  if (dx && p.few_dx) {
+    if (dtype == PF_F16) few_dx<PF_F16>(p.dgu, p.wide, weight, rows, ffn, D, p.parts, p.depth, p.splits, st);
+    else few_dx<PF_BF16>(p.dgu, p.wide, weight, rows, ffn, D, p.parts, p.depth, p.splits, st);
+    join();
+  } else if (dx) {
     const bool parts = p.parts != nullptr;
     void* c = parts ? (void*)p.parts : dx;
     const int64_t ldc = parts ? p.depth : D, n = parts && !f32 ? round_up(D, 8) : D;
@@ -511,14 +634,12 @@ extern "C" int pf_gated_linear_bwd(const void* x, int dtype, int64_t rows, int64
       if (rc == PF_OK) rc = product(dtype, c_dtype, 0, 0, rows, n, 2 * p.wide, p.dgu, 2 * p.wide, p.wt, 2 * p.wide, c, ldc, 0, st, p.splits);
     }
     if (rc != PF_OK) return rc;
-    if (parts) {
-      const int64_t lanes = D % 8 == 0 ? 512 : 64, units = (rows * ((D + lanes - 1) / lanes) + 3) / 4;
-      const dim3 grid((unsigned)(units < 16384 ? units : 16384));
-      if (D % 8 == 0) hipLaunchKernelGGL(gated_join_kernel<8>, grid, dim3(256), 0, st, p.parts, p.depth, p.splits, rows, D, dx, dtype);
-      else hipLaunchKernelGGL(gated_join_kernel<1>, grid, dim3(256), 0, st, p.parts, p.depth, p.splits, rows, D, dx, dtype);
-    }
+    if (parts) join();
   }
-  if (dweight) {
+  if (dweight && p.few_dw) {
+    if (dtype == PF_F16) few_dw<PF_F16>(p.dgu, p.wide, x, rows, ffn, D, dweight, st);
+    else few_dw<PF_BF16>(p.dgu, p.wide, x, rows, ffn, D, dweight, st);
+  } else if (dweight) {
     char* out = p.narrow ? p.dw : (char*)dweight;
     const int64_t ldc = p.narrow ? p.depth : D, n = p.narrow ? round_up(D, 8) : D;
     const int64_t m = halves == 1 ? 2 * ffn : ffn;

@@ -135,3 +135,19 @@ def test_embedding_gradient_of_a_few_ids_in_wide_rows(dtype, n, V, D):
     dw, = torch.autograd.grad(embedding(ids, w, scale=1.5), w, up)
     rw, ew = table_reference(ids, w, 1.5, None, up)
     within(dw, rw, ew, dtype)
+
+
+@pytest.mark.parametrize("n,D,ffn", [(1, 1030, 333), (4, 515, 40), (3, 8, 1), (4, 2048, 2050), (5, 77, 129), (16, 513, 31), (17, 513, 31), (2, 64, 9000)])
+@pytest.mark.parametrize("dtype,kept", [(torch.float16, "16bit"), (torch.bfloat16, "8bit")])
+def test_gated_linear_backward_of_a_few_rows(dtype, kept, n, D, ffn):
+    """Kernels of their own up to 4 rows (x) and 16 (weight): widths that end inside a lane's eight columns, a block of rows, a half."""
+    from pfeife_amd.layers import gated_linear
+    from test_decoder_ops_gpu import gated_check
+
+    g = torch.Generator().manual_seed(n + D)
+    x = torch.randn(n, D, generator=g).to(dtype).cuda().requires_grad_()
+    w = (torch.randn(2 * ffn, D, generator=g) * D ** -0.5).to(dtype).cuda().requires_grad_()
+    up = torch.randn(n, ffn, generator=g).to(dtype).cuda()
+    y = gated_linear(x, w, act="gelu", kept=kept)
+    dx, dw = torch.autograd.grad(y, (x, w), up)
+    gated_check(x.detach(), w.detach(), "gelu", kept, up, y.detach(), dx, dw)
