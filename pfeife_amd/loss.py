@@ -495,15 +495,15 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
         strides = grad.stride() if reduction == 0 else (0, 0)
         _call(hidden, "pf_linear_ce_bwd", *head, z_loss, int(reduction == 1), kept.data_ptr(), grad.data_ptr(), *strides, _at(dh), _at(dw), work.data_ptr())
         if scaled and dh is not None:
-            dh._pf_times = dh._version, functools.partial(_hidden_times, (head[7], dtype, B * T, D, V), dh, (weight, kept, work))
+            # (not dh itself: a cycle would keep the workspace until Python looks for one; of the weight only where it lies)
+            dh._pf_times = dh._version, functools.partial(_hidden_times, (head[7], dtype, B * T, D, V), (dh.shape, dh.dtype, dh.device), kept, work)
         return dh, dw, None
 
 
-def _hidden_times(sizes, like, keep, factor, out):
+def _hidden_times(sizes, like, kept, work, factor, out):
     """The hidden state's gradient times a loss scale, rounded once, from the fp32 sums that the backward pass left; -> is it written."""
-    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or not out.is_contiguous():
+    if (out.shape, out.dtype, out.device) != like or not out.is_contiguous():
         return False
-    _, kept, work = keep
     _call(out, "pf_linear_ce_hidden_grad", *sizes, kept.data_ptr(), factor.data_ptr(), out.data_ptr(), work.data_ptr())
     return True
 
