@@ -486,6 +486,8 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
         hidden, weight, kept = ctx.saved_tensors
         z_loss, reduction, scaled = ctx.cfg
         B, T, D = hidden.shape
+        if grad.numel() == 0:      # ("none" of no token: a gradient without an address)
+            return *(torch.zeros(t.shape, dtype=t.dtype, device=t.device) if n else None for t, n in zip((hidden, weight), ctx.needs_input_grad)), None
         V, dtype, dev = weight.shape[0], _CODE[hidden.dtype], hidden.device
         head = (hidden.data_ptr(), dtype, B, T, D, *hidden.stride()[:2], weight.data_ptr(), V)
         work = torch.empty((_need(hidden, "pf_linear_ce_workspace", head[7], dtype, B * T, D, V, 1),), dtype=torch.uint8, device=dev)

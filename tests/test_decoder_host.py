@@ -63,3 +63,16 @@ def test_what_a_scaled_gradient_is_written_to(on_the_cpu):
         assert not loss.scaled_gradient(grad, scale, out)
     grad.add_(1)      # (it is another gradient now)
     assert not loss.scaled_gradient(grad, scale, torch.empty(2, 3, 8, dtype=torch.float16))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shape,shift", [((2, 1), True), ((0, 4), False), ((0, 4), True), ((3, 0), False)])
+def test_a_loss_of_no_token_has_a_gradient_of_zeros(on_the_cpu, dtype, shape, shift):
+    """reduction "none" of nothing: its own gradient has no memory that a kernel could be shown."""
+    h, w = torch.ones(*shape, 8, dtype=dtype).requires_grad_(), torch.ones(5, 8, dtype=dtype).requires_grad_()
+    out = loss.linear_cross_entropy(h, w, torch.zeros(shape, dtype=torch.int64), shift=shift, reduction="none")
+    assert out.numel() == 0
+    loss._tables[-1].lib = None      # (a backward pass that asks the library for anything fails)
+    dh, dw = torch.autograd.grad(out.sum(), (h, w))
+    assert dh.shape == h.shape and dw.shape == w.shape and dh.dtype == dw.dtype == dtype
+    assert not dh.any() and not dw.any()
