@@ -5,6 +5,7 @@ They are ordinary autograd nodes, for the parts of a model that run beside a run
 compiled for a runner a call is one node of the captured graph (`torch.ops.pfeife_amd`), which the stages' lowering knows
 (`executor/lowering.py`)."""
 import math
+from typing import Tuple
 
 import torch
 
@@ -30,14 +31,17 @@ class _EmbeddingFn(torch.autograd.Function):
     @_once
     def backward(ctx, dout):
         ids, = ctx.saved_tensors
-        vocab, scale, padding = ctx.cfg
-        dim, n, dtype = dout.shape[-1], ids.numel(), _CODE[dout.dtype]
-        dout = dout.contiguous()
-        dw = torch.empty((vocab, dim), dtype=dout.dtype, device=dout.device)
-        need = _need(dout, "pf_embedding_sorted_workspace", n, dim)
-        work = torch.empty((need,), dtype=torch.uint8, device=dout.device) if need else None
-        _call(dout, "pf_embedding_sorted_bwd", dout.data_ptr(), dtype, ids.data_ptr(), dw.data_ptr(), dtype, n, dim, vocab, padding, scale, 0, _at(work))
-        return dw, None
+        return _table_gradient(dout, ids, *ctx.cfg), None
+
+
+def _table_gradient(dout, ids, vocab, scale, padding):
+    dim, n, dtype = dout.shape[-1], ids.numel(), _CODE[dout.dtype]
+    dout = dout.contiguous()
+    dw = torch.empty((vocab, dim), dtype=dout.dtype, device=dout.device)
+    need = _need(dout, "pf_embedding_sorted_workspace", n, dim)
+    work = torch.empty((need,), dtype=torch.uint8, device=dout.device) if need else None
+    _call(dout, "pf_embedding_sorted_bwd", dout.data_ptr(), dtype, ids.data_ptr(), dw.data_ptr(), dtype, n, dim, vocab, padding, scale, 0, _at(work))
+    return dw
 
 
 def embedding(ids, weight, *, scale=1.0, padding_idx=None):
@@ -89,17 +93,7 @@ class _GatedLinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, args, want=True):
         act, keep = args
-        keep = keep if want else 0
-        rows, D = x.shape
-        ffn, dtype, dev = weight.shape[0] // 2, _CODE[x.dtype], x.device
-        at, w = x.data_ptr(), weight.data_ptr()
-        kept = None
-        if want:
-            kept = torch.empty((_need(x, "pf_gated_linear_kept", dtype, rows, ffn, keep),), dtype=torch.uint8, device=dev)
-        need = _need(x, "pf_gated_linear_workspace", at, w, dtype, rows, D, ffn, keep, 0)
-        work = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
-        y = torch.empty((rows, ffn), dtype=x.dtype, device=dev)
-        _call(x, "pf_gated_linear_fwd", at, dtype, rows, D, w, ffn, act, keep, y.data_ptr(), _at(kept), _at(work))
+        y, kept = _gated_forward(x, weight, act, keep if want else 0)
         if want:
             ctx.save_for_backward(x, weight, kept)
             ctx.cfg = act, keep
@@ -107,17 +101,34 @@ class _GatedLinearFn(torch.autograd.Function):
 
     @_once
     def backward(ctx, dy):
-        x, weight, kept = ctx.saved_tensors
-        act, keep = ctx.cfg
-        rows, D = x.shape
-        ffn, dtype, dev = weight.shape[0] // 2, _CODE[x.dtype], x.device
-        at, w = x.data_ptr(), weight.data_ptr()
-        work = torch.empty((_need(x, "pf_gated_linear_workspace", at, w, dtype, rows, D, ffn, keep, 1),), dtype=torch.uint8, device=dev)
-        dx = torch.empty((rows, D), dtype=x.dtype, device=dev) if ctx.needs_input_grad[0] else None
-        dw = torch.empty((2 * ffn, D), dtype=x.dtype, device=dev) if ctx.needs_input_grad[1] else None
-        dy = dy.contiguous()
-        _call(x, "pf_gated_linear_bwd", at, dtype, rows, D, w, ffn, act, keep, kept.data_ptr(), dy.data_ptr(), _at(dx), _at(dw), work.data_ptr())
-        return dx, dw, None
+        return *_gated_gradients(dy, *ctx.saved_tensors, *ctx.cfg, *ctx.needs_input_grad[:2]), None
+
+
+def _gated_forward(x, weight, act, keep):
+    """-> (y, what the backward pass starts from; None: nothing)"""
+    rows, D = x.shape
+    ffn, dtype, dev = weight.shape[0] // 2, _CODE[x.dtype], x.device
+    at, w = x.data_ptr(), weight.data_ptr()
+    kept = None
+    if keep:
+        kept = torch.empty((_need(x, "pf_gated_linear_kept", dtype, rows, ffn, keep),), dtype=torch.uint8, device=dev)
+    need = _need(x, "pf_gated_linear_workspace", at, w, dtype, rows, D, ffn, keep, 0)
+    work = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+    y = torch.empty((rows, ffn), dtype=x.dtype, device=dev)
+    _call(x, "pf_gated_linear_fwd", at, dtype, rows, D, w, ffn, act, keep, y.data_ptr(), _at(kept), _at(work))
+    return y, kept
+
+
+def _gated_gradients(dy, x, weight, kept, act, keep, want_x, want_weight):
+    rows, D = x.shape
+    ffn, dtype, dev = weight.shape[0] // 2, _CODE[x.dtype], x.device
+    at, w = x.data_ptr(), weight.data_ptr()
+    work = torch.empty((_need(x, "pf_gated_linear_workspace", at, w, dtype, rows, D, ffn, keep, 1),), dtype=torch.uint8, device=dev)
+    dx = torch.empty((rows, D), dtype=x.dtype, device=dev) if want_x else None
+    dw = torch.empty((2 * ffn, D), dtype=x.dtype, device=dev) if want_weight else None
+    dy = dy.contiguous()
+    _call(x, "pf_gated_linear_bwd", at, dtype, rows, D, w, ffn, act, keep, kept.data_ptr(), dy.data_ptr(), _at(dx), _at(dw), work.data_ptr())
+    return dx, dw
 
 
 def gated_linear(x, weight, *, act="silu", kept="16bit"):
@@ -165,8 +176,9 @@ def _check_gated(x, weight, act, kept):
         raise RuntimeError("%s: kept is '16bit', or for 16-bit operands '8bit' (got %r for %s)" % (who, kept, x.dtype))
 
 
-# A call inside a graph that is being captured is a node of it.  What its result looks like is all that capturing asks; a runner's stages run the
-# nodes by their lowering, and whatever else runs a captured graph (the compiler's other backends) finds the functions above.
+# A call inside a graph that is being captured is a node of it, and so is its backward pass where that is traced as well.  What their results look
+# like is all that capturing asks; a runner's stages run the forward nodes by their lowering, and whatever else runs a captured graph (the compiler's
+# other backends) runs the functions above.
 @torch.library.custom_op("pfeife_amd::embedding", mutates_args=())
 def _embedding_op(ids: torch.Tensor, weight: torch.Tensor, scale: float, padding_idx: int) -> torch.Tensor:
     return embedding(ids, weight.detach(), scale=scale, padding_idx=None if padding_idx < 0 else padding_idx)
@@ -176,6 +188,17 @@ def _embedding_op(ids: torch.Tensor, weight: torch.Tensor, scale: float, padding
 def _(ids, weight, scale, padding_idx):
     _check_embedding(ids, weight, scale, None if padding_idx < 0 else padding_idx)
     return weight.new_empty(tuple(ids.shape) + (weight.shape[1],))
+
+
+@torch.library.custom_op("pfeife_amd::embedding_backward", mutates_args=())
+def _embedding_backward_op(grad: torch.Tensor, ids: torch.Tensor, rows: int, scale: float, padding_idx: int) -> torch.Tensor:
+    _table(grad, "embedding")
+    return _table_gradient(grad, ids.contiguous(), rows, scale, padding_idx)
+
+
+@_embedding_backward_op.register_fake
+def _(grad, ids, rows, scale, padding_idx):
+    return grad.new_empty((rows, grad.shape[-1]))
 
 
 @torch.library.custom_op("pfeife_amd::gated_linear", mutates_args=())
@@ -189,26 +212,44 @@ def _(x, weight, act, kept):
     return x.new_empty(tuple(x.shape[:-1]) + (weight.shape[0] // 2,))
 
 
-def _save(ctx, inputs, output):
+# An operator of the graph hands over one result, so both products are formed again here (rounded as kept says, as where they are kept); what is not wanted
+# is empty
+@torch.library.custom_op("pfeife_amd::gated_linear_backward", mutates_args=())
+def _gated_linear_backward_op(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, act: str, kept: str, want_x: bool,
+                              want_weight: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    _table(x, "gated_linear")
+    rows, weight = x.reshape(math.prod(x.shape[:-1]), x.shape[-1]).contiguous(), weight.contiguous()
+    _, held = _gated_forward(rows, weight, ACTS[act], KEPT[kept])
+    dx, dw = _gated_gradients(grad, rows, weight, held, ACTS[act], KEPT[kept], want_x, want_weight)
+    return dx.reshape(x.shape) if want_x else x.new_empty(0), dw if want_weight else weight.new_empty(0)
+
+
+@_gated_linear_backward_op.register_fake
+def _(grad, x, weight, act, kept, want_x, want_weight):
+    return x.new_empty(x.shape if want_x else 0), weight.new_empty(weight.shape if want_weight else 0)
+
+
+def _save_embedding(ctx, inputs, output):
+    ids, weight, scale, padding = inputs
+    ctx.save_for_backward(ids)
+    ctx.rest = weight.shape[0], scale, padding
+
+
+def _embedding_backward(ctx, grad):
+    ids, = ctx.saved_tensors
+    return None, torch.ops.pfeife_amd.embedding_backward.default(grad, ids, *ctx.rest), None, None
+
+
+def _save_gated_linear(ctx, inputs, output):
     ctx.save_for_backward(*inputs[:2])
     ctx.rest = inputs[2:]
 
 
-def _embedding_backward(ctx, grad):
-    ids, weight = ctx.saved_tensors
-    scale, padding = ctx.rest
-    with torch.enable_grad():
-        w = weight.detach().requires_grad_()
-        out = embedding(ids, w, scale=scale, padding_idx=None if padding < 0 else padding)
-    return None, torch.autograd.grad(out, w, grad)[0], None, None
-
-
 def _gated_linear_backward(ctx, grad):
-    x, weight = (t.detach().requires_grad_() for t in ctx.saved_tensors)
-    with torch.enable_grad():
-        y = gated_linear(x, weight, act=ctx.rest[0], kept=ctx.rest[1])
-    return *torch.autograd.grad(y, (x, weight), grad), None, None
+    want = ctx.needs_input_grad[:2]
+    grads = torch.ops.pfeife_amd.gated_linear_backward.default(grad, *ctx.saved_tensors, *ctx.rest, *want)
+    return *(g if w else None for g, w in zip(grads, want)), None, None
 
 
-_embedding_op.register_autograd(_embedding_backward, setup_context=_save)
-_gated_linear_op.register_autograd(_gated_linear_backward, setup_context=_save)
+_embedding_op.register_autograd(_embedding_backward, setup_context=_save_embedding)
+_gated_linear_op.register_autograd(_gated_linear_backward, setup_context=_save_gated_linear)

@@ -1,0 +1,70 @@
+"""`layers.embedding` and `layers.gated_linear` in graphs that something else than a runner compiles or records, without a GPU: tensors of the CPU
+stand for the GPU's, and nothing is launched (results hold whatever their memory held)."""
+import pytest
+import torch
+import torch.nn as nn
+
+from pfeife_amd import layers
+from test_decoder_host import on_the_cpu  # noqa: F401  (a fixture)
+
+
+class Layers(nn.Module):
+    def __init__(self, kept="16bit", dtype=torch.bfloat16):
+        super().__init__()
+        self.table = nn.Parameter(torch.zeros(11, 16, dtype=dtype))
+        self.up = nn.Parameter(torch.zeros(24, 16, dtype=dtype))
+        self.kept = kept
+
+    def forward(self, ids):
+        return layers.gated_linear(layers.embedding(ids, self.table, scale=2.0, padding_idx=-2), self.up, act="gelu", kept=self.kept)
+
+
+IDS = torch.zeros(2, 3, dtype=torch.int64)
+
+
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+@pytest.mark.parametrize("kept,dtype", [("16bit", torch.bfloat16), ("8bit", torch.bfloat16), ("16bit", torch.float32)])
+def test_a_model_that_trains(on_the_cpu, backend, kept, dtype):  # noqa: F811
+    """Forward and backward pass as the compiler's backends take them, those that trace the backward pass among them."""
+    torch._dynamo.reset()
+    model = Layers(kept, dtype)
+    out = torch.compile(model, backend=backend, fullgraph=True)(IDS)
+    assert out.shape == (2, 3, 12) and out.dtype == dtype
+    grads = torch.autograd.grad(out, list(model.parameters()), torch.zeros_like(out))
+    assert [(g.shape, g.dtype) for g in grads] == [(p.shape, dtype) for p in model.parameters()]
+
+
+@pytest.mark.parametrize("frozen", ["table", "up"])
+def test_a_model_with_a_frozen_part(on_the_cpu, frozen):  # noqa: F811
+    torch._dynamo.reset()
+    model = Layers()
+    getattr(model, frozen).requires_grad_(False)
+    out = torch.compile(model, backend="aot_eager", fullgraph=True)(IDS)
+    out.sum().backward()
+    assert all((p.grad is None) == (n == frozen) for n, p in model.named_parameters())
+
+
+def test_the_backward_pass_is_a_node_of_the_traced_graph(on_the_cpu):  # noqa: F811
+    from torch._dynamo.backends.common import aot_autograd
+
+    torch._dynamo.reset()
+    seen = []
+
+    def keep(graph, inputs):
+        seen.append({str(n.target) for n in graph.graph.nodes if n.op == "call_function"})
+        return graph.forward
+
+    out = torch.compile(Layers(), backend=aot_autograd(fw_compiler=keep, bw_compiler=keep), fullgraph=True)(IDS)
+    out.sum().backward()
+    assert {"pfeife_amd.embedding.default", "pfeife_amd.gated_linear.default"} <= seen[0]
+    assert {"pfeife_amd.embedding_backward.default", "pfeife_amd.gated_linear_backward.default"} <= seen[1]
+
+
+def test_second_derivatives_are_refused_there_too(on_the_cpu):  # noqa: F811
+    torch._dynamo.reset()
+    model = Layers()
+    out = torch.compile(model, backend="eager", fullgraph=True)(IDS)
+    for p in (model.up, model.table):
+        g, = torch.autograd.grad(out, p, torch.zeros_like(out).requires_grad_(), create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum() + model.up.square().sum(), model.up)
