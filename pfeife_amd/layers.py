@@ -10,7 +10,7 @@ from typing import Tuple
 import torch
 
 from .hip import ACT_GELU, ACT_GELU_TANH, ACT_RELU, ACT_SILU
-from .loss import _CODE, _LOGITS, _NoContext, _at, _call, _dual, _has_tangent, _need, _once, _table
+from .loss import _CODE, _LOGITS, _NoContext, _at, _call, _dual, _has_tangent, _need, _once, _recorded, _table
 
 ACTS = {"silu": ACT_SILU, "gelu": ACT_GELU, "gelu_tanh": ACT_GELU_TANH, "relu": ACT_RELU}
 KEPT = {"16bit": 1, "8bit": 2}
@@ -52,8 +52,12 @@ def embedding(ids, weight, *, scale=1.0, padding_idx=None):
     out by the tokens, so a token that fills half of a batch costs no more than others.  There are no second and no forward-mode
     derivatives.  A backward pass is captured into a graph, as any of torch's, only while no autograd graph made outside the capture holds
     the same leaves."""
-    if torch.compiler.is_compiling():
+    if torch.compiler.is_compiling() or _recorded():
         return torch.ops.pfeife_amd.embedding.default(ids, weight, float(scale), _table_row(weight, padding_idx))
+    return _embedding(ids, weight, scale, padding_idx)
+
+
+def _embedding(ids, weight, scale, padding_idx):
     if not torch.is_tensor(ids) or not torch.is_tensor(weight):
         raise RuntimeError("embedding: ids and weight are tensors")
     _table(weight, "embedding")
@@ -140,8 +144,12 @@ def gated_linear(x, weight, *, act="silu", kept="16bit"):
     of two, in 17/32 of the memory; the result itself is the same.  The gradient flows to x and weight.  There are no second and no
     forward-mode derivatives.  A backward pass is captured into a graph, as any of torch's, only while no autograd graph made outside the
     capture holds the same leaves."""
-    if torch.compiler.is_compiling():
+    if torch.compiler.is_compiling() or _recorded():
         return torch.ops.pfeife_amd.gated_linear.default(x, weight, act, kept)
+    return _gated_linear(x, weight, act, kept)
+
+
+def _gated_linear(x, weight, act, kept):
     if not torch.is_tensor(x) or not torch.is_tensor(weight):
         raise RuntimeError("gated_linear: x and weight are tensors")
     _table(x, "gated_linear")
@@ -181,7 +189,7 @@ def _check_gated(x, weight, act, kept):
 # other backends) runs the functions above.
 @torch.library.custom_op("pfeife_amd::embedding", mutates_args=())
 def _embedding_op(ids: torch.Tensor, weight: torch.Tensor, scale: float, padding_idx: int) -> torch.Tensor:
-    return embedding(ids, weight.detach(), scale=scale, padding_idx=None if padding_idx < 0 else padding_idx)
+    return _embedding(ids, weight.detach(), scale, None if padding_idx < 0 else padding_idx)
 
 
 @_embedding_op.register_fake
@@ -203,7 +211,7 @@ def _(grad, ids, rows, scale, padding_idx):
 
 @torch.library.custom_op("pfeife_amd::gated_linear", mutates_args=())
 def _gated_linear_op(x: torch.Tensor, weight: torch.Tensor, act: str, kept: str) -> torch.Tensor:
-    return gated_linear(x.detach(), weight.detach(), act=act, kept="16bit")      # (nothing is kept: the backward pass comes here again)
+    return _gated_linear(x.detach(), weight.detach(), act, "16bit")      # (nothing is kept: the backward pass comes here again)
 
 
 @_gated_linear_op.register_fake

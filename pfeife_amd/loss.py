@@ -120,6 +120,21 @@ def _table(t, who):
     return k
 
 
+_C = torch._C
+
+
+def _recorded():
+    """Is a graph being recorded of the calls that are made (make_fx, torch.jit.trace)?  A kernel's launch would not be in it, only the memory that it
+    was about to fill."""
+    return (_C._get_tracing_state() is not None or _C._len_torch_dispatch_stack() > 0 and _C._get_dispatch_mode(_C._TorchDispatchModeKey.PROXY) is not None
+            or _C._dispatch_tls_is_dispatch_key_included(_C.DispatchKey.PreDispatch))
+
+
+def _refuse_recording(who):
+    if not torch.compiler.is_compiling() and _recorded():      # (the compiler leaves such a call out of its graph)
+        raise RuntimeError("%s: the call cannot be recorded in a graph (make_fx, torch.jit.trace)" % who)
+
+
 def _issue(t, launch):
     """On the current stream of the tensor's device, whichever device is the current one."""
     index = t.get_device()
@@ -173,6 +188,7 @@ def _check_rows(who, logits, labels, ignore_index, temperature, shift):
     """What the three losses ask of their logits and labels.  -> (logits [B, T, V] with unit stride over the classes, labels [B, T])"""
     if not torch.is_tensor(logits) or not torch.is_tensor(labels):
         raise RuntimeError("%s: logits and labels are tensors" % who)
+    _refuse_recording(who)
     _table(logits, who)
     shape = logits.shape
     if logits.dtype not in _LOGITS:
@@ -527,6 +543,7 @@ def linear_cross_entropy(hidden, weight, labels, *, ignore_index=-100, z_loss=0.
     who = "linear_cross_entropy"
     if not torch.is_tensor(hidden) or not torch.is_tensor(weight) or not torch.is_tensor(labels):
         raise RuntimeError("%s: hidden, weight and labels are tensors" % who)
+    _refuse_recording(who)
     _table(hidden, who)
     shape = hidden.shape
     if hidden.dtype not in _LOGITS or weight.dtype != hidden.dtype:

@@ -68,3 +68,51 @@ def test_second_derivatives_are_refused_there_too(on_the_cpu):  # noqa: F811
         g, = torch.autograd.grad(out, p, torch.zeros_like(out).requires_grad_(), create_graph=True)
         with pytest.raises(RuntimeError):
             torch.autograd.grad(g.sum() + model.up.square().sum(), model.up)
+
+
+def recorded_by_make_fx(fn, *args):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    return {str(n.target) for n in make_fx(fn)(*args).graph.nodes}
+
+
+def recorded_before_dispatch(fn, *args):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    return {str(n.target) for n in make_fx(fn, pre_dispatch=True)(*args).graph.nodes}
+
+
+def recorded_by_jit(fn, *args):
+    return {n.kind().replace("::", ".") + ".default" for n in torch.jit.trace(fn, args, check_trace=False).graph.nodes()}
+
+
+RECORDERS = pytest.mark.parametrize("record", [recorded_by_make_fx, recorded_before_dispatch, recorded_by_jit])
+
+
+@RECORDERS
+def test_calls_that_are_recorded_are_nodes(on_the_cpu, record):  # noqa: F811
+    """A graph recorded from real calls holds the operators, not the memory that they were about to fill."""
+    table, up = torch.zeros(11, 16), torch.zeros(24, 16)
+    assert "pfeife_amd.embedding.default" in record(lambda ids, w: layers.embedding(ids, w, scale=3.0), IDS, table)
+    assert "pfeife_amd.gated_linear.default" in record(lambda x, w: layers.gated_linear(x, w, act="relu"), torch.zeros(2, 16), up)
+
+
+def test_a_recorded_backward_pass_is_a_node(on_the_cpu):  # noqa: F811
+    up = torch.zeros(24, 16)
+
+    def step(x, w):
+        w = w.detach().requires_grad_()
+        return torch.autograd.grad(layers.gated_linear(x, w), w, torch.ones(2, 12))[0]
+
+    assert "pfeife_amd.gated_linear_backward.default" in recorded_by_make_fx(step, torch.zeros(2, 16), up)
+
+
+@RECORDERS
+def test_losses_that_are_recorded_are_refused(on_the_cpu, record):  # noqa: F811
+    from pfeife_amd import loss
+
+    h, w, y = torch.zeros(2, 3, 8), torch.zeros(5, 8), torch.zeros(2, 3, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="linear_cross_entropy: .*recorded"):
+        record(lambda h, w: loss.linear_cross_entropy(h, w, y), h, w)
+    with pytest.raises(RuntimeError, match="token_logprobs: .*recorded"):
+        record(lambda h: loss.token_logprobs(h, y), h)

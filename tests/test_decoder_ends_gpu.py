@@ -40,3 +40,19 @@ def test_compiled_without_a_runner(backend, kept, dtype):
     got = torch.compile(model, backend=backend, fullgraph=True)(ids)
     assert torch.equal(got, want)
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(got, list(model.parameters()), up), grads))
+
+
+def test_recorded_graphs_run():
+    """A graph recorded of the layers gives what the calls give, on other values too."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from pfeife_amd.layers import embedding, gated_linear
+
+    g = torch.Generator("cuda").manual_seed(6)
+    draw = lambda: (torch.randint(0, 50, (2, 9), device="cuda", generator=g), torch.randn(50, 24, device="cuda", generator=g), torch.randn(34, 24, device="cuda", generator=g))  # noqa: E731
+    both = lambda ids, table, up: gated_linear(embedding(ids, table, scale=0.5), up)  # noqa: E731
+    first = draw()
+    graphs = [make_fx(both)(*first), torch.jit.trace(both, first)]
+    for args in (first, draw()):
+        want = both(*args)
+        assert all(torch.equal(graph(*args), want) for graph in graphs)
