@@ -2584,8 +2584,8 @@ def lower_gated_linear(L, node):
     ffn = N // 2
     if K % 8 or ffn % 8:
         raise Unsupported("gated_linear of %d -> %d columns: both have to be multiples of 8" % (K, ffn))
-    if cd == torch.float32:
-        kept = layers.KEPT["16bit"]
+    if cd == torch.float32 and kept == layers.KEPT["8bit"]:
+        raise Unsupported("gated_linear: kept is '16bit', or for 16-bit operands '8bit' (the stages compute in fp32)")
     w_cd = L.params.shadow(w.buf, cd) if w.param is not None or not w.req_grad else None
     if w_cd is None or not w_cd.is_contiguous():
         raise Unsupported("gated_linear with a weight that is no contiguous parameter")

@@ -170,6 +170,7 @@ def _gated_linear(x, weight, act, kept):
 
 
 def _check_gated(x, weight, act, kept):
+    """(Not whether 8 bits go with the operands' type: a runner's stages compute in one of their own.)"""
     who = "gated_linear"
     if x.dtype not in _LOGITS or weight.dtype != x.dtype:
         raise RuntimeError("%s: x and weight are both fp32, fp16 or bf16 (got %s and %s)" % (who, x.dtype, weight.dtype))
@@ -211,7 +212,7 @@ def _(grad, ids, rows, scale, padding_idx):
 
 @torch.library.custom_op("pfeife_amd::gated_linear", mutates_args=())
 def _gated_linear_op(x: torch.Tensor, weight: torch.Tensor, act: str, kept: str) -> torch.Tensor:
-    return _gated_linear(x.detach(), weight.detach(), act, "16bit")      # (nothing is kept: the backward pass comes here again)
+    return _gated_linear(x.detach(), weight.detach(), act, kept)      # (nothing is kept: the backward pass forms both products again)
 
 
 @_gated_linear_op.register_fake

@@ -116,3 +116,53 @@ def test_losses_that_are_recorded_are_refused(on_the_cpu, record):  # noqa: F811
         record(lambda h, w: loss.linear_cross_entropy(h, w, y), h, w)
     with pytest.raises(RuntimeError, match="token_logprobs: .*recorded"):
         record(lambda h: loss.token_logprobs(h, y), h)
+
+
+@pytest.mark.parametrize("run", ["eager", "aot_eager", recorded_by_make_fx, recorded_by_jit])
+def test_8_bits_of_fp32_operands_are_refused_before_anything_runs(on_the_cpu, run):  # noqa: F811
+    """... as they are where nothing is compiled."""
+    torch._dynamo.reset()
+    model = Layers("8bit", torch.float32)
+    with pytest.raises(RuntimeError, match="kept is '16bit', or for 16-bit operands '8bit'"):
+        if callable(run):
+            run(model, IDS)
+        else:
+            torch.compile(model, backend=run, fullgraph=True)(IDS)
+
+
+def runner_step(model, mixed=None):
+    from oracle.kernels_oracle import OracleKernels
+    from pfeife_amd.mp import PartialRunner, initialize_pfeife, net_states, partial_compiler
+    from pfeife_amd.option import PipeOption
+
+    torch._dynamo.reset()
+    net_states._reset_state_for_tests()
+    initialize_pfeife(device="cpu")
+    runner = PartialRunner(PipeOption(device_cnt=1, batch_cnt=1, batch_size=2, mixed_precision=mixed, loss_scale=1.0, optimizer=dict(type="sgd", lr=0.0)),
+                           kernels=OracleKernels("cpu"))
+    compiled = torch.compile(model, backend=partial_compiler)
+
+    def fn(ids):
+        loss = compiled(ids).float().sum()
+        loss.backward()
+        return loss.detach()
+
+    runner.set_exec_fn(fn)
+    return runner.step(torch.zeros(2, 3, dtype=torch.int64))
+
+
+def test_8_bits_in_a_runner_go_by_what_it_computes_in():
+    """fp32 parameters under mixed precision are operands of 16 bits."""
+    from pfeife_amd.executor.lowering import Unsupported
+
+    assert len(runner_step(Wide("8bit"), "bf16")) == 1
+    with pytest.raises(Unsupported, match="kept is '16bit', or for 16-bit operands '8bit'"):
+        runner_step(Wide("8bit"))
+
+
+class Wide(Layers):
+    """(A runner's widths are multiples of 8.)"""
+
+    def __init__(self, kept):
+        super().__init__(kept, torch.float32)
+        self.up = nn.Parameter(torch.ones(32, 16))

@@ -56,3 +56,19 @@ def test_recorded_graphs_run():
     for args in (first, draw()):
         want = both(*args)
         assert all(torch.equal(graph(*args), want) for graph in graphs)
+
+
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_a_loss_in_a_compiled_function(backend):
+    """The compiler leaves the loss out of its graphs; values and gradients are those of the plain call."""
+    from pfeife_amd.loss import linear_cross_entropy
+
+    torch._dynamo.reset()
+    g = torch.Generator("cuda").manual_seed(8)
+    h = torch.randn(2, 20, 64, device="cuda", generator=g).requires_grad_()
+    w = torch.randn(90, 64, device="cuda", generator=g).requires_grad_()
+    y = torch.randint(0, 90, (2, 20), device="cuda", generator=g)
+    step = lambda h, w: linear_cross_entropy(h * 0.5, w, y, shift=True, z_loss=1e-3) * 2.0  # noqa: E731
+    want, got = step(h, w), torch.compile(step, backend=backend)(h, w)
+    assert torch.equal(got, want)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(got, (h, w)), torch.autograd.grad(want, (h, w))))
