@@ -470,7 +470,7 @@ int64_t piece_rows(int64_t n_max, int64_t V, int64_t size) {
   if (rows < 256) rows = 256;
   return rows < V ? rows : V;
 }
-// ... and of one whose weights a buffer's 32-bit offsets reach
+// Rows that a buffer's 32-bit offsets reach
 int64_t reach_rows(int64_t ldw) { return ((1ll << 31) / (ldw * 2) - 512) / 256 * 256; }
 
 struct Call {
@@ -499,8 +499,10 @@ bool sizes_of(const Call& c, Sizes& s, bool back) {
   s.piece = piece_rows(s.n_max, c.V, es);
   if (es == 2 && s.piece > reach_rows(s.depth)) s.piece = reach_rows(s.depth);
   if (back) s.shares = pf_head_shares(c.dtype, es == 4 && s.n > 0 ? s.n : s.n_max, s.depth, s.piece);
-  return s.n < (1ll << 24) && c.V < (1ll << 31) && s.n_max * s.depth * 4 < (1ll << 31) - 64 && s.piece * s.n_max * es < (1ll << 31) - 64 &&
-         s.depth < (1ll << 19);
+  if (s.n >= (1ll << 24) || c.V >= (1ll << 31) || s.depth >= (1ll << 19)) return false;
+  // what is addressed by 32-bit offsets: forward the gathered rows (fp32: and a piece's logits), backward the fp32 sums of their gradient and a piece's dz
+  if (es == 2 && !back) return s.n_max <= reach_rows(s.depth);
+  return s.n_max * s.depth * 4 < (1ll << 31) - 64 && s.piece * s.n_max * es < (1ll << 31) - 64;
 }
 
 // A block of device memory handed out front to back, each part on a boundary of 256 bytes
@@ -537,12 +539,12 @@ Work carve(Carve& a, const Call& c, const Sizes& s, bool back) {
   return w;
 }
 
-int check_call(const Call& c, const Sizes& s, bool ok) {
+int check_call(const Call& c, const Sizes& s, bool back, bool ok) {
   if (c.dtype != PF_F32 && c.dtype != PF_F16 && c.dtype != PF_BF16) return bad(c.who, "bad dtype");
   if (c.B < 0 || c.T < 0 || c.D <= 0 || c.V <= 0) return bad(c.who, "bad sizes");
   if (!ok) {
-    pf_set_error("%s: %lld tokens of width %lld and %lld classes: too many for one call (the tokens' fp32 gradient has to stay below 2 GiB)", c.who, (long long)s.n,
-                 (long long)c.D, (long long)c.V);
+    pf_set_error("%s: %lld tokens of width %lld and %lld classes: too many for one call (the tokens%s to stay below 2 GiB)", c.who, (long long)s.n, (long long)c.D,
+                 (long long)c.V, back ? "' fp32 gradient has" : " have");
     return PF_ERR_INVALID;
   }
   return PF_OK;
@@ -591,7 +593,7 @@ extern "C" int64_t pf_linear_ce_kept(int64_t tokens) { return kept_bytes(round_u
 extern "C" int64_t pf_linear_ce_workspace(const void* weight, int dtype, int64_t tokens, int64_t D, int64_t V, int backward) {
   const Call c = {"pf_linear_ce_workspace", nullptr, dtype, 1, tokens, D, 0, D, weight, V};
   Sizes s = {};
-  const int rc = check_call(c, s, tokens < 0 || D <= 0 || V <= 0 || sizes_of(c, s, backward != 0));
+  const int rc = check_call(c, s, backward != 0, tokens < 0 || D <= 0 || V <= 0 || sizes_of(c, s, backward != 0));
   if (rc != PF_OK) return rc;
   Carve a = {nullptr};
   carve(a, c, s, backward != 0);
@@ -603,7 +605,7 @@ extern "C" int pf_linear_ce_fwd(const void* hidden, int dtype, int64_t B, int64_
                                 void* workspace, void* stream) {
   const Call c = {"pf_linear_ce_fwd", hidden, dtype, B, T, D, sb, st_, weight, V};
   Sizes s = {};
-  int rc = check_call(c, s, B < 0 || T < 0 || D <= 0 || V <= 0 || sizes_of(c, s, false));
+  int rc = check_call(c, s, false, B < 0 || T < 0 || D <= 0 || V <= 0 || sizes_of(c, s, false));
   if (rc != PF_OK) return rc;
   PF_REQUIRE((shift == 0 || shift == 1) && reduction >= 0 && reduction <= 2, "%s: shift is 0 or 1, reduction 0, 1 or 2", c.who);
   PF_REQUIRE(pf_aligned(kept, 16) && pf_aligned(workspace, 16), "%s: kept and the workspace lie on boundaries of 256 bytes", c.who);
@@ -640,7 +642,8 @@ extern "C" int pf_linear_ce_fwd(const void* hidden, int dtype, int64_t B, int64_
     p.ldw = s.depth; p.depth = s.depth;
     p.hc = w.hc; p.ldh = s.depth; p.n_max = s.n_max;
     p.count = k.count; p.lab = k.lab; p.zl = w.zl;
-    const int64_t reach = reach_rows(s.depth);
+    // (at most 2^23 workgroups of 512 threads to a launch)
+    const int64_t most = (1ll << 23) / ((s.n_max + 127) / 128) * 256, reach = reach_rows(s.depth) < most ? reach_rows(s.depth) : most;
     for (int64_t v0 = 0; v0 < V; v0 += reach) {
       p.v0 = v0;
       p.rows = V - v0 < reach ? V - v0 : reach;
@@ -667,7 +670,7 @@ extern "C" int pf_linear_ce_bwd(const void* hidden, int dtype, int64_t B, int64_
                                 void* workspace, void* stream) {
   const Call c = {"pf_linear_ce_bwd", hidden, dtype, B, T, D, sb, st_, weight, V};
   Sizes s = {};
-  int rc = check_call(c, s, B < 0 || T < 0 || D <= 0 || V <= 0 || sizes_of(c, s, true));
+  int rc = check_call(c, s, true, B < 0 || T < 0 || D <= 0 || V <= 0 || sizes_of(c, s, true));
   if (rc != PF_OK) return rc;
   PF_REQUIRE(kept && workspace && weight && grad && (s.n == 0 || hidden), "%s: null pointer", c.who);
   PF_REQUIRE(pf_aligned(kept, 16) && pf_aligned(workspace, 16), "%s: kept and the workspace lie on boundaries of 256 bytes", c.who);
@@ -747,7 +750,7 @@ extern "C" int pf_linear_ce_hidden_grad(const void* weight, int dtype, int64_t t
                                         const void* workspace, void* stream) {
   const Call c = {"pf_linear_ce_hidden_grad", nullptr, dtype, 1, tokens, D, 0, D, weight, V};
   Sizes s = {};
-  const int rc = check_call(c, s, tokens < 0 || D <= 0 || V <= 0 || sizes_of(c, s, true));
+  const int rc = check_call(c, s, true, tokens < 0 || D <= 0 || V <= 0 || sizes_of(c, s, true));
   if (rc != PF_OK) return rc;
   if (s.n == 0) return PF_OK;
   PF_REQUIRE(kept && dhidden && workspace, "%s: null pointer", c.who);

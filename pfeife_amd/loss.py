@@ -158,12 +158,13 @@ def _call(t, entry, *args):
         raise RuntimeError("%s failed: %s" % (entry, _tables[index].lib.pf_last_error().decode()))
 
 
-def _need(t, entry, *args):
-    """Bytes that an entry point asks for."""
+def _need(t, entry, *args, who=None):
+    """Bytes that an entry point asks for; who: refuses in its place."""
     lib = _tables[t.get_device()].lib
     need = getattr(lib, entry)(*args)
     if need < 0:
-        raise RuntimeError(lib.pf_last_error().decode())
+        said = lib.pf_last_error().decode()
+        raise RuntimeError(said if who is None else said.replace(entry, who, 1))
     return need
 
 
@@ -571,6 +572,9 @@ def linear_cross_entropy(hidden, weight, labels, *, ignore_index=-100, z_loss=0.
     args = (labels.reshape(x.shape[:-1]).contiguous(), int(shift), ignore_index, float(z_loss), _REDUCTIONS[reduction])
     weight = weight.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        tokens = x.shape[0] * x.shape[1]
+        if (tokens + 64) * (shape[-1] + 64) >= 1 << 28:      # (fewer are never too many for a gradient)
+            _need(x, "pf_linear_ce_workspace", weight.data_ptr(), _CODE[x.dtype], tokens, shape[-1], weight.shape[0], 1, who=who)
         out = _LinearCrossEntropyFn.apply(x, weight, args)
     else:
         out = _LinearCrossEntropyFn.forward(_NoContext, x, weight, args, False)

@@ -72,3 +72,30 @@ def test_a_loss_in_a_compiled_function(backend):
     want, got = step(h, w), torch.compile(step, backend=backend)(h, w)
     assert torch.equal(got, want)
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(got, (h, w)), torch.autograd.grad(want, (h, w))))
+
+
+# rows of 1 GiB, whose gradient in fp32 no call could hold; more workgroups than one launch has
+@pytest.mark.parametrize("tokens,D,V", [(131072, 4096, 300), (1 << 22, 64, 66000)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_scores_of_a_long_batch(dtype, tokens, D, V):
+    """A forward pass alone, tokens scored at its ends and here and there."""
+    from test_decoder_ops_gpu import IGNORE, head_reference, within
+
+    from pfeife_amd.loss import linear_cross_entropy
+
+    g = torch.Generator("cuda").manual_seed(9)
+    w = (torch.randn(V, D, device="cuda", generator=g) * D ** -0.5).to(dtype)
+    h = torch.empty(1, tokens, D, device="cuda", dtype=dtype)
+    for part in h.split(1 << 16, dim=1):
+        part.copy_(torch.randn(part.shape, device="cuda", generator=g))
+    at = torch.cat([torch.tensor([0, 1, tokens - 2, tokens - 1], device="cuda"), torch.randint(2, tokens - 2, (600,), device="cuda", generator=g)]).unique()
+    y = torch.full((1, tokens), IGNORE, device="cuda")
+    y[0, at] = torch.randint(0, V, at.shape, device="cuda", generator=g)
+    loss = linear_cross_entropy(h, w, y, reduction="none")
+    every = linear_cross_entropy(h, w, torch.where(y == IGNORE, 7, y), reduction="none")
+    assert torch.isfinite(every).all() and torch.equal(every[0, at], loss[0, at])      # (what is scored beside a token changes nothing of it)
+    rest = loss.clone()
+    rest[0, at] = 0
+    assert not rest.any()
+    term, bound = head_reference(h[:, at], w, y[:, at], 0, "none", 0.0, torch.ones((), device="cuda"))[:2]
+    within(loss[:, at], term, bound, torch.float32)

@@ -76,3 +76,37 @@ def test_a_loss_of_no_token_has_a_gradient_of_zeros(on_the_cpu, dtype, shape, sh
     dh, dw = torch.autograd.grad(out.sum(), (h, w))
     assert dh.shape == h.shape and dw.shape == w.shape and dh.dtype == dw.dtype == dtype
     assert not dh.any() and not dw.any()
+
+
+@pytest.mark.parametrize("dtype,size", [(0, 4), (1, 2), (2, 2)])
+@pytest.mark.parametrize("D", [64, 1024, 4096, 8192])
+def test_how_many_tokens_a_call_takes(dtype, size, D):
+    """A forward pass holds the gathered rows (16 bits: and 512 more rows in reach of a buffer's offsets), a backward pass their gradient in fp32."""
+    from pfeife_amd import hip
+
+    lib = hip.load()
+    in_fp32 = ((1 << 31) - 65) // (D * 4) // 64 * 64
+    for backward, most in ((0, in_fp32 if size == 4 else min(((1 << 31) // (D * 2) - 512) // 256 * 256, (1 << 24) - 1)), (1, in_fp32)):
+        need = lambda n: lib.pf_linear_ce_workspace(None, dtype, n, D, 50, backward)  # noqa: E731
+        assert need(most) > most * D * (4 if backward else size)
+        assert need(most + 1) == -1 and b"too many for one call" in lib.pf_last_error()
+
+
+def test_a_loss_without_a_possible_gradient_is_refused_before_it_runs(on_the_cpu):
+    """... and scored where none is asked for."""
+    from pfeife_amd import hip
+
+    lib = hip.load()
+
+    class Sizes(NothingLaunched):
+        pf_linear_ce_workspace = staticmethod(lambda *args: 1 << 20 if lib.pf_linear_ce_workspace(*args) > 0 else -1)
+        pf_last_error = staticmethod(lib.pf_last_error)
+
+    loss._tables[-1].lib = Sizes()
+    h = torch.zeros(1, dtype=torch.bfloat16).expand(1, 131072, 4096)
+    w, y = torch.zeros(5, 4096, dtype=torch.bfloat16), torch.zeros(1, dtype=torch.int64).expand(1, 131072)
+    assert loss.linear_cross_entropy(h, w, y, reduction="none").shape == (1, 131072)
+    for a, b in ((h.detach().requires_grad_(), w), (h, w.clone().requires_grad_())):
+        with pytest.raises(RuntimeError, match="linear_cross_entropy: .*too many for one call"):
+            loss.linear_cross_entropy(a, b, y)
+    assert loss.linear_cross_entropy(h[:, :65000], w.clone().requires_grad_(), y[:, :65000]).requires_grad
