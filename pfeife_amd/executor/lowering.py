@@ -2564,12 +2564,17 @@ def lower_scaled_embedding(L, node):
 
     def bwd(B):
         g = B.grad_of(outv)
-        if g is None or table.param is None:
+        if g is None:
             return
         gc = g if g.is_contiguous() else _compact(B, g)
         need = B.k.embedding_sorted_workspace(n, dim)
         ws = L.pool.scratch("sorted_ids", (need,), torch.uint8) if need else None
-        B.emit(B.k.embedding_sorted_bwd(gc, ids.buf, L.params.grad(table.param), n, dim, vocab, padding_idx, scale, True, ws))
+        if table.param is not None:
+            B.emit(B.k.embedding_sorted_bwd(gc, ids.buf, L.params.grad(table.param), n, dim, vocab, padding_idx, scale, True, ws))
+            return
+        dtable = B.temp((vocab, dim), gc.dtype)      # (of a table that is computed, or a parameter's view)
+        B.emit(B.k.embedding_sorted_bwd(gc, ids.buf, dtable, n, dim, vocab, padding_idx, scale, False, ws))
+        B.contribute(table, dtable)
 
     if table.req_grad:
         L.add_backward(bwd)

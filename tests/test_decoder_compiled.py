@@ -130,7 +130,7 @@ def test_8_bits_of_fp32_operands_are_refused_before_anything_runs(on_the_cpu, ru
             torch.compile(model, backend=run, fullgraph=True)(IDS)
 
 
-def runner_step(model, mixed=None):
+def runner_step(model, mixed=None, ids=IDS):
     from oracle.kernels_oracle import OracleKernels
     from pfeife_amd.mp import PartialRunner, initialize_pfeife, net_states, partial_compiler
     from pfeife_amd.option import PipeOption
@@ -148,7 +148,7 @@ def runner_step(model, mixed=None):
         return loss.detach()
 
     runner.set_exec_fn(fn)
-    return runner.step(torch.zeros(2, 3, dtype=torch.int64))
+    return runner.step(ids)
 
 
 def test_8_bits_in_a_runner_go_by_what_it_computes_in():
@@ -166,3 +166,36 @@ class Wide(Layers):
     def __init__(self, kept):
         super().__init__(kept, torch.float32)
         self.up = nn.Parameter(torch.ones(32, 16))
+
+
+class Computed(nn.Module):
+    """A table that the model computes, once from all of a parameter and once from some of its columns"""
+
+    def __init__(self, plain):
+        super().__init__()
+        self.table = nn.Parameter(torch.linspace(-1, 1, 11 * 16).view(11, 16))
+        self.plain = plain
+
+    def forward(self, ids):
+        look = (lambda t, s: nn.functional.embedding(ids, t, padding_idx=3) * s) if self.plain else lambda t, s: layers.embedding(ids, t, scale=s, padding_idx=3)
+        return look(self.table * 2.0, 0.5) + look(self.table.float(), 3.0) + look(self.table.to(torch.bfloat16), 2.0).float()
+
+
+def test_a_table_that_is_computed_in_a_runner():
+    """Its gradient reaches the parameter."""
+    ids = torch.tensor([[1, 5, 3], [5, 5, 10]])
+    model, plain = Computed(False), Computed(True)
+    got = runner_step(model, ids=ids)
+    want = plain(ids).float().sum()
+    want.backward()
+    assert abs(float(got[0]) - float(want.detach())) <= 1e-5 * abs(float(want.detach()))
+    assert torch.allclose(model.table.grad, plain.table.grad, rtol=1e-5, atol=1e-6) and plain.table.grad[5].any() and not model.table.grad[3].any()
+
+
+def test_a_table_that_learns_nothing_in_a_runner():
+    model = Computed(False)
+    model.table.requires_grad_(False)
+    model.bias = nn.Parameter(torch.zeros(16))
+    model.forward = lambda ids: layers.embedding(ids, model.table * 2.0) + model.bias
+    runner_step(model)
+    assert model.bias.grad is not None and model.table.grad is None

@@ -99,3 +99,37 @@ def test_scores_of_a_long_batch(dtype, tokens, D, V):
     assert not rest.any()
     term, bound = head_reference(h[:, at], w, y[:, at], 0, "none", 0.0, torch.ones((), device="cuda"))[:2]
     within(loss[:, at], term, bound, torch.float32)
+
+
+@pytest.mark.parametrize("sequences", [8, 400])
+def test_a_table_that_is_computed_in_a_runner(sequences):
+    """Four micro-batches, ids sorted and not: the table's gradient reaches its parameter through what it is computed from, three ways."""
+    from test_decoder_compiled import Computed
+    from test_pipeline_gpu import _fresh_runner
+
+    from pfeife_amd.mp import partial_compiler
+    from pfeife_amd.option import PipeOption
+
+    model, plain = Computed(False).cuda(), Computed(True).cuda()
+    g = torch.Generator("cuda").manual_seed(3)
+    ids = torch.randint(0, 11, (sequences, 5), device="cuda", generator=g)
+    weight = torch.linspace(-1, 1, 16, device="cuda")
+    runner = _fresh_runner(PipeOption(device_cnt=1, batch_cnt=4, batch_size=sequences // 4, optimizer=dict(type="sgd", lr=0.0)))
+    compiled = torch.compile(model, backend=partial_compiler)
+
+    def fn(ids):
+        loss = (compiled(ids).float() * weight).sum()
+        loss.backward()
+        return loss.detach()
+
+    runner.set_exec_fn(fn)
+    for _ in range(3):
+        model.table.grad = plain.table.grad = None
+        losses = runner.step(ids)
+        torch.cuda.synchronize()
+        want = (plain(ids).float() * weight).sum()
+        want.backward()
+        # (sums of some thousand terms in fp32, of which the bf16 table's lookup rounds its gradient to 8 bits)
+        assert abs(sum(float(v) for v in losses) - float(want.detach())) <= 1e-3 * float((plain(ids).float() * weight).abs().sum().detach())
+        assert (model.table.grad - plain.table.grad).norm() <= 3 * 2.0 ** -8 * plain.table.grad.norm()
+        assert not model.table.grad[3].any()
