@@ -443,7 +443,8 @@ bool plan_of(Plan& p, const void* x, const void* w, int dtype, int64_t rows, int
   p.few_dw = back && !f32 && rows <= FEW_DW;
   p.narrow = !f32 && D % 8 != 0;
   const int64_t blocks = (ffn + 31) / 32 * 2;      // (of the weight's rows, to four wavefronts each)
-  p.splits = !back ? 1 : p.few_dx ? (int)(blocks < 4 * FEW_PARTS ? (blocks + 3) / 4 : FEW_PARTS) : splits_of(dtype, rows, D, p.wide == ffn ? 2 * ffn : ffn);
+  const int64_t deep = f32 && p.wide != ffn ? ffn : 2 * p.wide;      // (16 bits: one sum over both halves, whatever ffn is)
+  p.splits = !back ? 1 : p.few_dx ? (int)(blocks < 4 * FEW_PARTS ? (blocks + 3) / 4 : FEW_PARTS) : splits_of(dtype, rows, D, deep);
   // rows of one launch: everything it addresses by 32-bit offsets stays below 2 GiB
   const int64_t widest = p.depth > 2 * p.half ? p.depth : 2 * p.half;
   p.chunk = ((1ll << 31) / (widest * p.es) - 512) / 256 * 256;

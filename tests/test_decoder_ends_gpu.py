@@ -133,3 +133,19 @@ def test_a_table_that_is_computed_in_a_runner(sequences):
         assert abs(sum(float(v) for v in losses) - float(want.detach())) <= 1e-3 * float((plain(ids).float() * weight).abs().sum().detach())
         assert (model.table.grad - plain.table.grad).norm() <= 3 * 2.0 ** -8 * plain.table.grad.norm()
         assert not model.table.grad[3].any()
+
+
+@pytest.mark.parametrize("rows,D,ffn", [(1024, 256, 5630), (2048, 64, 4097), (1024, 1030, 5630)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gated_linear_in_shares_of_an_odd_depth(dtype, rows, D, ffn):
+    from test_decoder_ops_gpu import gated_check
+
+    from pfeife_amd.layers import gated_linear
+
+    g = torch.Generator("cuda").manual_seed(12)
+    x = torch.randn(rows, D, device="cuda", generator=g).to(dtype).requires_grad_()
+    w = (torch.randn(2 * ffn, D, device="cuda", generator=g) * D ** -0.5).to(dtype).requires_grad_()
+    up = torch.randn(rows, ffn, device="cuda", generator=g).to(dtype)
+    y = gated_linear(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), up)
+    gated_check(x.detach(), w.detach(), "silu", "16bit", up, y.detach(), dx, dw)

@@ -110,3 +110,13 @@ def test_a_loss_without_a_possible_gradient_is_refused_before_it_runs(on_the_cpu
         with pytest.raises(RuntimeError, match="linear_cross_entropy: .*too many for one call"):
             loss.linear_cross_entropy(a, b, y)
     assert loss.linear_cross_entropy(h[:, :65000], w.clone().requires_grad_(), y[:, :65000]).requires_grad
+
+
+@pytest.mark.parametrize("rows,D,ffn", [(1024, 2048, 5630), (777, 1000, 2732), (300, 512, 1001), (64, 4096, 999), (2048, 64, 4097)])
+def test_shares_of_a_sum_go_by_its_depth(rows, D, ffn):
+    """In 16 bits the gradient of x is one sum over both halves, padded to multiples of 8: as many shares of it, and so as much memory, as at that width."""
+    from pfeife_amd import hip
+
+    lib = hip.load()
+    need = lambda columns: lib.pf_gated_linear_workspace(None, None, 2, rows, D, columns, 1, 1)  # noqa: E731
+    assert need(ffn) == need(-(-ffn // 8) * 8) > 0
