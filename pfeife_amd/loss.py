@@ -120,14 +120,14 @@ def _table(t, who):
     return k
 
 
-_C = torch._C
+_modes, _mode, _proxies = torch._C._len_torch_dispatch_stack, torch._C._get_dispatch_mode, torch._C._TorchDispatchModeKey.PROXY
+_tracing, _key_is_on, _before = torch._C._is_tracing, torch._C._dispatch_tls_is_dispatch_key_included, torch._C.DispatchKey.PreDispatch
 
 
 def _recorded():
     """Is a graph being recorded of the calls that are made (make_fx, torch.jit.trace)?  A kernel's launch would not be in it, only the memory that it
     was about to fill."""
-    return (_C._get_tracing_state() is not None or _C._len_torch_dispatch_stack() > 0 and _C._get_dispatch_mode(_C._TorchDispatchModeKey.PROXY) is not None
-            or _C._dispatch_tls_is_dispatch_key_included(_C.DispatchKey.PreDispatch))
+    return _tracing() or _modes() > 0 and _mode(_proxies) is not None or _key_is_on(_before)
 
 
 def _refuse_recording(who):
